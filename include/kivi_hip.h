@@ -396,6 +396,76 @@ int kivi_packed_decode_attention_append(
     int32_t group_size_v, int32_t chunk_capacity, int32_t num_chunks, int32_t res_capacity,
     int32_t res_start, int32_t res_len, float softmax_scale, int32_t num_splits, void* stream);
 
+/* ---- paged cache -----------------------------------------------------------
+ * No reference counterpart (the reference serves one fixed batch).  A cache for
+ * sequences that come and go: k_pages and v_pages are [num_pages][kv_heads]
+ * [page_size][head_dim] of dtype (0 f32, 1 bf16, 2 f16), 16-byte aligned;
+ * position p of a sequence lies on page page_table[p / page_size] at offset
+ * p % page_size.  page_size is 16, 32, 64, 128 or 256, head_dim a multiple of
+ * 16 up to 256, num_pages * page_size below 2^31. */
+
+/* The number of words of kivi_paged_plan's info. */
+#define KIVI_PAGED_INFO 16
+
+/* Writes a step's plan: which sequences bring how many new tokens, where these
+ * go, and how the attention's work is shared out.  Host work only: every array
+ * is host memory.  Sequence s brings new_lens[s] tokens (0: it sits this step
+ * out) and is context_lens[s] tokens long with them; its pages are
+ * page_table[s*table_stride + 0 .. ceil(context/page_size)-1], table_pages
+ * entries at most.  Pages may be shared between sequences (a common prefix), but
+ * no slot may be given to two new tokens.  With plan NULL only info is written:
+ * info[0] is the size of the plan in int32 words, info[1] its tokens.  The
+ * caller copies the plan to the device once per step and gives the copy and info
+ * to every layer's calls; it holds for pools of num_pages pages and the
+ * geometry it was made for. */
+int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* context_lens,
+                    const int32_t* page_table, int64_t table_stride, int32_t table_pages,
+                    int32_t page_size, int64_t num_pages, int32_t dtype, int32_t q_heads,
+                    int32_t kv_heads, int32_t head_dim, int32_t* plan, int64_t plan_words,
+                    int64_t* info);
+
+/* Appends a step's new tokens to the pages: token t of k and v (element
+ * (t, h, d) at t*token_stride + h*head_stride + d, in elements of dtype) goes
+ * to the plan's slot t.  tokens is info[1] (rows behind it are not read).  q
+ * (NULL: none) is [tokens][q_heads][head_dim] with strides of its own and goes
+ * to q_out, contiguous.  On the way, in fp32 with one rounding at the end:
+ * - q_norm, k_norm (NULL: none): head_dim weights of norm_dtype; each head row x
+ *   of q or k becomes x * rsqrt(mean(x^2) + eps) * weight;
+ * - rotary_dim > 0 (a multiple of 16): the first rotary_dim channels of q and k
+ *   rows are rotated by the angles of the token's position p, row p of cos and
+ *   sin ([positions][rotary_dim/2] f32): channels i and i + rotary_dim/2, or 2i
+ *   and 2i+1 with interleaved.  The tables must reach info[12] positions.
+ * Values are copied bit for bit. */
+int kivi_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                      const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                      const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                      int32_t dtype, void* q_out, void* k_pages, void* v_pages,
+                      int64_t num_pages, int32_t page_size, int32_t q_heads, int32_t kv_heads,
+                      int32_t head_dim, const int32_t* plan, int32_t tokens, const float* cos,
+                      const float* sin, int32_t rotary_dim, int32_t interleaved,
+                      const void* q_norm, const void* k_norm, int32_t norm_dtype, float eps,
+                      void* stream);
+
+/* Bytes of workspace of kivi_paged_attention for a plan (0: none is needed). */
+size_t kivi_paged_attention_workspace_size(const int64_t* info, int32_t kv_heads,
+                                           int32_t head_dim);
+
+/* Attention of a step's new tokens over the pages, their own keys and values
+ * included (append them first): new token i of a sequence with n new ones in a
+ * context of c sees positions 0 .. c - n + i.  q is [tokens][q_heads][head_dim]
+ * of dtype with strides of whole 16-byte vectors, out the same, contiguous; query
+ * head h reads kv head h / (q_heads / kv_heads).  softmax_scale must be positive.
+ * Scores, softmax and sums are fp32; weights are rounded to dtype for the product
+ * with the values.  What lies behind a sequence's end or in positions that a
+ * token does not see, infinities and NaN too, does not reach it.  Rows of out
+ * behind the last token are left as they were. */
+int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                         int32_t dtype, const void* k_pages, const void* v_pages,
+                         int64_t num_pages, int32_t page_size, int32_t q_heads,
+                         int32_t kv_heads, int32_t head_dim, const int32_t* plan,
+                         const int64_t* info, float softmax_scale, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

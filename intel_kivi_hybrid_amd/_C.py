@@ -697,3 +697,270 @@ def packed_attention_typed(q, store, softmax_scale=None, kv_start=None, hidden=N
             D ** -0.5 if softmax_scale is None else float(softmax_scale), 0,
             _stream_of(q.device)), "packed_attention")
     return out
+
+
+# --------------------------------------------------------------------------
+# Paged cache (no reference counterpart; see include/kivi_hip.h): sequences of
+# unequal lengths on pages of one pool.
+# --------------------------------------------------------------------------
+def _check_inference(*tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            _check(t is None or not t.requires_grad, "inference only: a tensor requires a "
+                   "gradient; call it under torch.no_grad()")
+
+
+def _host_ints(values, name: str) -> torch.Tensor:
+    """Counts as a contiguous int32 host tensor."""
+    t = torch.as_tensor(values)
+    if t.numel() == 0:
+        t = t.to(torch.int64)
+    _check(t.dim() == 1 and t.device.type == "cpu" and t.dtype in (torch.int32, torch.int64),
+           name, " must hold one int for each sequence, on the host")
+    if t.dtype is torch.int64:
+        _check(t.numel() == 0 or (int(t.min()) >= 0 and int(t.max()) < 1 << 31), name,
+               " must lie in [0, 2^31)")
+        t = t.to(torch.int32)
+    return t.contiguous()
+
+
+class PagedPlan:
+    """One step over a paged cache (:func:`paged_plan`): which sequences bring
+    how many new tokens, and where these lie, as one device array that every
+    layer's :func:`paged_append` and :func:`paged_attention` read.  It belongs to
+    pools of ``num_pages`` pages and to the geometry it was made for."""
+
+    __slots__ = ("device", "tokens", "context", "num_pages", "page_size", "q_heads", "kv_heads",
+                 "head_dim", "dtype", "_code", "_buf", "_ptr", "_info", "_info_ptr",
+                 "_workspace", "_stream", "_event", "_settled")
+
+    def wait(self) -> None:
+        """Waits until the plan is on the device.  Needed only before a graph is
+        captured with it (which reads the plan's memory at every replay: keep the
+        plan as long as the graph); other calls order themselves behind its copy."""
+        self._event.synchronize()
+        self._settled = True
+
+    def _enter(self, device: int) -> int:
+        """The current stream's handle, ordered behind the plan's copy."""
+        handle = stream_handle(device)
+        if handle != self._stream and not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(device)
+            if not self._settled:
+                stream.wait_event(self._event)
+            # (its memory is not given away while this stream may read it)
+            self._buf.record_stream(stream)
+        elif handle != self._stream:
+            _check(self._settled, "call the plan's wait() before capturing a graph with it")
+        return handle
+
+
+def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_heads, kv_heads,
+               head_dim, dtype=torch.bfloat16, device="cuda") -> PagedPlan:
+    """The plan of a step in which sequence s, ``context_lens[s]`` tokens long
+    with them, brings its last ``new_lens[s]`` tokens (0: it sits this step out).
+    ``page_table`` (int32 host tensor ``[sequences, pages]``): its pages, position
+    p on entry ``p // page_size``; entries behind its last position are not read.
+    Tokens are numbered sequence by sequence.  Host work and one copy to
+    ``device``, once per step for all layers."""
+    _check(isinstance(page_table, torch.Tensor) and page_table.dim() == 2
+           and page_table.dtype is torch.int32 and page_table.device.type == "cpu",
+           "page_table must be an int32 [sequences, pages] tensor on the host")
+    _check(dtype in _IO_DTYPES, "dtype must be float32, bfloat16 or float16, got ",
+           _dtype_name(dtype))
+    dev = torch.device(device)
+    _check(dev.type == _DEVICE_TYPE, "device must be on ", _DEVICE_TYPE, " but got ", dev.type)
+    page_size, q_heads, kv_heads, head_dim = (
+        _check_int(x, n) for x, n in ((page_size, "page_size"), (q_heads, "q_heads"),
+                                      (kv_heads, "kv_heads"), (head_dim, "head_dim")))
+    num_pages = _check_int(num_pages, "num_pages")
+    table = page_table.contiguous()
+    ctx, new = _host_ints(context_lens, "context_lens"), _host_ints(new_lens, "new_lens")
+    n_seqs = table.shape[0]
+    _check(ctx.numel() == n_seqs and new.numel() == n_seqs,
+           "context_lens and new_lens must hold one entry for each of the table's ", n_seqs,
+           " sequences")
+    p = PagedPlan()
+    info = (ctypes.c_int64 * 16)()
+    p._info, p._info_ptr = info, ctypes.addressof(info)
+    args = (n_seqs, new.data_ptr(), ctx.data_ptr(), table.data_ptr(), table.shape[1],
+            table.shape[1], page_size, num_pages, _IO_DTYPES[dtype], q_heads, kv_heads, head_dim)
+    _native.check(_lib.kivi_paged_plan(*args, None, 0, p._info_ptr), "paged_plan")
+    p.device = torch.device(_DEVICE_TYPE, device_index(dev))
+    _check(not torch.cuda.is_current_stream_capturing(),
+           "a plan is made outside of a graph's capture")
+    p.tokens, p.context = info[1], info[12]
+    p.num_pages, p.page_size, p.dtype, p._code = num_pages, page_size, dtype, _IO_DTYPES[dtype]
+    p.q_heads, p.kv_heads, p.head_dim = q_heads, kv_heads, head_dim
+    host = torch.empty(max(info[0], 1), dtype=torch.int32, pin_memory=True)
+    _native.check(_lib.kivi_paged_plan(*args, host.data_ptr(), host.numel(), p._info_ptr),
+                  "paged_plan")
+    with on_device(p.device):
+        p._buf = host.to(p.device, non_blocking=True)
+        p._event = torch.cuda.Event()
+        p._event.record()
+        p._stream = stream_handle(p.device)
+    p._settled = False
+    p._ptr = p._buf.data_ptr()
+    p._workspace = int(_lib.kivi_paged_attention_workspace_size(p._info_ptr, kv_heads, head_dim))
+    return p
+
+
+def _check_pages(plan, k_pages, v_pages) -> None:
+    shape = (plan.num_pages, plan.kv_heads, plan.page_size, plan.head_dim)
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if not (t.shape == shape and t.dtype is plan.dtype and t.is_contiguous()
+                and t.device == plan.device and t.data_ptr() % 16 == 0):
+            _fail(name, " must be a contiguous, 16-byte aligned ", list(shape), " tensor of ",
+                  _dtype_name(plan.dtype), " on ", plan.device, ", got ", list(t.shape), " of ",
+                  _dtype_name(t.dtype), " on ", t.device)
+
+
+def _check_tokens(t, name: str, plan, heads: int) -> None:
+    """A step's rows ``[>= tokens, heads, head_dim]``, any strides of whole rows."""
+    if not (t.dim() == 3 and t.shape[0] >= plan.tokens and t.shape[1] == heads
+            and t.shape[2] == plan.head_dim and t.dtype is plan.dtype
+            and t.device == plan.device):
+        _fail(name, " must be [>= ", plan.tokens, ", ", heads, ", ", plan.head_dim, "] of ",
+              _dtype_name(plan.dtype), " on ", plan.device, ", got ", list(t.shape), " of ",
+              _dtype_name(t.dtype), " on ", t.device)
+    _check(t.stride(2) == 1, name, "'s channels must be contiguous")
+
+
+def _new_rows(t, plan):
+    """An output beside a step's rows ``t``; rows behind the step's tokens, which
+    no kernel writes, are zeros."""
+    make = torch.zeros if t.shape[0] > plan.tokens else torch.empty
+    return make(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _check_out(out, name: str, like) -> None:
+    _check(out.shape == like.shape and out.dtype is like.dtype and out.device == like.device
+           and out.is_contiguous() and out.data_ptr() % 16 == 0, name,
+           " must be a contiguous, 16-byte aligned ", list(like.shape), " tensor of ",
+           _dtype_name(like.dtype), " on ", like.device)
+
+
+def paged_append(k, v, k_pages, v_pages, plan, q=None, q_out=None, cos=None, sin=None,
+                 interleaved=False, q_norm=None, k_norm=None, eps=1e-6):
+    """Write a step's new keys and values ``[tokens, Hkv, D]`` to their pages,
+    normed and rotated on the way, and return its queries ``q`` ``[tokens, Hq, D]``
+    normed and rotated likewise (None without ``q``): one launch.
+
+    ``q_norm``, ``k_norm`` ``[D]``: weights of an RMS norm over each head's
+    channels (``eps`` inside the root).  ``cos``, ``sin`` ``[positions, r / 2]``
+    fp32 (:func:`rotary_tables`): the first r channels are rotated by the angles of
+    the token's position in its sequence, channel i with i + r/2, or 2i with 2i + 1
+    if ``interleaved``.  Both in fp32, rounded once.  Values are copied.  Rows may
+    have any strides, as slices of one projection have; rows behind the plan's
+    tokens are not read, and stay as they are in ``q_out``, which may be ``q``."""
+    _check_inference(k, v, q, q_norm, k_norm)
+    _check_pages(plan, k_pages, v_pages)
+    _check_tokens(k, "k", plan, plan.kv_heads)
+    _check_tokens(v, "v", plan, plan.kv_heads)
+    rot = 0
+    if cos is not None or sin is not None:
+        _check(cos is not None and sin is not None, "rotation needs cos and sin")
+        rot = 2 * cos.shape[-1]
+        _check(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype is torch.float32
+               and sin.dtype is torch.float32 and cos.is_contiguous() and sin.is_contiguous()
+               and cos.device == plan.device and sin.device == plan.device,
+               "cos and sin must be contiguous [positions, rotated / 2] float32 tensors on ",
+               plan.device)
+        _check(cos.shape[0] >= plan.context, "cos and sin reach ", cos.shape[0],
+               " positions, the step's longest sequence has ", plan.context)
+    norm_dt = None
+    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if t is None:
+            continue
+        _check(t.dim() == 1 and t.shape[0] == plan.head_dim and t.dtype in _IO_DTYPES
+               and t.is_contiguous() and t.device == plan.device, name, " must be a contiguous [",
+               plan.head_dim, "] tensor of a float type on ", plan.device)
+        _check(norm_dt is None or norm_dt is t.dtype, "q_norm and k_norm must have one type")
+        norm_dt = t.dtype
+    if q is not None:
+        _check_tokens(q, "q", plan, plan.q_heads)
+        if q_out is None:
+            q_out = _new_rows(q, plan)
+        else:
+            _check_out(q_out, "q_out", q)
+    else:
+        _check(q_out is None and q_norm is None, "q_out and q_norm need q")
+    dev = plan.device.index
+    with on_device(dev):
+        _native.check(_lib.kivi_paged_append(
+            0 if q is None else q.data_ptr(), 0 if q is None else q.stride(0),
+            0 if q is None else q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+            v.data_ptr(), v.stride(0), v.stride(1), plan._code,
+            0 if q is None else q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+            plan.num_pages, plan.page_size, plan.q_heads, plan.kv_heads, plan.head_dim,
+            plan._ptr, plan.tokens, 0 if cos is None else cos.data_ptr(),
+            0 if sin is None else sin.data_ptr(), rot, 1 if interleaved else 0,
+            0 if q_norm is None else q_norm.data_ptr(),
+            0 if k_norm is None else k_norm.data_ptr(),
+            0 if norm_dt is None else _IO_DTYPES[norm_dt], eps, plan._enter(dev)),
+            "paged_append")
+    return q_out
+
+
+def rotary_tables(positions, rotary_dim, base=10000.0, inv_freq=None, device="cuda"):
+    """cos and sin ``[positions, rotary_dim / 2]`` fp32 of position x frequency,
+    the angles formed in fp64.  Frequencies: ``inv_freq`` (a model's own, scaled
+    as it scales them), else ``base ** (-2 i / rotary_dim)``."""
+    _check(rotary_dim > 0 and rotary_dim % 16 == 0,
+           "rotary_dim must be a positive multiple of 16, got ", rotary_dim)
+    if inv_freq is None:
+        inv_freq = base ** (-torch.arange(rotary_dim // 2, dtype=torch.float64)
+                            / (rotary_dim // 2))
+    f = inv_freq.detach().to("cpu", torch.float64)
+    _check(f.dim() == 1 and f.shape[0] == rotary_dim // 2, "inv_freq must hold ",
+           rotary_dim // 2, " frequencies, got ", list(f.shape))
+    ang = torch.arange(positions, dtype=torch.float64)[:, None] * f[None, :]
+    return ang.cos().float().to(device), ang.sin().float().to(device)
+
+
+def _call_workspace(device, nbytes: int):
+    """:func:`_workspace`, but memory of its own for each call of a graph: two
+    captured graphs may run at once."""
+    if nbytes and torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=torch.device(_DEVICE_TYPE, device))
+    return _workspace(device, nbytes)
+
+
+def paged_attention(q, k_pages, v_pages, plan, softmax_scale=None, out=None, workspace=None):
+    """Attention of a step's new tokens ``q [tokens, Hq, D]`` over their
+    sequences' pages, their own keys and values included (:func:`paged_append`
+    first): token i of n new ones in a context of c sees positions 0 .. c - n + i.
+    Returns ``[tokens, Hq, D]`` in q's type.  Chunks of prompts, verification
+    passes and single tokens may share a call.  Rows behind the plan's tokens are
+    not read, and stay as they are in ``out``.  Launched on the current stream."""
+    _check_inference(q)
+    _check_pages(plan, k_pages, v_pages)
+    _check_tokens(q, "q", plan, plan.q_heads)
+    per = 16 // q.element_size()
+    if q.data_ptr() % 16 or q.stride(0) % per or q.stride(1) % per:
+        q = q.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        out = _new_rows(q, plan)
+    else:
+        _check_out(out, "out", q)
+    dev = plan.device.index
+    with on_device(dev):
+        need = plan._workspace
+        if workspace is None:
+            workspace = _call_workspace(dev, need)
+        elif need:
+            _check(workspace.is_contiguous() and workspace.device == plan.device
+                   and workspace.data_ptr() % 16 == 0
+                   and workspace.numel() * workspace.element_size() >= need,
+                   "workspace must be a contiguous, 16-byte aligned tensor of ", need,
+                   " bytes on ", plan.device)
+        _native.check(_lib.kivi_paged_attention(
+            q.data_ptr(), q.stride(0), q.stride(1), plan._code, k_pages.data_ptr(),
+            v_pages.data_ptr(), plan.num_pages, plan.page_size, plan.q_heads, plan.kv_heads,
+            plan.head_dim, plan._ptr, plan._info_ptr,
+            plan.head_dim ** -0.5 if softmax_scale is None else float(softmax_scale),
+            out.data_ptr(), 0 if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel() * workspace.element_size(),
+            plan._enter(dev)), "paged_attention")
+    return out

@@ -80,6 +80,15 @@ SIGNATURES = {
     "kivi_packed_decode_attention_noalloc": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32,
                                              _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
                                              _i32, _i32, _i32, _i32, _f32, _i32, _vp],
+    # host arrays throughout
+    "kivi_paged_plan": [_i32, _vp, _vp, _vp, _i64, _i32, _i32, _i64, _i32, _i32, _i32, _i32,
+                        _vp, _i64, _vp],
+    "kivi_paged_append": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp,
+                          _i64, _i32, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _vp,
+                          _vp, _i32, _f32, _vp],
+    "kivi_paged_attention_workspace_size": [_vp, _i32, _i32],
+    "kivi_paged_attention": [_vp, _i64, _i64, _i32, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp,
+                             _vp, _f32, _vp, _vp, ctypes.c_size_t, _vp],
 }
 
 _RESTYPES = {
@@ -87,6 +96,7 @@ _RESTYPES = {
     "kivi_clear_error": None,
     "kivi_packed_decode_attention_workspace_size": ctypes.c_size_t,
     "kivi_packed_attention_workspace_size": ctypes.c_size_t,
+    "kivi_paged_attention_workspace_size": ctypes.c_size_t,
 }
 
 _lib = None

@@ -1,0 +1,474 @@
+// Paged K/V cache: a step's plan (host) and the append of its new tokens.
+//
+// The append takes a projection's queries, keys and values of the step's
+// tokens, token-major as a model's projections leave them.  For a head row x
+// of the queries or keys:
+//   y = x * rsqrt(mean(x^2) + eps) * weight          (where a weight is given)
+//   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin)   for each rotated pair
+// with the token's position's row of the tables, all in fp32 and rounded once
+// to the tensors' type; values are copied.  Keys and values go to their pages,
+// queries to an output of their own: one launch, each element read and
+// written once.  Memory-bound for prompts, launch-bound for single tokens.
+//
+// A lane takes two 8-element vectors of a head that hold whole pairs: i and
+// i + r/2 of the first r channels rotated by halves, neighbours otherwise;
+// so a rotation never crosses lanes, and only the norm's sum does, over the
+// D / 16 lanes of the head (a power of two of them, DPP steps).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "kivi_common.hpp"
+#include "kivi_paged.hpp"
+#include "../../include/kivi_hip.h"
+
+namespace kivi {
+namespace {
+
+constexpr int kAppendBlock = 256;
+
+struct AppendArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
+    void* q_out;
+    void* k_pages;
+    void* v_pages;
+    const int2* tokens;          // slot, position
+    const float* cos;
+    const float* sin;
+    const void* q_norm;
+    const void* k_norm;
+    float eps;
+    int n_tokens, Hq, Hkv, D, page_shift, rot, lanes_log2;
+    int norm_dt, interleaved, vec;
+};
+
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t i, bool vec, float (&x)[8]) {
+    if (vec) {
+        const float4 a = load4_vec<DT>(p, i), b = load4_vec<DT>(p, i + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = widen<DT>(p, i + j);
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(void* p, int64_t i, const float (&x)[8]) {
+    if constexpr (DT == kSrcF32) {
+        float4* o = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+        o[0] = make_float4(x[0], x[1], x[2], x[3]);
+        o[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint16_t lo, hi;
+            if constexpr (DT == kSrcBF16) {
+                lo = __builtin_bit_cast(uint16_t, (__bf16)x[2 * j]);
+                hi = __builtin_bit_cast(uint16_t, (__bf16)x[2 * j + 1]);
+            } else {
+                lo = __builtin_bit_cast(uint16_t, (_Float16)x[2 * j]);
+                hi = __builtin_bit_cast(uint16_t, (_Float16)x[2 * j + 1]);
+            }
+            w[j] = lo | (uint32_t)hi << 16;
+        }
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) =
+            make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// Sum over aligned segments of 1 << log2 lanes.
+__device__ __forceinline__ float seg_sum(float v, int log2) {
+    if (log2 > 0) v += seg_partner<1>(v);
+    if (log2 > 1) v += seg_partner<2>(v);
+    if (log2 > 2) v += seg_partner<4>(v);
+    if (log2 > 3) v += seg_partner<8>(v);
+    return v;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kAppendBlock) paged_append_kernel(AppendArgs a) {
+    const int heads = a.Hq + 2 * a.Hkv;
+    const int64_t t = (int64_t)blockIdx.x * kAppendBlock + threadIdx.x;
+    const int64_t row = t >> a.lanes_log2;
+    if (row >= (int64_t)a.n_tokens * heads) return;      // (whole segments leave)
+    const int unit = (int)t & ((1 << a.lanes_log2) - 1);
+    const bool live = unit < a.D / 16;
+    const int tok = (int)(row / heads), h = (int)(row - (int64_t)tok * heads);
+    const int half = a.rot / 2;
+    const int2 place = a.tokens[tok];
+
+    // the lane's two vectors of 8 channels, and the first of its pairs
+    const bool turned = live && 16 * unit < a.rot && h < a.Hq + a.Hkv;
+    int c0 = 16 * unit, c1 = 16 * unit + 8;
+    if (16 * unit < a.rot && !a.interleaved) {
+        c0 = 8 * unit;
+        c1 = half + 8 * unit;
+    }
+
+    const void* src = a.v;
+    int64_t from = tok * a.v_st + (int64_t)(h - a.Hq - a.Hkv) * a.v_sh;
+    const void* norm = nullptr;
+    if (h < a.Hq) {
+        src = a.q;
+        from = tok * a.q_st + h * a.q_sh;
+        norm = a.q_norm;
+    } else if (h < a.Hq + a.Hkv) {
+        src = a.k;
+        from = tok * a.k_st + (int64_t)(h - a.Hq) * a.k_sh;
+        norm = a.k_norm;
+    }
+    float x[8], y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = y[j] = 0.f;
+    if (live) {
+        load8<DT>(src, from + c0, a.vec, x);
+        load8<DT>(src, from + c1, a.vec, y);
+    }
+    if (norm != nullptr) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf(x[j], x[j], fmaf(y[j], y[j], s));
+        s = seg_sum(s, a.lanes_log2);
+        const float r = 1.0f / sqrtf(s / (float)a.D + a.eps);
+        if (live) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = x[j] * r * load1_dt(norm, c0 + j, a.norm_dt);
+                y[j] = y[j] * r * load1_dt(norm, c1 + j, a.norm_dt);
+            }
+        }
+    }
+    if (!live) return;
+    if (turned) {
+        const float* cs = a.cos + (int64_t)place.y * half + 8 * unit;
+        const float* sn = a.sin + (int64_t)place.y * half + 8 * unit;
+        float u[8], w[8];
+        if (a.interleaved) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {          // pair j: channels 2j, 2j + 1
+                const float p = j < 4 ? x[2 * (j % 4)] : y[2 * (j % 4)];
+                const float q = j < 4 ? x[2 * (j % 4) + 1] : y[2 * (j % 4) + 1];
+                u[j] = fmaf(p, cs[j], -(q * sn[j]));
+                w[j] = fmaf(q, cs[j], p * sn[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[2 * j] = u[j];
+                x[2 * j + 1] = w[j];
+                y[2 * j] = u[j + 4];
+                y[2 * j + 1] = w[j + 4];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                u[j] = fmaf(x[j], cs[j], -(y[j] * sn[j]));
+                w[j] = fmaf(y[j], cs[j], x[j] * sn[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                x[j] = u[j];
+                y[j] = w[j];
+            }
+        }
+    }
+    void* dst = a.q_out;
+    int64_t to = ((int64_t)tok * a.Hq + h) * a.D;
+    if (h >= a.Hq) {
+        const int kvh = h < a.Hq + a.Hkv ? h - a.Hq : h - a.Hq - a.Hkv;
+        const int64_t page = place.x >> a.page_shift;
+        const int off = place.x & ((1 << a.page_shift) - 1);
+        dst = h < a.Hq + a.Hkv ? a.k_pages : a.v_pages;
+        to = (((page * a.Hkv + kvh) << a.page_shift) + off) * a.D;
+    }
+    store8<DT>(dst, to + c0, x);
+    store8<DT>(dst, to + c1, y);
+}
+
+int page_shift_of(int32_t page_size) {
+    for (int s = 4; s <= 8; ++s)
+        if (page_size == 1 << s) return s;
+    return -1;
+}
+
+int check_pool(int32_t dtype, int64_t num_pages, int32_t page_size, int32_t q_heads,
+               int32_t kv_heads, int32_t head_dim) {
+    if (dtype < 0 || dtype > 2)
+        return set_error(kErrInvalidArgument, "dtype %d is not 0 (f32), 1 (bf16) or 2 (f16)", dtype);
+    if (page_shift_of(page_size) < 0)
+        return set_error(kErrInvalidArgument,
+                         "page_size must be 16, 32, 64, 128 or 256, got %d", page_size);
+    if (num_pages < 1 || num_pages * page_size > INT32_MAX)
+        return set_error(kErrInvalidArgument,
+                         "num_pages must be positive and hold fewer than 2^31 tokens, got %lld",
+                         (long long)num_pages);
+    if (kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0)
+        return set_error(kErrInvalidArgument,
+                         "q_heads (%d) must be a positive multiple of kv_heads (%d)", q_heads,
+                         kv_heads);
+    if (head_dim < 16 || head_dim > 256 || head_dim % 16 != 0)
+        return set_error(kErrUnsupported,
+                         "head_dim must be a multiple of 16 up to 256, got %d", head_dim);
+    return kOk;
+}
+
+struct Tile {
+    int seq, kind, row0;
+    int64_t begin, end;          // positions that its rows see
+};
+
+}  // namespace
+}  // namespace kivi
+
+using namespace kivi;
+
+extern "C" {
+
+int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* context_lens,
+                    const int32_t* page_table, int64_t table_stride, int32_t table_pages,
+                    int32_t page_size, int64_t num_pages, int32_t dtype, int32_t q_heads,
+                    int32_t kv_heads, int32_t head_dim, int32_t* plan, int64_t plan_ints,
+                    int64_t* info) {
+    int rc = check_pool(dtype, num_pages, page_size, q_heads, kv_heads, head_dim);
+    if (rc) return rc;
+    if (n_seqs < 0 || info == nullptr || table_pages < 0 || table_stride < table_pages ||
+        (n_seqs > 0 && (new_lens == nullptr || context_lens == nullptr ||
+                        (page_table == nullptr && table_pages > 0))))
+        return set_error(kErrInvalidArgument, "null or negative plan argument");
+    const int shift = page_shift_of(page_size);
+    const int hg = q_heads / kv_heads;
+    const bool f32 = dtype == 0;
+    try {
+        int64_t tokens = 0, pages = 0, longest = 0;
+        for (int s = 0; s < n_seqs; ++s) {
+            const int64_t n = new_lens[s], c = context_lens[s];
+            if (n < 0 || c < n)
+                return set_error(kErrInvalidArgument,
+                                 "sequence %d: %lld new tokens in a context of %lld", s,
+                                 (long long)n, (long long)c);
+            const int64_t p = (c + page_size - 1) >> shift;
+            if (p > table_pages)
+                return set_error(kErrInvalidArgument,
+                                 "sequence %d: a context of %lld needs %lld pages, the table has "
+                                 "%d", s, (long long)c, (long long)p, table_pages);
+            if (n == 0) continue;
+            for (int64_t j = 0; j < p; ++j) {
+                const int32_t page = page_table[s * table_stride + j];
+                if (page < 0 || page >= num_pages)
+                    return set_error(kErrInvalidArgument,
+                                     "sequence %d: page %d outside the pool of %lld", s, page,
+                                     (long long)num_pages);
+            }
+            tokens += n;
+            pages += p;
+            longest = std::max(longest, c);
+        }
+        if (tokens > INT32_MAX / 4 || tokens * (int64_t)hg > INT32_MAX || pages > INT32_MAX / 4)
+            return set_error(kErrInvalidArgument, "a step of %lld tokens over %lld pages is too "
+                             "large", (long long)tokens, (long long)pages);
+
+        // No slot is written twice: the new tokens' stretches of pages, sorted.
+        struct Run { int32_t page, from, to; };
+        std::vector<Run> runs;
+        for (int s = 0; s < n_seqs; ++s) {
+            if (new_lens[s] == 0) continue;
+            const int64_t first = context_lens[s] - new_lens[s], last = context_lens[s] - 1;
+            for (int64_t j = first >> shift; j <= last >> shift; ++j)
+                runs.push_back({page_table[s * table_stride + j],
+                                (int32_t)(std::max(first, j << shift) - (j << shift)),
+                                (int32_t)(std::min<int64_t>(last, (j << shift) + page_size - 1) -
+                                          (j << shift))});
+        }
+        std::sort(runs.begin(), runs.end(), [](const Run& a, const Run& b) {
+            return a.page != b.page ? a.page < b.page : a.from < b.from;
+        });
+        for (size_t i = 1; i < runs.size(); ++i)
+            if (runs[i].page == runs[i - 1].page && runs[i].from <= runs[i - 1].to)
+                return set_error(kErrInvalidArgument, "page %d: a slot is given to two new tokens",
+                                 runs[i].page);
+
+        // Row tiles, and the positions that the last row of each sees.
+        std::vector<Tile> tiles;
+        int64_t work[kPagedKinds] = {0, 0, 0, 0}, count[kPagedKinds] = {0, 0, 0, 0};
+        for (int s = 0; s < n_seqs; ++s) {
+            const int64_t n = new_lens[s], rows = n * hg;
+            if (n == 0) continue;
+            const int kind = paged_kind(rows, f32, head_dim);
+            const int step = paged_tile_rows(kind);
+            for (int64_t r = 0; r < rows; r += step) {
+                const int64_t last = std::min(rows, r + step) - 1;
+                const int64_t end = context_lens[s] - n + last / hg + 1;
+                tiles.push_back({s, kind, (int)r, 0, end});
+                work[kind] += end;
+                count[kind] += 1;
+            }
+        }
+        // Splits: enough workgroups for the card's 256 CUs, each kept long
+        // enough to be worth its partial.
+        int64_t target[kPagedKinds];
+        for (int kind = 0; kind < kPagedKinds; ++kind) {
+            const int64_t want = kind == kMany ? 512 : 1024;
+            const int64_t least = kind == kMany ? 512 : 256;
+            const int64_t total = work[kind] * kv_heads;
+            target[kind] = std::max(least, (total + want - 1) / want);
+            if (count[kind] * kv_heads >= want) target[kind] = std::max(target[kind], longest);
+            target[kind] = (target[kind] + 63) / 64 * 64;
+        }
+        int64_t items = 0, merges = 0, parts = 0, part_rows = 0, kinds[kPagedKinds] = {0, 0, 0, 0};
+        for (const Tile& t : tiles) {
+            const int64_t len = t.end - t.begin;
+            const int64_t splits = std::max<int64_t>(1, (len + target[t.kind] - 1) / target[t.kind]);
+            items += splits;
+            kinds[t.kind] += splits;
+            if (splits > 1) {
+                merges += 1;
+                parts += splits;
+                part_rows = std::max<int64_t>(part_rows, paged_tile_rows(t.kind));
+            }
+        }
+        const int64_t pages_at = 2 * tokens, items_at = (pages_at + pages + 7) / 8 * 8;
+        const int64_t merges_at = items_at + 8 * items, ints = merges_at + 8 * merges;
+        if (ints > INT32_MAX || parts > INT32_MAX / 64)
+            return set_error(kErrInvalidArgument, "a plan of %lld words is too large",
+                             (long long)ints);
+        for (int i = 0; i < kInfoCount; ++i) info[i] = 0;
+        info[kInfoInts] = ints;
+        info[kInfoTokens] = tokens;
+        info[kInfoPagesAt] = pages_at;
+        info[kInfoItemsAt] = items_at;
+        info[kInfoMergesAt] = merges_at;
+        info[kInfoMerges] = merges;
+        for (int i = 0; i < kPagedKinds; ++i) info[kInfoItems + i] = kinds[i];
+        info[kInfoParts] = parts;
+        info[kInfoPartRows] = part_rows;
+        info[kInfoContext] = longest;
+        if (plan == nullptr) return kOk;
+        if (plan_ints < ints)
+            return set_error(kErrInvalidArgument, "the plan needs %lld words, got %lld",
+                             (long long)ints, (long long)plan_ints);
+
+        std::vector<int32_t> tok0(n_seqs), page0(n_seqs);
+        int32_t t = 0, pg = 0;
+        for (int s = 0; s < n_seqs; ++s) {
+            tok0[s] = t;
+            page0[s] = pg;
+            if (new_lens[s] == 0) continue;
+            const int32_t* row = page_table + s * table_stride;
+            const int64_t np = ((int64_t)context_lens[s] + page_size - 1) >> shift;
+            for (int64_t j = 0; j < np; ++j) plan[pages_at + pg + j] = row[j];
+            pg += (int32_t)np;
+            for (int32_t i = 0; i < new_lens[s]; ++i, ++t) {
+                const int32_t pos = context_lens[s] - new_lens[s] + i;
+                plan[2 * t] = row[pos >> shift] * page_size + (pos & (page_size - 1));
+                plan[2 * t + 1] = pos;
+            }
+        }
+        for (int64_t i = pages_at + pages; i < items_at; ++i) plan[i] = 0;
+        PagedItem* item = reinterpret_cast<PagedItem*>(plan + items_at);
+        PagedMerge* merge = reinterpret_cast<PagedMerge*>(plan + merges_at);
+        int32_t part = 0;
+        for (int kind = 0; kind < kPagedKinds; ++kind) {
+            // longest first: the last workgroups to start are short ones
+            std::vector<const Tile*> of;
+            for (const Tile& x : tiles)
+                if (x.kind == kind) of.push_back(&x);
+            std::stable_sort(of.begin(), of.end(), [](const Tile* a, const Tile* b) {
+                return a->end - a->begin > b->end - b->begin;
+            });
+            for (const Tile* x : of) {
+                const int64_t len = x->end - x->begin;
+                const int64_t splits = std::max<int64_t>(1, (len + target[kind] - 1) / target[kind]);
+                // (whole units of 64 positions, shared out evenly)
+                const int64_t units = (len + 63) / 64;
+                const int s = x->seq;
+                if (splits > 1) {
+                    *merge++ = PagedMerge{tok0[s], new_lens[s], x->row0, (int32_t)splits, part,
+                                          paged_tile_rows(kind), {0, 0}};
+                }
+                for (int64_t i = 0; i < splits; ++i) {
+                    const int64_t b = x->begin + units * i / splits * 64;
+                    const int64_t e = std::min(x->end, x->begin + units * (i + 1) / splits * 64);
+                    *item++ = PagedItem{tok0[s], new_lens[s], context_lens[s], page0[s], x->row0,
+                                        (int32_t)b, (int32_t)e, splits > 1 ? part++ : -1};
+                }
+            }
+        }
+        return kOk;
+    } catch (const std::bad_alloc&) {
+        return set_error(kErrRuntime, "out of host memory for a plan");
+    }
+}
+
+int kivi_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                      const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                      const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                      int32_t dtype, void* q_out, void* k_pages, void* v_pages,
+                      int64_t num_pages, int32_t page_size, int32_t q_heads, int32_t kv_heads,
+                      int32_t head_dim, const int32_t* plan, int32_t tokens, const float* cos,
+                      const float* sin, int32_t rotary_dim, int32_t interleaved,
+                      const void* q_norm, const void* k_norm, int32_t norm_dtype, float eps,
+                      void* stream) {
+    const int32_t hq = q == nullptr ? 0 : q_heads;
+    int rc = check_pool(dtype, num_pages, page_size, q == nullptr ? kv_heads : q_heads, kv_heads,
+                        head_dim);
+    if (rc) return rc;
+    if (tokens < 0) return set_error(kErrInvalidArgument, "tokens %d must not be negative", tokens);
+    if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 16 != 0)
+        return set_error(kErrInvalidArgument,
+                         "rotary_dim must be a multiple of 16 up to head_dim, got %d", rotary_dim);
+    if (rotary_dim > 0 && (cos == nullptr || sin == nullptr))
+        return set_error(kErrInvalidArgument, "rotation needs cos and sin");
+    if (norm_dtype < 0 || norm_dtype > 2)
+        return set_error(kErrInvalidArgument, "norm_dtype %d is not 0, 1 or 2", norm_dtype);
+    if (tokens == 0) return kOk;
+    if (k == nullptr || v == nullptr || k_pages == nullptr || v_pages == nullptr ||
+        plan == nullptr || (q != nullptr && q_out == nullptr))
+        return set_error(kErrInvalidArgument, "null pointer");
+    const uintptr_t align = 15;
+    if (((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)(q != nullptr ? q_out : nullptr)) &
+        align)
+        return set_error(kErrInvalidArgument, "pages and q_out must be 16-byte aligned");
+    AppendArgs a{};
+    a.q = q; a.k = k; a.v = v;
+    a.q_st = q_token_stride; a.q_sh = q_head_stride;
+    a.k_st = k_token_stride; a.k_sh = k_head_stride;
+    a.v_st = v_token_stride; a.v_sh = v_head_stride;
+    a.q_out = q_out; a.k_pages = k_pages; a.v_pages = v_pages;
+    a.tokens = reinterpret_cast<const int2*>(plan);
+    a.cos = cos; a.sin = sin;
+    a.q_norm = q_norm; a.k_norm = k_norm; a.norm_dt = norm_dtype;
+    a.eps = eps;
+    a.n_tokens = tokens; a.Hq = hq; a.Hkv = kv_heads; a.D = head_dim;
+    a.page_shift = page_shift_of(page_size);
+    a.rot = rotary_dim; a.interleaved = interleaved != 0;
+    a.lanes_log2 = 0;
+    while ((1 << a.lanes_log2) < head_dim / 16) ++a.lanes_log2;
+    // four elements per load (8 or 16 bytes) where every row starts on one
+    const uintptr_t bytes = 4 * src_size(dtype) - 1;
+    int64_t strides = k_token_stride | k_head_stride | v_token_stride | v_head_stride;
+    uintptr_t bases = (uintptr_t)k | (uintptr_t)v;
+    if (q != nullptr) {
+        strides |= q_token_stride | q_head_stride;
+        bases |= (uintptr_t)q;
+    }
+    a.vec = (strides & 3) == 0 && (bases & bytes) == 0;
+    const int64_t lanes = (int64_t)tokens * (hq + 2 * kv_heads) << a.lanes_log2;
+    const int64_t blocks = (lanes + kAppendBlock - 1) / kAppendBlock;
+    if (blocks > INT32_MAX)
+        return set_error(kErrInvalidArgument, "%d tokens are too many for one launch", tokens);
+    hipStream_t s = (hipStream_t)stream;
+    const dim3 grid((unsigned)blocks);
+    if (dtype == kSrcF32) paged_append_kernel<kSrcF32><<<grid, kAppendBlock, 0, s>>>(a);
+    else if (dtype == kSrcBF16) paged_append_kernel<kSrcBF16><<<grid, kAppendBlock, 0, s>>>(a);
+    else paged_append_kernel<kSrcF16><<<grid, kAppendBlock, 0, s>>>(a);
+    return check_launch("paged_append");
+}
+
+}  // extern "C"

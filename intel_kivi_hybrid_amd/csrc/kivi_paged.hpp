@@ -1,0 +1,100 @@
+// The plan of one step over a paged cache, shared by the host that writes it
+// (kivi_paged.hip) and the kernels that read it.
+//
+// A paged cache holds keys and values as [num_pages][kv_heads][page_size]
+// [head_dim] of the model's type; a sequence's position p lies on its page
+// p / page_size.  A step brings n new tokens to each of some sequences.  The
+// plan is one int32 array, written and checked on the host once per step and
+// read by every layer's launches:
+//   tokens  [tokens][2]   slot (page * page_size + offset) and position of
+//                         each new token, the sequences one after the other
+//   pages   [pages]       the sequences' page lists, one after the other
+//   items   [items][8]    PagedItem: one workgroup's work for one kv head
+//   merges  [merges][8]   PagedMerge: row tiles whose context is split
+#pragma once
+
+#include "kivi_common.hpp"
+
+namespace kivi {
+
+// Query rows of a sequence and kv head: row r is new token r / hg, head
+// r % hg of the kv head's hg = q_heads / kv_heads.  Token i sees positions
+// 0 .. ctx - n + i.
+struct PagedItem {
+    int32_t tok0;        // the sequence's first new token among the step's
+    int32_t n;           // its new tokens
+    int32_t ctx;         // its length, the new tokens included
+    int32_t page0;       // where its page list starts
+    int32_t row0;        // first row of the tile
+    int32_t kv_begin;    // positions of the split
+    int32_t kv_end;
+    int32_t part;        // the split's partial (-1: the only one, written out)
+};
+
+struct PagedMerge {
+    int32_t tok0;
+    int32_t n;
+    int32_t row0;
+    int32_t splits;
+    int32_t part;        // first partial
+    int32_t rows;        // of the tile (the last one's may end earlier)
+    int32_t pad[2];
+};
+
+static_assert(sizeof(PagedItem) == 32 && sizeof(PagedMerge) == 32, "plan records");
+
+// Kinds of attention items, by the rows of a tile: a kind is one launch.
+enum PagedKind : int { kFew16 = 0, kFew32 = 1, kFew64 = 2, kMany = 3, kPagedKinds = 4 };
+
+constexpr int kManyRows = 128;
+constexpr int paged_tile_rows(int kind) {
+    return kind == kFew16 ? 16 : kind == kFew32 ? 32 : kind == kFew64 ? 64 : kManyRows;
+}
+// The most rows of a kv head that a few-row kernel holds: their queries and
+// outputs, with a unit's keys and values, fill a wave's registers.
+constexpr int paged_few_rows(bool f32, int head_dim) {
+    if (f32) return head_dim <= 64 ? 64 : head_dim <= 128 ? 32 : 16;
+    return head_dim <= 96 ? 64 : head_dim <= 128 ? 32 : 16;
+}
+// The kind that takes a sequence's rows.  fp32 has no kMany kernel: its products
+// run at a sixteenth of the 16-bit rate, so sharing tiles through LDS gains
+// nothing there.
+constexpr int paged_kind(int64_t rows, bool f32, int head_dim) {
+    const int few = paged_few_rows(f32, head_dim);
+    if (rows > few && !f32) return kMany;
+    const int64_t tile = rows < few ? rows : few;
+    return tile <= 16 ? kFew16 : tile <= 32 ? kFew32 : kFew64;
+}
+
+// info[] of kivi_paged_plan
+enum PagedInfo : int {
+    kInfoInts = 0,        // int32s of the plan
+    kInfoTokens = 1,
+    kInfoPagesAt = 2,     // offset of the page lists
+    kInfoItemsAt = 3,
+    kInfoMergesAt = 4,
+    kInfoMerges = 5,
+    kInfoItems = 6,       // items of each kind, in order
+    kInfoParts = 10,      // partials of a kv head
+    kInfoPartRows = 11,   // rows of a partial (the largest tile among the split ones)
+    kInfoContext = 12,    // the longest sequence
+    kInfoCount = 16,
+};
+
+struct PagedLaunch {
+    const void* q;
+    int64_t q_st, q_sh;           // strides of tokens and heads, in elements
+    const void* k_pages;
+    const void* v_pages;
+    void* out;                    // [tokens][q_heads][head_dim]
+    float* part_o;                // [kv head][partial][rows][head_dim]
+    float* part_ml;               // [kv head][partial][rows][2]: maximum and sum
+    const int32_t* pages;
+    const PagedItem* items;
+    const PagedMerge* merges;
+    int n_items, n_merges, n_parts, part_rows;
+    int Hq, Hkv, hg, D, page_shift;
+    float qscale;                 // softmax scale * log2 e
+};
+
+}  // namespace kivi

@@ -1,0 +1,160 @@
+// Attention of a step's new tokens over a paged cache: the launches of a plan
+// and the merge of split contexts.
+//
+// For sequence b with n new tokens in a context of c (these included), query
+// head h of kv head h / (q_heads / kv_heads), new token i:
+//   o = sum_p softmax_p(q . k_p * scale) v_p   over positions p <= c - n + i.
+// A plan's items are workgroups' shares of this (kivi_paged.hpp); each kind of
+// row tile is one launch.  Block b takes kv head b % kv_heads: blocks go to the
+// eight XCDs in turn, so with 8 kv heads (or a multiple) the tiles that read
+// one head's pages meet in one XCD's L2.
+#include <hip/hip_runtime.h>
+
+#include <math.h>
+
+#include "kivi_paged_attention.hpp"
+#include "../../include/kivi_hip.h"
+
+namespace kivi {
+namespace {
+
+constexpr int kMergeBlock = 256;
+
+// Joins a row's partials: 64 lanes take a row, four channels each.
+template <int DT>
+__global__ void __launch_bounds__(kMergeBlock) paged_merge_kernel(PagedLaunch a) {
+    const int groups = (a.part_rows + 3) / 4;          // of four rows, one a wave
+    const int tile = blockIdx.x / groups;
+    const int kvh = tile % a.Hkv;
+    const PagedMerge g = a.merges[tile / a.Hkv];
+    const int row = blockIdx.x % groups * 4 + threadIdx.x / kWave;
+    const int r = g.row0 + row, lane = threadIdx.x % kWave, c = 4 * lane;
+    // (rows of other tiles' sizes: a tile's own rows end at the next tile's)
+    if (row >= a.part_rows || row >= g.rows || r >= g.n * a.hg) return;
+    const int64_t p0 = ((int64_t)kvh * a.n_parts + g.part) * a.part_rows + row;
+    float top = -FLT_MAX;
+    for (int s = lane; s < g.splits; s += kWave)
+        top = fmaxf(top, a.part_ml[2 * (p0 + (int64_t)s * a.part_rows)]);
+    top = wave_max(top);
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < g.splits; ++s) {
+        const int64_t p = p0 + (int64_t)s * a.part_rows;
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
+        const float f = exp2_fast(ml.x - top);
+        sum = fmaf(ml.y, f, sum);
+        if (c < a.D) {
+            const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part_o + p * a.D + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = fmaf(x[i], f, o[i]);
+        }
+    }
+    if (c >= a.D) return;
+    const int i = r / a.hg;
+    const int64_t at =
+        ((int64_t)(g.tok0 + i) * a.Hq + kvh * a.hg + (r - i * a.hg)) * a.D;
+    store4<DT>(a.out, at + c, o * inverse_sum(sum));
+}
+
+int64_t part_floats(const int64_t* info, int32_t kv_heads, int32_t head_dim) {
+    return info[kInfoParts] * info[kInfoPartRows] * kv_heads * (head_dim + 2);
+}
+
+}  // namespace
+}  // namespace kivi
+
+using namespace kivi;
+
+extern "C" {
+
+size_t kivi_paged_attention_workspace_size(const int64_t* info, int32_t kv_heads,
+                                           int32_t head_dim) {
+    if (info == nullptr || kv_heads < 1 || head_dim < 1) return 0;
+    return (size_t)part_floats(info, kv_heads, head_dim) * 4;
+}
+
+int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                         int32_t dtype, const void* k_pages, const void* v_pages,
+                         int64_t num_pages, int32_t page_size, int32_t q_heads,
+                         int32_t kv_heads, int32_t head_dim, const int32_t* plan,
+                         const int64_t* info, float softmax_scale, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+    if (info == nullptr) return set_error(kErrInvalidArgument, "null plan info");
+    if (dtype < 0 || dtype > 2)
+        return set_error(kErrInvalidArgument, "dtype %d is not 0 (f32), 1 (bf16) or 2 (f16)", dtype);
+    int shift = -1;
+    for (int s = 4; s <= 8; ++s)
+        if (page_size == 1 << s) shift = s;
+    if (shift < 0 || num_pages < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0 ||
+        head_dim < 16 || head_dim > 256 || head_dim % 16 != 0)
+        return set_error(kErrInvalidArgument,
+                         "unsupported geometry: page_size %d, %d query heads over %d kv heads, "
+                         "head_dim %d", page_size, q_heads, kv_heads, head_dim);
+    if (!(softmax_scale > 0.f) || !isfinite(softmax_scale))
+        return set_error(kErrInvalidArgument, "softmax_scale must be positive and finite, got %g",
+                         (double)softmax_scale);
+    if (info[kInfoTokens] == 0) return kOk;
+    if (q == nullptr || k_pages == nullptr || v_pages == nullptr || plan == nullptr ||
+        out == nullptr)
+        return set_error(kErrInvalidArgument, "null pointer");
+    const int per = 16 / src_size(dtype);
+    if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out |
+         (uintptr_t)workspace) & 15 || q_token_stride % per != 0 || q_head_stride % per != 0)
+        return set_error(kErrInvalidArgument,
+                         "q's rows, pages, out and workspace must be 16-byte aligned");
+    const int64_t floats = part_floats(info, kv_heads, head_dim);
+    if (floats > 0 && (workspace == nullptr || workspace_bytes < (size_t)floats * 4))
+        return set_error(kErrInvalidArgument, "workspace must hold %lld bytes, got %zu",
+                         (long long)floats * 4, workspace_bytes);
+    PagedLaunch a{};
+    a.q = q;
+    a.q_st = q_token_stride;
+    a.q_sh = q_head_stride;
+    a.k_pages = k_pages;
+    a.v_pages = v_pages;
+    a.out = out;
+    a.pages = plan + info[kInfoPagesAt];
+    a.merges = reinterpret_cast<const PagedMerge*>(plan + info[kInfoMergesAt]);
+    a.n_merges = (int)info[kInfoMerges];
+    a.n_parts = (int)info[kInfoParts];
+    a.part_rows = (int)info[kInfoPartRows];
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + (int64_t)a.n_parts * a.part_rows * kv_heads * head_dim;
+    a.Hq = q_heads;
+    a.Hkv = kv_heads;
+    a.hg = q_heads / kv_heads;
+    a.D = head_dim;
+    a.page_shift = shift;
+    a.qscale = softmax_scale * (float)M_LOG2E;
+    hipStream_t s = (hipStream_t)stream;
+    const PagedItem* items = reinterpret_cast<const PagedItem*>(plan + info[kInfoItemsAt]);
+    // (the largest tiles first: the small ones fill in behind them)
+    for (int kind = kPagedKinds - 1; kind >= 0; --kind) {
+        int64_t before = 0;
+        for (int j = 0; j < kind; ++j) before += info[kInfoItems + j];
+        a.items = items + before;
+        a.n_items = (int)info[kInfoItems + kind];
+        if (a.n_items == 0) continue;
+        if ((int64_t)a.n_items * kv_heads > INT32_MAX)
+            return set_error(kErrInvalidArgument, "%d items are too many for one launch",
+                             a.n_items);
+        if (kind == kMany) launch_paged_many(a, dtype, s);
+        else if (dtype == kSrcF32) launch_paged_f32(a, kind, s);
+        else launch_paged_few(a, dtype, kind, s);
+        const int rc = check_launch("paged_attention");
+        if (rc) return rc;
+    }
+    if (a.n_merges == 0) return kOk;
+    const int64_t blocks = (int64_t)a.n_merges * kv_heads * ((a.part_rows + 3) / 4);
+    if (blocks > INT32_MAX)
+        return set_error(kErrInvalidArgument, "%lld rows to merge are too many for one launch",
+                         (long long)blocks * 4);
+    const dim3 grid((unsigned)blocks);
+    if (dtype == kSrcF32) paged_merge_kernel<kSrcF32><<<grid, kMergeBlock, 0, s>>>(a);
+    else if (dtype == kSrcBF16) paged_merge_kernel<kSrcBF16><<<grid, kMergeBlock, 0, s>>>(a);
+    else paged_merge_kernel<kSrcF16><<<grid, kMergeBlock, 0, s>>>(a);
+    return check_launch("paged_merge");
+}
+
+}  // extern "C"

@@ -1,0 +1,157 @@
+// Pieces shared by the paged-attention kernels: operand types, the products
+// of each type, a step's rows and pages, and what is written at the end.
+//
+// All kernels form scores transposed, S^T = K Q^T, and outputs transposed,
+// O^T = V^T P^T: a lane then holds scores, sums and outputs of one query row,
+// so a row's softmax state is a per-lane scalar, and the weights go from the
+// score registers into the second product's operand without moving between
+// lanes (the order of a product's inner index is free as long as both operands
+// agree).  Scores, softmax and outputs are fp32; the weights are rounded to
+// the cache's type for the second product (fp32 caches keep them), which is
+// off by at most half a step of that type, as the values themselves are.
+//
+// The softmax is online in the log2 domain.  A row's maximum moves only when
+// exceeded by more than 8 (weights <= 256, in range of every type), so most
+// steps rescale nothing.
+#pragma once
+
+#include <float.h>
+
+#include "kivi_common.hpp"
+#include "kivi_mfma.hpp"
+#include "kivi_paged.hpp"
+
+namespace kivi {
+namespace {
+
+constexpr float kMoveMax = 8.0f;       // log2 units
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+
+template <int DT>
+__device__ __forceinline__ f32x4_t mfma16(u32x4_t a, u32x4_t b, f32x4_t c) {
+    if constexpr (DT == kSrcBF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a),
+                                                      __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+    if constexpr (DT == kSrcBF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
+                                                      __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// Two values rounded to nearest even.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (DT == kSrcBF16) {
+        return pack_bf16x2(a, b);
+    } else {
+        const f16x2_t v = {(_Float16)a, (_Float16)b};
+        return __builtin_bit_cast(uint32_t, v);
+    }
+}
+// The low or high half of a word, widened.
+template <int DT>
+__device__ __forceinline__ float half_of(uint32_t w, int hi) {
+    const uint32_t h = hi ? w >> 16 : w & 0xffffu;
+    if constexpr (DT == kSrcBF16) return __uint_as_float(h << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
+
+// Whether a word holds an infinity or a NaN (an exponent of ones).
+template <int DT>
+__device__ __forceinline__ bool non_finite(uint32_t w) {
+    constexpr uint32_t e = DT == kSrcBF16 ? 0x7f80u : 0x7c00u;
+    return (w & e) == e || (w >> 16 & e) == e;
+}
+
+// Four rows' 16-bit elements, read transposed: the 16 lanes of a group give the
+// addresses of 4 consecutive elements each, lane 4r + c of row r's columns 4c ..
+// 4c + 3; lane i receives column i of rows 0 .. 3.
+__device__ __forceinline__ uint2 read_transposed(const unsigned char* p) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4_t*)(p)));
+}
+
+// A workgroup's item and where its sequence's pages lie.
+struct Work {
+    PagedItem it;
+    int kvh, rows, hg;
+    const int32_t* pages;
+    int64_t head_off;            // of the kv head within a page, in elements
+    int64_t page_elems;
+};
+
+__device__ __forceinline__ Work work_of(const PagedLaunch& a) {
+    Work w;
+    const int item = blockIdx.x / a.Hkv;
+    w.kvh = blockIdx.x - item * a.Hkv;
+    w.it = a.items[item];
+    w.hg = a.hg;
+    w.rows = w.it.n * a.hg;
+    w.pages = a.pages + w.it.page0;
+    w.head_off = ((int64_t)w.kvh << a.page_shift) * a.D;
+    w.page_elems = ((int64_t)a.Hkv << a.page_shift) * a.D;
+    return w;
+}
+
+// Positions are loaded in blocks of 16, which never cross a page.  A block's
+// page id (the block of the last position for blocks past the end), and the
+// address of its first row.
+__device__ __forceinline__ int block_page(const PagedLaunch& a, const Work& w, int t) {
+    return w.pages[min(t, w.it.kv_end - 1) >> a.page_shift];
+}
+template <class T>
+__device__ __forceinline__ const T* block_at(const PagedLaunch& a, const Work& w,
+                                             const void* pool, int page, int t) {
+    const int off = min(t, (w.it.kv_end - 1) & ~15) & ((1 << a.page_shift) - 1);
+    return static_cast<const T*>(pool) + page * w.page_elems + w.head_off + off * a.D;
+}
+
+// Positions that row r sees, within the split.
+__device__ __forceinline__ int row_limit(const Work& w, int r) {
+    return min(w.it.ctx - w.it.n + r / w.hg + 1, w.it.kv_end);
+}
+__device__ __forceinline__ int64_t out_offset(const PagedLaunch& a, const Work& w, int r) {
+    const int i = r / w.hg;
+    return ((int64_t)(w.it.tok0 + i) * a.Hq + w.kvh * w.hg + (r - i * w.hg)) * a.D;
+}
+__device__ __forceinline__ int64_t q_offset(const PagedLaunch& a, const Work& w, int r) {
+    const int i = r / w.hg;
+    return (w.it.tok0 + i) * a.q_st + (int64_t)(w.kvh * w.hg + (r - i * w.hg)) * a.q_sh;
+}
+__device__ __forceinline__ int64_t part_row(const PagedLaunch& a, const Work& w, int r) {
+    return ((int64_t)w.kvh * a.n_parts + w.it.part) * a.part_rows + (r - w.it.row0);
+}
+
+// Four consecutive channels of an output row, rounded once.
+template <int DT>
+__device__ __forceinline__ void store4(void* out, int64_t i, f32x4_t x) {
+    if constexpr (DT == kSrcF32)
+        *reinterpret_cast<f32x4_t*>(static_cast<float*>(out) + i) = x;
+    else
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i) =
+            make_uint2(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]));
+}
+
+// 1 / sum; a row that saw nothing has sum 0 and comes out as zeros.
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }
+
+}  // namespace
+
+void launch_paged_few(const PagedLaunch& a, int dtype, int kind, hipStream_t s);
+void launch_paged_f32(const PagedLaunch& a, int kind, hipStream_t s);
+void launch_paged_many(const PagedLaunch& a, int dtype, hipStream_t s);
+
+}  // namespace kivi
