@@ -466,6 +466,29 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
                          const int64_t* info, float softmax_scale, void* out, void* workspace,
                          size_t workspace_bytes, void* stream);
 
+/* ---- sampling ---------------------------------------------------------------
+ * Next tokens out[rows] from logits [rows][vocab] (dtype 0 f32, 1 bf16, 2 f16;
+ * rows row_stride elements apart; vocab at most 2^20) and uniforms[rows] in [0, 1)
+ * (f32, or f64 with uniforms_f64).  Replaces the selection of sample_token
+ * (src/kivi_sycl/generation/sampling.py:10-25: temperature, top-k, a multinomial
+ * draw), with top-p and min-p and the random numbers given by the caller.
+ *
+ * A row's tokens are ordered by (logit descending, index ascending); with w =
+ * exp((x - max) / temperature), kept are the first top_k of them (0 or less:
+ * all), of these the shortest prefix whose mass reaches top_p of theirs (1 or
+ * more: all), of these the ones with w >= min_p; the first token always.  The
+ * result is the first token whose running mass in that order exceeds u times the
+ * kept mass.  temperature <= 0: the first token.  Settings are the scalars, or one
+ * value per row (device arrays) where a pointer is given.  NaN logits count as
+ * -infinity; a row with nothing above that gives -1.  Of tokens of infinite logit
+ * all weigh 1, any others 0.  Weights are fp64, summed in units of 2^-43 of the
+ * largest: exactly, in any order, the same token at every call. */
+int kivi_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows,
+                int32_t vocab, const void* uniforms, int32_t uniforms_f64,
+                const float* temperatures, double temperature, const int32_t* top_ks,
+                int32_t top_k, const float* top_ps, double top_p, const float* min_ps,
+                double min_p, int64_t* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

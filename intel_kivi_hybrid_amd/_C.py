@@ -964,3 +964,64 @@ def paged_attention(q, k_pages, v_pages, plan, softmax_scale=None, out=None, wor
             0 if workspace is None else workspace.numel() * workspace.element_size(),
             plan._enter(dev)), "paged_attention")
     return out
+
+
+# --------------------------------------------------------------------------
+# Sampling (sampling.py:10-25 in the reference, with top-p, min-p and given
+# random numbers; see include/kivi_hip.h).
+# --------------------------------------------------------------------------
+def _setting(value, name: str, rows: int, dtype, dev):
+    """A setting as (pointer of a per-row tensor or 0, scalar)."""
+    if isinstance(value, torch.Tensor):
+        _check(value.dtype is dtype and value.dim() == 1 and value.shape[0] == rows
+               and value.is_contiguous() and value.device == dev, name,
+               " must be a number or a contiguous [", rows, "] tensor of ", _dtype_name(dtype),
+               " on ", dev)
+        return value.data_ptr(), 0
+    return 0, value
+
+
+def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+    """Next tokens ``[rows]`` (int64) from ``logits [rows, vocab]`` (fp32, bf16 or
+    fp16) and ``uniforms [rows]`` in [0, 1) (fp32 or fp64): one launch on the
+    current stream.
+
+    In the order (logit descending, index ascending) with weights
+    ``exp((x - max) / temperature)``: the first ``top_k`` tokens (0: all), of these
+    the shortest prefix with ``top_p`` of their mass (1: all), of these the ones of
+    weight ``min_p`` or more (0: all), the first one always; the result is the
+    first whose running mass exceeds ``u`` times the kept mass.  ``temperature``
+    0: the largest logit.  Each setting is a number or a tensor with one value per
+    row (float32; top_k int32).  NaN logits are never taken; a row without any
+    logit above -infinity gives -1."""
+    if not (isinstance(logits, torch.Tensor) and logits.dim() == 2
+            and logits.dtype in _IO_DTYPES and logits.is_cuda):
+        _fail("logits must be a [rows, vocab] tensor of a float type on ", _DEVICE_TYPE)
+    _check(logits.stride(1) == 1 or logits.shape[1] == 1, "a row's logits must be contiguous")
+    rows, vocab = logits.shape
+    dev = logits.device
+    _check(uniforms.dtype in (torch.float32, torch.float64) and uniforms.dim() == 1
+           and uniforms.shape[0] == rows and uniforms.is_contiguous() and uniforms.device == dev,
+           "uniforms must be a contiguous [", rows, "] float32 or float64 tensor on ", dev)
+    tp, t = _setting(temperature, "temperature", rows, torch.float32, dev)
+    kp, k = _setting(top_k, "top_k", rows, torch.int32, dev)
+    pp, p = _setting(top_p, "top_p", rows, torch.float32, dev)
+    mp, m = _setting(min_p, "min_p", rows, torch.float32, dev)
+    _check(t >= 0.0, "temperature must not be negative, got ", t)
+    _check(p >= 0.0, "top_p must not be negative, got ", p)
+    _check(0.0 <= m <= 1.0, "min_p must lie in [0, 1], got ", m)
+    k = min(_check_int(k, "top_k"), vocab)
+    _check(k >= 0, "top_k must not be negative, got ", k)
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=dev)
+    else:
+        _check(out.dtype is torch.int64 and out.shape == (rows,) and out.is_contiguous()
+               and out.device == dev, "out must be a contiguous [", rows, "] int64 tensor on ",
+               dev)
+    index = dev.index
+    with on_device(index):
+        _native.check(_lib.kivi_sample(
+            logits.data_ptr(), _IO_DTYPES[logits.dtype], logits.stride(0), rows, vocab,
+            uniforms.data_ptr(), 1 if uniforms.dtype is torch.float64 else 0, tp, t, kp, k, pp, p,
+            mp, m, out.data_ptr(), stream_handle(index)), "sample")
+    return out

@@ -89,6 +89,8 @@ SIGNATURES = {
     "kivi_paged_attention_workspace_size": [_vp, _i32, _i32],
     "kivi_paged_attention": [_vp, _i64, _i64, _i32, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp,
                              _vp, _f32, _vp, _vp, ctypes.c_size_t, _vp],
+    "kivi_sample": [_vp, _i32, _i64, _i32, _i32, _vp, _i32, _vp, ctypes.c_double, _vp, _i32, _vp,
+                    ctypes.c_double, _vp, ctypes.c_double, _vp, _vp],
 }
 
 _RESTYPES = {
