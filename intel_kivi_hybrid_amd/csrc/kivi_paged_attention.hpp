@@ -88,7 +88,8 @@ __device__ __forceinline__ uint2 read_transposed(const unsigned char* p) {
 struct Work {
     PagedItem it;
     int kvh, rows, hg;
-    const int32_t* pages;
+    // (the constant address space: scalar loads, whatever else is written)
+    const __attribute__((address_space(4))) int32_t* pages;
     int64_t head_off;            // of the kv head within a page, in elements
     int64_t page_elems;
 };
@@ -100,7 +101,7 @@ __device__ __forceinline__ Work work_of(const PagedLaunch& a) {
     w.it = a.items[item];
     w.hg = a.hg;
     w.rows = w.it.n * a.hg;
-    w.pages = a.pages + w.it.page0;
+    w.pages = (const __attribute__((address_space(4))) int32_t*)(a.pages + w.it.page0);
     w.head_off = ((int64_t)w.kvh << a.page_shift) * a.D;
     w.page_elems = ((int64_t)a.Hkv << a.page_shift) * a.D;
     return w;
