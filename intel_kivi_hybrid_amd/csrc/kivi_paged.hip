@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <functional>
 #include <new>
 #include <vector>
 
@@ -220,9 +221,65 @@ int check_pool(int32_t dtype, int64_t num_pages, int32_t page_size, int32_t q_he
 }
 
 struct Tile {
-    int seq, kind, row0;
-    int64_t begin, end;          // positions that its rows see
+    int seq, row0;
+    int64_t end;                 // positions that its rows see
 };
+
+// How one kind's tiles (the longest first) are cut: the first `whole` stay
+// whole, the others into pieces of at most `length` positions (a multiple of 64).
+struct Cut {
+    size_t whole;
+    int64_t length;
+    int64_t pieces(size_t tile, int64_t len) const {
+        return tile < whole ? 1 : std::max<int64_t>(1, (len + length - 1) / length);
+    }
+};
+
+// Costs in positions, as measured: an item's start; what a row of a partial
+// adds to it (written, then read by the merge); the merge's launch.
+constexpr int64_t kStart = 64, kPartialRow = 4, kMerge = 96;
+
+// The cut whose items, dealt in order to `machines` workgroups as these come
+// free, end first.
+Cut best_cut(const std::vector<Tile>& tiles, const std::vector<int>& rows, int64_t machines) {
+    Cut best{tiles.size(), 64};
+    int64_t best_end = INT64_MAX;
+    const int64_t longest = tiles.empty() ? 0 : tiles.front().end;
+    std::vector<int64_t> busy;                    // a heap: when each comes free
+    const size_t rounds = tiles.size() / (size_t)machines * (size_t)machines;
+    for (int64_t n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+        const int64_t T = ((longest + n - 1) / n + 63) / 64 * 64;
+        if (n > 1 && T < 128) break;
+        // (with whole rounds of tiles first, only the rest is cut)
+        for (int keep = 0; keep < (n > 1 && rounds > 0 ? 2 : 1); ++keep) {
+            const Cut cut{keep ? rounds : 0, T};
+            int64_t items = 0;
+            for (size_t i = 0; i < tiles.size(); ++i) items += cut.pieces(i, tiles[i].end);
+            if (n > 1 && items > 16 * machines) continue;
+            busy.assign((size_t)machines, 0);
+            int64_t end = 0;
+            bool merge = false;
+            for (size_t i = 0; i < tiles.size(); ++i) {
+                const int64_t k = cut.pieces(i, tiles[i].end);
+                merge |= k > 1;
+                const int64_t each =
+                    tiles[i].end / k + kStart + (k > 1 ? kPartialRow * rows[i] : 0);
+                for (int64_t j = 0; j < k; ++j) {
+                    std::pop_heap(busy.begin(), busy.end(), std::greater<int64_t>());
+                    busy.back() += each;
+                    end = std::max(end, busy.back());
+                    std::push_heap(busy.begin(), busy.end(), std::greater<int64_t>());
+                }
+            }
+            if (merge) end += kMerge;
+            if (end < best_end) {
+                best_end = end;
+                best = cut;
+            }
+        }
+    }
+    return best;
+}
 
 }  // namespace
 }  // namespace kivi
@@ -294,43 +351,48 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
                 return set_error(kErrInvalidArgument, "page %d: a slot is given to two new tokens",
                                  runs[i].page);
 
-        // Row tiles, and the positions that the last row of each sees.
-        std::vector<Tile> tiles;
-        int64_t work[kPagedKinds] = {0, 0, 0, 0}, count[kPagedKinds] = {0, 0, 0, 0};
+        // Row tiles, and the positions that the last row of each sees.  The
+        // sequences of few rows take one kind, the largest that one of them needs:
+        // one launch then streams all their pages.
+        const int few = paged_few_rows(f32, head_dim);
+        int64_t few_rows = 0;
+        for (int s = 0; s < n_seqs; ++s) {
+            const int64_t rows = (int64_t)new_lens[s] * hg;
+            if (rows <= few) few_rows = std::max(few_rows, rows);
+        }
+        std::vector<Tile> tiles[kPagedKinds];
         for (int s = 0; s < n_seqs; ++s) {
             const int64_t n = new_lens[s], rows = n * hg;
             if (n == 0) continue;
-            const int kind = paged_kind(rows, f32, head_dim);
+            const int kind = paged_kind(rows <= few ? few_rows : rows, f32, head_dim);
             const int step = paged_tile_rows(kind);
             for (int64_t r = 0; r < rows; r += step) {
                 const int64_t last = std::min(rows, r + step) - 1;
-                const int64_t end = context_lens[s] - n + last / hg + 1;
-                tiles.push_back({s, kind, (int)r, 0, end});
-                work[kind] += end;
-                count[kind] += 1;
+                tiles[kind].push_back({s, (int)r, context_lens[s] - n + last / hg + 1});
             }
         }
-        // Splits: enough workgroups for the card's 256 CUs, each kept long
-        // enough to be worth its partial.
-        int64_t target[kPagedKinds];
-        for (int kind = 0; kind < kPagedKinds; ++kind) {
-            const int64_t want = kind == kMany ? 512 : 1024;
-            const int64_t least = kind == kMany ? 512 : 256;
-            const int64_t total = work[kind] * kv_heads;
-            target[kind] = std::max(least, (total + want - 1) / want);
-            if (count[kind] * kv_heads >= want) target[kind] = std::max(target[kind], longest);
-            target[kind] = (target[kind] + 63) / 64 * 64;
-        }
+        Cut cuts[kPagedKinds];
         int64_t items = 0, merges = 0, parts = 0, part_rows = 0, kinds[kPagedKinds] = {0, 0, 0, 0};
-        for (const Tile& t : tiles) {
-            const int64_t len = t.end - t.begin;
-            const int64_t splits = std::max<int64_t>(1, (len + target[t.kind] - 1) / target[t.kind]);
-            items += splits;
-            kinds[t.kind] += splits;
-            if (splits > 1) {
-                merges += 1;
-                parts += splits;
-                part_rows = std::max<int64_t>(part_rows, paged_tile_rows(t.kind));
+        for (int kind = 0; kind < kPagedKinds; ++kind) {
+            // longest first: the last workgroups to start are short ones
+            std::vector<Tile>& of = tiles[kind];
+            std::stable_sort(of.begin(), of.end(),
+                             [](const Tile& a, const Tile& b) { return a.end > b.end; });
+            std::vector<int> rows;
+            for (const Tile& t : of)
+                rows.push_back((int)std::min<int64_t>(paged_tile_rows(kind),
+                                                      (int64_t)new_lens[t.seq] * hg - t.row0));
+            const int64_t slots = paged_slots(kind, head_dim);
+            cuts[kind] = best_cut(of, rows, std::max<int64_t>(1, slots / kv_heads));
+            for (size_t i = 0; i < of.size(); ++i) {
+                const int64_t splits = cuts[kind].pieces(i, of[i].end);
+                items += splits;
+                kinds[kind] += splits;
+                if (splits > 1) {
+                    merges += 1;
+                    parts += splits;
+                    part_rows = std::max<int64_t>(part_rows, paged_tile_rows(kind));
+                }
             }
         }
         const int64_t pages_at = 2 * tokens, items_at = (pages_at + pages + 7) / 8 * 8;
@@ -375,27 +437,19 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
         PagedMerge* merge = reinterpret_cast<PagedMerge*>(plan + merges_at);
         int32_t part = 0;
         for (int kind = 0; kind < kPagedKinds; ++kind) {
-            // longest first: the last workgroups to start are short ones
-            std::vector<const Tile*> of;
-            for (const Tile& x : tiles)
-                if (x.kind == kind) of.push_back(&x);
-            std::stable_sort(of.begin(), of.end(), [](const Tile* a, const Tile* b) {
-                return a->end - a->begin > b->end - b->begin;
-            });
-            for (const Tile* x : of) {
-                const int64_t len = x->end - x->begin;
-                const int64_t splits = std::max<int64_t>(1, (len + target[kind] - 1) / target[kind]);
+            for (size_t j = 0; j < tiles[kind].size(); ++j) {
+                const Tile& x = tiles[kind][j];
+                const int64_t splits = cuts[kind].pieces(j, x.end);
                 // (whole units of 64 positions, shared out evenly)
-                const int64_t units = (len + 63) / 64;
-                const int s = x->seq;
-                if (splits > 1) {
-                    *merge++ = PagedMerge{tok0[s], new_lens[s], x->row0, (int32_t)splits, part,
+                const int64_t units = (x.end + 63) / 64;
+                const int s = x.seq;
+                if (splits > 1)
+                    *merge++ = PagedMerge{tok0[s], new_lens[s], x.row0, (int32_t)splits, part,
                                           paged_tile_rows(kind), {0, 0}};
-                }
                 for (int64_t i = 0; i < splits; ++i) {
-                    const int64_t b = x->begin + units * i / splits * 64;
-                    const int64_t e = std::min(x->end, x->begin + units * (i + 1) / splits * 64);
-                    *item++ = PagedItem{tok0[s], new_lens[s], context_lens[s], page0[s], x->row0,
+                    const int64_t b = units * i / splits * 64;
+                    const int64_t e = std::min(x.end, units * (i + 1) / splits * 64);
+                    *item++ = PagedItem{tok0[s], new_lens[s], context_lens[s], page0[s], x.row0,
                                         (int32_t)b, (int32_t)e, splits > 1 ? part++ : -1};
                 }
             }

@@ -54,16 +54,25 @@ constexpr int paged_tile_rows(int kind) {
 // outputs, with a unit's keys and values, fill a wave's registers.
 constexpr int paged_few_rows(bool f32, int head_dim) {
     if (f32) return head_dim <= 64 ? 64 : head_dim <= 128 ? 32 : 16;
-    return head_dim <= 96 ? 64 : head_dim <= 128 ? 32 : 16;
+    return head_dim <= 128 ? 64 : 16;
 }
-// The kind that takes a sequence's rows.  fp32 has no kMany kernel: its products
-// run at a sixteenth of the 16-bit rate, so sharing tiles through LDS gains
-// nothing there.
+// The kind that takes `rows` rows.  fp32 has no kMany kernel: its products run at
+// a sixteenth of the 16-bit rate, so sharing tiles through LDS gains nothing
+// there.
 constexpr int paged_kind(int64_t rows, bool f32, int head_dim) {
     const int few = paged_few_rows(f32, head_dim);
     if (rows > few && !f32) return kMany;
     const int64_t tile = rows < few ? rows : few;
     return tile <= 16 ? kFew16 : tile <= 32 ? kFew32 : kFew64;
+}
+// Workgroups that the card holds at once: 256 CUs, and as many on each as the
+// kernels' registers (few rows) or LDS (many) leave room for.
+constexpr int paged_slots(int kind, int head_dim) {
+    const int per_cu = kind == kMany    ? (head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1)
+                       : kind == kFew16 ? (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1)
+                       : kind == kFew32 ? (head_dim <= 64 ? 2 : 1)
+                                        : 1;
+    return 256 * per_cu;
 }
 
 // info[] of kivi_paged_plan

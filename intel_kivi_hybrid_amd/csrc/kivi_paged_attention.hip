@@ -20,41 +20,39 @@ namespace {
 
 constexpr int kMergeBlock = 256;
 
-// Joins a row's partials: 64 lanes take a row, four channels each.
+// Joins partials: a thread takes four channels of a row.
 template <int DT>
 __global__ void __launch_bounds__(kMergeBlock) paged_merge_kernel(PagedLaunch a) {
-    const int groups = (a.part_rows + 3) / 4;          // of four rows, one a wave
-    const int tile = blockIdx.x / groups;
+    const int per_row = a.D / 4;
+    const int blocks = (a.part_rows * per_row + kMergeBlock - 1) / kMergeBlock;   // of a tile
+    const int tile = blockIdx.x / blocks;
     const int kvh = tile % a.Hkv;
     const PagedMerge g = a.merges[tile / a.Hkv];
-    const int row = blockIdx.x % groups * 4 + threadIdx.x / kWave;
-    const int r = g.row0 + row, lane = threadIdx.x % kWave, c = 4 * lane;
-    // (rows of other tiles' sizes: a tile's own rows end at the next tile's)
-    if (row >= a.part_rows || row >= g.rows || r >= g.n * a.hg) return;
+    const int at = (blockIdx.x - tile * blocks) * kMergeBlock + threadIdx.x;
+    const int row = at / per_row, c = (at - row * per_row) * 4, r = g.row0 + row;
+    // (partials are as large as the largest tile's)
+    if (row >= g.rows || r >= g.n * a.hg) return;
     const int64_t p0 = ((int64_t)kvh * a.n_parts + g.part) * a.part_rows + row;
+    const float* ml = a.part_ml + 2 * p0;
+    const float* po = a.part_o + p0 * a.D + c;
+    const int64_t next_ml = 2 * (int64_t)a.part_rows, next_o = (int64_t)a.part_rows * a.D;
     float top = -FLT_MAX;
-    for (int s = lane; s < g.splits; s += kWave)
-        top = fmaxf(top, a.part_ml[2 * (p0 + (int64_t)s * a.part_rows)]);
-    top = wave_max(top);
+#pragma unroll 4
+    for (int s = 0; s < g.splits; ++s) top = fmaxf(top, ml[s * next_ml]);
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
 #pragma unroll 4
     for (int s = 0; s < g.splits; ++s) {
-        const int64_t p = p0 + (int64_t)s * a.part_rows;
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * p);
-        const float f = exp2_fast(ml.x - top);
-        sum = fmaf(ml.y, f, sum);
-        if (c < a.D) {
-            const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part_o + p * a.D + c);
+        const float2 x = *reinterpret_cast<const float2*>(ml + s * next_ml);
+        const f32x4_t y = *reinterpret_cast<const f32x4_t*>(po + s * next_o);
+        const float f = exp2_fast(x.x - top);
+        sum = fmaf(x.y, f, sum);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = fmaf(x[i], f, o[i]);
-        }
+        for (int i = 0; i < 4; ++i) o[i] = fmaf(y[i], f, o[i]);
     }
-    if (c >= a.D) return;
     const int i = r / a.hg;
-    const int64_t at =
-        ((int64_t)(g.tok0 + i) * a.Hq + kvh * a.hg + (r - i * a.hg)) * a.D;
-    store4<DT>(a.out, at + c, o * inverse_sum(sum));
+    store4<DT>(a.out, ((int64_t)(g.tok0 + i) * a.Hq + kvh * a.hg + (r - i * a.hg)) * a.D + c,
+               o * inverse_sum(sum));
 }
 
 int64_t part_floats(const int64_t* info, int32_t kv_heads, int32_t head_dim) {
@@ -146,10 +144,11 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
         if (rc) return rc;
     }
     if (a.n_merges == 0) return kOk;
-    const int64_t blocks = (int64_t)a.n_merges * kv_heads * ((a.part_rows + 3) / 4);
+    const int64_t blocks = (int64_t)a.n_merges * kv_heads *
+                           ((a.part_rows * (head_dim / 4) + kMergeBlock - 1) / kMergeBlock);
     if (blocks > INT32_MAX)
-        return set_error(kErrInvalidArgument, "%lld rows to merge are too many for one launch",
-                         (long long)blocks * 4);
+        return set_error(kErrInvalidArgument, "%d tiles to merge are too many for one launch",
+                         a.n_merges);
     const dim3 grid((unsigned)blocks);
     if (dtype == kSrcF32) paged_merge_kernel<kSrcF32><<<grid, kMergeBlock, 0, s>>>(a);
     else if (dtype == kSrcBF16) paged_merge_kernel<kSrcBF16><<<grid, kMergeBlock, 0, s>>>(a);

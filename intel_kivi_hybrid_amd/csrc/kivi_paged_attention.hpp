@@ -69,11 +69,22 @@ __device__ __forceinline__ float half_of(uint32_t w, int hi) {
     else return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
 }
 
-// Whether a word holds an infinity or a NaN (an exponent of ones).
+// A value that a row must not see still meets it as 0 * value, which is NaN for
+// an infinity or a NaN.  In steps where some row stops short, such elements
+// enter the products as 0, and the rows that do see them get them back at the
+// end (odd_values()): a weight is positive, so what they make of the sum does not
+// depend on it.
+
+// Zeroes the non-finite ones (an exponent of ones) of two 16-bit values.
 template <int DT>
-__device__ __forceinline__ bool non_finite(uint32_t w) {
+__device__ __forceinline__ uint32_t finite_part(uint32_t w) {
     constexpr uint32_t e = DT == kSrcBF16 ? 0x7f80u : 0x7c00u;
-    return (w & e) == e || (w >> 16 & e) == e;
+    if ((w & e) == e) w &= 0xffff0000u;
+    if ((w >> 16 & e) == e) w &= 0xffffu;
+    return w;
+}
+__device__ __forceinline__ bool non_finite(float x) {
+    return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u;
 }
 
 // Four rows' 16-bit elements, read transposed: the 16 lanes of a group give the
@@ -144,6 +155,28 @@ __device__ __forceinline__ void store4(void* out, int64_t i, f32x4_t x) {
     else
         *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i) =
             make_uint2(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]));
+}
+
+// The sum of the non-finite values of positions t .. lim - 1 in four channels.
+template <int DT>
+__device__ __forceinline__ f32x4_t odd_values(const PagedLaunch& a, const Work& w, int t, int lim,
+                                           int c) {
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+    for (; t < lim; ++t) {
+        const int64_t at = w.pages[t >> a.page_shift] * w.page_elems + w.head_off +
+                           (int64_t)(t & ((1 << a.page_shift) - 1)) * a.D + c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = widen<DT>(a.v_pages, at + i);
+            if (non_finite(x)) sum[i] += x;
+        }
+    }
+    return sum;
+}
+// Where these start: the first step of `unit` positions that some row of the
+// tile (all of which see `all` positions) does not see to its end.
+__device__ __forceinline__ int odd_from(const Work& w, int all, int unit) {
+    return w.it.kv_begin + max(0, all - w.it.kv_begin) / unit * unit;
 }
 
 // 1 / sum; a row that saw nothing has sum 0 and comes out as zeros.

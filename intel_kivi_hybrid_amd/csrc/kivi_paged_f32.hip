@@ -30,6 +30,7 @@ __global__ void __launch_bounds__(kBlock) paged_f32_kernel(PagedLaunch a) {
     constexpr int OS = DP + 4;             // joining rows, padded by one vector
     __shared__ __align__(16) float jo[kWaves * 16 * OS];
     __shared__ float join_m[kWaves][RT * 16], join_l[kWaves][RT * 16];
+    __shared__ int join_odd[kWaves];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, col = lane % 16, gq = lane / 16;
     const Work w = work_of(a);
@@ -61,30 +62,48 @@ __global__ void __launch_bounds__(kBlock) paged_f32_kernel(PagedLaunch a) {
     const int end = w.it.kv_end;
 
     f32x4_t kf[KK], vf[CG][4];
+    const bool full = a.D == DP;
     auto load_k = [&](int t0, int page) {
         const float* p = block_at<float>(a, w, a.k_pages, page, t0);
+        const uint32_t off = col * a.D + 4 * gq;
+        if (full) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            const int c = 16 * kk + 4 * gq;
-            kf[kk] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            if (c < a.D) kf[kk] = *reinterpret_cast<const f32x4_t*>(p + col * a.D + c);
+            for (int kk = 0; kk < KK; ++kk)
+                kf[kk] = *reinterpret_cast<const f32x4_t*>(p + off + 16 * kk);
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                kf[kk] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                if (16 * kk + 4 * gq < a.D)
+                    kf[kk] = *reinterpret_cast<const f32x4_t*>(p + off + 16 * kk);
+            }
         }
     };
     auto load_v = [&](int t0, int page) {
         const float* p = block_at<float>(a, w, a.v_pages, page, t0);
+        const uint32_t off = 4 * gq * a.D + 4 * col;
+        if (full && t0 + kUnit <= end) {
 #pragma unroll
-        for (int cg = 0; cg < CG; ++cg) {
+            for (int cg = 0; cg < CG; ++cg) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = 4 * gq + i, c = 64 * cg + 4 * col;
-                // (zeros past the end: whatever lies there has weight 0)
-                vf[cg][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-                if (t0 + t < end && c < a.D)
-                    vf[cg][i] = *reinterpret_cast<const f32x4_t*>(p + t * a.D + c);
+                for (int i = 0; i < 4; ++i)
+                    vf[cg][i] = *reinterpret_cast<const f32x4_t*>(p + off + i * a.D + 64 * cg);
+            }
+        } else {
+#pragma unroll
+            for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // (zeros past the end: whatever lies there has weight 0)
+                    vf[cg][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                    if (t0 + 4 * gq + i < end && 64 * cg + 4 * col < a.D)
+                        vf[cg][i] = *reinterpret_cast<const f32x4_t*>(p + off + i * a.D + 64 * cg);
+                }
             }
         }
     };
 
+    bool odd = false;                     // some of the lane's values were not finite
     int t0 = w.it.kv_begin + wave * kUnit, page = 0, ahead = 0;
     if (t0 < end) {
         page = block_page(a, w, t0);
@@ -105,26 +124,25 @@ __global__ void __launch_bounds__(kBlock) paged_f32_kernel(PagedLaunch a) {
                 for (int rt = 0; rt < RT; ++rt) s[rt] = mfma4(kf[kk][c], qf[rt][kk][c], s[rt]);
             }
         }
-        const int here = page;
         page = ahead;
         if (next < end) {
             load_k(next, page);
             ahead = block_page(a, w, next + kWaves * kUnit);
         }
         const bool masked = t0 + kUnit > min(all_see, end);
-        // (a value that some row must not see: see the 16-bit kernel)
-        bool odd = false;
         if (t0 + kUnit > all_see) {
 #pragma unroll
             for (int cg = 0; cg < CG; ++cg) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        odd |= (__float_as_uint(vf[cg][i][c]) & 0x7f800000u) == 0x7f800000u;
+                    for (int c = 0; c < 4; ++c) {
+                        if (!non_finite(vf[cg][i][c])) continue;
+                        vf[cg][i][c] = 0.f;
+                        odd = true;
+                    }
                 }
             }
-            odd = __builtin_amdgcn_ballot_w64(odd) != 0;
         }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -150,41 +168,15 @@ __global__ void __launch_bounds__(kBlock) paged_f32_kernel(PagedLaunch a) {
                 l[rt] += s[rt][i];
             }
         }
-        if (!odd) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int cg = 0; cg < CG; ++cg) {
+            for (int cg = 0; cg < CG; ++cg) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 4; ++c) {
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-                            O[rt][cg][c] = mfma4(vf[cg][i][c], s[rt][i], O[rt][cg][c]);
-                    }
-                }
-            }
-        } else {
-            const float* p = block_at<float>(a, w, a.v_pages, here, t0);
-            for (int j = 0; j < kUnit && t0 + j < end; ++j) {
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const f32x4_t f = s[rt];
-                    const int i = j % 4;
-                    const float own = i < 2 ? (i == 0 ? f[0] : f[1]) : (i == 2 ? f[2] : f[3]);
-                    const float wt = fmaxf(__shfl(own, col + 16 * (j / 4)), FLT_MIN);
-                    if (t0 + j >= lim[rt]) continue;
-#pragma unroll
-                    for (int cg = 0; cg < CG; ++cg) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int c0 = 64 * cg + 16 * gq + 4 * r;
-                            if (c0 >= a.D) continue;
-                            const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p + j * a.D + c0);
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                O[rt][cg][c][r] = fmaf(wt, x[c], O[rt][cg][c][r]);
-                        }
-                    }
+                    for (int rt = 0; rt < RT; ++rt)
+                        O[rt][cg][c] = mfma4(vf[cg][i][c], s[rt][i], O[rt][cg][c]);
                 }
             }
         }
@@ -192,6 +184,8 @@ __global__ void __launch_bounds__(kBlock) paged_f32_kernel(PagedLaunch a) {
     }
 
     // Join the waves: a row's largest maximum, then the rescaled sums.
+    if (lane == 0) join_odd[wave] = 0;
+    if (__builtin_amdgcn_ballot_w64(odd) != 0 && lane == 0) join_odd[wave] = 1;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         l[rt] += __shfl_xor(l[rt], 16);
@@ -231,8 +225,11 @@ __global__ void __launch_bounds__(kBlock) paged_f32_kernel(PagedLaunch a) {
                 o += *reinterpret_cast<const f32x4_t*>(jo + (i * 16 + row) * OS + c);
                 sum += join_l[i][16 * rt + row] * exp2_fast(join_m[i][16 * rt + row] - mt);
             }
+            if (w.it.part < 0) o *= inverse_sum(sum);
+            if (join_odd[0] | join_odd[1] | join_odd[2] | join_odd[3])
+                o += odd_values<kSrcF32>(a, w, odd_from(w, all_see, kUnit), row_limit(w, r), c);
             if (w.it.part < 0) {
-                store4<kSrcF32>(a.out, out_offset(a, w, r) + c, o * inverse_sum(sum));
+                store4<kSrcF32>(a.out, out_offset(a, w, r) + c, o);
             } else {
                 const int64_t pr = part_row(a, w, r);
                 *reinterpret_cast<f32x4_t*>(a.part_o + pr * a.D + c) = o;

@@ -41,6 +41,7 @@ __global__ void __launch_bounds__(kBlock) paged_few_kernel(PagedLaunch a) {
     using F = Few<DT, DP, RT>;
     __shared__ __align__(16) unsigned char lds[F::LDS];
     __shared__ float join_m[kWaves][RT * 16], join_l[kWaves][RT * 16];
+    __shared__ int join_odd[kWaves];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     const int col = lane % 16, gq = lane / 16;
     const Work w = work_of(a);
@@ -77,32 +78,47 @@ __global__ void __launch_bounds__(kBlock) paged_few_kernel(PagedLaunch a) {
     auto pages_of = [&](int t0) {
         return Pages{{block_page(a, w, t0), block_page(a, w, t0 + 16)}};
     };
+    const bool full = a.D == DP;
     auto load_k = [&](int t0, Pages pg) {
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb) {
             const uint16_t* p = block_at<uint16_t>(a, w, a.k_pages, pg.p[tb], t0 + 16 * tb);
+            const uint32_t off = col * a.D + 8 * gq;
+            if (full) {
 #pragma unroll
-            for (int ks = 0; ks < F::KS; ++ks) {
-                const int c = 32 * ks + 8 * gq;
-                kf[tb][ks] = u32x4_t{0, 0, 0, 0};
-                if (c < a.D) kf[tb][ks] = *reinterpret_cast<const u32x4_t*>(p + col * a.D + c);
+                for (int ks = 0; ks < F::KS; ++ks)
+                    kf[tb][ks] = *reinterpret_cast<const u32x4_t*>(p + off + 32 * ks);
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < F::KS; ++ks) {
+                    kf[tb][ks] = u32x4_t{0, 0, 0, 0};
+                    if (32 * ks + 8 * gq < a.D)
+                        kf[tb][ks] = *reinterpret_cast<const u32x4_t*>(p + off + 32 * ks);
+                }
             }
         }
     };
     auto load_v = [&](int t0, Pages pg) {
+        const bool whole = full && t0 + kUnit <= end;
 #pragma unroll
         for (int i = 0; i < F::VL; ++i) {
             constexpr int kPer = F::VL / 2;               // loads of a block
             const int at = i % kPer * kWave + lane, t = at / F::CH, c = at % F::CH * 8;
             const int tb = i / kPer;
             const uint16_t* p = block_at<uint16_t>(a, w, a.v_pages, pg.p[tb], t0 + 16 * tb);
-            // (zeros past the end: whatever lies there has weight 0)
-            vf[i] = u32x4_t{0, 0, 0, 0};
-            if (t0 + 16 * tb + t < end && c < a.D)
-                vf[i] = *reinterpret_cast<const u32x4_t*>(p + t * a.D + c);
+            const uint32_t off = t * a.D + c;
+            if (whole) {
+                vf[i] = *reinterpret_cast<const u32x4_t*>(p + off);
+            } else {
+                // (zeros past the end: whatever lies there has weight 0)
+                vf[i] = u32x4_t{0, 0, 0, 0};
+                if (t0 + 16 * tb + t < end && c < a.D)
+                    vf[i] = *reinterpret_cast<const u32x4_t*>(p + off);
+            }
         }
     };
 
+    bool odd = false;                     // some of the lane's values were not finite
     int t0 = w.it.kv_begin + wave * kUnit;
     Pages ahead = {{0, 0}};
     if (t0 < end) {
@@ -130,15 +146,16 @@ __global__ void __launch_bounds__(kBlock) paged_few_kernel(PagedLaunch a) {
             ahead = pages_of(next + kWaves * kUnit);
         }
         const bool masked = t0 + kUnit > min(all_see, end);
-        // A value that some row must not see reaches it as 0 * value: where one
-        // is not finite, the unit's second product goes row by row.
-        bool odd = false;
         if (t0 + kUnit > all_see) {
 #pragma unroll
-            for (int i = 0; i < F::VL; ++i)
-                odd |= non_finite<DT>(vf[i][0]) || non_finite<DT>(vf[i][1]) ||
-                       non_finite<DT>(vf[i][2]) || non_finite<DT>(vf[i][3]);
-            odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+            for (int i = 0; i < F::VL; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t x = finite_part<DT>(vf[i][j]);
+                    odd |= x != vf[i][j];
+                    vf[i][j] = x;
+                }
+            }
         }
         wave_sync();                      // the last unit's reads, before these writes
 #pragma unroll
@@ -179,48 +196,22 @@ __global__ void __launch_bounds__(kBlock) paged_few_kernel(PagedLaunch a) {
             for (int i = 0; i < 4; ++i) pf[rt][i] = pack2<DT>(p[2 * i], p[2 * i + 1]);
         }
         wave_sync();
-        if (!odd) {
-            // rows of a transposed read: tokens 4 gq .. + 3, and 16 further on,
-            // in the order in which a lane holds the weights
-            const unsigned char* vr = vl + (4 * gq + col / 4) * F::VS + col % 4 * 8;
+        // rows of a transposed read: tokens 4 gq .. + 3, and 16 further on, in the
+        // order in which a lane holds the weights
+        const unsigned char* vr = vl + (4 * gq + col / 4) * F::VS + col % 4 * 8;
 #pragma unroll
-            for (int cb = 0; cb < F::CB; ++cb) {
-                const uint2 lo = read_transposed(vr + cb * 32);
-                const uint2 hi = read_transposed(vr + 16 * F::VS + cb * 32);
-                const u32x4_t vt = {lo.x, lo.y, hi.x, hi.y};
+        for (int cb = 0; cb < F::CB; ++cb) {
+            const uint2 lo = read_transposed(vr + cb * 32);
+            const uint2 hi = read_transposed(vr + 16 * F::VS + cb * 32);
+            const u32x4_t vt = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) O[rt][cb] = mfma16<DT>(vt, pf[rt], O[rt][cb]);
-            }
-        } else {
-            for (int j = 0; j < kUnit && t0 + j < end; ++j) {
-                const uint16_t* vrow = block_at<uint16_t>(a, w, a.v_pages,
-                                                          block_page(a, w, t0 + j),
-                                                          (t0 + j) & ~15) + (j & 15) * a.D;
-                const int from = col + 16 * (j % 16 / 4), e = j / 16 * 4 + j % 4;
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const u32x4_t f = pf[rt];
-                    const uint32_t word = e < 4 ? (e < 2 ? f[0] : f[1]) : (e < 6 ? f[2] : f[3]);
-                    const float p = half_of<DT>(__shfl(word, from), e & 1);
-                    if (t0 + j >= lim[rt]) continue;
-#pragma unroll
-                    for (int cb = 0; cb < F::CB; ++cb) {
-                        const int c = 16 * cb + 4 * gq;
-                        if (c >= a.D) continue;
-                        const uint2 x = *reinterpret_cast<const uint2*>(vrow + c);
-                        // (a weight that rounds to 0 still carries an infinity)
-                        const float pp = fmaxf(p, FLT_MIN);
-                        O[rt][cb][0] = fmaf(pp, half_of<DT>(x.x, 0), O[rt][cb][0]);
-                        O[rt][cb][1] = fmaf(pp, half_of<DT>(x.x, 1), O[rt][cb][1]);
-                        O[rt][cb][2] = fmaf(pp, half_of<DT>(x.y, 0), O[rt][cb][2]);
-                        O[rt][cb][3] = fmaf(pp, half_of<DT>(x.y, 1), O[rt][cb][3]);
-                    }
-                }
-            }
+            for (int rt = 0; rt < RT; ++rt) O[rt][cb] = mfma16<DT>(vt, pf[rt], O[rt][cb]);
         }
     }
 
     // Join the waves: a row's largest maximum, then the rescaled sums.
+    if (lane == 0) join_odd[wave] = 0;
+    if (__builtin_amdgcn_ballot_w64(odd) != 0 && lane == 0) join_odd[wave] = 1;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         l[rt] += __shfl_xor(l[rt], 16);
@@ -257,8 +248,11 @@ __global__ void __launch_bounds__(kBlock) paged_few_kernel(PagedLaunch a) {
                 o += *reinterpret_cast<const f32x4_t*>(jo + (i * 16 + row) * F::OS + c);
                 sum += join_l[i][16 * rt + row] * exp2_fast(join_m[i][16 * rt + row] - mt);
             }
+            if (w.it.part < 0) o *= inverse_sum(sum);
+            if (join_odd[0] | join_odd[1] | join_odd[2] | join_odd[3])
+                o += odd_values<DT>(a, w, odd_from(w, all_see, kUnit), row_limit(w, r), c);
             if (w.it.part < 0) {
-                store4<DT>(a.out, out_offset(a, w, r) + c, o * inverse_sum(sum));
+                store4<DT>(a.out, out_offset(a, w, r) + c, o);
             } else {
                 const int64_t pr = part_row(a, w, r);
                 *reinterpret_cast<f32x4_t*>(a.part_o + pr * a.D + c) = o;
@@ -277,7 +271,7 @@ void launch_rows(const PagedLaunch& a, int kind, hipStream_t s) {
     } else if (kind == kFew32) {
         if constexpr (DP <= 128) paged_few_kernel<DT, DP, 2><<<grid, kBlock, 0, s>>>(a);
     } else {
-        if constexpr (DP <= 96) paged_few_kernel<DT, DP, 4><<<grid, kBlock, 0, s>>>(a);
+        if constexpr (DP <= 128) paged_few_kernel<DT, DP, 4><<<grid, kBlock, 0, s>>>(a);
     }
 }
 

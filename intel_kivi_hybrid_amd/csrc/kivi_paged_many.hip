@@ -64,7 +64,7 @@ struct ManyRows {
 
     // A tile of keys (kb) and values (vb) in LDS, positions t0 ..
     __device__ __forceinline__ void tile(const unsigned char* kb, const unsigned char* vb,
-                                         int t0, int end, float qscale, bool odd) {
+                                         int t0, int end, float qscale) {
         const int lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
         f32x16_t s[M::TB];
 #pragma unroll
@@ -119,49 +119,18 @@ struct ManyRows {
             for (int i = 0; i < 8; ++i)
                 pf[2 * tb + i / 4][i % 4] = pack2<DT>(s[tb][2 * i], s[tb][2 * i + 1]);
         }
-        if (!odd) {
-            // transposed: lanes of 16 take tokens 4 half .. + 3 of 16 channels
-            const int t = 4 * half + lane % 16 / 4;
-            const int c = lane / 16 % 2 * 2 + lane % 4 / 2;
-            const uint32_t vrow =
-                t * M::ROW + ((c ^ M::value_swizzle(t)) << 4) + lane % 2 * 8;
+        // transposed: lanes of 16 take tokens 4 half .. + 3 of 16 channels
+        const int t = 4 * half + lane % 16 / 4;
+        const int c = lane / 16 % 2 * 2 + lane % 4 / 2;
+        const uint32_t vrow = t * M::ROW + ((c ^ M::value_swizzle(t)) << 4) + lane % 2 * 8;
 #pragma unroll
-            for (int j = 0; j < 2 * M::TB; ++j) {
+        for (int j = 0; j < 2 * M::TB; ++j) {
 #pragma unroll
-                for (int cb = 0; cb < M::CB; ++cb) {
-                    const unsigned char* p = vb + (vrow ^ (64 * cb)) + 16 * j * M::ROW;
-                    const uint2 lo = read_transposed(p);
-                    const uint2 hi = read_transposed(p + 8 * M::ROW);
-                    O[cb] = mfma32<DT>(u32x4_t{lo.x, lo.y, hi.x, hi.y}, pf[j], O[cb]);
-                }
-            }
-        } else {
-            // A value that some row must not see would reach it as 0 * value:
-            // token by token, for the rows that see it.
-            for (int j = 0; j < M::TILE && t0 + j < end; ++j) {
-                // token 16 j4 + 8 (e / 4) + 4 h + e % 4 is element e of pf[j4]
-                const int j4 = j / 16, e = j % 16 / 8 * 4 + j % 4, h = j / 4 % 2;
-                u32x4_t f = pf[0];
-#pragma unroll
-                for (int i = 1; i < 2 * M::TB; ++i)
-                    if (j4 == i) f = pf[i];
-                const uint32_t word = e < 4 ? (e < 2 ? f[0] : f[1]) : (e < 6 ? f[2] : f[3]);
-                // (a weight that rounds to 0 still carries an infinity)
-                const float p = fmaxf(half_of<DT>(__shfl(word, col + 32 * h), e & 1), FLT_MIN);
-                if (t0 + j >= lim) continue;
-#pragma unroll
-                for (int cb = 0; cb < M::CB; ++cb) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int slot = (4 * cb + i) ^ M::value_swizzle(j);
-                        const uint2 x = *reinterpret_cast<const uint2*>(
-                            vb + j * M::ROW + 16 * slot + 8 * half);
-                        O[cb][4 * i] = fmaf(p, half_of<DT>(x.x, 0), O[cb][4 * i]);
-                        O[cb][4 * i + 1] = fmaf(p, half_of<DT>(x.x, 1), O[cb][4 * i + 1]);
-                        O[cb][4 * i + 2] = fmaf(p, half_of<DT>(x.y, 0), O[cb][4 * i + 2]);
-                        O[cb][4 * i + 3] = fmaf(p, half_of<DT>(x.y, 1), O[cb][4 * i + 3]);
-                    }
-                }
+            for (int cb = 0; cb < M::CB; ++cb) {
+                const unsigned char* p = vb + (vrow ^ (64 * cb)) + 16 * j * M::ROW;
+                const uint2 lo = read_transposed(p);
+                const uint2 hi = read_transposed(p + 8 * M::ROW);
+                O[cb] = mfma32<DT>(u32x4_t{lo.x, lo.y, hi.x, hi.y}, pf[j], O[cb]);
             }
         }
     }
@@ -174,10 +143,7 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) paged_many_kernel(P
     // one's loads, which the compiler knows to write the other array)
     __shared__ __align__(16) unsigned char buf0[2 * M::BYTES];
     __shared__ __align__(16) unsigned char buf1[2 * M::BYTES];
-    // Whether tile k's values are not all finite, at k % 3: set before tile k's
-    // barrier, read after it, cleared after the next one (three, so that a
-    // barrier lies between a clearing and the next setting too).
-    __shared__ int odd_tile[3];
+    __shared__ int odd;                    // some values were not finite
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
     const Work w = work_of(a);
@@ -242,32 +208,37 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) paged_many_kernel(P
     };
     // Waits for the wave's part of the tile.  What lies behind the end has
     // weight 0: zeros there, as it may be anything.
-    auto arrive = [&](unsigned char* buf, int t0, int slot) {
+    auto arrive = [&](unsigned char* buf, int t0) {
         wait_loads();
         if (t0 + M::TILE > min(wg_all, end)) {
-            bool odd = false;
+            bool any = false;
 #pragma unroll
             for (int i = 0; i < M::LD; ++i) {
                 u32x4_t* v = reinterpret_cast<u32x4_t*>(buf + M::BYTES +
                                                         (i * kWaves + wave) * 1024 + lane * 16);
-                const u32x4_t x = *v;
-                if (t0 + block_of(i) + vec_off(i, false).x >= end) *v = u32x4_t{0, 0, 0, 0};
-                else
-                    odd |= non_finite<DT>(x[0]) || non_finite<DT>(x[1]) || non_finite<DT>(x[2]) ||
-                           non_finite<DT>(x[3]);
+                u32x4_t x = *v;
+                if (t0 + block_of(i) + vec_off(i, false).x >= end) {
+                    x = u32x4_t{0, 0, 0, 0};
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t y = finite_part<DT>(x[j]);
+                        any |= y != x[j];
+                        x[j] = y;
+                    }
+                }
+                *v = x;
             }
-            if (odd) odd_tile[slot] = 1;
+            if (any) odd = 1;
         }
         lds_barrier();
     };
-    int t0 = w.it.kv_begin, slot = 0;
+    int t0 = w.it.kv_begin;
     auto step = [&](unsigned char* now, unsigned char* next) {
-        arrive(now, t0, slot);
+        arrive(now, t0);
         if (t0 + M::TILE < end) issue(next, t0 + M::TILE);
-        if (threadIdx.x == 0) odd_tile[slot == 0 ? 2 : slot - 1] = 0;
-        if (t0 < rows.last) rows.tile(now, now + M::BYTES, t0, end, a.qscale, odd_tile[slot] != 0);
+        if (t0 < rows.last) rows.tile(now, now + M::BYTES, t0, end, a.qscale);
         t0 += M::TILE;
-        slot = slot == 2 ? 0 : slot + 1;
     };
 
     pages_of(t0);
@@ -278,7 +249,7 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) paged_many_kernel(P
             reinterpret_cast<u32x4_t*>(buf1)[i] = u32x4_t{0, 0, 0, 0};
         }
     }
-    if (threadIdx.x < 3) odd_tile[threadIdx.x] = 0;
+    if (threadIdx.x == 0) odd = 0;
     lds_barrier();
     issue(buf0, t0);
     while (true) {
@@ -291,8 +262,8 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) paged_many_kernel(P
     float l = rows.l;
     l += __shfl_xor(l, 32);
     if (!live) return;
-    const float inv = inverse_sum(l);
     const bool whole = w.it.part < 0;
+    const float inv = whole ? inverse_sum(l) : 1.0f;
     const int64_t at = whole ? out_offset(a, w, r) : part_row(a, w, r);
 #pragma unroll
     for (int cb = 0; cb < M::CB; ++cb) {
@@ -301,8 +272,10 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) paged_many_kernel(P
             const int c = 32 * cb + 8 * i + 4 * half;
             if (c >= a.D) continue;
             const f32x16_t& O = rows.O[cb];
-            const f32x4_t o = {O[4 * i], O[4 * i + 1], O[4 * i + 2], O[4 * i + 3]};
-            if (whole) store4<DT>(a.out, at + c, o * inv);
+            f32x4_t o = {O[4 * i], O[4 * i + 1], O[4 * i + 2], O[4 * i + 3]};
+            o *= inv;
+            if (odd != 0) o += odd_values<DT>(a, w, odd_from(w, wg_all, M::TILE), rows.lim, c);
+            if (whole) store4<DT>(a.out, at + c, o);
             else *reinterpret_cast<f32x4_t*>(a.part_o + at * a.D + c) = o;
         }
     }
