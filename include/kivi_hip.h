@@ -481,13 +481,18 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
  * kept mass.  temperature <= 0: the first token.  Settings are the scalars, or one
  * value per row (device arrays) where a pointer is given.  NaN logits count as
  * -infinity; a row with nothing above that gives -1.  Of tokens of infinite logit
- * all weigh 1, any others 0.  Weights are fp64, summed in units of 2^-43 of the
- * largest: exactly, in any order, the same token at every call. */
+ * all weigh 1, any others 0.  Weights are formed in fp64 from x / temperature and
+ * summed as integers (2^-36 of a token's weight, 2^-43 of the largest): exactly, in
+ * any order, the same token at every call.  workspace (16-byte aligned): scratch
+ * of kivi_sample_workspace_size(rows, vocab) bytes. */
+size_t kivi_sample_workspace_size(int32_t rows, int32_t vocab);
+
 int kivi_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows,
                 int32_t vocab, const void* uniforms, int32_t uniforms_f64,
                 const float* temperatures, double temperature, const int32_t* top_ks,
                 int32_t top_k, const float* top_ps, double top_p, const float* min_ps,
-                double min_p, int64_t* out, void* stream);
+                double min_p, int64_t* out, void* workspace, size_t workspace_bytes,
+                void* stream);
 
 #ifdef __cplusplus
 }

@@ -983,8 +983,8 @@ def _setting(value, name: str, rows: int, dtype, dev):
 
 def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     """Next tokens ``[rows]`` (int64) from ``logits [rows, vocab]`` (fp32, bf16 or
-    fp16) and ``uniforms [rows]`` in [0, 1) (fp32 or fp64): one launch on the
-    current stream.
+    fp16) and ``uniforms [rows]`` in [0, 1) (fp32 or fp64), launched on the current
+    stream.
 
     In the order (logit descending, index ascending) with weights
     ``exp((x - max) / temperature)``: the first ``top_k`` tokens (0: all), of these
@@ -1020,8 +1020,11 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out
                dev)
     index = dev.index
     with on_device(index):
+        need = _lib.kivi_sample_workspace_size(rows, vocab)
+        workspace = _call_workspace(index, need)
         _native.check(_lib.kivi_sample(
             logits.data_ptr(), _IO_DTYPES[logits.dtype], logits.stride(0), rows, vocab,
             uniforms.data_ptr(), 1 if uniforms.dtype is torch.float64 else 0, tp, t, kp, k, pp, p,
-            mp, m, out.data_ptr(), stream_handle(index)), "sample")
+            mp, m, out.data_ptr(), 0 if workspace is None else workspace.data_ptr(), need,
+            stream_handle(index)), "sample")
     return out

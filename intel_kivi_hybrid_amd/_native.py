@@ -90,7 +90,8 @@ SIGNATURES = {
     "kivi_paged_attention": [_vp, _i64, _i64, _i32, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp,
                              _vp, _f32, _vp, _vp, ctypes.c_size_t, _vp],
     "kivi_sample": [_vp, _i32, _i64, _i32, _i32, _vp, _i32, _vp, ctypes.c_double, _vp, _i32, _vp,
-                    ctypes.c_double, _vp, ctypes.c_double, _vp, _vp],
+                    ctypes.c_double, _vp, ctypes.c_double, _vp, _vp, ctypes.c_size_t, _vp],
+    "kivi_sample_workspace_size": [_i32, _i32],
 }
 
 _RESTYPES = {
@@ -99,6 +100,7 @@ _RESTYPES = {
     "kivi_packed_decode_attention_workspace_size": ctypes.c_size_t,
     "kivi_packed_attention_workspace_size": ctypes.c_size_t,
     "kivi_paged_attention_workspace_size": ctypes.c_size_t,
+    "kivi_sample_workspace_size": ctypes.c_size_t,
 }
 
 _lib = None

@@ -53,7 +53,7 @@ constexpr int paged_tile_rows(int kind) {
 // The most rows of a kv head that a few-row kernel holds: their queries and
 // outputs, with a unit's keys and values, fill a wave's registers.
 constexpr int paged_few_rows(bool f32, int head_dim) {
-    if (f32) return head_dim <= 64 ? 64 : head_dim <= 128 ? 32 : 16;
+    if (f32) return head_dim <= 128 ? 32 : 16;
     return head_dim <= 128 ? 64 : 16;
 }
 // The kind that takes `rows` rows.  fp32 has no kMany kernel: its products run at

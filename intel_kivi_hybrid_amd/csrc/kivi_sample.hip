@@ -9,18 +9,21 @@
 // where its running count or mass crosses a border, three times at most for the
 // kept prefix and once for the token.
 //
-// A border is found by bucket, then within one: the row's 4096 buckets are
-// 1/128 wide in (max - x) / temperature, whose counts and masses one pass sums;
-// a second pass collects the border's bucket (a few tokens; where it holds more
-// than a workgroup's threads, sub-buckets of its keys narrow it first), and its
-// tokens are ranked against each other.
+// Two launches.  The first sums counts and masses of a row's buckets, 1/16 wide
+// in x / temperature, a workgroup for each slice of 8192 tokens.  The borders lie
+// in a few buckets that these sums name (the second to last border moves the
+// last by less than a bucket's mass); the second launch, a workgroup for each
+// row, goes through the row once for their tokens and ranks those against each
+// other, by sub-buckets where they are many.
 //
-// Precision: neighbouring tokens' borders lie as close as a token's share of the
-// mass, 1e-6 and less, and sums of fp32 weights over 10^5 tokens are off by more
-// than that.  Weights are computed in fp64 (2^-47 relative) and summed as
-// integers in units of 2^-43 of the largest weight, exactly and in any order.
-// Tokens below half a unit (w < 2^-44) have no mass: all of a million of them
-// together are below 2^-24 of it.
+// Precision: neighbouring borders lie as close as a token's share of the mass,
+// 1e-6 and less, and sums of fp32 weights over 10^5 tokens are off by more than
+// that.  A token's weight is formed in fp64 as (edge of its bucket) x rel, with
+// rel in [1, e^(1/16)) rounded to 2^-36 and summed as an integer, exactly and in
+// any order; a bucket's sum is rounded to 2^-43 of the row's largest edge.  Tokens
+// below e^-32 of a slice's largest have no mass (2^-46 of it, each).
+//
+// 64 rows of 128256 bf16 logits with settings of their own: see kivi_sample().
 #include <hip/hip_runtime.h>
 
 #include <math.h>
@@ -32,17 +35,24 @@
 namespace kivi {
 namespace {
 
-constexpr int kBlock = 1024;
-constexpr int kBuckets = 4096;
-constexpr float kPerUnit = 128.f;         // buckets per unit of (max - x) / t
-constexpr int kUnitBits = 43;
-constexpr int kMaxVocab = 1 << 20;        // (sums stay below 2^63)
+constexpr int kSlice = 8192;              // tokens of a workgroup
+constexpr int kBlock = 512;               // its threads
+constexpr int kPickBlock = 1024;
+constexpr int kFew = 128;                 // tokens that are ranked against each other
+constexpr int kBuckets = 512;
+constexpr double kPerUnit = 16.0;         // buckets per unit of x / t
+constexpr int kRelBits = 36, kMassBits = 43;
+constexpr int kCountShift = 50;           // a slice's rels stay below 2^50
+constexpr uint64_t kRelMask = (1ull << kCountShift) - 1;
+constexpr int kMaxVocab = 1 << 20;        // (a row's rels stay below 2^57)
+constexpr int kList = 6144;               // tokens that a row's list holds
+constexpr int kSeen = 1024;               // threads of the first launch that it is made from
 constexpr int kSub = 2048;                // sub-buckets of a crowded bucket
 
 struct SampleArgs {
     const void* logits;
     int64_t stride;
-    int V;
+    int V, slices;
     const void* u;
     int u_f64;
     const float* t_row;      // per row, or NULL: the scalar
@@ -52,75 +62,100 @@ struct SampleArgs {
     double t, p, m;
     int k;
     int64_t* out;
+    // workspace
+    uint64_t* hist;          // [row][slice][bucket]: count << 50 | sum of rels
+    uint64_t* best;          // [row][slice]: the first token's key
+    float* tops;             // [row][slice][thread]: the largest of its tokens
 };
 
-// Order-preserving bits of a logit, largest first: keys ascend as logits
-// descend.  -0 counts as 0, NaN as -infinity.
+struct Settings {
+    double t, p, m, u;
+    int k;
+    bool first;              // the first token of the order, whatever u
+};
+
+__device__ __forceinline__ Settings settings_of(const SampleArgs& a, int row) {
+    Settings s;
+    s.t = a.t_row ? (double)a.t_row[row] : a.t;
+    s.p = a.p_row ? (double)a.p_row[row] : a.p;
+    s.m = a.m_row ? (double)a.m_row[row] : a.m;
+    s.k = a.k_row ? a.k_row[row] : a.k;
+    const double u = a.u_f64 ? static_cast<const double*>(a.u)[row]
+                             : (double)static_cast<const float*>(a.u)[row];
+    s.u = u > 0.0 ? fmin(u, 1.0) : 0.0;                  // (NaN: 0)
+    s.first = !(s.t > 0.0) || s.k == 1 || s.p <= 0.0;
+    return s;
+}
+
+// Order-preserving bits of a logit: they ascend as logits descend.  -0 counts
+// as 0, NaN as -infinity.
 __device__ __forceinline__ uint32_t order_bits(float x) {
     x = x == 0.f ? 0.f : x;
     x = x != x ? -INFINITY : x;
     const uint32_t b = __float_as_uint(x);
     return b & 0x80000000u ? b : ~b & 0x7fffffffu;
 }
-__device__ __forceinline__ float logit_of(uint32_t bits) {
+__device__ __forceinline__ float logit_of(uint64_t key) {
+    const uint32_t bits = (uint32_t)(key >> 32);
     return __uint_as_float(bits & 0x80000000u ? bits : ~bits & 0x7fffffffu);
 }
 
-// The tokens' weights in units of 2^-43 of the largest.
-struct Weights {
-    double top, per;         // the largest logit, log2(e) / temperature
-    float top32, bucket;     // buckets per unit of logit
+// Buckets and weights of a row or slice whose largest logit is `top`.
+struct Scale {
+    float top;
+    double inv_t, edge;      // 1 / temperature; the largest logit's bucket
 
-    __device__ __forceinline__ void set(float mx, double t) {
-        top = mx;
-        top32 = mx;
-        per = 1.4426950408889634074 / t;
-        bucket = (float)(kPerUnit / t);
+    __device__ __forceinline__ void set(float largest, double t) {
+        top = largest;
+        inv_t = 1.0 / t;
+        edge = floor((double)top * inv_t * kPerUnit);
     }
-    // 2^y by its series in y ln 2 around the nearest integer: the eleventh
-    // power's remainder is 0.35^12 / 12! < 2^-46.
-    __device__ __forceinline__ uint64_t mass(float x) const {
-        const double y = ((double)x - top) * per;
-        if (x == top32) return 1ull << kUnitBits;          // (infinities too)
-        if (!(y > -46.0)) return 0;
-        const double n = __builtin_rint(y), z = (y - n) * 0.69314718055994530942;
-        double e = 1.0 / 39916800.0;
-        e = __builtin_fma(e, z, 1.0 / 3628800.0);
-        e = __builtin_fma(e, z, 1.0 / 362880.0);
-        e = __builtin_fma(e, z, 1.0 / 40320.0);
-        e = __builtin_fma(e, z, 1.0 / 5040.0);
-        e = __builtin_fma(e, z, 1.0 / 720.0);
-        e = __builtin_fma(e, z, 1.0 / 120.0);
-        e = __builtin_fma(e, z, 1.0 / 24.0);
-        e = __builtin_fma(e, z, 1.0 / 6.0);
-        e = __builtin_fma(e, z, 0.5);
-        e = __builtin_fma(e, z, 1.0);
-        e = __builtin_fma(e, z, 1.0);
-        return (uint64_t)__builtin_rint(ldexp(e, (int)n + kUnitBits));
-    }
-    // (monotone: each step rounds monotonely; at 4096 w is below 2^-46)
-    __device__ __forceinline__ int bucket_of(float x) const {
-        if (x == top32) return 0;
-        const float b = (top32 - x) * bucket;
-        return b < (float)kBuckets ? (int)b : kBuckets;
+    // Buckets below the largest's (kBuckets: no mass), and rel.
+    __device__ __forceinline__ int bucket(float x, uint64_t& rel) const {
+        rel = 1ull << kRelBits;
+        if (x == top && isinf(x)) return 0;
+        const double z = (double)x * inv_t, e = floor(z * kPerUnit), below = edge - e;
+        if (!(below < (double)kBuckets)) return kBuckets;      // (NaN too)
+        // e^r, r in [0, 1/16]: the series' remainder is r^7 / 7! < 2^-40
+        const double r = __builtin_fma(e, -1.0 / kPerUnit, z);
+        double w = 1.0 / 720.0;
+        w = __builtin_fma(w, r, 1.0 / 120.0);
+        w = __builtin_fma(w, r, 1.0 / 24.0);
+        w = __builtin_fma(w, r, 1.0 / 6.0);
+        w = __builtin_fma(w, r, 0.5);
+        w = __builtin_fma(w, r, 1.0);
+        w = __builtin_fma(w, r, 1.0);
+        // (rounded to an integer in the low bits by the 2^52 added)
+        w = __builtin_fma(w, (double)(1ull << kRelBits), 0x1p52);
+        rel = __double_as_longlong(w) & ((1ull << 52) - 1);
+        return (int)below;
     }
 };
 
-// f(x, index) for the row's tokens: 16-byte loads between the first and the last
-// 16-byte border, single ones outside.
-template <int DT, class F>
-__device__ __forceinline__ void each_token(const SampleArgs& a, int row, F f) {
-    constexpr int kSize = src_size(DT), kVec = 16 / kSize;
-    const char* base = static_cast<const char*>(a.logits) + row * a.stride * kSize;
-    const int head = min(a.V, (int)((16 - ((uintptr_t)base & 15)) & 15) / kSize);
-    const int vecs = (a.V - head) / kVec, tail = head + vecs * kVec;
-    if ((int)threadIdx.x < head) f(widen<DT>(base, threadIdx.x), (int)threadIdx.x);
-    if ((int)threadIdx.x < a.V - tail)
-        f(widen<DT>(base, tail + threadIdx.x), tail + (int)threadIdx.x);
-    const uint4* v = reinterpret_cast<const uint4*>(base + head * kSize);
-#pragma unroll 2
-    for (int i = threadIdx.x; i < vecs; i += kBlock) {
-        const uint4 w = v[i];
+__device__ __forceinline__ int bucket_gap(double row_edge, double slice_edge) {
+    if (row_edge == slice_edge) return 0;                // (infinities too)
+    const double d = row_edge - slice_edge;
+    return d < (double)kBuckets ? (int)d : kBuckets;
+}
+
+// A row as 16-byte vectors between its first and last 16-byte borders, and the
+// tokens before and behind them.
+template <int DT>
+struct RowView {
+    static constexpr int kVec = 16 / src_size(DT);
+    const char* base;
+    const uint4* vecs;
+    int head, n_vecs, tail;              // tail: the first token behind
+    __device__ __forceinline__ RowView(const SampleArgs& a, int row) {
+        base = static_cast<const char*>(a.logits) + row * a.stride * src_size(DT);
+        head = min(a.V, (int)((16 - ((uintptr_t)base & 15)) & 15) / src_size(DT));
+        n_vecs = (a.V - head) / kVec;
+        tail = head + n_vecs * kVec;
+        vecs = reinterpret_cast<const uint4*>(base + head * src_size(DT));
+    }
+    // f(logit, index) for the tokens of vector i, loaded as w
+    template <class F>
+    __device__ __forceinline__ void tokens(uint4 w, int i, F f) const {
         const uint32_t words[4] = {w.x, w.y, w.z, w.w};
         const int at = head + i * kVec;
 #pragma unroll
@@ -136,270 +171,809 @@ __device__ __forceinline__ void each_token(const SampleArgs& a, int row, F f) {
             }
         }
     }
-}
-
-struct Shared {
-    uint64_t mass[kBuckets];         // then the running sum before each bucket
-    uint32_t count[kBuckets];
-    union {
-        struct {
-            uint64_t key[kBlock];
-            uint64_t mass[kBlock];
-        } list;
-        struct {
-            uint64_t mass[kSub];
-            uint32_t count[kSub];
-        } sub;
-    };
-    uint64_t wave_mass[kBlock / kWave];
-    uint32_t wave_count[kBlock / kWave];
-    uint64_t key_min, key_max, hit_mass;
-    uint32_t listed, hit;
+    // The same without unrolling, for bodies of some size: code that runs once is
+    // bound by its own fetch.
+    template <class F>
+    __device__ __forceinline__ void tokens_rolled(uint4 w, int i, F f) const {
+        int at = head + i * kVec;
+#pragma unroll 1
+        for (int j = 0; j < kVec; ++j, ++at) {
+            float x;
+            if constexpr (DT == kSrcF32) {
+                x = __uint_as_float(w.x);
+            } else {
+                x = DT == kSrcBF16 ? __uint_as_float(w.x << 16)
+                                   : (float)__builtin_bit_cast(_Float16, (uint16_t)(w.x & 0xffffu));
+                w.x >>= 16;
+            }
+            if (DT == kSrcF32 || j % 2 == 1) {
+                w.x = w.y;
+                w.y = w.z;
+                w.z = w.w;
+            }
+            f(x, at);
+        }
+    }
+    // the token before or behind the vectors that a thread takes (-1: none):
+    // the first slice takes those before, the last slice those behind
+    __device__ __forceinline__ int single(int tid, int slice, int slices, int V) const {
+        if (slice == 0 && tid < head) return tid;
+        if (slice == slices - 1 && tid >= 8 && tid - 8 < V - tail) return tail + tid - 8;
+        return -1;
+    }
 };
 
-// A place in the order: the running count or mass to be reached.
+// A slice's tokens in registers.
+template <int DT>
+struct Slice {
+    using R = RowView<DT>;
+    static constexpr int kLoads = kSlice / R::kVec / kBlock;
+    R row;
+    uint4 w[kLoads];
+    int first, single;
+    float lone;
+    // a thread's first vector, the others kBlock further each
+    static __device__ __forceinline__ int vec_of(int slice, int thread) {
+        return slice * (kSlice / R::kVec) + thread;
+    }
+    __device__ __forceinline__ Slice(const SampleArgs& a, int r, int slice) : row(a, r) {
+        first = vec_of(slice, threadIdx.x);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int v = first + i * kBlock;
+            if (v < row.n_vecs) w[i] = row.vecs[v];
+        }
+        single = row.single(threadIdx.x, slice, a.slices, a.V);
+        lone = single >= 0 ? widen<DT>(row.base, single) : 0.f;
+    }
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int v = first + i * kBlock;
+            if (v < row.n_vecs) row.tokens(w[i], v, f);
+        }
+        if (single >= 0) f(lone, single);
+    }
+};
+
+template <int DT>
+__global__ void __launch_bounds__(kBlock) sample_sums_kernel(SampleArgs a) {
+    __shared__ uint64_t hist[kBuckets];
+    __shared__ float wave_top[kBlock / kWave];
+    __shared__ uint32_t first;
+    const int row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
+    const int tid = threadIdx.x;
+    const Slice<DT> tokens(a, row, slice);
+    const Settings s = settings_of(a, row);
+    hist[tid] = 0;
+    static_assert(kBuckets == kBlock, "a thread for each bucket");
+    if (tid == 0) first = ~0u;
+    float top = -INFINITY;
+    tokens.each([&](float x, int) { top = fmaxf(top, x); });       // (NaN never)
+    a.tops[(int64_t)blockIdx.x * kBlock + tid] = top;
+    top = wave_max(top);
+    if (tid % kWave == 0) wave_top[tid / kWave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kBlock / kWave; ++i) top = fmaxf(top, wave_top[i]);
+    uint32_t index = ~0u;
+    if (s.first || !(top > -INFINITY)) {
+        tokens.each([&](float x, int i) { index = x == top ? min(index, (uint32_t)i) : index; });
+    } else {
+        Scale scale;
+        scale.set(top, s.t);
+        tokens.each([&](float x, int i) {
+            index = x == top ? min(index, (uint32_t)i) : index;
+            uint64_t rel;
+            const int b = scale.bucket(x, rel);
+            if (b < kBuckets)
+                atomicAdd((unsigned long long*)&hist[b],
+                          (unsigned long long)(rel | 1ull << kCountShift));
+        });
+    }
+    if (index != ~0u) atomicMin(&first, index);
+    __syncthreads();
+    const int64_t at = (int64_t)row * a.slices + slice;
+    if (tid == 0) a.best[at] = (uint64_t)order_bits(top) << 32 | first;
+    if (!s.first) a.hist[at * kBuckets + tid] = hist[tid];
+}
+
+// The first token of a row from its slices' (every lane).
+__device__ __forceinline__ uint64_t first_of(const SampleArgs& a, int row) {
+    uint64_t best = ~0ull;
+    for (int i = threadIdx.x % kWave; i < a.slices; i += kWave)
+        best = min(best, a.best[(int64_t)row * a.slices + i]);
+    for (int d = 1; d < kWave; d *= 2)
+        best = min(best, (uint64_t)__shfl_xor((unsigned long long)best, d));
+    return best;
+}
+
+// A row's running sums before each bucket (entry kBuckets: the totals).
+struct Sums {
+    uint64_t mass[kBuckets + 1];
+    uint32_t count[kBuckets + 1];
+    uint64_t rel[kBuckets];              // the buckets' sums of rels
+};
+
+// Inclusive running sums over the wave's lanes.
+__device__ __forceinline__ void wave_scan(uint64_t& m, uint32_t& c) {
+    const int lane = threadIdx.x % kWave;
+    for (int d = 1; d < kWave; d *= 2) {
+        const uint64_t om = __shfl_up((unsigned long long)m, d);
+        const uint32_t oc = __shfl_up(c, d);
+        if (lane >= d) {
+            m += om;
+            c += oc;
+        }
+    }
+}
+
+// The border kinds, and whether entry i of running sums crosses one (exactly one
+// does, for a border within the total).
 enum Border : int {
     kByCount,       // the token that is number `at`
     kByMass,        // the first whose running sum reaches `at`
     kPast,          // the first whose running sum exceeds `at`
 };
+template <class T>
+__device__ __forceinline__ bool crosses(const T* sums, int i, Border kind, uint64_t at) {
+    const uint64_t from = sums[i], to = sums[i + 1];
+    return kind == kPast ? from <= at && at < to : from < at && at <= to;
+}
+
+__device__ __forceinline__ uint64_t mass_wanted(double p, uint64_t kept) {
+    const uint64_t want = (uint64_t)ceil(p * (double)kept);
+    return want < 1 ? 1 : want > kept ? kept : want;
+}
+__device__ __forceinline__ uint64_t mass_passed(double u, uint64_t kept) {
+    const uint64_t past = (uint64_t)(u * (double)kept);
+    return past >= kept ? kept - 1 : past;
+}
+
+// min_p: w >= m where x / t reaches this.
+__device__ __forceinline__ double min_p_border(const Scale& s, double m) {
+    return (double)s.top * s.inv_t + log(m);
+}
+// its bucket (kBuckets: it cuts nothing that has mass)
+__device__ __forceinline__ int min_p_bucket(const Scale& s, double border) {
+    if (isinf(s.top)) return 0;
+    const double below = s.edge - floor(border * kPerUnit);
+    return below < (double)kBuckets ? (int)below : kBuckets;
+}
+
+// Ranges of buckets that may hold a border (lo > hi: none).
+struct Wanted {
+    int lo[4], hi[4];
+};
+
+// The logits of the wanted buckets lie within these (fp32, a little wider): what
+// is outside needs no fp64.  Mostly two of the ranges are there or meet.
+struct Window {
+    float lo[4], hi[4], least;
+    bool two, odd;                       // the last two are empty; bounds are infinite
+    __device__ __forceinline__ void set(const Wanted& w, const Scale& s, double t) {
+        odd = isinf(s.top) || isinf(s.edge);
+        int n = 0;
+        least = INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            lo[i] = INFINITY;
+            hi[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (w.lo[i] > w.hi[i]) continue;
+            const double a = (s.edge - w.hi[i]) / kPerUnit * t;
+            const double b = (s.edge - w.lo[i] + 1.0) / kPerUnit * t;
+            // (rounding: x / t and its bucket, 2^-52 of x; these bounds, 2^-23)
+            const float l = odd ? -INFINITY : (float)(a - fabs(a) * 1e-6 - 1e-30);
+            const float h = odd ? INFINITY : (float)(b + fabs(b) * 1e-6 + 1e-30);
+            least = fminf(least, l);
+            bool met = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (met || !(l <= hi[j] && h >= lo[j])) continue;
+                lo[j] = fminf(lo[j], l);
+                hi[j] = fmaxf(hi[j], h);
+                met = true;
+            }
+            if (met) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j != n) continue;
+                lo[j] = l;
+                hi[j] = h;
+            }
+            ++n;
+        }
+        two = n <= 2;
+    }
+    __device__ __forceinline__ bool has(float x) const {
+        bool in = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) in |= (x >= lo[i]) & (x <= hi[i]);
+        return in;
+    }
+};
+
+// The same as the sign of min |x - middle| - half, in a few vector instructions
+// and no mask: finite bounds, a little wider again.
+template <int N>
+struct Near {
+    float middle[N], half[N];
+    __device__ __forceinline__ explicit Near(const Window& w) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool none = w.lo[i] > w.hi[i];
+            const float l = none ? 0.f : w.lo[i], h = none ? 0.f : w.hi[i];
+            middle[i] = 0.5f * l + 0.5f * h;
+            half[i] = none ? -1.f : 0.5f * h - 0.5f * l + 1e-6f * (fabsf(l) + fabsf(h)) + 1e-30f;
+        }
+    }
+    __device__ __forceinline__ float side(float x) const {
+        float d = fabsf(x - middle[0]) - half[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) d = fminf(d, fabsf(x - middle[i]) - half[i]);
+        return d;
+    }
+};
+
+// Where the borders can lie: each is known up to its bucket, so the kept mass
+// lies between two of the running sums.  By all threads of a workgroup.
+__device__ void wanted_buckets(const Settings& s, const Scale& scale, const Sums& sums,
+                               Wanted& w) {
+    const int b = threadIdx.x;
+    if (b < 4) {
+        w.lo[b] = 1;
+        w.hi[b] = 0;
+    }
+    __syncthreads();
+    uint64_t low = sums.mass[kBuckets], high = low;
+    if (s.k > 0 && (uint32_t)s.k < sums.count[kBuckets]) {
+        if (b < kBuckets && crosses(sums.count, b, kByCount, (uint64_t)s.k))
+            w.lo[0] = w.hi[0] = b;
+        __syncthreads();
+        low = max(sums.mass[w.lo[0]], (uint64_t)1);
+        high = max(sums.mass[w.hi[0] + 1], (uint64_t)1);
+    }
+    if (s.p < 1.0) {
+        if (b < kBuckets) {
+            if (crosses(sums.mass, b, kByMass, mass_wanted(s.p, low))) w.lo[1] = b;
+            if (crosses(sums.mass, b, kByMass, mass_wanted(s.p, high))) w.hi[1] = b;
+        }
+        __syncthreads();
+        low = max(sums.mass[w.lo[1]], (uint64_t)1);
+        high = min(high, sums.mass[w.hi[1] + 1]);
+    }
+    if (s.m > 0.0) {
+        const int at = min_p_bucket(scale, min_p_border(scale, s.m));
+        if (at < kBuckets) {
+            if (b == 0) w.lo[2] = w.hi[2] = at;
+            low = min(low, max(sums.mass[at], (uint64_t)1));
+            high = min(high, max(sums.mass[at + 1], (uint64_t)1));
+        }
+    }
+    if (b < kBuckets) {
+        if (crosses(sums.mass, b, kPast, mass_passed(s.u, low))) w.lo[3] = b;
+        if (crosses(sums.mass, b, kPast, mass_passed(s.u, high))) w.hi[3] = b;
+    }
+    __syncthreads();
+}
 
 template <int DT>
-struct Sampler {
+struct Picker {
+    struct Shared {
+        Sums sums;
+        uint64_t key[kList];             // the wanted buckets' tokens
+        uint64_t rel[kList];             // bucket << 40 | rel
+        union {
+            struct {
+                uint64_t key[kFew], rel[kFew], before[kPickBlock / kFew][kFew];
+                uint32_t count[kPickBlock / kFew][kFew];
+            } few;
+            struct {
+                uint64_t rel[kSub + 1];
+                uint32_t count[kSub + 1];
+            } sub;
+            int thread[kSeen];           // threads that saw a token within reach
+        };
+        Wanted wanted;
+        uint64_t wave_rel[kPickBlock / kWave];
+        uint32_t wave_count[kPickBlock / kWave];
+        int gap[kMaxVocab / kSlice];
+        uint64_t hit_rel;
+        uint32_t bits_min, bits_max, n, hit, listed, seen;
+        int entry;
+    };
     const SampleArgs& a;
     Shared& s;
     int row;
-    Weights w;
-    uint64_t all_mass;
-    uint32_t all_count;
+    Scale scale;
+    int listed;                          // tokens of the list, -1: too many
 
-    // Exclusive running sums of n counts and masses, in place; the totals.
-    __device__ void scan(uint64_t* mass, uint32_t* count, int n, uint64_t& tm, uint32_t& tc) {
-        const int tid = threadIdx.x, lane = tid % kWave, per = n / kBlock;
-        uint64_t m = 0;
-        uint32_t c = 0;
-        for (int i = 0; i < per; ++i) {
-            m += mass[tid * per + i];
-            c += count[tid * per + i];
+    // f(key, rel) for the tokens of bucket b
+    template <class F>
+    __device__ __forceinline__ void each(int b, F f) {
+        if (listed >= 0) {
+            for (int i = threadIdx.x; i < listed; i += kPickBlock) {
+                const uint64_t rel = s.rel[i];
+                if ((int)(rel >> 40) == b) f(s.key[i], rel & ((1ull << 40) - 1));
+            }
+            return;
         }
-        uint64_t im = m;
-        uint32_t ic = c;
-        for (int d = 1; d < kWave; d *= 2) {
-            const uint64_t om = __shfl_up(im, d);
-            const uint32_t oc = __shfl_up(ic, d);
-            if (lane >= d) {
-                im += om;
-                ic += oc;
+        const RowView<DT> r(a, row);
+        auto token = [&](float x, int i) {
+            uint64_t rel;
+            if (scale.bucket(x, rel) == b) f((uint64_t)order_bits(x) << 32 | (uint32_t)i, rel);
+        };
+        const int single = r.single(threadIdx.x, 0, 1, a.V);
+        if (single >= 0) token(widen<DT>(r.base, single), single);
+#pragma unroll 1
+        for (int i = threadIdx.x; i < r.n_vecs; i += kPickBlock) r.tokens_rolled(r.vecs[i], i, token);
+    }
+
+    // Vector i of those of the threads seen.
+    __device__ __forceinline__ int seen_vec(int i) const {
+        constexpr int kLoads = Slice<DT>::kLoads;
+        const int t = s.thread[i / kLoads];
+        return Slice<DT>::vec_of(t / kBlock, t % kBlock) + i % kLoads * kBlock;
+    }
+
+    // The tokens of vectors vec(0 .. n - 1) within the window, to the list.  A
+    // thread marks a few vectors' first: one round trip to the list's end for
+    // all of them, not one each.
+    template <int N, class F>
+    __device__ __forceinline__ void take(const Window& window, int n, F vec) {
+        constexpr int kVec = RowView<DT>::kVec, kAhead = 32 / kVec;
+        const RowView<DT> r(a, row);
+        if (r.n_vecs == 0) return;               // (a row of single tokens)
+        const Near<N> near(window);
+        const uint32_t always = window.odd ? ~0u : 0u;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < n; i += kAhead * kPickBlock) {
+            uint4 w[kAhead];
+            uint32_t there = 0;                  // token k of the 32 at bit 31 - k
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const int at = i + j * kPickBlock, v = vec(min(at, n - 1));
+                w[j] = r.vecs[min(v, r.n_vecs - 1)];
+                if (at < n && v < r.n_vecs)
+                    there |= ((1u << kVec) - 1) << (32 - kVec - j * kVec);
+            }
+            uint32_t mark = 0;
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                r.tokens(w[j], 0, [&](float x, int) {
+                    mark = mark << 1 | __float_as_uint(near.side(x)) >> 31;
+                });
+            mark = (mark | always) & there;
+            if (mark == 0) continue;
+            uint32_t to = atomicAdd(&s.listed, (uint32_t)__popc(mark));
+#pragma unroll 1
+            for (; mark != 0; ++to) {
+                const int at = __clz(mark);
+                mark &= ~(0x80000000u >> at);
+                const int token = vec(i + at / kVec * kPickBlock) * kVec + at % kVec;
+                if (to < kList) s.key[to] = (uint64_t)(r.head + token);
             }
         }
+    }
+
+    // The row's sums from its slices', and the buckets that may hold a border;
+    // their tokens to the list.
+    __device__ void collect(const Settings& set) {
+        const int tid = threadIdx.x, bucket = tid % kBuckets, lane = tid % kWave;
+        static_assert(kPickBlock == 2 * kBuckets, "two threads for each bucket");
+        // (buckets that each slice's lie below the row's)
+        for (int i = tid; i < a.slices; i += kPickBlock) {
+            Scale other;
+            other.set(logit_of(a.best[(int64_t)row * a.slices + i]), set.t);
+            s.gap[i] = other.top == -INFINITY ? kBuckets : bucket_gap(scale.edge, other.edge);
+        }
+        if (tid == 0) s.listed = s.seen = 0;
+        __syncthreads();
+        uint64_t rel = 0;
+        uint32_t count = 0;
+        const uint64_t* hist = a.hist + (int64_t)row * a.slices * kBuckets;
+#pragma unroll 4
+        for (int i = tid / kBuckets; i < a.slices; i += 2) {
+            const int b = bucket - s.gap[i];
+            const uint64_t h = b >= 0 ? hist[i * kBuckets + b] : 0;
+            rel += h & kRelMask;
+            count += (uint32_t)(h >> kCountShift);
+        }
+        if (tid >= kBuckets) {
+            s.sums.rel[bucket] = rel;
+            s.sums.count[bucket] = count;
+        }
+        __syncthreads();
+        uint64_t mass = 0;
+        if (tid < kBuckets) {
+            rel += s.sums.rel[tid];
+            count += s.sums.count[tid];
+            s.sums.rel[tid] = rel;
+            const double unit = exp(-tid / kPerUnit) * (double)(1ull << (kMassBits - kRelBits));
+            mass = (uint64_t)__builtin_rint((double)rel * unit);
+            wave_scan(mass, count);
+            if (lane == kWave - 1) {
+                s.wave_rel[tid / kWave] = mass;
+                s.wave_count[tid / kWave] = count;
+            }
+        }
+        __syncthreads();
+        if (tid < kBuckets) {
+            for (int i = 0; i < tid / kWave; ++i) {
+                mass += s.wave_rel[i];
+                count += s.wave_count[i];
+            }
+            s.sums.mass[tid + 1] = mass;
+            s.sums.count[tid + 1] = count;
+            if (tid == 0) {
+                s.sums.mass[0] = 0;
+                s.sums.count[0] = 0;
+            }
+        }
+        __syncthreads();
+        wanted_buckets(set, scale, s.sums, s.wanted);
+        Window window;
+        window.set(s.wanted, scale, set.t);
+        // The wanted buckets lie at the order's head: of most rows few of the first
+        // launch's threads saw a token that reaches them.  Those threads' tokens,
+        // or the whole row where they are many.
+        const float* tops = a.tops + (int64_t)row * a.slices * kBlock;
+        for (int i = tid; i < a.slices * kBlock; i += kPickBlock) {
+            const uint64_t lanes = __builtin_amdgcn_ballot_w64(tops[i] >= window.least);
+            if (lanes == 0) continue;
+            uint32_t n = 0;
+            if (lane == 0) n = atomicAdd(&s.seen, (uint32_t)__popcll(lanes));
+            n = __builtin_amdgcn_readfirstlane(n) +
+                __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32),
+                                          __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+            if ((lanes >> lane & 1) && n < kSeen) s.thread[n] = i;
+        }
+        __syncthreads();
+        if (s.seen <= kSeen) {
+            // (a thread's vectors of a slice to one thread each)
+            constexpr int kLoads = Slice<DT>::kLoads;
+            const int n = (int)s.seen * kLoads;
+            if (window.two) take<2>(window, n, [&](int i) { return seen_vec(i); });
+            else take<4>(window, n, [&](int i) { return seen_vec(i); });
+        } else {
+            const int n = RowView<DT>(a, row).n_vecs;
+            if (window.two) take<2>(window, n, [&](int i) { return i; });
+            else take<4>(window, n, [&](int i) { return i; });
+        }
+        const RowView<DT> r(a, row);
+        const int single = r.single(tid, 0, 1, a.V);
+        if (single >= 0) {
+            const float x = widen<DT>(r.base, single);
+            if (window.has(x)) {
+                const uint32_t n = atomicAdd(&s.listed, 1u);
+                if (n < kList) s.key[n] = (uint64_t)single;
+            }
+        }
+        __syncthreads();
+        listed = s.listed <= kList ? (int)s.listed : -1;
+#pragma unroll 1
+        for (int j = tid; j < listed; j += kPickBlock) {
+            const uint32_t i = (uint32_t)s.key[j];
+            const float x = widen<DT>(r.base, i);
+            uint64_t rel;
+            const int b = scale.bucket(x, rel);
+            s.key[j] = (uint64_t)order_bits(x) << 32 | i;
+            s.rel[j] = (uint64_t)b << 40 | rel;
+        }
+        __syncthreads();
+    }
+
+    // The sub-buckets' running sums, in place.
+    __device__ void scan_sub() {
+        constexpr int kPer = kSub / kPickBlock;
+        const int tid = threadIdx.x, lane = tid % kWave;
+        uint64_t r[kPer], sum = 0;
+        uint32_t c[kPer], n = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            r[i] = s.sub.rel[kPer * tid + i];
+            c[i] = s.sub.count[kPer * tid + i];
+            sum += r[i];
+            n += c[i];
+        }
+        uint64_t ir = sum;
+        uint32_t ic = n;
+        wave_scan(ir, ic);
         if (lane == kWave - 1) {
-            s.wave_mass[tid / kWave] = im;
+            s.wave_rel[tid / kWave] = ir;
             s.wave_count[tid / kWave] = ic;
         }
         __syncthreads();
-        uint64_t bm = im - m;
-        uint32_t bc = ic - c;
-        tm = tc = 0;
-        for (int i = 0; i < kBlock / kWave; ++i) {
-            if (i < tid / kWave) {
-                bm += s.wave_mass[i];
-                bc += s.wave_count[i];
-            }
-            tm += s.wave_mass[i];
-            tc += s.wave_count[i];
+        ir -= sum;
+        ic -= n;
+        for (int i = 0; i < tid / kWave; ++i) {
+            ir += s.wave_rel[i];
+            ic += s.wave_count[i];
         }
-        for (int i = 0; i < per; ++i) {
-            const uint64_t xm = mass[tid * per + i];
-            const uint32_t xc = count[tid * per + i];
-            mass[tid * per + i] = bm;
-            count[tid * per + i] = bc;
-            bm += xm;
-            bc += xc;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            s.sub.rel[kPer * tid + i] = ir;
+            s.sub.count[kPer * tid + i] = ic;
+            ir += r[i];
+            ic += c[i];
+        }
+        if (tid == kPickBlock - 1) {
+            s.sub.rel[kSub] = ir;
+            s.sub.count[kSub] = ic;
         }
         __syncthreads();
     }
 
-    // The last of n entries whose running sum before it has not reached the
-    // border: the one that crosses it.
-    __device__ static int crossing(const uint64_t* mass, const uint32_t* count, int n, Border kind,
-                                   uint64_t at) {
-        int lo = 0, hi = n - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            const uint64_t v = kind == kByCount ? count[mid] : mass[mid];
-            if (kind == kPast ? v <= at : v < at) lo = mid;
-            else hi = mid - 1;
+    // A border within bucket b: a number of tokens, or a sum of rels.
+    struct Need {
+        uint64_t base, mass, rels, at;
+        double per;
+    };
+    __device__ __forceinline__ Need need_of(Border kind, uint64_t at, int b) const {
+        Need x;
+        x.base = s.sums.mass[b];
+        x.mass = s.sums.mass[b + 1] - x.base;
+        x.rels = s.sums.rel[b];
+        x.per = (double)x.rels / (double)x.mass;
+        if (kind == kByCount) {
+            x.at = at - s.sums.count[b];
+        } else if (kind == kByMass) {
+            const uint64_t need = (uint64_t)ceil((double)(at - x.base) * x.per);
+            x.at = need < 1 ? 1 : need > x.rels ? x.rels : need;
+        } else {
+            const uint64_t need = (uint64_t)((double)(at - x.base) * x.per);
+            x.at = need >= x.rels ? x.rels - 1 : need;
         }
-        return lo;
+        return x;
+    }
+    // Whether a token with `r` rels and `c` tokens before it is the border's.
+    static __device__ __forceinline__ bool hits(Border kind, uint64_t at, uint64_t r, uint32_t c,
+                                                uint64_t rel) {
+        return kind == kByCount  ? c + 1 == at
+               : kind == kByMass ? r < at && at <= r + rel
+                                 : r <= at && at < r + rel;
+    }
+    static __device__ __forceinline__ uint64_t mass_at(const Need& x, uint64_t rel) {
+        const uint64_t part = (uint64_t)__builtin_rint((double)rel / x.per);
+        return x.base + (part < 1 ? 1 : part > x.mass ? x.mass : part);
     }
 
-    // The running sum up to and with the token at the border, and its index.
-    // `at` lies in the total of all buckets.
-    __device__ uint64_t find(Border kind, uint64_t at, int& index) {
+    // One wave, a token of the list for each lane: its rank in its bucket.
+    uint64_t my_key, my_rel, my_before;
+    uint32_t my_count;
+    int my_bucket;
+    __device__ void gather_wave() {
+        const int lane = threadIdx.x;
+        my_key = my_rel = my_before = 0;
+        my_count = 0;
+        my_bucket = -1;
+        if (lane < listed) {
+            my_key = s.key[lane];
+            my_rel = s.rel[lane] & ((1ull << 40) - 1);
+            my_bucket = (int)(s.rel[lane] >> 40);
+        }
+#pragma unroll 1
+        for (int j = 0; j < listed; ++j) {
+            const uint64_t rel = s.rel[j];
+            const bool ahead = (int)(rel >> 40) == my_bucket && s.key[j] < my_key;
+            my_before += ahead ? rel & ((1ull << 40) - 1) : 0;
+            my_count += ahead;
+        }
+    }
+    __device__ uint64_t find_wave(Border kind, uint64_t at, uint32_t& index) {
+        int b = 0;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < kBuckets; i += kWave) {
+            const uint64_t lanes = __builtin_amdgcn_ballot_w64(
+                kind == kByCount ? crosses(s.sums.count, i, kind, at)
+                                 : crosses(s.sums.mass, i, kind, at));
+            if (lanes == 0) continue;
+            b = __builtin_amdgcn_readfirstlane(i) + __ffsll((unsigned long long)lanes) - 1;
+            break;
+        }
+        const Need x = need_of(kind, at, b);
+        const uint64_t lanes = __builtin_amdgcn_ballot_w64(
+            my_bucket == b && hits(kind, x.at, my_before, my_count, my_rel));
+        const int lane = __ffsll((unsigned long long)lanes) - 1;
+        index = __shfl((uint32_t)my_key, lane);
+        return mass_at(x, __shfl((unsigned long long)(my_before + my_rel), lane));
+    }
+    __device__ uint64_t min_p_mass_wave(double m) {
+        const double border = min_p_border(scale, m);
+        const int b = min_p_bucket(scale, border);
+        if (b >= kBuckets) return s.sums.mass[kBuckets];
+        const float t = logit_of(my_key);
+        const bool in = my_bucket == b && (t == scale.top || (double)t * scale.inv_t >= border);
+        uint64_t sum = in ? my_rel : 0;
+        for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor((unsigned long long)sum, d);
+        return sum == 0 ? s.sums.mass[b] : mass_at(need_of(kByCount, 0, b), sum);
+    }
+
+    // The running mass up to and with the token at the border, and its index.
+    // `at` lies in the row's total.
+    __device__ uint64_t find(Border kind, uint64_t at, uint32_t& index) {
         const int tid = threadIdx.x;
-        const int b = crossing(s.mass, s.count, kBuckets, kind, at);
-        uint64_t base_mass = s.mass[b], lo = 0, hi = ~0ull;
-        uint32_t base_count = s.count[b];
-        while (true) {
-            // collect the bucket's tokens between two keys
+        if (tid < kBuckets && (kind == kByCount ? crosses(s.sums.count, tid, kind, at)
+                                                : crosses(s.sums.mass, tid, kind, at)))
+            s.entry = tid;
+        __syncthreads();
+        const int b = s.entry;
+        const Need x = need_of(kind, at, b);
+        uint64_t lo = 0, hi = ~0ull, before_rel = 0;
+        uint32_t before_count = 0, n = s.sums.count[b + 1] - s.sums.count[b];
+        while (n > kFew) {
+            // counts and sums of 2048 stretches of the keys between lo and hi, from
+            // the least to the most logit (or index, where all are equal)
             __syncthreads();
             if (tid == 0) {
-                s.listed = 0;
-                s.key_min = ~0ull;
-                s.key_max = 0;
+                s.bits_min = ~0u;
+                s.bits_max = 0;
             }
-            __syncthreads();
-            uint64_t mn = ~0ull, mx = 0;
-            each_token<DT>(a, row, [&](float x, int i) {
-                if (w.bucket_of(x) != b) return;
-                const uint64_t key = (uint64_t)order_bits(x) << 32 | (uint32_t)i;
-                if (key < lo || key > hi) return;
-                mn = min(mn, key);
-                mx = max(mx, key);
-                const uint32_t n = atomicAdd(&s.listed, 1u);
-                if (n < kBlock) s.list.key[n] = key;
-            });
-            if (mx >= mn) {
-                atomicMin((unsigned long long*)&s.key_min, (unsigned long long)mn);
-                atomicMax((unsigned long long*)&s.key_max, (unsigned long long)mx);
-            }
-            __syncthreads();
-            const uint32_t n = s.listed;
-            if (n <= kBlock) {
-                uint64_t key = 0, mass = 0;
-                if (tid < (int)n) {
-                    key = s.list.key[tid];
-                    mass = w.mass(logit_of((uint32_t)(key >> 32)));
-                    s.list.mass[tid] = mass;
-                }
-                __syncthreads();
-                if (tid < (int)n) {
-                    uint64_t before = base_mass;
-                    uint32_t rank = base_count;
-                    for (uint32_t j = 0; j < n; ++j) {
-                        if (s.list.key[j] < key) {
-                            before += s.list.mass[j];
-                            ++rank;
-                        }
-                    }
-                    const bool hit = kind == kByCount  ? rank + 1 == at
-                                     : kind == kByMass ? before < at && at <= before + mass
-                                                       : before <= at && at < before + mass;
-                    if (hit) {
-                        s.hit = (uint32_t)key;
-                        s.hit_mass = before + mass;
-                    }
-                }
-                __syncthreads();
-                index = (int)s.hit;
-                return s.hit_mass;
-            }
-            // too many: counts and masses of 2048 stretches of their keys
-            const uint64_t first = s.key_min, span = s.key_max - first;
-            int shift = 0;
-            while (span >> shift >= kSub) ++shift;
-            __syncthreads();
-            for (int i = tid; i < kSub; i += kBlock) {
-                s.sub.mass[i] = 0;
+            for (int i = tid; i < kSub; i += kPickBlock) {
+                s.sub.rel[i] = 0;
                 s.sub.count[i] = 0;
             }
             __syncthreads();
-            each_token<DT>(a, row, [&](float x, int i) {
-                if (w.bucket_of(x) != b) return;
-                const uint64_t key = (uint64_t)order_bits(x) << 32 | (uint32_t)i;
+            uint32_t mn = ~0u, mx = 0;
+            each(b, [&](uint64_t key, uint64_t) {
                 if (key < lo || key > hi) return;
-                const int at_sub = (int)((key - first) >> shift);
-                atomicAdd((unsigned long long*)&s.sub.mass[at_sub], (unsigned long long)w.mass(x));
-                atomicAdd(&s.sub.count[at_sub], 1u);
+                mn = min(mn, (uint32_t)(key >> 32));
+                mx = max(mx, (uint32_t)(key >> 32));
+            });
+            for (int d = 1; d < kWave; d *= 2) {
+                mn = min(mn, (uint32_t)__shfl_xor(mn, d));
+                mx = max(mx, (uint32_t)__shfl_xor(mx, d));
+            }
+            if (tid % kWave == 0) {
+                atomicMin(&s.bits_min, mn);
+                atomicMax(&s.bits_max, mx);
+            }
+            __syncthreads();
+            const uint64_t first = max((uint64_t)s.bits_min << 32, lo);
+            const uint64_t span = min(((uint64_t)s.bits_max << 32) + a.V - 1, hi) - first;
+            int shift = 0;
+            while (span >> shift >= kSub) ++shift;
+            each(b, [&](uint64_t key, uint64_t rel) {
+                if (key < lo || key > hi) return;
+                const int i = (int)((key - first) >> shift);
+                atomicAdd((unsigned long long*)&s.sub.rel[i], (unsigned long long)rel);
+                atomicAdd(&s.sub.count[i], 1u);
             });
             __syncthreads();
-            uint64_t tm;
-            uint32_t tc;
-            scan(s.sub.mass, s.sub.count, kSub, tm, tc);
-            const uint64_t rest = kind == kByCount ? at - base_count : at - base_mass;
-            const int at_sub = crossing(s.sub.mass, s.sub.count, kSub, kind, rest);
-            base_mass += s.sub.mass[at_sub];
-            base_count += s.sub.count[at_sub];
-            lo = first + ((uint64_t)at_sub << shift);
+            scan_sub();
+            const uint64_t rest = x.at - (kind == kByCount ? before_count : before_rel);
+            for (int j = tid; j < kSub; j += kPickBlock)
+                if (kind == kByCount ? crosses(s.sub.count, j, kind, rest)
+                                     : crosses(s.sub.rel, j, kind, rest))
+                    s.entry = j;
+            __syncthreads();
+            const int i = s.entry;
+            before_rel += s.sub.rel[i];
+            before_count += s.sub.count[i];
+            n = s.sub.count[i + 1] - s.sub.count[i];
+            lo = first + ((uint64_t)i << shift);
             hi = lo + ((1ull << shift) - 1);
         }
+        __syncthreads();
+        if (tid == 0) s.n = 0;
+        __syncthreads();
+        each(b, [&](uint64_t key, uint64_t rel) {
+            if (key < lo || key > hi) return;
+            const uint32_t i = atomicAdd(&s.n, 1u);
+            s.few.key[i] = key;
+            s.few.rel[i] = rel;
+        });
+        __syncthreads();
+        // each against the others, an eighth of them a thread
+        constexpr int kParts = kPickBlock / kFew;
+        const int mine = tid % kFew, part = tid / kFew;
+        const uint64_t key = mine < (int)n ? s.few.key[mine] : 0;
+        uint64_t r = 0;
+        uint32_t c = 0;
+        for (int j = part; j < (int)n; j += kParts) {
+            const bool ahead = s.few.key[j] < key;
+            r += ahead ? s.few.rel[j] : 0;
+            c += ahead;
+        }
+        s.few.before[part][mine] = r;
+        s.few.count[part][mine] = c;
+        __syncthreads();
+        if (tid < (int)n) {
+            const uint64_t rel = s.few.rel[tid];
+            r = before_rel;
+            c = before_count;
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                r += s.few.before[i][tid];
+                c += s.few.count[i][tid];
+            }
+            if (hits(kind, x.at, r, c, rel)) {
+                s.hit = (uint32_t)key;
+                s.hit_rel = r + rel;
+            }
+        }
+        __syncthreads();
+        index = s.hit;
+        return mass_at(x, s.hit_rel);
+    }
+
+    // The running mass of the tokens with w >= m.
+    __device__ uint64_t min_p_mass(double m) {
+        const double border = min_p_border(scale, m);
+        const int b = min_p_bucket(scale, border);
+        if (b >= kBuckets) return s.sums.mass[kBuckets];
+        __syncthreads();
+        if (threadIdx.x == 0) s.hit_rel = 0;
+        __syncthreads();
+        uint64_t sum = 0;
+        each(b, [&](uint64_t key, uint64_t rel) {
+            const float x = logit_of(key);
+            if (x == scale.top || (double)x * scale.inv_t >= border) sum += rel;
+        });
+        if (sum) atomicAdd((unsigned long long*)&s.hit_rel, (unsigned long long)sum);
+        __syncthreads();
+        return s.hit_rel == 0 ? s.sums.mass[b] : mass_at(need_of(kByCount, 0, b), s.hit_rel);
     }
 };
 
 template <int DT>
-__global__ void __launch_bounds__(kBlock) sample_kernel(SampleArgs a) {
-    __shared__ Shared s;
+__global__ void __launch_bounds__(kPickBlock) sample_pick_kernel(SampleArgs a) {
+    using P = Picker<DT>;
+    __shared__ typename P::Shared s;
     const int row = blockIdx.x, tid = threadIdx.x;
-    Sampler<DT> r{a, s, row, {}, 0, 0};
-
-    // the first token of the order
-    uint64_t best = ~0ull;
-    each_token<DT>(a, row, [&](float x, int i) {
-        best = min(best, (uint64_t)order_bits(x) << 32 | (uint32_t)i);
-    });
-    for (int d = 1; d < kWave; d *= 2) best = min(best, (uint64_t)__shfl_xor(best, d));
-    if (tid % kWave == 0) s.wave_mass[tid / kWave] = best;
-    for (int i = tid; i < kBuckets; i += kBlock) {
-        s.mass[i] = 0;
-        s.count[i] = 0;
-    }
-    __syncthreads();
-    for (int i = 0; i < kBlock / kWave; ++i) best = min(best, s.wave_mass[i]);
-    const float top = logit_of((uint32_t)(best >> 32));
-
-    const double t = a.t_row ? (double)a.t_row[row] : a.t;
-    const double p = a.p_row ? (double)a.p_row[row] : a.p;
-    const double m = a.m_row ? (double)a.m_row[row] : a.m;
-    const int k = a.k_row ? a.k_row[row] : a.k;
-    double u = a.u_f64 ? static_cast<const double*>(a.u)[row]
-                       : (double)static_cast<const float*>(a.u)[row];
-    u = u > 0.0 ? fmin(u, 1.0) : 0.0;          // (NaN: 0)
-
-    const bool none = top == -INFINITY;
-    if (none || !(t > 0.0) || k == 1 || p <= 0.0) {
+    const Settings set = settings_of(a, row);
+    const uint64_t best = first_of(a, row);
+    P p{a, s, row, {}, 0, 0, 0, 0, 0, 0};
+    p.scale.set(logit_of(best), set.t);
+    const bool none = p.scale.top == -INFINITY;
+    if (none || set.first) {
         if (tid == 0) a.out[row] = none ? -1 : (int64_t)(uint32_t)best;
         return;
     }
-    r.w.set(top, t);
-    __syncthreads();                           // (wave_mass was read)
-    each_token<DT>(a, row, [&](float x, int) {
-        const int b = r.w.bucket_of(x);
-        if (b >= kBuckets) return;
-        atomicAdd((unsigned long long*)&s.mass[b], (unsigned long long)r.w.mass(x));
-        atomicAdd(&s.count[b], 1u);
-    });
-    __syncthreads();
-    uint64_t kept;
-    uint32_t count;
-    r.scan(s.mass, s.count, kBuckets, kept, count);
-    int index = 0;
-    if (k > 0 && (uint32_t)k < count) kept = r.find(kByCount, (uint64_t)k, index);
-    if (p < 1.0) {
-        uint64_t want = (uint64_t)ceil(p * (double)kept);
-        want = want < 1 ? 1 : want > kept ? kept : want;
-        kept = r.find(kByMass, want, index);
+    p.collect(set);
+    uint64_t kept = s.sums.mass[kBuckets];
+    uint32_t index = 0;
+    // (few tokens: one wave, without barriers)
+    const bool alone = p.listed >= 0 && p.listed <= kWave;
+    if (alone) {
+        if (tid >= kWave) return;
+        p.gather_wave();
     }
-    if (m > 0.0) {
-        // the running sum of tokens with w >= min_p (the first one at least)
-        const double unit = (double)(1ull << kUnitBits);
-        uint64_t sum = 0;
-        __syncthreads();
-        if (tid == 0) s.hit_mass = 0;
-        __syncthreads();
-        each_token<DT>(a, row, [&](float x, int) {
-            const uint64_t mass = r.w.mass(x);
-            if ((double)mass >= m * unit) sum += mass;
-        });
-        for (int d = 1; d < kWave; d *= 2) sum += __shfl_xor(sum, d);
-        if (tid % kWave == 0) atomicAdd((unsigned long long*)&s.hit_mass, (unsigned long long)sum);
-        __syncthreads();
-        sum = s.hit_mass;
-        kept = min(kept, max(sum, (uint64_t)1 << kUnitBits));
+    // (one loop for the three borders: one copy of the search's code)
+#pragma unroll 1
+    for (int step = 0; step < 3; ++step) {
+        Border kind;
+        uint64_t at;
+        if (step == 0) {
+            if (set.k <= 0 || (uint32_t)set.k >= s.sums.count[kBuckets]) continue;
+            kind = kByCount;
+            at = (uint64_t)set.k;
+        } else if (step == 1) {
+            if (!(set.p < 1.0)) continue;
+            kind = kByMass;
+            at = mass_wanted(set.p, kept);
+        } else {
+            if (set.m > 0.0)
+                kept = max(min(kept, alone ? p.min_p_mass_wave(set.m) : p.min_p_mass(set.m)),
+                           (uint64_t)1);
+            kind = kPast;
+            at = mass_passed(set.u, kept);
+        }
+        kept = alone ? p.find_wave(kind, at, index) : p.find(kind, at, index);
     }
-    uint64_t past = (uint64_t)(u * (double)kept);
-    past = past >= kept ? kept - 1 : past;
-    r.find(kPast, past, index);
-    if (tid == 0) a.out[row] = index;
+    if (tid == 0) a.out[row] = (int64_t)index;
+}
+
+int64_t slices_of(int32_t vocab) { return ((int64_t)vocab + kSlice - 1) / kSlice; }
+
+template <int DT>
+void launch(const SampleArgs& a, int rows, hipStream_t s) {
+    sample_sums_kernel<DT><<<(unsigned)(rows * a.slices), kBlock, 0, s>>>(a);
+    sample_pick_kernel<DT><<<rows, kPickBlock, 0, s>>>(a);
 }
 
 }  // namespace
@@ -409,26 +983,41 @@ using namespace kivi;
 
 extern "C" {
 
+size_t kivi_sample_workspace_size(int32_t rows, int32_t vocab) {
+    if (rows < 1 || vocab < 1 || vocab > kMaxVocab) return 0;
+    return (size_t)(rows * slices_of(vocab)) * (8 * (kBuckets + 1) + 4 * kBlock);
+}
+
 int kivi_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows,
                 int32_t vocab, const void* uniforms, int32_t uniforms_f64,
                 const float* temperatures, double temperature, const int32_t* top_ks,
                 int32_t top_k, const float* top_ps, double top_p, const float* min_ps,
-                double min_p, int64_t* out, void* stream) {
+                double min_p, int64_t* out, void* workspace, size_t workspace_bytes,
+                void* stream) {
     if (dtype < 0 || dtype > 2)
         return set_error(kErrInvalidArgument, "dtype %d is not 0 (f32), 1 (bf16) or 2 (f16)", dtype);
     if (rows < 0 || vocab < 1 || vocab > kMaxVocab)
         return set_error(kErrInvalidArgument, "logits of %d rows and %d tokens (1 to %d)", rows,
                          vocab, kMaxVocab);
-    if (rows == 0) return kOk;
     if (row_stride < 0)
         return set_error(kErrInvalidArgument, "row_stride %lld must not be negative",
                          (long long)row_stride);
+    if (rows == 0) return kOk;
     if (logits == nullptr || uniforms == nullptr || out == nullptr)
         return set_error(kErrInvalidArgument, "null pointer");
+    const int64_t slices = slices_of(vocab);
+    if (rows * slices > INT32_MAX)
+        return set_error(kErrInvalidArgument, "%d rows of %d tokens are too many for one launch",
+                         rows, vocab);
+    const size_t need = kivi_sample_workspace_size(rows, vocab);
+    if (workspace == nullptr || ((uintptr_t)workspace & 15) || workspace_bytes < need)
+        return set_error(kErrInvalidArgument, "workspace must be 16-byte aligned and hold %zu "
+                         "bytes, got %zu", need, workspace_bytes);
     SampleArgs a{};
     a.logits = logits;
     a.stride = row_stride;
     a.V = vocab;
+    a.slices = (int)slices;
     a.u = uniforms;
     a.u_f64 = uniforms_f64 != 0;
     a.t_row = temperatures;
@@ -440,10 +1029,15 @@ int kivi_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t r
     a.p = top_p;
     a.m = min_p;
     a.out = out;
+    uint64_t* w = static_cast<uint64_t*>(workspace);
+    const int64_t n = rows * slices;
+    a.hist = w;
+    a.best = a.hist + n * kBuckets;
+    a.tops = reinterpret_cast<float*>(a.best + n);
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == kSrcF32) sample_kernel<kSrcF32><<<rows, kBlock, 0, s>>>(a);
-    else if (dtype == kSrcBF16) sample_kernel<kSrcBF16><<<rows, kBlock, 0, s>>>(a);
-    else sample_kernel<kSrcF16><<<rows, kBlock, 0, s>>>(a);
+    if (dtype == kSrcF32) launch<kSrcF32>(a, rows, s);
+    else if (dtype == kSrcBF16) launch<kSrcBF16>(a, rows, s);
+    else launch<kSrcF16>(a, rows, s);
     return check_launch("sample");
 }
 
