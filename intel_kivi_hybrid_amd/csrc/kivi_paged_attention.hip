@@ -139,7 +139,8 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
                              a.n_items);
         if (kind == kMany) launch_paged_many(a, dtype, s);
         else if (dtype == kSrcF32) launch_paged_f32(a, kind, s);
-        else launch_paged_few(a, dtype, kind, s);
+        else if (kind == kFew16) launch_paged_few(a, dtype, s);
+        else launch_paged_mid(a, dtype, kind, s);
         const int rc = check_launch("paged_attention");
         if (rc) return rc;
     }

@@ -182,9 +182,51 @@ __device__ __forceinline__ int odd_from(const Work& w, int all, int unit) {
 // 1 / sum; a row that saw nothing has sum 0 and comes out as zeros.
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
+// Four channels of row r of an item that is done: `o` of sum `sum` at maximum
+// `top`.  odd: some values of a step (of `unit` positions) that not all rows see
+// to its end were not finite.
+template <int DT>
+__device__ __forceinline__ void finish(const PagedLaunch& a, const Work& w, int r, int c,
+                                       f32x4_t o, float top, float sum, bool odd, int unit) {
+    if (w.it.part < 0) o *= inverse_sum(sum);
+    if (odd) {
+        const int all = w.it.ctx - w.it.n + w.it.row0 / w.hg + 1;
+        o += odd_values<DT>(a, w, odd_from(w, all, unit), row_limit(w, r), c);
+    }
+    if (w.it.part < 0) {
+        store4<DT>(a.out, out_offset(a, w, r) + c, o);
+    } else {
+        const int64_t at = part_row(a, w, r);
+        *reinterpret_cast<f32x4_t*>(a.part_o + at * a.D + c) = o;
+        if (c == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(top, sum);
+    }
+}
+
+// Joins four waves' results of ROWS rows (row i of wave j at jo(j) + i * stride, each
+// scaled to the largest of the waves' maxima) and finishes the rows from row0.
+template <int DT, int DP, int ROWS, class F>
+__device__ __forceinline__ void join_waves(const PagedLaunch& a, const Work& w, int row0, F jo,
+                                           int stride, const float (*m)[ROWS],
+                                           const float (*l)[ROWS], const int* odd, int unit) {
+    for (int at = threadIdx.x; at < ROWS * (DP / 4); at += 4 * kWave) {
+        const int row = at / (DP / 4), c = at % (DP / 4) * 4, r = row0 + row;
+        if (r >= w.rows || c >= a.D) continue;
+        const float top = fmaxf(fmaxf(m[0][row], m[1][row]), fmaxf(m[2][row], m[3][row]));
+        f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o += *reinterpret_cast<const f32x4_t*>(jo(i) + row * stride + c);
+            sum += l[i][row] * exp2_fast(m[i][row] - top);
+        }
+        finish<DT>(a, w, r, c, o, top, sum, (odd[0] | odd[1] | odd[2] | odd[3]) != 0, unit);
+    }
+}
+
 }  // namespace
 
-void launch_paged_few(const PagedLaunch& a, int dtype, int kind, hipStream_t s);
+void launch_paged_few(const PagedLaunch& a, int dtype, hipStream_t s);
+void launch_paged_mid(const PagedLaunch& a, int dtype, int kind, hipStream_t s);
 void launch_paged_f32(const PagedLaunch& a, int kind, hipStream_t s);
 void launch_paged_many(const PagedLaunch& a, int dtype, hipStream_t s);
 

@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kBlock) paged_f32_kernel(PagedLaunch a) {
     constexpr int KK = DP / 16, CG = DP / 64;
     constexpr int OS = DP + 4;             // joining rows, padded by one vector
     __shared__ __align__(16) float jo[kWaves * 16 * OS];
-    __shared__ float join_m[kWaves][RT * 16], join_l[kWaves][RT * 16];
+    __shared__ float join_m[kWaves][16], join_l[kWaves][16];
     __shared__ int join_odd[kWaves];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, col = lane % 16, gq = lane / 16;
@@ -184,25 +184,19 @@ __global__ void __launch_bounds__(kBlock) paged_f32_kernel(PagedLaunch a) {
     }
 
     // Join the waves: a row's largest maximum, then the rescaled sums.
-    if (lane == 0) join_odd[wave] = 0;
-    if (__builtin_amdgcn_ballot_w64(odd) != 0 && lane == 0) join_odd[wave] = 1;
+    const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+    if (lane == 0) join_odd[wave] = any_odd;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         l[rt] += __shfl_xor(l[rt], 16);
         l[rt] += __shfl_xor(l[rt], 32);
         if (gq == 0) {
-            join_m[wave][16 * rt + col] = m[rt];
-            join_l[wave][16 * rt + col] = l[rt];
+            join_m[wave][col] = m[rt];
+            join_l[wave][col] = l[rt];
         }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int jr = 16 * rt + col;
-        const float top = fmaxf(fmaxf(join_m[0][jr], join_m[1][jr]),
-                                fmaxf(join_m[2][jr], join_m[3][jr]));
-        const float f = exp2_fast(m[rt] - top);
-        if (rt > 0) __syncthreads();
+        __syncthreads();
+        const float f = exp2_fast(m[rt] - fmaxf(fmaxf(join_m[0][col], join_m[1][col]),
+                                                fmaxf(join_m[2][col], join_m[3][col])));
 #pragma unroll
         for (int cg = 0; cg < CG; ++cg) {
 #pragma unroll
@@ -212,30 +206,10 @@ __global__ void __launch_bounds__(kBlock) paged_f32_kernel(PagedLaunch a) {
                     f32x4_t{O[rt][cg][0][r], O[rt][cg][1][r], O[rt][cg][2][r], O[rt][cg][3][r]} * f;
         }
         __syncthreads();
-        for (int at = threadIdx.x; at < 16 * (DP / 4); at += kBlock) {
-            const int row = at / (DP / 4), c = at % (DP / 4) * 4;
-            const int r = w.it.row0 + 16 * rt + row;
-            if (r >= w.rows || c >= a.D) continue;
-            f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-            float sum = 0.f, mt = -FLT_MAX;
-#pragma unroll
-            for (int i = 0; i < kWaves; ++i) mt = fmaxf(mt, join_m[i][16 * rt + row]);
-#pragma unroll
-            for (int i = 0; i < kWaves; ++i) {
-                o += *reinterpret_cast<const f32x4_t*>(jo + (i * 16 + row) * OS + c);
-                sum += join_l[i][16 * rt + row] * exp2_fast(join_m[i][16 * rt + row] - mt);
-            }
-            if (w.it.part < 0) o *= inverse_sum(sum);
-            if (join_odd[0] | join_odd[1] | join_odd[2] | join_odd[3])
-                o += odd_values<kSrcF32>(a, w, odd_from(w, all_see, kUnit), row_limit(w, r), c);
-            if (w.it.part < 0) {
-                store4<kSrcF32>(a.out, out_offset(a, w, r) + c, o);
-            } else {
-                const int64_t pr = part_row(a, w, r);
-                *reinterpret_cast<f32x4_t*>(a.part_o + pr * a.D + c) = o;
-                if (c == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = make_float2(mt, sum);
-            }
-        }
+        join_waves<kSrcF32, DP, 16>(a, w, w.it.row0 + 16 * rt,
+                                    [&](int i) { return jo + i * 16 * OS; }, OS, join_m, join_l,
+                                    join_odd, kUnit);
+        __syncthreads();
     }
 }
 
@@ -245,10 +219,8 @@ void launch_rows(const PagedLaunch& a, int kind, hipStream_t s) {
     // (paged_few_rows(): the kinds that a head_dim comes with)
     if (kind == kFew16) {
         paged_f32_kernel<DP, 1><<<grid, kBlock, 0, s>>>(a);
-    } else if (kind == kFew32) {
-        if constexpr (DP <= 128) paged_f32_kernel<DP, 2><<<grid, kBlock, 0, s>>>(a);
     } else {
-        if constexpr (DP <= 64) paged_f32_kernel<DP, 4><<<grid, kBlock, 0, s>>>(a);
+        if constexpr (DP <= 128) paged_f32_kernel<DP, 2><<<grid, kBlock, 0, s>>>(a);
     }
 }
 

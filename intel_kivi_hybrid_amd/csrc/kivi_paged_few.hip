@@ -1,5 +1,5 @@
-// Attention over a paged cache for up to 64 query rows per kv head, 16-bit
-// types (gfx950 matrix cores): single tokens, verification passes.
+// Attention over a paged cache for up to 16 query rows per kv head, 16-bit
+// types (gfx950 matrix cores): single tokens.
 //
 // Such calls read every key and value once for a few products: memory-bound.
 // A workgroup's four waves walk the item's positions in units of 32, each wave
@@ -7,7 +7,9 @@
 // in flight while it computes.  Keys go from memory into the A operand of
 // v_mfma_f32_16x16x32 as they lie (a lane takes 8 channels of one token); values
 // need the token as the inner index and pass through the wave's own LDS, from
-// which they are read transposed.  The waves' results are joined in LDS at the
+// which they are read transposed.  The products cost nothing beside the loads, so
+// the weights enter as two pieces (rounded, and what that left out): their
+// rounding then does not show.  The waves' results are joined in LDS at the
 // end; splits of a context are joined by a second launch.
 #include <hip/hip_runtime.h>
 
@@ -20,7 +22,7 @@ constexpr int kWaves = 4;
 constexpr int kBlock = kWaves * kWave;
 constexpr int kUnit = 32;
 
-template <int DT, int DP, int RT>
+template <int DP>
 struct Few {
     static constexpr int KS = DP / 32;            // k-steps of a score
     static constexpr int CB = DP / 16;            // blocks of 16 output channels
@@ -36,39 +38,36 @@ struct Few {
     static constexpr int LDS = kWaves * V_BYTES > JOIN_BYTES ? kWaves * V_BYTES : JOIN_BYTES;
 };
 
-template <int DT, int DP, int RT>
+template <int DT, int DP>
 __global__ void __launch_bounds__(kBlock) paged_few_kernel(PagedLaunch a) {
-    using F = Few<DT, DP, RT>;
+    using F = Few<DP>;
     __shared__ __align__(16) unsigned char lds[F::LDS];
-    __shared__ float join_m[kWaves][RT * 16], join_l[kWaves][RT * 16];
+    __shared__ float join_m[kWaves][16], join_l[kWaves][16];
     __shared__ int join_odd[kWaves];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     const int col = lane % 16, gq = lane / 16;
     const Work w = work_of(a);
     unsigned char* vl = lds + wave * F::V_BYTES;
 
-    u32x4_t qf[RT][F::KS];
-    int lim[RT];
-    float m[RT], l[RT];
-    f32x4_t O[RT][F::CB];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int r = w.it.row0 + 16 * rt + col;
+    u32x4_t qf[F::KS];
+    f32x4_t O[F::CB];
+    float m = -FLT_MAX, l = 0.f;
+    int lim = 0;
+    {
+        const int r = w.it.row0 + col;
         const bool live = r < w.rows;
-        lim[rt] = live ? row_limit(w, r) : 0;
-        m[rt] = -FLT_MAX;
-        l[rt] = 0.f;
+        if (live) lim = row_limit(w, r);
         const uint16_t* q = static_cast<const uint16_t*>(a.q) + (live ? q_offset(a, w, r) : 0);
 #pragma unroll
         for (int ks = 0; ks < F::KS; ++ks) {
             const int c = 32 * ks + 8 * gq;
-            qf[rt][ks] = u32x4_t{0, 0, 0, 0};
-            if (live && c < a.D) qf[rt][ks] = *reinterpret_cast<const u32x4_t*>(q + c);
+            qf[ks] = u32x4_t{0, 0, 0, 0};
+            if (live && c < a.D) qf[ks] = *reinterpret_cast<const u32x4_t*>(q + c);
         }
-#pragma unroll
-        for (int cb = 0; cb < F::CB; ++cb) O[rt][cb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-    // positions that every row sees, and whether some row is short of the end
+#pragma unroll
+    for (int cb = 0; cb < F::CB; ++cb) O[cb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    // positions that every row sees
     const int all_see = w.it.ctx - w.it.n + w.it.row0 / w.hg + 1;
     const int end = w.it.kv_end;
 
@@ -129,16 +128,12 @@ __global__ void __launch_bounds__(kBlock) paged_few_kernel(PagedLaunch a) {
     }
     for (; t0 < end; t0 += kWaves * kUnit) {
         const int next = t0 + kWaves * kUnit;
-        f32x4_t s[RT][2];
+        f32x4_t s[2];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
+        for (int tb = 0; tb < 2; ++tb) {
+            s[tb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int tb = 0; tb < 2; ++tb) {
-                s[rt][tb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int ks = 0; ks < F::KS; ++ks)
-                    s[rt][tb] = mfma16<DT>(kf[tb][ks], qf[rt][ks], s[rt][tb]);
-            }
+            for (int ks = 0; ks < F::KS; ++ks) s[tb] = mfma16<DT>(kf[tb][ks], qf[ks], s[tb]);
         }
         const Pages pg = ahead;
         if (next < end) {
@@ -165,35 +160,34 @@ __global__ void __launch_bounds__(kBlock) paged_few_kernel(PagedLaunch a) {
         }
         if (next < end) load_v(next, pg);
 
-        u32x4_t pf[RT];
+        float x[8];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float x[8];
+        for (int i = 0; i < 8; ++i) {
+            x[i] = s[i / 4][i % 4];
+            if (masked && t0 + 16 * (i / 4) + 4 * gq + i % 4 >= lim) x[i] = -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                         fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        mx *= a.qscale;
+        if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax) != 0) {
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float to = fmaxf(m, mx), f = exp2_fast(m - to);
+            m = to;
+            l *= f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = s[rt][i / 4][i % 4];
-                if (masked && t0 + 16 * (i / 4) + 4 * gq + i % 4 >= lim[rt]) x[i] = -INFINITY;
-            }
-            float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                             fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            mx *= a.qscale;
-            if (__builtin_amdgcn_ballot_w64(mx > m[rt] + kMoveMax) != 0) {
-                mx = fmaxf(mx, __shfl_xor(mx, 16));
-                mx = fmaxf(mx, __shfl_xor(mx, 32));
-                const float to = fmaxf(m[rt], mx), f = exp2_fast(m[rt] - to);
-                m[rt] = to;
-                l[rt] *= f;
+            for (int cb = 0; cb < F::CB; ++cb) O[cb] *= f;
+        }
 #pragma unroll
-                for (int cb = 0; cb < F::CB; ++cb) O[rt][cb] *= f;
-            }
-            float p[8];
+        for (int i = 0; i < 8; ++i) {
+            x[i] = exp2_fast(fmaf(x[i], a.qscale, -m));
+            l += x[i];
+        }
+        u32x4_t hi, lo;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                p[i] = exp2_fast(fmaf(x[i], a.qscale, -m[rt]));
-                l[rt] += p[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) pf[rt][i] = pack2<DT>(p[2 * i], p[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) {
+            hi[i] = pack2<DT>(x[2 * i], x[2 * i + 1]);
+            lo[i] = pack2<DT>(x[2 * i] - half_of<DT>(hi[i], 0), x[2 * i + 1] - half_of<DT>(hi[i], 1));
         }
         wave_sync();
         // rows of a transposed read: tokens 4 gq .. + 3, and 16 further on, in the
@@ -201,93 +195,49 @@ __global__ void __launch_bounds__(kBlock) paged_few_kernel(PagedLaunch a) {
         const unsigned char* vr = vl + (4 * gq + col / 4) * F::VS + col % 4 * 8;
 #pragma unroll
         for (int cb = 0; cb < F::CB; ++cb) {
-            const uint2 lo = read_transposed(vr + cb * 32);
-            const uint2 hi = read_transposed(vr + 16 * F::VS + cb * 32);
-            const u32x4_t vt = {lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) O[rt][cb] = mfma16<DT>(vt, pf[rt], O[rt][cb]);
+            const uint2 v0 = read_transposed(vr + cb * 32);
+            const uint2 v1 = read_transposed(vr + 16 * F::VS + cb * 32);
+            const u32x4_t vt = {v0.x, v0.y, v1.x, v1.y};
+            O[cb] = mfma16<DT>(vt, lo, O[cb]);
+            O[cb] = mfma16<DT>(vt, hi, O[cb]);
         }
     }
 
     // Join the waves: a row's largest maximum, then the rescaled sums.
-    if (lane == 0) join_odd[wave] = 0;
-    if (__builtin_amdgcn_ballot_w64(odd) != 0 && lane == 0) join_odd[wave] = 1;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        l[rt] += __shfl_xor(l[rt], 16);
-        l[rt] += __shfl_xor(l[rt], 32);
-        if (gq == 0) {
-            join_m[wave][16 * rt + col] = m[rt];
-            join_l[wave][16 * rt + col] = l[rt];
-        }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (gq == 0) {
+        join_m[wave][col] = m;
+        join_l[wave][col] = l;
     }
+    const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
+    if (lane == 0) join_odd[wave] = any_odd;
     __syncthreads();
     float* jo = reinterpret_cast<float*>(lds);
+    const float f = exp2_fast(m - fmaxf(fmaxf(join_m[0][col], join_m[1][col]),
+                                        fmaxf(join_m[2][col], join_m[3][col])));
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int jr = 16 * rt + col;
-        const float top = fmaxf(fmaxf(join_m[0][jr], join_m[1][jr]),
-                                fmaxf(join_m[2][jr], join_m[3][jr]));
-        const float f = exp2_fast(m[rt] - top);
-        if (rt > 0) __syncthreads();
-#pragma unroll
-        for (int cb = 0; cb < F::CB; ++cb)
-            *reinterpret_cast<f32x4_t*>(jo + (wave * 16 + col) * F::OS + 16 * cb + 4 * gq) =
-                O[rt][cb] * f;
-        __syncthreads();
-        for (int at = threadIdx.x; at < 16 * (DP / 4); at += kBlock) {
-            const int row = at / (DP / 4), c = at % (DP / 4) * 4;
-            const int r = w.it.row0 + 16 * rt + row;
-            if (r >= w.rows || c >= a.D) continue;
-            f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-            float sum = 0.f, mt = -FLT_MAX;
-#pragma unroll
-            for (int i = 0; i < kWaves; ++i) mt = fmaxf(mt, join_m[i][16 * rt + row]);
-#pragma unroll
-            for (int i = 0; i < kWaves; ++i) {
-                o += *reinterpret_cast<const f32x4_t*>(jo + (i * 16 + row) * F::OS + c);
-                sum += join_l[i][16 * rt + row] * exp2_fast(join_m[i][16 * rt + row] - mt);
-            }
-            if (w.it.part < 0) o *= inverse_sum(sum);
-            if (join_odd[0] | join_odd[1] | join_odd[2] | join_odd[3])
-                o += odd_values<DT>(a, w, odd_from(w, all_see, kUnit), row_limit(w, r), c);
-            if (w.it.part < 0) {
-                store4<DT>(a.out, out_offset(a, w, r) + c, o);
-            } else {
-                const int64_t pr = part_row(a, w, r);
-                *reinterpret_cast<f32x4_t*>(a.part_o + pr * a.D + c) = o;
-                if (c == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = make_float2(mt, sum);
-            }
-        }
-    }
-}
-
-template <int DT, int DP>
-void launch_rows(const PagedLaunch& a, int kind, hipStream_t s) {
-    const dim3 grid((unsigned)(a.n_items * a.Hkv));
-    // (paged_few_rows(): the kinds that a head_dim comes with)
-    if (kind == kFew16) {
-        paged_few_kernel<DT, DP, 1><<<grid, kBlock, 0, s>>>(a);
-    } else if (kind == kFew32) {
-        if constexpr (DP <= 128) paged_few_kernel<DT, DP, 2><<<grid, kBlock, 0, s>>>(a);
-    } else {
-        if constexpr (DP <= 128) paged_few_kernel<DT, DP, 4><<<grid, kBlock, 0, s>>>(a);
-    }
+    for (int cb = 0; cb < F::CB; ++cb)
+        *reinterpret_cast<f32x4_t*>(jo + (wave * 16 + col) * F::OS + 16 * cb + 4 * gq) = O[cb] * f;
+    __syncthreads();
+    join_waves<DT, DP, 16>(a, w, w.it.row0, [&](int i) { return jo + i * 16 * F::OS; }, F::OS,
+                           join_m, join_l, join_odd, kUnit);
 }
 
 template <int DT>
-void launch_dim(const PagedLaunch& a, int kind, hipStream_t s) {
-    if (a.D <= 64) launch_rows<DT, 64>(a, kind, s);
-    else if (a.D <= 96) launch_rows<DT, 96>(a, kind, s);
-    else if (a.D <= 128) launch_rows<DT, 128>(a, kind, s);
-    else launch_rows<DT, 256>(a, kind, s);
+void launch_dim(const PagedLaunch& a, hipStream_t s) {
+    const dim3 grid((unsigned)(a.n_items * a.Hkv));
+    if (a.D <= 64) paged_few_kernel<DT, 64><<<grid, kBlock, 0, s>>>(a);
+    else if (a.D <= 96) paged_few_kernel<DT, 96><<<grid, kBlock, 0, s>>>(a);
+    else if (a.D <= 128) paged_few_kernel<DT, 128><<<grid, kBlock, 0, s>>>(a);
+    else paged_few_kernel<DT, 256><<<grid, kBlock, 0, s>>>(a);
 }
 
 }  // namespace
 
-void launch_paged_few(const PagedLaunch& a, int dtype, int kind, hipStream_t s) {
-    if (dtype == kSrcBF16) launch_dim<kSrcBF16>(a, kind, s);
-    else launch_dim<kSrcF16>(a, kind, s);
+void launch_paged_few(const PagedLaunch& a, int dtype, hipStream_t s) {
+    if (dtype == kSrcBF16) launch_dim<kSrcBF16>(a, s);
+    else launch_dim<kSrcF16>(a, s);
 }
 
 }  // namespace kivi

@@ -1,0 +1,237 @@
+// Tiles of keys and values in LDS and the products of 32 query rows with them
+// (16-bit types), for the kernels that load their tiles straight into LDS.
+//
+// Such a load (64 lanes of 16 bytes) fills 1024 consecutive bytes, so token rows
+// lie unpadded there, and the vectors of a token are permuted instead, by the
+// address that each lane loads from.
+#pragma once
+
+#include "kivi_paged_attention.hpp"
+
+namespace kivi {
+namespace {
+
+template <int DP, int TOKENS>
+struct TileShape {
+    static constexpr int TILE = TOKENS, TB = TILE / 32;
+    static constexpr int KS = DP / 16;                 // k-steps of a score
+    static constexpr int CB = DP / 32;                 // blocks of 32 output channels
+    // slots of 16 bytes of a token's row in LDS (DP 96: the last four unused)
+    static constexpr int SL = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;
+    static constexpr int ROW = SL * 16;
+    static constexpr int BYTES = TILE * ROW;           // of a tile's keys
+    static constexpr int ROWS = kWave / SL;            // tokens of a load
+
+    // Slot c ^ swizzle(t) holds vector c of token t.  The 16 tokens of a
+    // half-wave's key reads then start on 16 different bank groups, and the 8
+    // tokens of a transposed read (64 bytes each) meet each bank twice.
+    static __device__ __forceinline__ int key_swizzle(int t) {
+        return SL == 8 ? t / 2 % 8 : t % 16;
+    }
+    static __device__ __forceinline__ int value_swizzle(int t) {
+        return SL == 8 ? t / 2 % 2 * 4 : t % 4 * 4;
+    }
+};
+
+// 64 lanes' 16 bytes from memory to 1024 consecutive bytes of LDS.
+__device__ __forceinline__ void load_lds(const uint16_t* base, uint32_t off, unsigned char* lds) {
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void*)(base + off),
+        (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+// All of the wave's loads have arrived.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
+// A wave's 32 query rows (lane: row lane % 32) and their softmax state.
+// Q_LDS: the queries lie in LDS (q_lds, a vector for each k-step and lane), where
+// registers are short.
+template <int DT, int DP, int TOKENS, bool Q_LDS = false>
+struct TileRows {
+    using M = TileShape<DP, TOKENS>;
+    u32x4_t qf[Q_LDS ? 1 : M::KS];
+    const u32x4_t* ql;
+    f32x16_t O[M::CB];
+    float m, l;
+    int lim;                 // positions that the lane's row sees
+    int all, last;           // that all, and any, of the 32 rows see
+
+    // rows row0 .. row0 + 31 of the item's sequence
+    __device__ __forceinline__ void init(const PagedLaunch& a, const Work& w, int row0,
+                                         u32x4_t* q_lds = nullptr) {
+        const int lane = threadIdx.x % kWave, half = lane / 32, r = row0 + lane % 32;
+        const bool live = r < w.rows;
+        lim = live ? row_limit(w, r) : 0;
+        m = -FLT_MAX;
+        l = 0.f;
+        const uint16_t* q = static_cast<const uint16_t*>(a.q) + (live ? q_offset(a, w, r) : 0);
+#pragma unroll
+        for (int ks = 0; ks < M::KS; ++ks) {
+            const int c = 16 * ks + 8 * half;
+            u32x4_t x = {0, 0, 0, 0};
+            if (live && c < a.D) x = *reinterpret_cast<const u32x4_t*>(q + c);
+            if constexpr (Q_LDS) q_lds[ks * kWave + lane] = x;
+            else qf[ks] = x;
+        }
+        ql = q_lds + lane;
+#pragma unroll
+        for (int cb = 0; cb < M::CB; ++cb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) O[cb][i] = 0.f;
+        }
+        const int base = w.it.ctx - w.it.n + 1;
+        all = base + row0 / w.hg;
+        last = row0 < w.rows ? min(base + min(row0 + 31, w.rows - 1) / w.hg, w.it.kv_end) : 0;
+    }
+
+    // A tile of keys (kb) and values (vb) in LDS, positions t0 ..
+    __device__ __forceinline__ void tile(const unsigned char* kb, const unsigned char* vb,
+                                         int t0, int end, float qscale) {
+        const int lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
+        f32x16_t s[M::TB];
+#pragma unroll
+        for (int tb = 0; tb < M::TB; ++tb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[tb][i] = 0.f;
+        }
+        const uint32_t krow = col * M::ROW + ((half ^ M::key_swizzle(col)) << 4);
+#pragma unroll
+        for (int ks = 0; ks < M::KS; ++ks) {
+            u32x4_t q;
+            if constexpr (Q_LDS) q = ql[ks * kWave];
+            else q = qf[ks];
+#pragma unroll
+            for (int tb = 0; tb < M::TB; ++tb) {
+                const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(
+                    kb + (krow ^ (32 * ks)) + 32 * tb * M::ROW);
+                s[tb] = mfma32<DT>(kf, q, s[tb]);
+            }
+        }
+        // score i of block tb: token 32 tb + 8 (i / 4) + 4 half + i % 4
+        if (t0 + M::TILE > min(all, end)) {
+#pragma unroll
+            for (int tb = 0; tb < M::TB; ++tb) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (t0 + 32 * tb + 8 * (i / 4) + 4 * half + i % 4 >= lim)
+                        s[tb][i] = -INFINITY;
+            }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int tb = 0; tb < M::TB; ++tb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tb][i]);
+        }
+        mx *= qscale;
+        if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax) != 0) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float to = fmaxf(m, mx), f = exp2_fast(m - to);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int cb = 0; cb < M::CB; ++cb) O[cb] *= f;
+        }
+        u32x4_t pf[2 * M::TB];        // weights of tokens 16 j .. + 15
+#pragma unroll
+        for (int tb = 0; tb < M::TB; ++tb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[tb][i] = exp2_fast(fmaf(s[tb][i], qscale, -m));
+                l += s[tb][i];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                pf[2 * tb + i / 4][i % 4] = pack2<DT>(s[tb][2 * i], s[tb][2 * i + 1]);
+        }
+        // transposed: lanes of 16 take tokens 4 half .. + 3 of 16 channels
+        const int t = 4 * half + lane % 16 / 4;
+        const int c = lane / 16 % 2 * 2 + lane % 4 / 2;
+        const uint32_t vrow = t * M::ROW + ((c ^ M::value_swizzle(t)) << 4) + lane % 2 * 8;
+#pragma unroll
+        for (int j = 0; j < 2 * M::TB; ++j) {
+#pragma unroll
+            for (int cb = 0; cb < M::CB; ++cb) {
+                const unsigned char* p = vb + (vrow ^ (64 * cb)) + 16 * j * M::ROW;
+                const uint2 lo = read_transposed(p);
+                const uint2 hi = read_transposed(p + 8 * M::ROW);
+                O[cb] = mfma32<DT>(u32x4_t{lo.x, lo.y, hi.x, hi.y}, pf[j], O[cb]);
+            }
+        }
+    }
+};
+
+// How a workgroup's or wave's lanes load a tile: load i of GROUP waves covers
+// ROWS tokens of one block of 16 positions, whose page is the same for the whole
+// wave; a lane's place in the block is the same for every tile.
+template <int DP, int TOKENS, int GROUP>
+struct TileLoads {
+    using M = TileShape<DP, TOKENS>;
+    static constexpr int LD = TOKENS / M::ROWS / GROUP;     // loads of a wave for a tile's keys
+    int wave;                                               // within the group
+    int page[LD];
+
+    __device__ __forceinline__ int block_of(int i) const {
+        return (i * GROUP + wave) * M::ROWS / 16 * 16;
+    }
+    // the token (of its block) and channel that the lane loads
+    __device__ __forceinline__ int token(int i) const {
+        return ((i * GROUP + wave) * M::ROWS + threadIdx.x % kWave / M::SL) % 16;
+    }
+    __device__ __forceinline__ int channel(int i, bool key) const {
+        const int t = token(i), slot = threadIdx.x % kWave % M::SL;
+        return (slot ^ (key ? M::key_swizzle(t) : M::value_swizzle(t))) * 8;
+    }
+    __device__ __forceinline__ void pages_of(const PagedLaunch& a, const Work& w, int t0) {
+#pragma unroll
+        for (int i = 0; i < LD; ++i) page[i] = block_page(a, w, t0 + block_of(i));
+    }
+    // Loads the tile at t0 (whose pages are known), then its successor's pages.
+    __device__ __forceinline__ void issue(const PagedLaunch& a, const Work& w, unsigned char* buf,
+                                          int t0, int next) {
+        const bool full = a.D == M::SL * 8;
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int t = t0 + block_of(i);
+            const uint16_t* k = block_at<uint16_t>(a, w, a.k_pages, page[i], t);
+            const uint16_t* v = block_at<uint16_t>(a, w, a.v_pages, page[i], t);
+            unsigned char* to = buf + (i * GROUP + wave) * 1024;
+            const int row = token(i) * a.D, kc = channel(i, true), vc = channel(i, false);
+            if (full) {
+                load_lds(k, row + kc, to);
+                load_lds(v, row + vc, to + M::BYTES);
+            } else {
+                if (kc < a.D) load_lds(k, row + kc, to);
+                if (vc < a.D) load_lds(v, row + vc, to + M::BYTES);
+            }
+        }
+        pages_of(a, w, next);
+    }
+    // The lane's own part of a tile that has arrived and that some row does not see
+    // to its end: zeros behind the end (weight 0 of whatever lies there) and for
+    // non-finite values.  Whether there was one of the latter.
+    template <int DT>
+    __device__ __forceinline__ bool mend(unsigned char* buf, int t0, int end) const {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            u32x4_t* v = reinterpret_cast<u32x4_t*>(buf + M::BYTES + (i * GROUP + wave) * 1024 +
+                                                    threadIdx.x % kWave * 16);
+            u32x4_t x = *v;
+            if (t0 + block_of(i) + token(i) >= end) {
+                x = u32x4_t{0, 0, 0, 0};
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t y = finite_part<DT>(x[j]);
+                    any |= y != x[j];
+                    x[j] = y;
+                }
+            }
+            *v = x;
+        }
+        return any;
+    }
+};
+
+}  // namespace
+}  // namespace kivi
