@@ -352,19 +352,18 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
                                  runs[i].page);
 
         // Row tiles, and the positions that the last row of each sees.  The
-        // sequences of few rows take one kind, the largest that one of them needs:
-        // one launch then streams all their pages.
-        const int few = paged_few_rows(f32, head_dim);
-        int64_t few_rows = 0;
+        // 16-bit sequences of up to 64 rows take one kind, the larger that one of
+        // them needs: one launch then streams all their pages.
+        int few = kFew16;
         for (int s = 0; s < n_seqs; ++s) {
-            const int64_t rows = (int64_t)new_lens[s] * hg;
-            if (rows <= few) few_rows = std::max(few_rows, rows);
+            const int kind = paged_kind((int64_t)new_lens[s] * hg, f32, head_dim);
+            if (kind == kFew64) few = kFew64;
         }
         std::vector<Tile> tiles[kPagedKinds];
         for (int s = 0; s < n_seqs; ++s) {
             const int64_t n = new_lens[s], rows = n * hg;
             if (n == 0) continue;
-            const int kind = paged_kind(rows <= few ? few_rows : rows, f32, head_dim);
+            const int kind = std::max(few, paged_kind(rows, f32, head_dim));
             const int step = paged_tile_rows(kind);
             for (int64_t r = 0; r < rows; r += step) {
                 const int64_t last = std::min(rows, r + step) - 1;

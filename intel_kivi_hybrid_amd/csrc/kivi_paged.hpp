@@ -46,31 +46,24 @@ static_assert(sizeof(PagedItem) == 32 && sizeof(PagedMerge) == 32, "plan records
 // Kinds of attention items, by the rows of a tile: a kind is one launch.
 enum PagedKind : int { kFew16 = 0, kFew32 = 1, kFew64 = 2, kMany = 3, kPagedKinds = 4 };
 
-constexpr int kManyRows = 128;
-constexpr int paged_tile_rows(int kind) {
-    return kind == kFew16 ? 16 : kind == kFew32 ? 32 : kind == kFew64 ? 64 : kManyRows;
-}
-// The most rows of a kv head that a few-row kernel holds: their queries and
-// outputs, with a unit's keys and values, fill a wave's registers.
-constexpr int paged_few_rows(bool f32, int head_dim) {
-    if (f32) return head_dim <= 128 ? 32 : 16;
-    return head_dim <= 128 ? 64 : 16;
-}
-// The kind that takes `rows` rows.  fp32 has no kMany kernel: its products run at
-// a sixteenth of the 16-bit rate, so sharing tiles through LDS gains nothing
-// there.
+constexpr int paged_tile_rows(int kind) { return kind == kMany ? 128 : 16 << kind; }
+
+// The kind that takes `rows` rows of a kv head.  fp32 has a kernel of 16 rows and
+// one of 32 (whose outputs no longer fit the registers above 128 channels), more
+// rows in tiles of these; the 16-bit types one of 16, one of 64 (four buffers of
+// tiles fit the LDS up to 128 channels) and one for many.
 constexpr int paged_kind(int64_t rows, bool f32, int head_dim) {
-    const int few = paged_few_rows(f32, head_dim);
-    if (rows > few && !f32) return kMany;
-    const int64_t tile = rows < few ? rows : few;
-    return tile <= 16 ? kFew16 : tile <= 32 ? kFew32 : kFew64;
+    if (rows <= 16) return kFew16;
+    if (f32) return head_dim <= 128 ? kFew32 : kFew16;
+    return rows <= 64 && head_dim <= 128 ? kFew64 : kMany;
 }
-// Workgroups that the card holds at once: 256 CUs, and as many on each as the
-// kernels' registers (few rows) or LDS (many) leave room for.
+// Workgroups that the card works on at once: 256 CUs, and as many on each as the
+// kernels' registers or LDS leave room for (kFew32, fp32 alone: one, two would
+// share the matrix cores that bound it).
 constexpr int paged_slots(int kind, int head_dim) {
     const int per_cu = kind == kMany    ? (head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1)
                        : kind == kFew16 ? (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1)
-                       : kind == kFew32 ? (head_dim <= 64 ? 2 : 1)
+                       : kind == kFew64 ? (head_dim <= 64 ? 2 : 1)
                                         : 1;
     return 256 * per_cu;
 }

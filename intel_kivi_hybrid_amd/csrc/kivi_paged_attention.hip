@@ -140,7 +140,7 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
         if (kind == kMany) launch_paged_many(a, dtype, s);
         else if (dtype == kSrcF32) launch_paged_f32(a, kind, s);
         else if (kind == kFew16) launch_paged_few(a, dtype, s);
-        else launch_paged_mid(a, dtype, kind, s);
+        else launch_paged_mid(a, dtype, s);
         const int rc = check_launch("paged_attention");
         if (rc) return rc;
     }

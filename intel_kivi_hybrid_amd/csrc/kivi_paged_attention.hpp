@@ -202,31 +202,34 @@ __device__ __forceinline__ void finish(const PagedLaunch& a, const Work& w, int 
     }
 }
 
-// Joins four waves' results of ROWS rows (row i of wave j at jo(j) + i * stride, each
-// scaled to the largest of the waves' maxima) and finishes the rows from row0.
-template <int DT, int DP, int ROWS, class F>
+// Joins WAVES waves' results of ROWS rows (row i of wave j at jo(j) + i * stride,
+// each scaled to the largest of the waves' maxima) and finishes the rows from
+// row0.  By all 256 threads of a workgroup.
+template <int DT, int DP, int ROWS, int WAVES, class F>
 __device__ __forceinline__ void join_waves(const PagedLaunch& a, const Work& w, int row0, F jo,
                                            int stride, const float (*m)[ROWS],
-                                           const float (*l)[ROWS], const int* odd, int unit) {
+                                           const float (*l)[ROWS], bool odd, int unit) {
     for (int at = threadIdx.x; at < ROWS * (DP / 4); at += 4 * kWave) {
         const int row = at / (DP / 4), c = at % (DP / 4) * 4, r = row0 + row;
         if (r >= w.rows || c >= a.D) continue;
-        const float top = fmaxf(fmaxf(m[0][row], m[1][row]), fmaxf(m[2][row], m[3][row]));
+        float top = m[0][row];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) top = fmaxf(top, m[i][row]);
         f32x4_t o = {0.f, 0.f, 0.f, 0.f};
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < WAVES; ++i) {
             o += *reinterpret_cast<const f32x4_t*>(jo(i) + row * stride + c);
             sum += l[i][row] * exp2_fast(m[i][row] - top);
         }
-        finish<DT>(a, w, r, c, o, top, sum, (odd[0] | odd[1] | odd[2] | odd[3]) != 0, unit);
+        finish<DT>(a, w, r, c, o, top, sum, odd, unit);
     }
 }
 
 }  // namespace
 
 void launch_paged_few(const PagedLaunch& a, int dtype, hipStream_t s);
-void launch_paged_mid(const PagedLaunch& a, int dtype, int kind, hipStream_t s);
+void launch_paged_mid(const PagedLaunch& a, int dtype, hipStream_t s);
 void launch_paged_f32(const PagedLaunch& a, int kind, hipStream_t s);
 void launch_paged_many(const PagedLaunch& a, int dtype, hipStream_t s);
 

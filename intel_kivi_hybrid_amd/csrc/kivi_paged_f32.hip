@@ -206,9 +206,9 @@ __global__ void __launch_bounds__(kBlock) paged_f32_kernel(PagedLaunch a) {
                     f32x4_t{O[rt][cg][0][r], O[rt][cg][1][r], O[rt][cg][2][r], O[rt][cg][3][r]} * f;
         }
         __syncthreads();
-        join_waves<kSrcF32, DP, 16>(a, w, w.it.row0 + 16 * rt,
-                                    [&](int i) { return jo + i * 16 * OS; }, OS, join_m, join_l,
-                                    join_odd, kUnit);
+        join_waves<kSrcF32, DP, 16, kWaves>(
+            a, w, w.it.row0 + 16 * rt, [&](int i) { return jo + i * 16 * OS; }, OS, join_m,
+            join_l, (join_odd[0] | join_odd[1] | join_odd[2] | join_odd[3]) != 0, kUnit);
         __syncthreads();
     }
 }
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kBlock) paged_f32_kernel(PagedLaunch a) {
 template <int DP>
 void launch_rows(const PagedLaunch& a, int kind, hipStream_t s) {
     const dim3 grid((unsigned)(a.n_items * a.Hkv));
-    // (paged_few_rows(): the kinds that a head_dim comes with)
+    // (paged_kind(): the kinds that a head_dim comes with)
     if (kind == kFew16) {
         paged_f32_kernel<DP, 1><<<grid, kBlock, 0, s>>>(a);
     } else {

@@ -220,8 +220,9 @@ __global__ void __launch_bounds__(kBlock) paged_few_kernel(PagedLaunch a) {
     for (int cb = 0; cb < F::CB; ++cb)
         *reinterpret_cast<f32x4_t*>(jo + (wave * 16 + col) * F::OS + 16 * cb + 4 * gq) = O[cb] * f;
     __syncthreads();
-    join_waves<DT, DP, 16>(a, w, w.it.row0, [&](int i) { return jo + i * 16 * F::OS; }, F::OS,
-                           join_m, join_l, join_odd, kUnit);
+    join_waves<DT, DP, 16, kWaves>(
+        a, w, w.it.row0, [&](int i) { return jo + i * 16 * F::OS; }, F::OS, join_m, join_l,
+        (join_odd[0] | join_odd[1] | join_odd[2] | join_odd[3]) != 0, kUnit);
 }
 
 template <int DT>

@@ -39,25 +39,25 @@ __device__ __forceinline__ void load_lds(const uint16_t* base, uint32_t off, uns
         (const __attribute__((address_space(1))) void*)(base + off),
         (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
-// All of the wave's loads have arrived.
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+// All but the wave's last N loads have arrived (they do in order).
+template <int N = 0>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N < 64, "the counter's range");
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+}
 
 // A wave's 32 query rows (lane: row lane % 32) and their softmax state.
-// Q_LDS: the queries lie in LDS (q_lds, a vector for each k-step and lane), where
-// registers are short.
-template <int DT, int DP, int TOKENS, bool Q_LDS = false>
+template <int DT, int DP, int TOKENS>
 struct TileRows {
     using M = TileShape<DP, TOKENS>;
-    u32x4_t qf[Q_LDS ? 1 : M::KS];
-    const u32x4_t* ql;
+    u32x4_t qf[M::KS];
     f32x16_t O[M::CB];
     float m, l;
     int lim;                 // positions that the lane's row sees
     int all, last;           // that all, and any, of the 32 rows see
 
     // rows row0 .. row0 + 31 of the item's sequence
-    __device__ __forceinline__ void init(const PagedLaunch& a, const Work& w, int row0,
-                                         u32x4_t* q_lds = nullptr) {
+    __device__ __forceinline__ void init(const PagedLaunch& a, const Work& w, int row0) {
         const int lane = threadIdx.x % kWave, half = lane / 32, r = row0 + lane % 32;
         const bool live = r < w.rows;
         lim = live ? row_limit(w, r) : 0;
@@ -67,12 +67,9 @@ struct TileRows {
 #pragma unroll
         for (int ks = 0; ks < M::KS; ++ks) {
             const int c = 16 * ks + 8 * half;
-            u32x4_t x = {0, 0, 0, 0};
-            if (live && c < a.D) x = *reinterpret_cast<const u32x4_t*>(q + c);
-            if constexpr (Q_LDS) q_lds[ks * kWave + lane] = x;
-            else qf[ks] = x;
+            qf[ks] = u32x4_t{0, 0, 0, 0};
+            if (live && c < a.D) qf[ks] = *reinterpret_cast<const u32x4_t*>(q + c);
         }
-        ql = q_lds + lane;
 #pragma unroll
         for (int cb = 0; cb < M::CB; ++cb) {
 #pragma unroll
@@ -96,14 +93,11 @@ struct TileRows {
         const uint32_t krow = col * M::ROW + ((half ^ M::key_swizzle(col)) << 4);
 #pragma unroll
         for (int ks = 0; ks < M::KS; ++ks) {
-            u32x4_t q;
-            if constexpr (Q_LDS) q = ql[ks * kWave];
-            else q = qf[ks];
 #pragma unroll
             for (int tb = 0; tb < M::TB; ++tb) {
                 const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(
                     kb + (krow ^ (32 * ks)) + 32 * tb * M::ROW);
-                s[tb] = mfma32<DT>(kf, q, s[tb]);
+                s[tb] = mfma32<DT>(kf, qf[ks], s[tb]);
             }
         }
         // score i of block tb: token 32 tb + 8 (i / 4) + 4 half + i % 4
