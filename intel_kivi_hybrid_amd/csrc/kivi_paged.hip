@@ -217,6 +217,8 @@ int check_pool(int32_t dtype, int64_t num_pages, int32_t page_size, int32_t q_he
     if (head_dim < 16 || head_dim > 256 || head_dim % 16 != 0)
         return set_error(kErrUnsupported,
                          "head_dim must be a multiple of 16 up to 256, got %d", head_dim);
+    if ((int64_t)kv_heads * page_size * head_dim > INT32_MAX)
+        return set_error(kErrUnsupported, "a page of %d kv heads is too large", kv_heads);
     return kOk;
 }
 

@@ -85,7 +85,8 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     for (int s = 4; s <= 8; ++s)
         if (page_size == 1 << s) shift = s;
     if (shift < 0 || num_pages < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0 ||
-        head_dim < 16 || head_dim > 256 || head_dim % 16 != 0)
+        head_dim < 16 || head_dim > 256 || head_dim % 16 != 0 ||
+        (int64_t)kv_heads * page_size * head_dim > INT32_MAX)
         return set_error(kErrInvalidArgument,
                          "unsupported geometry: page_size %d, %d query heads over %d kv heads, "
                          "head_dim %d", page_size, q_heads, kv_heads, head_dim);

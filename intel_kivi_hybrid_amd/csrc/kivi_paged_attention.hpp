@@ -101,8 +101,8 @@ struct Work {
     int kvh, rows, hg;
     // (the constant address space: scalar loads, whatever else is written)
     const __attribute__((address_space(4))) int32_t* pages;
-    int64_t head_off;            // of the kv head within a page, in elements
-    int64_t page_elems;
+    uint32_t head_off;           // of the kv head within a page, in elements
+    uint32_t page_elems;
 };
 
 __device__ __forceinline__ Work work_of(const PagedLaunch& a) {
@@ -113,8 +113,8 @@ __device__ __forceinline__ Work work_of(const PagedLaunch& a) {
     w.hg = a.hg;
     w.rows = w.it.n * a.hg;
     w.pages = (const __attribute__((address_space(4))) int32_t*)(a.pages + w.it.page0);
-    w.head_off = ((int64_t)w.kvh << a.page_shift) * a.D;
-    w.page_elems = ((int64_t)a.Hkv << a.page_shift) * a.D;
+    w.head_off = ((uint32_t)w.kvh << a.page_shift) * a.D;
+    w.page_elems = ((uint32_t)a.Hkv << a.page_shift) * a.D;
     return w;
 }
 
@@ -128,7 +128,8 @@ template <class T>
 __device__ __forceinline__ const T* block_at(const PagedLaunch& a, const Work& w,
                                              const void* pool, int page, int t) {
     const int off = min(t, (w.it.kv_end - 1) & ~15) & ((1 << a.page_shift) - 1);
-    return static_cast<const T*>(pool) + page * w.page_elems + w.head_off + off * a.D;
+    return static_cast<const T*>(pool) + (uint64_t)(uint32_t)page * w.page_elems + w.head_off +
+           (uint32_t)(off * a.D);
 }
 
 // Positions that row r sees, within the split.
@@ -163,8 +164,8 @@ __device__ __forceinline__ f32x4_t odd_values(const PagedLaunch& a, const Work& 
                                            int c) {
     f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
     for (; t < lim; ++t) {
-        const int64_t at = w.pages[t >> a.page_shift] * w.page_elems + w.head_off +
-                           (int64_t)(t & ((1 << a.page_shift) - 1)) * a.D + c;
+        const int64_t at = (int64_t)w.pages[t >> a.page_shift] * w.page_elems + w.head_off +
+                           (t & ((1 << a.page_shift) - 1)) * a.D + c;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float x = widen<DT>(a.v_pages, at + i);

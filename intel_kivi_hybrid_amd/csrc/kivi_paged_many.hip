@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) paged_many_kernel(P
     rows.init(a, w, w.it.row0 + 32 * wave);
     const int wg_all = w.it.ctx - w.it.n + 1 + w.it.row0 / w.hg;
     TileLoads<DP, kTile, kWaves> loads;
-    loads.wave = wave;
+    loads.init(a, wave);
 
     int t0 = w.it.kv_begin;
     auto step = [&](unsigned char* now, unsigned char* next) {

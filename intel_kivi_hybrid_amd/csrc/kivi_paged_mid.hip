@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(kBlock) paged_mid_kernel(PagedLaunch a) {
     rows.init(a, w, w.it.row0 + 32 * group);
     const int all_see = w.it.ctx - w.it.n + 1 + w.it.row0 / w.hg;
     TileLoads<DP, kTile, kWaves> loads;
-    loads.wave = wave;
+    loads.init(a, wave);
     constexpr int kLoads = 2 * TileLoads<DP, kTile, kWaves>::LD;      // of a tile
 
     int t0 = w.it.kv_begin;

@@ -46,6 +46,9 @@ __device__ __forceinline__ void wait_loads() {
     __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
 }
 
+// Instruction kinds of __builtin_amdgcn_sched_group_barrier.
+constexpr int kSchedValu = 0x2, kSchedMfma = 0x8, kSchedLdsRead = 0x100;
+
 // A wave's 32 query rows (lane: row lane % 32) and their softmax state.
 template <int DT, int DP, int TOKENS>
 struct TileRows {
@@ -100,6 +103,16 @@ struct TileRows {
                 s[tb] = mfma32<DT>(kf, qf[ks], s[tb]);
             }
         }
+        // (key vectors three k-steps ahead of their products: left to itself the
+        // compiler waits for each pair)
+        constexpr int kReads = M::KS * M::TB, kAhead = 3 * M::TB;
+        __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, kAhead, 0);
+#pragma unroll
+        for (int i = 0; i < kReads - kAhead; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, kAhead, 0);
         // score i of block tb: token 32 tb + 8 (i / 4) + 4 half + i % 4
         if (t0 + M::TILE > min(all, end)) {
 #pragma unroll
@@ -125,45 +138,71 @@ struct TileRows {
 #pragma unroll
             for (int cb = 0; cb < M::CB; ++cb) O[cb] *= f;
         }
-        u32x4_t pf[2 * M::TB];        // weights of tokens 16 j .. + 15
-#pragma unroll
-        for (int tb = 0; tb < M::TB; ++tb) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[tb][i] = exp2_fast(fmaf(s[tb][i], qscale, -m));
-                l += s[tb][i];
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                pf[2 * tb + i / 4][i % 4] = pack2<DT>(s[tb][2 * i], s[tb][2 * i + 1]);
-        }
         // transposed: lanes of 16 take tokens 4 half .. + 3 of 16 channels
         const int t = 4 * half + lane % 16 / 4;
         const int c = lane / 16 % 2 * 2 + lane % 4 / 2;
         const uint32_t vrow = t * M::ROW + ((c ^ M::value_swizzle(t)) << 4) + lane % 2 * 8;
+        constexpr int kSteps = 2 * M::TB;          // of 16 tokens
 #pragma unroll
-        for (int j = 0; j < 2 * M::TB; ++j) {
+        for (int j = 0; j < kSteps; ++j) {
+            u32x4_t pf;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = s[j / 2][j % 2 * 8 + 2 * i];
+                const float y = s[j / 2][j % 2 * 8 + 2 * i + 1];
+                const float p0 = exp2_fast(fmaf(x, qscale, -m)), p1 = exp2_fast(fmaf(y, qscale, -m));
+                l += p0 + p1;
+                pf[i] = pack2<DT>(p0, p1);
+            }
 #pragma unroll
             for (int cb = 0; cb < M::CB; ++cb) {
                 const unsigned char* p = vb + (vrow ^ (64 * cb)) + 16 * j * M::ROW;
                 const uint2 lo = read_transposed(p);
                 const uint2 hi = read_transposed(p + 8 * M::ROW);
-                O[cb] = mfma32<DT>(u32x4_t{lo.x, lo.y, hi.x, hi.y}, pf[j], O[cb]);
+                O[cb] = mfma32<DT>(u32x4_t{lo.x, lo.y, hi.x, hi.y}, pf, O[cb]);
             }
         }
+        // A step's products run beside the next one's weights; its values are read
+        // a step ahead.
+        __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 2 * M::CB, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedValu, 28, 0);
+#pragma unroll
+        for (int j = 0; j + 1 < kSteps; ++j) {
+#pragma unroll
+            for (int cb = 0; cb < M::CB; ++cb) {
+                __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(kSchedValu, 28 / M::CB, 0);
+            }
+        }
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, M::CB, 0);
     }
 };
 
 // How a workgroup's or wave's lanes load a tile: load i of GROUP waves covers
 // ROWS tokens of one block of 16 positions, whose page is the same for the whole
-// wave; a lane's place in the block is the same for every tile.
+// wave; a lane's place in the block is the same for every tile.  Pages of at
+// least a tile's size hold the whole tile: one page and one address for it (four
+// of each, with their 64-bit products, were 160 scalar instructions a tile).
 template <int DP, int TOKENS, int GROUP>
 struct TileLoads {
     using M = TileShape<DP, TOKENS>;
     static constexpr int LD = TOKENS / M::ROWS / GROUP;     // loads of a wave for a tile's keys
     int wave;                                               // within the group
     int page[LD];
+    uint32_t k_off[LD], v_off[LD];                          // the lane's, in the tile's rows
+    bool whole;                                             // pages hold tiles
 
+    __device__ __forceinline__ void init(const PagedLaunch& a, int wave_in_group) {
+        wave = wave_in_group;
+        whole = 1 << a.page_shift >= TOKENS;
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int row = (whole ? block_of(i) : 0) + token(i);
+            k_off[i] = row * a.D + channel(i, true);
+            v_off[i] = row * a.D + channel(i, false);
+        }
+    }
     __device__ __forceinline__ int block_of(int i) const {
         return (i * GROUP + wave) * M::ROWS / 16 * 16;
     }
@@ -176,6 +215,10 @@ struct TileLoads {
         return (slot ^ (key ? M::key_swizzle(t) : M::value_swizzle(t))) * 8;
     }
     __device__ __forceinline__ void pages_of(const PagedLaunch& a, const Work& w, int t0) {
+        if (whole) {
+            page[0] = block_page(a, w, t0);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < LD; ++i) page[i] = block_page(a, w, t0 + block_of(i));
     }
@@ -183,19 +226,33 @@ struct TileLoads {
     __device__ __forceinline__ void issue(const PagedLaunch& a, const Work& w, unsigned char* buf,
                                           int t0, int next) {
         const bool full = a.D == M::SL * 8;
-#pragma unroll
-        for (int i = 0; i < LD; ++i) {
-            const int t = t0 + block_of(i);
-            const uint16_t* k = block_at<uint16_t>(a, w, a.k_pages, page[i], t);
-            const uint16_t* v = block_at<uint16_t>(a, w, a.v_pages, page[i], t);
-            unsigned char* to = buf + (i * GROUP + wave) * 1024;
-            const int row = token(i) * a.D, kc = channel(i, true), vc = channel(i, false);
+        unsigned char* to = buf + wave * 1024;
+        if (whole) {
+            const uint16_t* k = block_at<uint16_t>(a, w, a.k_pages, page[0], t0);
+            const uint16_t* v = block_at<uint16_t>(a, w, a.v_pages, page[0], t0);
             if (full) {
-                load_lds(k, row + kc, to);
-                load_lds(v, row + vc, to + M::BYTES);
+#pragma unroll
+                for (int i = 0; i < LD; ++i) {
+                    load_lds(k, k_off[i], to + i * GROUP * 1024);
+                    load_lds(v, v_off[i], to + i * GROUP * 1024 + M::BYTES);
+                }
             } else {
-                if (kc < a.D) load_lds(k, row + kc, to);
-                if (vc < a.D) load_lds(v, row + vc, to + M::BYTES);
+#pragma unroll
+                for (int i = 0; i < LD; ++i) {
+                    if (channel(i, true) < a.D) load_lds(k, k_off[i], to + i * GROUP * 1024);
+                    if (channel(i, false) < a.D)
+                        load_lds(v, v_off[i], to + i * GROUP * 1024 + M::BYTES);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < LD; ++i) {
+                const int t = t0 + block_of(i);
+                const uint16_t* k = block_at<uint16_t>(a, w, a.k_pages, page[i], t);
+                const uint16_t* v = block_at<uint16_t>(a, w, a.v_pages, page[i], t);
+                if (channel(i, true) < a.D) load_lds(k, k_off[i], to + i * GROUP * 1024);
+                if (channel(i, false) < a.D)
+                    load_lds(v, v_off[i], to + i * GROUP * 1024 + M::BYTES);
             }
         }
         pages_of(a, w, next);
