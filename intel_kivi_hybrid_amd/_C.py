@@ -864,9 +864,10 @@ def paged_append(k, v, k_pages, v_pages, plan, q=None, q_out=None, cos=None, sin
         rot = 2 * cos.shape[-1]
         _check(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype is torch.float32
                and sin.dtype is torch.float32 and cos.is_contiguous() and sin.is_contiguous()
-               and cos.device == plan.device and sin.device == plan.device,
-               "cos and sin must be contiguous [positions, rotated / 2] float32 tensors on ",
-               plan.device)
+               and cos.device == plan.device and sin.device == plan.device
+               and (cos.data_ptr() | sin.data_ptr()) % 16 == 0,
+               "cos and sin must be contiguous, 16-byte aligned [positions, rotated / 2] float32 "
+               "tensors on ", plan.device)
         _check(cos.shape[0] >= plan.context, "cos and sin reach ", cos.shape[0],
                " positions, the step's longest sequence has ", plan.context)
     norm_dt = None

@@ -10,10 +10,10 @@
 // queries to an output of their own: one launch, each element read and
 // written once.  Memory-bound for prompts, launch-bound for single tokens.
 //
-// A lane takes two 8-element vectors of a head that hold whole pairs: i and
-// i + r/2 of the first r channels rotated by halves, neighbours otherwise;
-// so a rotation never crosses lanes, and only the norm's sum does, over the
-// D / 16 lanes of the head (a power of two of them, DPP steps).
+// A lane takes two 8-element vectors of a head, D/2 apart (r/2 in a rotated part of
+// r channels), that hold whole pairs of either kind of rotation: neighbours, or
+// i and i + r/2.  So a rotation never crosses lanes, and only the norm's sum does,
+// over the D / 16 lanes of the head (a power of two of them, DPP steps).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -43,21 +43,44 @@ struct AppendArgs {
     const float* sin;
     const void* q_norm;
     const void* k_norm;
-    float eps;
+    float eps, inv_d;
     int n_tokens, Hq, Hkv, D, page_shift, rot, lanes_log2;
-    int norm_dt, interleaved, vec;
+    int norm_dt, norm_vec, interleaved, vec;
 };
 
+typedef unsigned int kivi_u4v __attribute__((ext_vector_type(4)));
+
+// Eight elements widened: one or two 16-byte loads (vec: aligned to 16), read once
+// by this kernel.
 template <int DT>
 __device__ __forceinline__ void load8(const void* p, int64_t i, bool vec, float (&x)[8]) {
-    if (vec) {
+    if (!vec) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = widen<DT>(p, i + j);
+    } else if constexpr (DT == kSrcF32) {
         const float4 a = load4_vec<DT>(p, i), b = load4_vec<DT>(p, i + 4);
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
         x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     } else {
+        const kivi_u4v w = __builtin_nontemporal_load(
+            reinterpret_cast<const kivi_u4v*>(static_cast<const uint16_t*>(p) + i));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = widen<DT>(p, i + j);
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == kSrcBF16) {
+                x[2 * j] = __uint_as_float(w[j] << 16);
+                x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            } else {
+                x[2 * j] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j] & 0xffffu));
+                x[2 * j + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j] >> 16));
+            }
+        }
     }
+}
+// The same of a type known at run time.
+__device__ __forceinline__ void load8_dt(const void* p, int i, int dt, bool vec, float (&x)[8]) {
+    if (dt == kSrcF32) load8<kSrcF32>(p, i, vec, x);
+    else if (dt == kSrcBF16) load8<kSrcBF16>(p, i, vec, x);
+    else load8<kSrcF16>(p, i, vec, x);
 }
 
 template <int DT>
@@ -94,37 +117,38 @@ __device__ __forceinline__ float seg_sum(float v, int log2) {
     return v;
 }
 
+// A segment of lanes takes a head of a token.  (Several heads to a segment, to
+// share the angles and have more loads in flight, cost more in waves on a SIMD
+// than it gave: 12.3K tokens of 32/8 heads with norms, 1 head 60 us, 2 heads 67, 4
+// heads 83.)
 template <int DT>
 __global__ void __launch_bounds__(kAppendBlock) paged_append_kernel(AppendArgs a) {
     const int heads = a.Hq + 2 * a.Hkv;
-    const int64_t t = (int64_t)blockIdx.x * kAppendBlock + threadIdx.x;
-    const int64_t row = t >> a.lanes_log2;
-    if (row >= (int64_t)a.n_tokens * heads) return;      // (whole segments leave)
-    const int unit = (int)t & ((1 << a.lanes_log2) - 1);
+    const uint32_t t = blockIdx.x * kAppendBlock + threadIdx.x;
+    const uint32_t row = t >> a.lanes_log2;
+    const int tok = (int)(row / (uint32_t)heads), h = (int)(row - (uint32_t)tok * heads);
+    if (tok >= a.n_tokens) return;                       // (whole segments leave)
+    const int unit = (int)(t & ((1u << a.lanes_log2) - 1));
     const bool live = unit < a.D / 16;
-    const int tok = (int)(row / heads), h = (int)(row - (int64_t)tok * heads);
-    const int half = a.rot / 2;
     const int2 place = a.tokens[tok];
 
-    // the lane's two vectors of 8 channels, and the first of its pairs
-    const bool turned = live && 16 * unit < a.rot && h < a.Hq + a.Hkv;
-    int c0 = 16 * unit, c1 = 16 * unit + 8;
-    if (16 * unit < a.rot && !a.interleaved) {
-        c0 = 8 * unit;
-        c1 = half + 8 * unit;
-    }
+    // the lane's two vectors of 8 channels: of the rotated part's halves, or of the
+    // rest's
+    const bool inside = 16 * unit < a.rot;
+    const int start = inside ? 0 : a.rot, at = 8 * unit - start / 2;
+    const int c0 = start + at, c1 = c0 + (inside ? a.rot : a.D - a.rot) / 2;
 
     const void* src = a.v;
-    int64_t from = tok * a.v_st + (int64_t)(h - a.Hq - a.Hkv) * a.v_sh;
     const void* norm = nullptr;
+    int64_t from = tok * a.v_st + (int64_t)(h - a.Hq - a.Hkv) * a.v_sh;
     if (h < a.Hq) {
         src = a.q;
-        from = tok * a.q_st + h * a.q_sh;
         norm = a.q_norm;
+        from = tok * a.q_st + (int64_t)h * a.q_sh;
     } else if (h < a.Hq + a.Hkv) {
         src = a.k;
-        from = tok * a.k_st + (int64_t)(h - a.Hq) * a.k_sh;
         norm = a.k_norm;
+        from = tok * a.k_st + (int64_t)(h - a.Hq) * a.k_sh;
     }
     float x[8], y[8];
 #pragma unroll
@@ -133,50 +157,53 @@ __global__ void __launch_bounds__(kAppendBlock) paged_append_kernel(AppendArgs a
         load8<DT>(src, from + c0, a.vec, x);
         load8<DT>(src, from + c1, a.vec, y);
     }
+    // angles: of pairs (c0 + j, c1 + j), or of the pairs in x and those in y
+    const bool turned = live && inside && h < a.Hq + a.Hkv;
+    const int half = a.rot / 2;
+    float4 cs[2], sn[2];
+    if (turned) {
+        const int64_t r = (int64_t)place.y * half;
+        const int i0 = a.interleaved ? c0 / 2 : c0, i1 = a.interleaved ? c1 / 2 : c0 + 4;
+        cs[0] = *reinterpret_cast<const float4*>(a.cos + r + i0);
+        cs[1] = *reinterpret_cast<const float4*>(a.cos + r + i1);
+        sn[0] = *reinterpret_cast<const float4*>(a.sin + r + i0);
+        sn[1] = *reinterpret_cast<const float4*>(a.sin + r + i1);
+    }
     if (norm != nullptr) {
+        float u[8], w[8];
+        if (live) {
+            load8_dt(norm, c0, a.norm_dt, a.norm_vec, u);
+            load8_dt(norm, c1, a.norm_dt, a.norm_vec, w);
+        }
         float s = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) s = fmaf(x[j], x[j], fmaf(y[j], y[j], s));
         s = seg_sum(s, a.lanes_log2);
-        const float r = 1.0f / sqrtf(s / (float)a.D + a.eps);
-        if (live) {
+        const float r = rsqrtf(fmaf(s, a.inv_d, a.eps));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] = x[j] * r * load1_dt(norm, c0 + j, a.norm_dt);
-                y[j] = y[j] * r * load1_dt(norm, c1 + j, a.norm_dt);
-            }
+        for (int j = 0; j < 8; ++j) {
+            x[j] = x[j] * r * u[j];
+            y[j] = y[j] * r * w[j];
         }
     }
     if (!live) return;
     if (turned) {
-        const float* cs = a.cos + (int64_t)place.y * half + 8 * unit;
-        const float* sn = a.sin + (int64_t)place.y * half + 8 * unit;
-        float u[8], w[8];
+        const float c[8] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w, cs[1].x, cs[1].y, cs[1].z, cs[1].w};
+        const float s[8] = {sn[0].x, sn[0].y, sn[0].z, sn[0].w, sn[1].x, sn[1].y, sn[1].z, sn[1].w};
         if (a.interleaved) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {          // pair j: channels 2j, 2j + 1
-                const float p = j < 4 ? x[2 * (j % 4)] : y[2 * (j % 4)];
-                const float q = j < 4 ? x[2 * (j % 4) + 1] : y[2 * (j % 4) + 1];
-                u[j] = fmaf(p, cs[j], -(q * sn[j]));
-                w[j] = fmaf(q, cs[j], p * sn[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[2 * j] = u[j];
-                x[2 * j + 1] = w[j];
-                y[2 * j] = u[j + 4];
-                y[2 * j + 1] = w[j + 4];
+            for (int j = 0; j < 8; ++j) {
+                float* v = j < 4 ? x + 2 * j : y + 2 * (j - 4);
+                const float p = v[0], q = v[1];
+                v[0] = fmaf(p, c[j], -(q * s[j]));
+                v[1] = fmaf(q, c[j], p * s[j]);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                u[j] = fmaf(x[j], cs[j], -(y[j] * sn[j]));
-                w[j] = fmaf(y[j], cs[j], x[j] * sn[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] = u[j];
-                y[j] = w[j];
+                const float p = x[j], q = y[j];
+                x[j] = fmaf(p, c[j], -(q * s[j]));
+                y[j] = fmaf(q, c[j], p * s[j]);
             }
         }
     }
@@ -480,6 +507,8 @@ int kivi_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stri
                          "rotary_dim must be a multiple of 16 up to head_dim, got %d", rotary_dim);
     if (rotary_dim > 0 && (cos == nullptr || sin == nullptr))
         return set_error(kErrInvalidArgument, "rotation needs cos and sin");
+    if (rotary_dim > 0 && (((uintptr_t)cos | (uintptr_t)sin) & 15))
+        return set_error(kErrInvalidArgument, "cos and sin must be 16-byte aligned");
     if (norm_dtype < 0 || norm_dtype > 2)
         return set_error(kErrInvalidArgument, "norm_dtype %d is not 0, 1 or 2", norm_dtype);
     if (tokens == 0) return kOk;
@@ -500,26 +529,26 @@ int kivi_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stri
     a.cos = cos; a.sin = sin;
     a.q_norm = q_norm; a.k_norm = k_norm; a.norm_dt = norm_dtype;
     a.eps = eps;
+    a.inv_d = 1.0f / (float)head_dim;
     a.n_tokens = tokens; a.Hq = hq; a.Hkv = kv_heads; a.D = head_dim;
     a.page_shift = page_shift_of(page_size);
     a.rot = rotary_dim; a.interleaved = interleaved != 0;
     a.lanes_log2 = 0;
     while ((1 << a.lanes_log2) < head_dim / 16) ++a.lanes_log2;
-    // four elements per load (8 or 16 bytes) where every row starts on one
-    const uintptr_t bytes = 4 * src_size(dtype) - 1;
+    // vectors of eight elements where every row starts on 16 bytes
     int64_t strides = k_token_stride | k_head_stride | v_token_stride | v_head_stride;
     uintptr_t bases = (uintptr_t)k | (uintptr_t)v;
     if (q != nullptr) {
         strides |= q_token_stride | q_head_stride;
         bases |= (uintptr_t)q;
     }
-    a.vec = (strides & 3) == 0 && (bases & bytes) == 0;
+    a.vec = (strides * src_size(dtype) & 15) == 0 && (bases & 15) == 0;
+    a.norm_vec = (((uintptr_t)q_norm | (uintptr_t)k_norm) & 15) == 0;
     const int64_t lanes = (int64_t)tokens * (hq + 2 * kv_heads) << a.lanes_log2;
-    const int64_t blocks = (lanes + kAppendBlock - 1) / kAppendBlock;
-    if (blocks > INT32_MAX)
+    if (lanes > INT32_MAX)
         return set_error(kErrInvalidArgument, "%d tokens are too many for one launch", tokens);
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)blocks);
+    const dim3 grid((unsigned)((lanes + kAppendBlock - 1) / kAppendBlock));
     if (dtype == kSrcF32) paged_append_kernel<kSrcF32><<<grid, kAppendBlock, 0, s>>>(a);
     else if (dtype == kSrcBF16) paged_append_kernel<kSrcBF16><<<grid, kAppendBlock, 0, s>>>(a);
     else paged_append_kernel<kSrcF16><<<grid, kAppendBlock, 0, s>>>(a);
