@@ -704,10 +704,9 @@ def packed_attention_typed(q, store, softmax_scale=None, kv_start=None, hidden=N
 # unequal lengths on pages of one pool.
 # --------------------------------------------------------------------------
 def _check_inference(*tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            _check(t is None or not t.requires_grad, "inference only: a tensor requires a "
-                   "gradient; call it under torch.no_grad()")
+    for t in tensors:
+        _check(t is None or not t.requires_grad, "inference only: a tensor requires a gradient; "
+               "call it under torch.no_grad()")
 
 
 def _host_ints(values, name: str) -> torch.Tensor:
@@ -731,8 +730,8 @@ class PagedPlan:
     pools of ``num_pages`` pages and to the geometry it was made for."""
 
     __slots__ = ("device", "tokens", "context", "num_pages", "page_size", "q_heads", "kv_heads",
-                 "head_dim", "dtype", "_code", "_buf", "_ptr", "_info", "_info_ptr",
-                 "_workspace", "_stream", "_event", "_settled")
+                 "head_dim", "dtype", "_code", "_index", "_pool", "_buf", "_ptr", "_info",
+                 "_info_ptr", "_workspace", "_stream", "_event", "_settled")
 
     def wait(self) -> None:
         """Waits until the plan is on the device.  Needed only before a graph is
@@ -792,6 +791,8 @@ def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_he
     p.tokens, p.context = info[1], info[12]
     p.num_pages, p.page_size, p.dtype, p._code = num_pages, page_size, dtype, _IO_DTYPES[dtype]
     p.q_heads, p.kv_heads, p.head_dim = q_heads, kv_heads, head_dim
+    p._index = p.device.index
+    p._pool = torch.Size((num_pages, kv_heads, page_size, head_dim))
     host = torch.empty(max(info[0], 1), dtype=torch.int32, pin_memory=True)
     _native.check(_lib.kivi_paged_plan(*args, host.data_ptr(), host.numel(), p._info_ptr),
                   "paged_plan")
@@ -806,32 +807,46 @@ def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_he
     return p
 
 
-def _check_pages(plan, k_pages, v_pages) -> None:
-    shape = (plan.num_pages, plan.kv_heads, plan.page_size, plan.head_dim)
-    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if not (t.shape == shape and t.dtype is plan.dtype and t.is_contiguous()
-                and t.device == plan.device and t.data_ptr() % 16 == 0):
-            _fail(name, " must be a contiguous, 16-byte aligned ", list(shape), " tensor of ",
-                  _dtype_name(plan.dtype), " on ", plan.device, ", got ", list(t.shape), " of ",
-                  _dtype_name(t.dtype), " on ", t.device)
+# The calls below are made once per layer of a step, so their checks are ordered
+# for the common case: one combined test each, the detailed messages (or the less
+# common ways to be right) only where it fails.
+def _check_pages(plan, k_pages, v_pages):
+    kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+    pool, dt, dev = plan._pool, plan.dtype, plan._index
+    if not (k_pages.shape == pool and v_pages.shape == pool and k_pages.dtype is dt
+            and v_pages.dtype is dt and k_pages.is_contiguous() and v_pages.is_contiguous()
+            and k_pages.get_device() == dev and v_pages.get_device() == dev
+            and not (kp | vp) & 15):
+        for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+            _check(t.shape == pool and t.dtype is dt and t.is_contiguous()
+                   and t.get_device() == dev and not t.data_ptr() & 15,
+                   name, " must be a contiguous, 16-byte aligned ", list(pool), " tensor of ",
+                   _dtype_name(dt), " on ", plan.device, ", got ", list(t.shape), " of ",
+                   _dtype_name(t.dtype), " on ", t.device)
+    return kp, vp
 
 
-def _check_tokens(t, name: str, plan, heads: int) -> None:
-    """A step's rows ``[>= tokens, heads, head_dim]``, any strides of whole rows."""
-    if not (t.dim() == 3 and t.shape[0] >= plan.tokens and t.shape[1] == heads
-            and t.shape[2] == plan.head_dim and t.dtype is plan.dtype
-            and t.device == plan.device):
-        _fail(name, " must be [>= ", plan.tokens, ", ", heads, ", ", plan.head_dim, "] of ",
-              _dtype_name(plan.dtype), " on ", plan.device, ", got ", list(t.shape), " of ",
-              _dtype_name(t.dtype), " on ", t.device)
-    _check(t.stride(2) == 1, name, "'s channels must be contiguous")
+def _check_tokens(t, name: str, plan, heads: int):
+    """A step's rows ``[>= tokens, heads, head_dim]``, any strides of whole rows;
+    the strides."""
+    sh, st = t.shape, t.stride()
+    if not (len(sh) == 3 and sh[0] >= plan.tokens and sh[1] == heads and sh[2] == plan.head_dim
+            and st[2] == 1 and t.dtype is plan.dtype and t.get_device() == plan._index):
+        _check(len(sh) == 3 and sh[0] >= plan.tokens and sh[1] == heads
+               and sh[2] == plan.head_dim and t.dtype is plan.dtype and t.device == plan.device,
+               name, " must be [>= ", plan.tokens, ", ", heads, ", ", plan.head_dim, "] of ",
+               _dtype_name(plan.dtype), " on ", plan.device, ", got ", list(sh), " of ",
+               _dtype_name(t.dtype), " on ", t.device)
+        _fail(name, "'s channels must be contiguous")
+    return st
 
 
 def _new_rows(t, plan):
     """An output beside a step's rows ``t``; rows behind the step's tokens, which
     no kernel writes, are zeros."""
-    make = torch.zeros if t.shape[0] > plan.tokens else torch.empty
-    return make(t.shape, dtype=t.dtype, device=t.device)
+    if t.shape[0] > plan.tokens:
+        return torch.zeros(t.shape, dtype=t.dtype, device=t.device)
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def _check_out(out, name: str, like) -> None:
@@ -854,53 +869,57 @@ def paged_append(k, v, k_pages, v_pages, plan, q=None, q_out=None, cos=None, sin
     if ``interleaved``.  Both in fp32, rounded once.  Values are copied.  Rows may
     have any strides, as slices of one projection have; rows behind the plan's
     tokens are not read, and stay as they are in ``q_out``, which may be ``q``."""
-    _check_inference(k, v, q, q_norm, k_norm)
-    _check_pages(plan, k_pages, v_pages)
-    _check_tokens(k, "k", plan, plan.kv_heads)
-    _check_tokens(v, "v", plan, plan.kv_heads)
-    rot = 0
+    if torch.is_grad_enabled():
+        _check_inference(k, v, q, q_norm, k_norm)
+    dev = plan._index
+    kp, vp = _check_pages(plan, k_pages, v_pages)
+    ks = _check_tokens(k, "k", plan, plan.kv_heads)
+    vs = _check_tokens(v, "v", plan, plan.kv_heads)
+    rot = cos_ptr = sin_ptr = 0
     if cos is not None or sin is not None:
         _check(cos is not None and sin is not None, "rotation needs cos and sin")
-        rot = 2 * cos.shape[-1]
-        _check(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype is torch.float32
+        sh = cos.shape
+        cos_ptr, sin_ptr = cos.data_ptr(), sin.data_ptr()
+        _check(len(sh) == 2 and sin.shape == sh and cos.dtype is torch.float32
                and sin.dtype is torch.float32 and cos.is_contiguous() and sin.is_contiguous()
-               and cos.device == plan.device and sin.device == plan.device
-               and (cos.data_ptr() | sin.data_ptr()) % 16 == 0,
+               and cos.get_device() == dev and sin.get_device() == dev
+               and not (cos_ptr | sin_ptr) & 15,
                "cos and sin must be contiguous, 16-byte aligned [positions, rotated / 2] float32 "
                "tensors on ", plan.device)
-        _check(cos.shape[0] >= plan.context, "cos and sin reach ", cos.shape[0],
+        _check(sh[0] >= plan.context, "cos and sin reach ", sh[0],
                " positions, the step's longest sequence has ", plan.context)
+        rot = 2 * sh[1]
     norm_dt = None
-    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if t is None:
-            continue
-        _check(t.dim() == 1 and t.shape[0] == plan.head_dim and t.dtype in _IO_DTYPES
-               and t.is_contiguous() and t.device == plan.device, name, " must be a contiguous [",
-               plan.head_dim, "] tensor of a float type on ", plan.device)
-        _check(norm_dt is None or norm_dt is t.dtype, "q_norm and k_norm must have one type")
-        norm_dt = t.dtype
+    if q_norm is not None or k_norm is not None:
+        for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+            if t is None:
+                continue
+            if not (t.shape == (plan.head_dim,) and t.dtype in _IO_DTYPES and t.is_contiguous()
+                    and t.get_device() == dev):
+                _fail(name, " must be a contiguous [", plan.head_dim,
+                      "] tensor of a float type on ", plan.device)
+            _check(norm_dt is None or norm_dt is t.dtype, "q_norm and k_norm must have one type")
+            norm_dt = t.dtype
+    q_ptr = q_st = q_sh = out_ptr = 0
     if q is not None:
-        _check_tokens(q, "q", plan, plan.q_heads)
+        st = _check_tokens(q, "q", plan, plan.q_heads)
         if q_out is None:
             q_out = _new_rows(q, plan)
         else:
             _check_out(q_out, "q_out", q)
+        q_ptr, q_st, q_sh, out_ptr = q.data_ptr(), st[0], st[1], q_out.data_ptr()
     else:
         _check(q_out is None and q_norm is None, "q_out and q_norm need q")
-    dev = plan.device.index
     with on_device(dev):
-        _native.check(_lib.kivi_paged_append(
-            0 if q is None else q.data_ptr(), 0 if q is None else q.stride(0),
-            0 if q is None else q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-            v.data_ptr(), v.stride(0), v.stride(1), plan._code,
-            0 if q is None else q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-            plan.num_pages, plan.page_size, plan.q_heads, plan.kv_heads, plan.head_dim,
-            plan._ptr, plan.tokens, 0 if cos is None else cos.data_ptr(),
-            0 if sin is None else sin.data_ptr(), rot, 1 if interleaved else 0,
-            0 if q_norm is None else q_norm.data_ptr(),
+        rc = _lib.kivi_paged_append(
+            q_ptr, q_st, q_sh, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+            plan._code, out_ptr, kp, vp, plan.num_pages, plan.page_size, plan.q_heads,
+            plan.kv_heads, plan.head_dim, plan._ptr, plan.tokens, cos_ptr, sin_ptr, rot,
+            1 if interleaved else 0, 0 if q_norm is None else q_norm.data_ptr(),
             0 if k_norm is None else k_norm.data_ptr(),
-            0 if norm_dt is None else _IO_DTYPES[norm_dt], eps, plan._enter(dev)),
-            "paged_append")
+            0 if norm_dt is None else _IO_DTYPES[norm_dt], eps, plan._enter(dev))
+    if rc:
+        _native.check(rc, "paged_append")
     return q_out
 
 
@@ -935,35 +954,37 @@ def paged_attention(q, k_pages, v_pages, plan, softmax_scale=None, out=None, wor
     Returns ``[tokens, Hq, D]`` in q's type.  Chunks of prompts, verification
     passes and single tokens may share a call.  Rows behind the plan's tokens are
     not read, and stay as they are in ``out``.  Launched on the current stream."""
-    _check_inference(q)
-    _check_pages(plan, k_pages, v_pages)
-    _check_tokens(q, "q", plan, plan.q_heads)
-    per = 16 // q.element_size()
-    if q.data_ptr() % 16 or q.stride(0) % per or q.stride(1) % per:
+    if torch.is_grad_enabled():
+        _check_inference(q)
+    kp, vp = _check_pages(plan, k_pages, v_pages)
+    st = _check_tokens(q, "q", plan, plan.q_heads)
+    q_ptr = q.data_ptr()
+    if q_ptr & 15 or (st[0] | st[1]) * q.element_size() & 15:
         q = q.clone(memory_format=torch.contiguous_format)
+        q_ptr, st = q.data_ptr(), q.stride()
     if out is None:
         out = _new_rows(q, plan)
     else:
         _check_out(out, "out", q)
-    dev = plan.device.index
+    dev = plan._index
+    need = plan._workspace
+    ws_ptr = ws_bytes = 0
     with on_device(dev):
-        need = plan._workspace
-        if workspace is None:
-            workspace = _call_workspace(dev, need)
-        elif need:
-            _check(workspace.is_contiguous() and workspace.device == plan.device
-                   and workspace.data_ptr() % 16 == 0
-                   and workspace.numel() * workspace.element_size() >= need,
+        if need:
+            if workspace is None:
+                workspace = _call_workspace(dev, need)
+            ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+            _check(workspace.is_contiguous() and workspace.get_device() == dev
+                   and not ws_ptr & 15 and ws_bytes >= need,
                    "workspace must be a contiguous, 16-byte aligned tensor of ", need,
                    " bytes on ", plan.device)
-        _native.check(_lib.kivi_paged_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), plan._code, k_pages.data_ptr(),
-            v_pages.data_ptr(), plan.num_pages, plan.page_size, plan.q_heads, plan.kv_heads,
-            plan.head_dim, plan._ptr, plan._info_ptr,
+        rc = _lib.kivi_paged_attention(
+            q_ptr, st[0], st[1], plan._code, kp, vp, plan.num_pages, plan.page_size,
+            plan.q_heads, plan.kv_heads, plan.head_dim, plan._ptr, plan._info_ptr,
             plan.head_dim ** -0.5 if softmax_scale is None else float(softmax_scale),
-            out.data_ptr(), 0 if workspace is None else workspace.data_ptr(),
-            0 if workspace is None else workspace.numel() * workspace.element_size(),
-            plan._enter(dev)), "paged_attention")
+            out.data_ptr(), ws_ptr, ws_bytes, plan._enter(dev))
+    if rc:
+        _native.check(rc, "paged_attention")
     return out
 
 
