@@ -9,12 +9,14 @@
 // where its running count or mass crosses a border, three times at most for the
 // kept prefix and once for the token.
 //
-// Two launches.  The first sums counts and masses of a row's buckets, 1/16 wide
-// in x / temperature, a workgroup for each slice of 8192 tokens.  The borders lie
-// in a few buckets that these sums name (the second to last border moves the
-// last by less than a bucket's mass); the second launch, a workgroup for each
-// row, goes through the row once for their tokens and ranks those against each
-// other, by sub-buckets where they are many.
+// Two launches.  The first, a workgroup for each slice of 8192 tokens, sums counts
+// and masses of the slice's buckets, 1/16 wide in x / temperature, and leaves its
+// tokens in the buckets' order (a token's place is its bucket's count when it was
+// added).  The borders lie in a few buckets that these sums name (the second to
+// last border moves the last by less than a bucket's mass); the second launch, a
+// workgroup for each row, takes their tokens from the slices and ranks those
+// against each other, by sub-buckets where they are many.  Where they are more than
+// fit its list (thousands of equal logits) it goes through the row instead.
 //
 // Precision: neighbouring borders lie as close as a token's share of the mass,
 // 1e-6 and less, and sums of fp32 weights over 10^5 tokens are off by more than
@@ -46,7 +48,8 @@ constexpr int kCountShift = 50;           // a slice's rels stay below 2^50
 constexpr uint64_t kRelMask = (1ull << kCountShift) - 1;
 constexpr int kMaxVocab = 1 << 20;        // (a row's rels stay below 2^57)
 constexpr int kList = 6144;               // tokens that a row's list holds
-constexpr int kSeen = 1024;               // threads of the first launch that it is made from
+constexpr int kOrder = kSlice + 16;       // a slice's tokens, and the ones outside of vectors
+constexpr int kStarts = kBuckets + 8;     // (whole 16 bytes)
 constexpr int kSub = 2048;                // sub-buckets of a crowded bucket
 
 struct SampleArgs {
@@ -65,7 +68,8 @@ struct SampleArgs {
     // workspace
     uint64_t* hist;          // [row][slice][bucket]: count << 50 | sum of rels
     uint64_t* best;          // [row][slice]: the first token's key
-    float* tops;             // [row][slice][thread]: the largest of its tokens
+    uint16_t* order;         // [row][slice][kOrder]: its tokens by bucket
+    uint16_t* starts;        // [row][slice][kStarts]: where each bucket's begin
 };
 
 struct Settings {
@@ -226,57 +230,114 @@ struct Slice {
         single = row.single(threadIdx.x, slice, a.slices, a.V);
         lone = single >= 0 ? widen<DT>(row.base, single) : 0.f;
     }
+    // f(logit, index, slot) for the thread's tokens: slots 0 .. kLone
+    static constexpr int kLone = kLoads * R::kVec;
     template <class F>
     __device__ __forceinline__ void each(F f) const {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int v = first + i * kBlock;
-            if (v < row.n_vecs) row.tokens(w[i], v, f);
+            if (v >= row.n_vecs) continue;
+            int slot = i * R::kVec;
+            row.tokens(w[i], v, [&](float x, int at) { f(x, at, slot++); });
         }
-        if (single >= 0) f(lone, single);
+        if (single >= 0) f(lone, single, kLone);
+    }
+    // A token's number within the slice, and the token of a number.
+    static __device__ __forceinline__ int number(int slot) {
+        return slot == kLone ? kSlice + (int)threadIdx.x
+                             : (slot / R::kVec * kBlock + (int)threadIdx.x) * R::kVec +
+                                   slot % R::kVec;
+    }
+    static __device__ __forceinline__ int token(const R& row, int slice, int number) {
+        if (number < kSlice) return row.head + slice * kSlice + number;
+        number -= kSlice;
+        return number < 8 ? number : row.tail + number - 8;
     }
 };
 
 template <int DT>
 __global__ void __launch_bounds__(kBlock) sample_sums_kernel(SampleArgs a) {
     __shared__ uint64_t hist[kBuckets];
+    __shared__ uint32_t starts[kBuckets];
+    __shared__ __align__(16) uint16_t order[kOrder];
     __shared__ float wave_top[kBlock / kWave];
-    __shared__ uint32_t first;
+    __shared__ uint32_t wave_count[kBlock / kWave], first;
     const int row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
     const int tid = threadIdx.x;
-    const Slice<DT> tokens(a, row, slice);
+    using S = Slice<DT>;
+    const S tokens(a, row, slice);
     const Settings s = settings_of(a, row);
     hist[tid] = 0;
     static_assert(kBuckets == kBlock, "a thread for each bucket");
     if (tid == 0) first = ~0u;
     float top = -INFINITY;
-    tokens.each([&](float x, int) { top = fmaxf(top, x); });       // (NaN never)
-    a.tops[(int64_t)blockIdx.x * kBlock + tid] = top;
+    tokens.each([&](float x, int, int) { top = fmaxf(top, x); });       // (NaN never)
     top = wave_max(top);
     if (tid % kWave == 0) wave_top[tid / kWave] = top;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kBlock / kWave; ++i) top = fmaxf(top, wave_top[i]);
+    const int64_t at = (int64_t)row * a.slices + slice;
     uint32_t index = ~0u;
-    if (s.first || !(top > -INFINITY)) {
-        tokens.each([&](float x, int i) { index = x == top ? min(index, (uint32_t)i) : index; });
-    } else {
-        Scale scale;
-        scale.set(top, s.t);
-        tokens.each([&](float x, int i) {
+    if (s.first) {
+        tokens.each([&](float x, int i, int) {
+            index = x == top ? min(index, (uint32_t)i) : index;
+        });
+        if (index != ~0u) atomicMin(&first, index);
+        __syncthreads();
+        if (tid == 0) a.best[at] = (uint64_t)order_bits(top) << 32 | first;
+        return;
+    }
+    Scale scale;
+    scale.set(top, s.t);
+    uint32_t place[S::kLone + 1];          // bucket << 16 | number in the bucket
+#pragma unroll
+    for (int i = 0; i <= S::kLone; ++i) place[i] = ~0u;
+    if (top > -INFINITY) {
+        tokens.each([&](float x, int i, int slot) {
             index = x == top ? min(index, (uint32_t)i) : index;
             uint64_t rel;
             const int b = scale.bucket(x, rel);
-            if (b < kBuckets)
-                atomicAdd((unsigned long long*)&hist[b],
-                          (unsigned long long)(rel | 1ull << kCountShift));
+            if (b >= kBuckets) return;
+            const uint64_t old = atomicAdd((unsigned long long*)&hist[b],
+                                           (unsigned long long)(rel | 1ull << kCountShift));
+            place[slot] = (uint32_t)b << 16 | (uint32_t)(old >> kCountShift);
         });
     }
     if (index != ~0u) atomicMin(&first, index);
     __syncthreads();
-    const int64_t at = (int64_t)row * a.slices + slice;
     if (tid == 0) a.best[at] = (uint64_t)order_bits(top) << 32 | first;
-    if (!s.first) a.hist[at * kBuckets + tid] = hist[tid];
+    const uint64_t sum = hist[tid];
+    a.hist[at * kBuckets + tid] = sum;
+    // where each bucket's tokens start
+    const int lane = tid % kWave;
+    const uint32_t count = (uint32_t)(sum >> kCountShift);
+    uint32_t end = count;
+    for (int d = 1; d < kWave; d *= 2) {
+        const uint32_t o = __shfl_up(end, d);
+        if (lane >= d) end += o;
+    }
+    if (lane == kWave - 1) wave_count[tid / kWave] = end;
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (int i = 0; i < kBlock / kWave; ++i) {
+        if (i < tid / kWave) end += wave_count[i];
+        all += wave_count[i];
+    }
+    starts[tid] = end - count;
+    a.starts[at * kStarts + tid] = (uint16_t)(end - count);
+    if (tid == 0) a.starts[at * kStarts + kBuckets] = (uint16_t)all;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i <= S::kLone; ++i)
+        if (place[i] != ~0u)
+            order[starts[place[i] >> 16] + (place[i] & 0xffffu)] = (uint16_t)S::number(i);
+    __syncthreads();
+    uint4* to = reinterpret_cast<uint4*>(a.order + at * kOrder);
+    for (uint32_t i = tid; i < (all + 7) / 8; i += kBlock)
+        to[i] = reinterpret_cast<const uint4*>(order)[i];
 }
 
 // The first token of a row from its slices' (every lane).
@@ -347,78 +408,6 @@ struct Wanted {
     int lo[4], hi[4];
 };
 
-// The logits of the wanted buckets lie within these (fp32, a little wider): what
-// is outside needs no fp64.  Mostly two of the ranges are there or meet.
-struct Window {
-    float lo[4], hi[4], least;
-    bool two, odd;                       // the last two are empty; bounds are infinite
-    __device__ __forceinline__ void set(const Wanted& w, const Scale& s, double t) {
-        odd = isinf(s.top) || isinf(s.edge);
-        int n = 0;
-        least = INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            lo[i] = INFINITY;
-            hi[i] = -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (w.lo[i] > w.hi[i]) continue;
-            const double a = (s.edge - w.hi[i]) / kPerUnit * t;
-            const double b = (s.edge - w.lo[i] + 1.0) / kPerUnit * t;
-            // (rounding: x / t and its bucket, 2^-52 of x; these bounds, 2^-23)
-            const float l = odd ? -INFINITY : (float)(a - fabs(a) * 1e-6 - 1e-30);
-            const float h = odd ? INFINITY : (float)(b + fabs(b) * 1e-6 + 1e-30);
-            least = fminf(least, l);
-            bool met = false;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (met || !(l <= hi[j] && h >= lo[j])) continue;
-                lo[j] = fminf(lo[j], l);
-                hi[j] = fmaxf(hi[j], h);
-                met = true;
-            }
-            if (met) continue;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j != n) continue;
-                lo[j] = l;
-                hi[j] = h;
-            }
-            ++n;
-        }
-        two = n <= 2;
-    }
-    __device__ __forceinline__ bool has(float x) const {
-        bool in = false;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) in |= (x >= lo[i]) & (x <= hi[i]);
-        return in;
-    }
-};
-
-// The same as the sign of min |x - middle| - half, in a few vector instructions
-// and no mask: finite bounds, a little wider again.
-template <int N>
-struct Near {
-    float middle[N], half[N];
-    __device__ __forceinline__ explicit Near(const Window& w) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const bool none = w.lo[i] > w.hi[i];
-            const float l = none ? 0.f : w.lo[i], h = none ? 0.f : w.hi[i];
-            middle[i] = 0.5f * l + 0.5f * h;
-            half[i] = none ? -1.f : 0.5f * h - 0.5f * l + 1e-6f * (fabsf(l) + fabsf(h)) + 1e-30f;
-        }
-    }
-    __device__ __forceinline__ float side(float x) const {
-        float d = fabsf(x - middle[0]) - half[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) d = fminf(d, fabsf(x - middle[i]) - half[i]);
-        return d;
-    }
-};
-
 // Where the borders can lie: each is known up to its bucket, so the kept mass
 // lies between two of the running sums.  By all threads of a workgroup.
 __device__ void wanted_buckets(const Settings& s, const Scale& scale, const Sums& sums,
@@ -476,14 +465,15 @@ struct Picker {
                 uint64_t rel[kSub + 1];
                 uint32_t count[kSub + 1];
             } sub;
-            int thread[kSeen];           // threads that saw a token within reach
         };
         Wanted wanted;
         uint64_t wave_rel[kPickBlock / kWave];
         uint32_t wave_count[kPickBlock / kWave];
         int gap[kMaxVocab / kSlice];
         uint64_t hit_rel;
-        uint32_t bits_min, bits_max, n, hit, listed, seen;
+        // a range of wanted buckets in a slice: its first token there, and in the list
+        uint32_t from[4 * kMaxVocab / kSlice], to[4 * kMaxVocab / kSlice + 1];
+        uint32_t bits_min, bits_max, n, hit;
         int entry;
     };
     const SampleArgs& a;
@@ -513,53 +503,6 @@ struct Picker {
         for (int i = threadIdx.x; i < r.n_vecs; i += kPickBlock) r.tokens_rolled(r.vecs[i], i, token);
     }
 
-    // Vector i of those of the threads seen.
-    __device__ __forceinline__ int seen_vec(int i) const {
-        constexpr int kLoads = Slice<DT>::kLoads;
-        const int t = s.thread[i / kLoads];
-        return Slice<DT>::vec_of(t / kBlock, t % kBlock) + i % kLoads * kBlock;
-    }
-
-    // The tokens of vectors vec(0 .. n - 1) within the window, to the list.  A
-    // thread marks a few vectors' first: one round trip to the list's end for
-    // all of them, not one each.
-    template <int N, class F>
-    __device__ __forceinline__ void take(const Window& window, int n, F vec) {
-        constexpr int kVec = RowView<DT>::kVec, kAhead = 32 / kVec;
-        const RowView<DT> r(a, row);
-        if (r.n_vecs == 0) return;               // (a row of single tokens)
-        const Near<N> near(window);
-        const uint32_t always = window.odd ? ~0u : 0u;
-#pragma unroll 1
-        for (int i = threadIdx.x; i < n; i += kAhead * kPickBlock) {
-            uint4 w[kAhead];
-            uint32_t there = 0;                  // token k of the 32 at bit 31 - k
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                const int at = i + j * kPickBlock, v = vec(min(at, n - 1));
-                w[j] = r.vecs[min(v, r.n_vecs - 1)];
-                if (at < n && v < r.n_vecs)
-                    there |= ((1u << kVec) - 1) << (32 - kVec - j * kVec);
-            }
-            uint32_t mark = 0;
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-                r.tokens(w[j], 0, [&](float x, int) {
-                    mark = mark << 1 | __float_as_uint(near.side(x)) >> 31;
-                });
-            mark = (mark | always) & there;
-            if (mark == 0) continue;
-            uint32_t to = atomicAdd(&s.listed, (uint32_t)__popc(mark));
-#pragma unroll 1
-            for (; mark != 0; ++to) {
-                const int at = __clz(mark);
-                mark &= ~(0x80000000u >> at);
-                const int token = vec(i + at / kVec * kPickBlock) * kVec + at % kVec;
-                if (to < kList) s.key[to] = (uint64_t)(r.head + token);
-            }
-        }
-    }
-
     // The row's sums from its slices', and the buckets that may hold a border;
     // their tokens to the list.
     __device__ void collect(const Settings& set) {
@@ -571,7 +514,6 @@ struct Picker {
             other.set(logit_of(a.best[(int64_t)row * a.slices + i]), set.t);
             s.gap[i] = other.top == -INFINITY ? kBuckets : bucket_gap(scale.edge, other.edge);
         }
-        if (tid == 0) s.listed = s.seen = 0;
         __syncthreads();
         uint64_t rel = 0;
         uint32_t count = 0;
@@ -616,52 +558,70 @@ struct Picker {
         }
         __syncthreads();
         wanted_buckets(set, scale, s.sums, s.wanted);
-        Window window;
-        window.set(s.wanted, scale, set.t);
-        // The wanted buckets lie at the order's head: of most rows few of the first
-        // launch's threads saw a token that reaches them.  Those threads' tokens,
-        // or the whole row where they are many.
-        const float* tops = a.tops + (int64_t)row * a.slices * kBlock;
-        for (int i = tid; i < a.slices * kBlock; i += kPickBlock) {
-            const uint64_t lanes = __builtin_amdgcn_ballot_w64(tops[i] >= window.least);
-            if (lanes == 0) continue;
-            uint32_t n = 0;
-            if (lane == 0) n = atomicAdd(&s.seen, (uint32_t)__popcll(lanes));
-            n = __builtin_amdgcn_readfirstlane(n) +
-                __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32),
-                                          __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
-            if ((lanes >> lane & 1) && n < kSeen) s.thread[n] = i;
+        // The ranges without what an earlier one has: each token once.
+        int lo[4], hi[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            lo[i] = s.wanted.lo[i];
+            hi[i] = s.wanted.hi[i];
         }
-        __syncthreads();
-        if (s.seen <= kSeen) {
-            // (a thread's vectors of a slice to one thread each)
-            constexpr int kLoads = Slice<DT>::kLoads;
-            const int n = (int)s.seen * kLoads;
-            if (window.two) take<2>(window, n, [&](int i) { return seen_vec(i); });
-            else take<4>(window, n, [&](int i) { return seen_vec(i); });
-        } else {
-            const int n = RowView<DT>(a, row).n_vecs;
-            if (window.two) take<2>(window, n, [&](int i) { return i; });
-            else take<4>(window, n, [&](int i) { return i; });
-        }
-        const RowView<DT> r(a, row);
-        const int single = r.single(tid, 0, 1, a.V);
-        if (single >= 0) {
-            const float x = widen<DT>(r.base, single);
-            if (window.has(x)) {
-                const uint32_t n = atomicAdd(&s.listed, 1u);
-                if (n < kList) s.key[n] = (uint64_t)single;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int j = 0; j < i; ++j) {
+                if (lo[i] > hi[i] || lo[j] > hi[j] || lo[i] > hi[j] + 1 || hi[i] < lo[j] - 1)
+                    continue;
+                // (they meet: one range, in the later's place)
+                lo[i] = min(lo[i], lo[j]);
+                hi[i] = max(hi[i], hi[j]);
+                lo[j] = 1;
+                hi[j] = 0;
             }
         }
+        // Their stretches of each slice's order, one after the other in the list.
+        const int stretches = 4 * a.slices;
+        uint64_t unused = 0;
+        uint32_t length = 0;
+        static_assert(4 * kMaxVocab / kSlice <= kBuckets, "a thread for each stretch");
+        if (tid < stretches) {
+            const int i = tid / a.slices, slice = tid - i * a.slices;
+            const int l = i == 0 ? lo[0] : i == 1 ? lo[1] : i == 2 ? lo[2] : lo[3];
+            const int h = i == 0 ? hi[0] : i == 1 ? hi[1] : i == 2 ? hi[2] : hi[3];
+            const int b0 = max(l - s.gap[slice], 0), b1 = min(h - s.gap[slice], kBuckets - 1);
+            if (l <= h && b0 <= b1) {
+                const uint16_t* starts = a.starts + ((int64_t)row * a.slices + slice) * kStarts;
+                s.from[tid] = starts[b0];
+                length = starts[b1 + 1] - starts[b0];
+            }
+        }
+        uint32_t to = length;
+        if (tid < kBuckets) {
+            wave_scan(unused, to);
+            if (lane == kWave - 1) s.wave_count[tid / kWave] = to;
+        }
         __syncthreads();
-        listed = s.listed <= kList ? (int)s.listed : -1;
+        uint32_t all = 0;
+        for (int i = 0; i < kBuckets / kWave; ++i) {
+            if (i < tid / kWave) to += s.wave_count[i];
+            all += s.wave_count[i];
+        }
+        if (tid < stretches) s.to[tid] = to - length;
+        if (tid == 0) s.to[stretches] = all;
+        __syncthreads();
+        listed = all <= (uint32_t)kList ? (int)all : -1;
+        const RowView<DT> r(a, row);
 #pragma unroll 1
         for (int j = tid; j < listed; j += kPickBlock) {
-            const uint32_t i = (uint32_t)s.key[j];
+            int at = 0;                              // the last stretch that starts by j
+            for (int d = kBuckets; d > 0; d /= 2)
+                if (at + d < stretches && s.to[at + d] <= (uint32_t)j) at += d;
+            const int slice = at % a.slices;
+            const uint16_t* order = a.order + ((int64_t)row * a.slices + slice) * kOrder;
+            const int i = Slice<DT>::token(r, slice, order[s.from[at] + (j - s.to[at])]);
             const float x = widen<DT>(r.base, i);
             uint64_t rel;
             const int b = scale.bucket(x, rel);
-            s.key[j] = (uint64_t)order_bits(x) << 32 | i;
+            s.key[j] = (uint64_t)order_bits(x) << 32 | (uint32_t)i;
             s.rel[j] = (uint64_t)b << 40 | rel;
         }
         __syncthreads();
@@ -985,7 +945,8 @@ extern "C" {
 
 size_t kivi_sample_workspace_size(int32_t rows, int32_t vocab) {
     if (rows < 1 || vocab < 1 || vocab > kMaxVocab) return 0;
-    return (size_t)(rows * slices_of(vocab)) * (8 * (kBuckets + 1) + 4 * kBlock);
+    return (size_t)(rows * slices_of(vocab)) *
+           (8 * kBuckets + 2 * kOrder + 2 * kStarts + 8);
 }
 
 int kivi_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows,
@@ -1032,8 +993,10 @@ int kivi_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t r
     uint64_t* w = static_cast<uint64_t*>(workspace);
     const int64_t n = rows * slices;
     a.hist = w;
-    a.best = a.hist + n * kBuckets;
-    a.tops = reinterpret_cast<float*>(a.best + n);
+    a.order = reinterpret_cast<uint16_t*>(a.hist + n * kBuckets);
+    a.starts = a.order + n * kOrder;
+    a.best = reinterpret_cast<uint64_t*>(a.starts + n * kStarts);
+    static_assert(kOrder % 8 == 0 && kStarts % 8 == 0, "whole 16 bytes");
     hipStream_t s = (hipStream_t)stream;
     if (dtype == kSrcF32) launch<kSrcF32>(a, rows, s);
     else if (dtype == kSrcBF16) launch<kSrcBF16>(a, rows, s);
