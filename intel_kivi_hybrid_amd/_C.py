@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import threading
 
 import torch
 
@@ -939,12 +940,23 @@ def rotary_tables(positions, rotary_dim, base=10000.0, inv_freq=None, device="cu
     return ang.cos().float().to(device), ang.sin().float().to(device)
 
 
-def _call_workspace(device, nbytes: int):
-    """:func:`_workspace`, but memory of its own for each call of a graph: two
-    captured graphs may run at once."""
-    if nbytes and torch.cuda.is_current_stream_capturing():
+_call_ws = threading.local()
+
+
+def _call_workspace(device: int, nbytes: int):
+    """Device memory for one call: kept for the next of the same host thread and
+    stream (two threads' launches on one stream may alternate).  A call that is
+    captured has memory of its own: two graphs may run at once."""
+    if nbytes == 0:
+        return None
+    if nbytes > _WS_KEPT or torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=torch.device(_DEVICE_TYPE, device))
-    return _workspace(device, nbytes)
+    kept, key = _call_ws.__dict__, (device, stream_handle(device))
+    buf = kept.get(key)
+    if buf is None or buf.numel() < nbytes:
+        buf = kept[key] = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8,
+                                      device=torch.device(_DEVICE_TYPE, device))
+    return buf
 
 
 def paged_attention(q, k_pages, v_pages, plan, softmax_scale=None, out=None, workspace=None):

@@ -87,7 +87,10 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int row) {
     const double u = a.u_f64 ? static_cast<const double*>(a.u)[row]
                              : (double)static_cast<const float*>(a.u)[row];
     s.u = u > 0.0 ? fmin(u, 1.0) : 0.0;                  // (NaN: 0)
-    s.first = !(s.t > 0.0) || s.k == 1 || s.p <= 0.0;
+    s.first = !(s.t > 0.0) || s.k == 1 || s.p <= 0.0 || s.m > 1.0;
+    // (of any fp32 logits, x / t and its multiples stay finite; beyond these bounds
+    // all others weigh nothing, or all the same)
+    s.t = fmin(fmax(s.t, 0x1p-300), 0x1p300);
     return s;
 }
 
@@ -765,7 +768,8 @@ struct Picker {
         const Need x = need_of(kind, at, b);
         uint64_t lo = 0, hi = ~0ull, before_rel = 0;
         uint32_t before_count = 0, n = s.sums.count[b + 1] - s.sums.count[b];
-        while (n > kFew) {
+        // (a round leaves a 2048th of a range of 2^64 at most: 6 rounds)
+        for (int round = 0; n > kFew && round < 6; ++round) {
             // counts and sums of 2048 stretches of the keys between lo and hi, from
             // the least to the most logit (or index, where all are equal)
             __syncthreads();
@@ -824,6 +828,7 @@ struct Picker {
         each(b, [&](uint64_t key, uint64_t rel) {
             if (key < lo || key > hi) return;
             const uint32_t i = atomicAdd(&s.n, 1u);
+            if (i >= (uint32_t)kFew) return;
             s.few.key[i] = key;
             s.few.rel[i] = rel;
         });

@@ -224,3 +224,92 @@ def test_refusals(hip_device):
         C.sample(x[0], u)
     with pytest.raises(RuntimeError, match="row's logits must be contiguous"):
         C.sample(x.t().contiguous().t(), u)
+
+
+def test_temperatures_at_the_ends(hip_device):
+    """Beyond all finite temperatures each token weighs the same, at the least ones
+    only the largest logit has any weight; infinite and zero logits included."""
+    V = 1000
+    x = torch.randn(3, V, generator=torch.Generator().manual_seed(1))
+    x[1, 5] = float("inf")
+    x[2] = -x[2].abs()
+    x[2, 9] = 0.0
+    u = torch.full((3,), (123 + 0.5) / V, dtype=torch.float64)
+    cold = [int(x[0].argmax()), 5, 9]
+    hot = [int(_order(x[0].numpy())[123]), 5, int(_order(x[2].numpy())[123])]
+    for t in (5e-324, 1e-310, 1e-45, 1e-30):
+        assert _c().sample(x.cuda(), u.cuda(), temperature=t).cpu().tolist() == cold
+    for t in (1e30, 1e300, float("inf")):
+        assert _c().sample(x.cuda(), u.cuda(), temperature=t).cpu().tolist() == hot
+    for t, want in ((1e-45, cold), (float("inf"), hot), (float("nan"), cold)):
+        ts = torch.full((3,), t, device="cuda:0")
+        for kw in (dict(), dict(top_p=0.9999), dict(top_k=V), dict(min_p=1e-3)):
+            assert _c().sample(x.cuda(), u.cuda(), temperature=ts, **kw).cpu().tolist() == want
+
+
+def test_settings_of_rows_outside_their_ranges(hip_device):
+    """Per-row settings are not read by the host: each has a meaning for any value."""
+    V = 300
+    x = torch.randn(6, V, generator=torch.Generator().manual_seed(2)).cuda()
+    u = _uniforms(6, 3).cuda()
+    nan = float("nan")
+    plain = _c().sample(x, u)
+    first = x.argmax(dim=-1)
+    dev = lambda v, d: torch.tensor(v, dtype=d, device="cuda:0")          # noqa: E731
+    got = _c().sample(x, u, top_p=dev([nan, 2.0, 1.0, -1.0, 0.0, 1e9], torch.float32))
+    assert torch.equal(got, torch.where(dev([1, 1, 1, 0, 0, 1], torch.bool), plain, first))
+    got = _c().sample(x, u, min_p=dev([nan, -1.0, 0.0, 2.0, 1e9, -nan], torch.float32))
+    assert torch.equal(got, torch.where(dev([1, 1, 1, 0, 0, 1], torch.bool), plain, first))
+    got = _c().sample(x, u, top_k=dev([-5, 0, V, 1, V + 9, 2 ** 31 - 1], torch.int32))
+    assert torch.equal(got, torch.where(dev([1, 1, 1, 0, 1, 1], torch.bool), plain, first))
+
+
+@pytest.mark.parametrize("where", ["cpu", "cuda:0"])
+def test_sample_token_with_cuts(hip_device, where):
+    """The generation loops' draw with top_p and min_p: the definition's token for
+    the random numbers of the device's generator."""
+    from intel_kivi_hybrid_amd.generation import sample_token
+    x = 2 * torch.randn(5, 700, generator=torch.Generator().manual_seed(7))
+    for kw in (dict(top_p=0.8), dict(min_p=0.1), dict(top_p=0.9, min_p=0.02)):
+        torch.manual_seed(11)
+        got = sample_token(x.to(where), 0.8, 50, True, **kw)
+        torch.manual_seed(11)
+        u = torch.rand(5, dtype=torch.float64, device=where).cpu().numpy()
+        assert got.shape == (5, 1) and got.device == torch.device(where)
+        for i in range(5):
+            want, margin = _reference(x[i].double().numpy(), u[i], 0.8, 50,
+                                      kw.get("top_p", 1.0), kw.get("min_p", 0.0))
+            assert margin > 2.0 ** -25 and int(got[i]) == want
+    x[2] = -float("inf")
+    with pytest.raises(ValueError, match="none above -infinity"):
+        sample_token(x.to(where), 0.8, None, True, top_p=0.9)
+
+
+def test_generate_packed_with_cuts(hip_device):
+    """The loop passes them on: with top_p so small that one token is left the draw
+    is the greedy one; with less cut it draws the same again after the same seed."""
+    import importlib
+    from transformers import GPT2Config, GPT2LMHeadModel
+    gen = importlib.import_module("intel_kivi_hybrid_amd.generation.generate")
+    torch.manual_seed(0)
+    model = GPT2LMHeadModel(GPT2Config(n_layer=2, n_head=2, n_embd=128, vocab_size=97,
+                                       n_positions=256)).eval().to("cuda:0")
+
+    class Tok:
+        eos_token_id = None
+
+        def __call__(self, prompt, return_tensors="pt"):
+            return type("Enc", (), {"input_ids": torch.tensor([[1 + ord(c) % 96 for c in prompt]])})
+
+        def decode(self, ids, skip_special_tokens=True):
+            return " ".join(str(int(t)) for t in ids)
+    args = (model, Tok(), "a prompt of some tokens")
+    kw = dict(max_new_tokens=12, group_size=32, residual_length=32)
+    greedy = gen.generate_packed(*args, **kw)
+    assert gen.generate_packed(*args, do_sample=True, top_p=1e-6, **kw) == greedy
+    assert gen.generate_packed(*args, do_sample=True, min_p=1.0, **kw) == greedy
+    texts = []
+    for seed in (5, 5, 6):
+        torch.manual_seed(seed)
+        texts.append(gen.generate_packed(*args, do_sample=True, temperature=3.0, top_p=0.95, **kw))
+    assert texts[0] == texts[1] != texts[2]
