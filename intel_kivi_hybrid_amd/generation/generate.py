@@ -69,14 +69,12 @@ def generate(model, tokenizer, prompt: str, max_new_tokens: int = 200, group_siz
 def generate_packed(model, tokenizer, prompt: str, max_new_tokens: int = 200,
                     group_size: int = 32, residual_length: int = 128, device: str = "cuda",
                     temperature: float = 1.0, top_k: Optional[int] = None,
-                    do_sample: bool = False, verbose: bool = False,
-                    top_p: Optional[float] = None, min_p: Optional[float] = None) -> str:
+                    do_sample: bool = False, verbose: bool = False) -> str:
     """:func:`generate` with the model attending straight from the 2-bit store.
 
     Same arguments, token selection and stopping rule as the reference's
-    ``generate`` (generate.py:13-89) -- and ``top_p``, ``min_p``, which cut what
-    is sampled from further (:func:`sample_token`) -- and the same cache semantics:
-    the prompt pass attends over its own fp32 K/V, every decode step attends over
+    ``generate`` (generate.py:13-89), and the same cache semantics: the
+    prompt pass attends over its own fp32 K/V, every decode step attends over
     [dequantised history ; fp32 residual ; new token], and the G oldest
     residual tokens are quantised after a step leaves R or more.  The cache is
     a :class:`KiviPackedCache` that the model updates itself, and the decode
@@ -90,15 +88,13 @@ def generate_packed(model, tokenizer, prompt: str, max_new_tokens: int = 200,
 
     with packed_attention(model):
         out = model(input_ids, past_key_values=cache, use_cache=True)
-        next_id = sample_token(out.logits[:, -1, :], temperature, top_k, do_sample,
-                               top_p, min_p)
+        next_id = sample_token(out.logits[:, -1, :], temperature, top_k, do_sample)
         generated = [next_id]
         for step in range(1, max_new_tokens):
             if eos_id is not None and next_id.item() == eos_id:
                 break
             out = model(next_id, past_key_values=cache, use_cache=True)
-            next_id = sample_token(out.logits[:, -1, :], temperature, top_k, do_sample,
-                                   top_p, min_p)
+            next_id = sample_token(out.logits[:, -1, :], temperature, top_k, do_sample)
             generated.append(next_id)
             if verbose and (step + 1) % 10 == 0:
                 print(".", end="", flush=True)

@@ -283,33 +283,3 @@ def test_sample_token_with_cuts(hip_device, where):
     x[2] = -float("inf")
     with pytest.raises(ValueError, match="none above -infinity"):
         sample_token(x.to(where), 0.8, None, True, top_p=0.9)
-
-
-def test_generate_packed_with_cuts(hip_device):
-    """The loop passes them on: with top_p so small that one token is left the draw
-    is the greedy one; with less cut it draws the same again after the same seed."""
-    import importlib
-    from transformers import GPT2Config, GPT2LMHeadModel
-    gen = importlib.import_module("intel_kivi_hybrid_amd.generation.generate")
-    torch.manual_seed(0)
-    model = GPT2LMHeadModel(GPT2Config(n_layer=2, n_head=2, n_embd=128, vocab_size=97,
-                                       n_positions=256)).eval().to("cuda:0")
-
-    class Tok:
-        eos_token_id = None
-
-        def __call__(self, prompt, return_tensors="pt"):
-            return type("Enc", (), {"input_ids": torch.tensor([[1 + ord(c) % 96 for c in prompt]])})
-
-        def decode(self, ids, skip_special_tokens=True):
-            return " ".join(str(int(t)) for t in ids)
-    args = (model, Tok(), "a prompt of some tokens")
-    kw = dict(max_new_tokens=12, group_size=32, residual_length=32)
-    greedy = gen.generate_packed(*args, **kw)
-    assert gen.generate_packed(*args, do_sample=True, top_p=1e-6, **kw) == greedy
-    assert gen.generate_packed(*args, do_sample=True, min_p=1.0, **kw) == greedy
-    texts = []
-    for seed in (5, 5, 6):
-        torch.manual_seed(seed)
-        texts.append(gen.generate_packed(*args, do_sample=True, temperature=3.0, top_p=0.95, **kw))
-    assert texts[0] == texts[1] != texts[2]

@@ -47,11 +47,9 @@ def test_entry_point_rejects_bad_arguments():
 
 
 def test_sample_token_takes_the_cuts_as_options():
-    from intel_kivi_hybrid_amd import generate_packed
     from intel_kivi_hybrid_amd.generation import sample_token
-    for f in (sample_token, generate_packed):
-        d = inspect.signature(f).parameters
-        assert d["top_p"].default is None and d["min_p"].default is None
+    d = inspect.signature(sample_token).parameters
+    assert d["top_p"].default is None and d["min_p"].default is None
     # greedy stays the argmax, whatever the cuts
     logits = torch.tensor([[0.1, 3.0, -1.0, 2.9], [5.0, 0.0, 0.0, 0.0]])
     assert sample_token(logits, 1.0, None, False, top_p=0.1, min_p=0.5).tolist() == [[1], [0]]
