@@ -266,11 +266,18 @@ struct Cut {
 
 // Costs in positions, as measured: an item's start; what a row of a partial
 // adds to it (written, then read by the merge); the merge's launch.
-constexpr int64_t kStart = 64, kPartialRow = 4, kMerge = 96;
+struct Costs {
+    int64_t start, partial_row, merge;
+};
+constexpr Costs paged_costs(int kind, bool f32) {
+    // (fp32's products of 64 rows take four times as long for a position)
+    return f32 && kind == kFew64 ? Costs{16, 1, 24} : Costs{64, 4, 96};
+}
 
 // The cut whose items, dealt in order to `machines` workgroups as these come
 // free, end first.
-Cut best_cut(const std::vector<Tile>& tiles, const std::vector<int>& rows, int64_t machines) {
+Cut best_cut(const std::vector<Tile>& tiles, const std::vector<int>& rows, int64_t machines,
+             Costs cost) {
     Cut best{tiles.size(), 64};
     int64_t best_end = INT64_MAX;
     const int64_t longest = tiles.empty() ? 0 : tiles.front().end;
@@ -292,7 +299,7 @@ Cut best_cut(const std::vector<Tile>& tiles, const std::vector<int>& rows, int64
                 const int64_t k = cut.pieces(i, tiles[i].end);
                 merge |= k > 1;
                 const int64_t each =
-                    tiles[i].end / k + kStart + (k > 1 ? kPartialRow * rows[i] : 0);
+                    tiles[i].end / k + cost.start + (k > 1 ? cost.partial_row * rows[i] : 0);
                 for (int64_t j = 0; j < k; ++j) {
                     std::pop_heap(busy.begin(), busy.end(), std::greater<int64_t>());
                     busy.back() += each;
@@ -300,7 +307,7 @@ Cut best_cut(const std::vector<Tile>& tiles, const std::vector<int>& rows, int64
                     std::push_heap(busy.begin(), busy.end(), std::greater<int64_t>());
                 }
             }
-            if (merge) end += kMerge;
+            if (merge) end += cost.merge;
             if (end < best_end) {
                 best_end = end;
                 best = cut;
@@ -386,7 +393,7 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
         int few = kFew16;
         for (int s = 0; s < n_seqs; ++s) {
             const int kind = paged_kind((int64_t)new_lens[s] * hg, f32, head_dim);
-            if (kind == kFew64) few = kFew64;
+            if (kind == kFew64 && !f32) few = kFew64;
         }
         std::vector<Tile> tiles[kPagedKinds];
         for (int s = 0; s < n_seqs; ++s) {
@@ -410,8 +417,9 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
             for (const Tile& t : of)
                 rows.push_back((int)std::min<int64_t>(paged_tile_rows(kind),
                                                       (int64_t)new_lens[t.seq] * hg - t.row0));
-            const int64_t slots = paged_slots(kind, head_dim);
-            cuts[kind] = best_cut(of, rows, std::max<int64_t>(1, slots / kv_heads));
+            const int64_t slots = paged_slots(kind, f32, head_dim);
+            cuts[kind] = best_cut(of, rows, std::max<int64_t>(1, slots / kv_heads),
+                                  paged_costs(kind, f32));
             for (size_t i = 0; i < of.size(); ++i) {
                 const int64_t splits = cuts[kind].pieces(i, of[i].end);
                 items += splits;
@@ -424,7 +432,8 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
             }
         }
         const int64_t pages_at = 2 * tokens, items_at = (pages_at + pages + 7) / 8 * 8;
-        const int64_t merges_at = items_at + 8 * items, ints = merges_at + 8 * merges;
+        const int64_t merges_at = items_at + 8 * items, zeros_at = merges_at + 8 * merges;
+        const int64_t ints = tokens > 0 ? zeros_at + 8 : 0;
         if (ints > INT32_MAX || parts > INT32_MAX / 64)
             return set_error(kErrInvalidArgument, "a plan of %lld words is too large",
                              (long long)ints);
@@ -439,7 +448,8 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
         info[kInfoParts] = parts;
         info[kInfoPartRows] = part_rows;
         info[kInfoContext] = longest;
-        if (plan == nullptr) return kOk;
+        info[kInfoZerosAt] = zeros_at;
+        if (plan == nullptr || tokens == 0) return kOk;
         if (plan_ints < ints)
             return set_error(kErrInvalidArgument, "the plan needs %lld words, got %lld",
                              (long long)ints, (long long)plan_ints);
@@ -461,6 +471,7 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
             }
         }
         for (int64_t i = pages_at + pages; i < items_at; ++i) plan[i] = 0;
+        for (int64_t i = zeros_at; i < ints; ++i) plan[i] = 0;
         PagedItem* item = reinterpret_cast<PagedItem*>(plan + items_at);
         PagedMerge* merge = reinterpret_cast<PagedMerge*>(plan + merges_at);
         int32_t part = 0;

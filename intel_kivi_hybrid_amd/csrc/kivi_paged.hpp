@@ -11,6 +11,7 @@
 //   pages   [pages]       the sequences' page lists, one after the other
 //   items   [items][8]    PagedItem: one workgroup's work for one kv head
 //   merges  [merges][8]   PagedMerge: row tiles whose context is split
+//   zeros   [8]           what lanes behind the head's channels load
 #pragma once
 
 #include "kivi_common.hpp"
@@ -43,28 +44,27 @@ struct PagedMerge {
 
 static_assert(sizeof(PagedItem) == 32 && sizeof(PagedMerge) == 32, "plan records");
 
-// Kinds of attention items, by the rows of a tile: a kind is one launch.
-enum PagedKind : int { kFew16 = 0, kFew32 = 1, kFew64 = 2, kMany = 3, kPagedKinds = 4 };
+// Kinds of attention items: kind k takes 16 << k rows (none 32), and is one launch.
+enum PagedKind : int { kFew16 = 0, kFew64 = 2, kMany = 3, kPagedKinds = 4 };
 
-constexpr int paged_tile_rows(int kind) { return kind == kMany ? 128 : 16 << kind; }
+constexpr int paged_tile_rows(int kind) { return 16 << kind; }
 
 // The kind that takes `rows` rows of a kv head.  fp32 has a kernel of 16 rows and
-// one of 32 (whose outputs no longer fit the registers above 128 channels), more
-// rows in tiles of these; the 16-bit types one of 16, one of 64 (four buffers of
-// tiles fit the LDS up to 128 channels) and one for many.
+// one of 64, which takes all larger numbers; the 16-bit types one of 16, one of 64
+// (four buffers of tiles fit the LDS up to 128 channels) and one of 128.
 constexpr int paged_kind(int64_t rows, bool f32, int head_dim) {
     if (rows <= 16) return kFew16;
-    if (f32) return head_dim <= 128 ? kFew32 : kFew16;
+    if (f32) return kFew64;
     return rows <= 64 && head_dim <= 128 ? kFew64 : kMany;
 }
 // Workgroups that the card works on at once: 256 CUs, and as many on each as the
-// kernels' registers or LDS leave room for (kFew32, fp32 alone: one, two would
-// share the matrix cores that bound it).
-constexpr int paged_slots(int kind, int head_dim) {
+// kernels' registers or LDS leave room for (fp32's 64 rows: as bring more, more
+// than that share the matrix cores that bound it).
+constexpr int paged_slots(int kind, bool f32, int head_dim) {
     const int per_cu = kind == kMany    ? (head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1)
                        : kind == kFew16 ? (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1)
-                       : kind == kFew64 ? (head_dim <= 64 ? 2 : 1)
-                                        : 1;
+                       : f32            ? 2
+                                        : (head_dim <= 64 ? 2 : 1);
     return 256 * per_cu;
 }
 
@@ -80,6 +80,7 @@ enum PagedInfo : int {
     kInfoParts = 10,      // partials of a kv head
     kInfoPartRows = 11,   // rows of a partial (the largest tile among the split ones)
     kInfoContext = 12,    // the longest sequence
+    kInfoZerosAt = 13,
     kInfoCount = 16,
 };
 
@@ -94,6 +95,7 @@ struct PagedLaunch {
     const int32_t* pages;
     const PagedItem* items;
     const PagedMerge* merges;
+    const int32_t* zeros;
     int n_items, n_merges, n_parts, part_rows;
     int Hq, Hkv, hg, D, page_shift;
     float qscale;                 // softmax scale * log2 e

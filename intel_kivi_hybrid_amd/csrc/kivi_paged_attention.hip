@@ -99,9 +99,9 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
         return set_error(kErrInvalidArgument, "null pointer");
     const int per = 16 / src_size(dtype);
     if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out |
-         (uintptr_t)workspace) & 15 || q_token_stride % per != 0 || q_head_stride % per != 0)
+         (uintptr_t)plan | (uintptr_t)workspace) & 15 || q_token_stride % per != 0 || q_head_stride % per != 0)
         return set_error(kErrInvalidArgument,
-                         "q's rows, pages, out and workspace must be 16-byte aligned");
+                         "q's rows, pages, plan, out and workspace must be 16-byte aligned");
     const int64_t floats = part_floats(info, kv_heads, head_dim);
     if (floats > 0 && (workspace == nullptr || workspace_bytes < (size_t)floats * 4))
         return set_error(kErrInvalidArgument, "workspace must hold %lld bytes, got %zu",
@@ -115,6 +115,7 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     a.out = out;
     a.pages = plan + info[kInfoPagesAt];
     a.merges = reinterpret_cast<const PagedMerge*>(plan + info[kInfoMergesAt]);
+    a.zeros = plan + info[kInfoZerosAt];
     a.n_merges = (int)info[kInfoMerges];
     a.n_parts = (int)info[kInfoParts];
     a.part_rows = (int)info[kInfoPartRows];

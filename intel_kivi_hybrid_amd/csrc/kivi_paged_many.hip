@@ -41,22 +41,15 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) paged_many_kernel(P
     auto step = [&](unsigned char* now, unsigned char* next) {
         wait_loads();
         if (t0 + kTile > min(wg_all, end) && loads.template mend<DT>(now, t0, end)) odd = 1;
-        lds_barrier();
+        tile_barrier();
         if (t0 + kTile < end) loads.issue(a, w, next, t0 + kTile, t0 + 2 * kTile);
         if (t0 < rows.last) rows.tile(now, now + M::BYTES, t0, end, a.qscale);
         t0 += kTile;
     };
 
     loads.pages_of(a, w, t0);
-    if (a.D != M::SL * 8) {
-        // (vectors behind the head's channels, which no load writes)
-        for (int i = threadIdx.x; i < 2 * M::BYTES / 16; i += kBlock) {
-            reinterpret_cast<u32x4_t*>(buf0)[i] = u32x4_t{0, 0, 0, 0};
-            reinterpret_cast<u32x4_t*>(buf1)[i] = u32x4_t{0, 0, 0, 0};
-        }
-    }
     if (threadIdx.x == 0) odd = 0;
-    lds_barrier();
+    tile_barrier();
     loads.issue(a, w, buf0, t0, t0 + kTile);
     while (true) {
         step(buf0, buf1);

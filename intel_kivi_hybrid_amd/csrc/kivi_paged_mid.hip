@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kBlock) paged_mid_kernel(PagedLaunch a) {
         else if (t0 + kTile < end) wait_loads<kLoads>();
         else wait_loads<0>();
         if (t0 + kTile > min(all_see, end) && loads.template mend<DT>(now, t0, end)) odd = 1;
-        lds_barrier();
+        tile_barrier();
         if (t0 + 3 * kTile < end) loads.issue(a, w, last, t0 + 3 * kTile, t0 + 4 * kTile);
         const int at = t0 + 32 * part;
         if (at < rows.last)
@@ -60,19 +60,10 @@ __global__ void __launch_bounds__(kBlock) paged_mid_kernel(PagedLaunch a) {
     };
 
     loads.pages_of(a, w, t0);
-    if (a.D != M::SL * 8) {
-        // (vectors behind the head's channels, which no load writes)
-        for (int i = threadIdx.x; i < 2 * M::BYTES / 16; i += kBlock) {
-            reinterpret_cast<u32x4_t*>(buf0)[i] = u32x4_t{0, 0, 0, 0};
-            reinterpret_cast<u32x4_t*>(buf1)[i] = u32x4_t{0, 0, 0, 0};
-            reinterpret_cast<u32x4_t*>(buf2)[i] = u32x4_t{0, 0, 0, 0};
-            reinterpret_cast<u32x4_t*>(buf3)[i] = u32x4_t{0, 0, 0, 0};
-        }
-    }
     if (threadIdx.x == 0) odd = 0;
     // (the queries' loads first: the waits count the tiles' alone)
     wait_loads<0>();
-    lds_barrier();
+    tile_barrier();
     loads.issue(a, w, buf0, t0, t0 + kTile);
     if (t0 + kTile < end) loads.issue(a, w, buf1, t0 + kTile, t0 + 2 * kTile);
     if (t0 + 2 * kTile < end) loads.issue(a, w, buf2, t0 + 2 * kTile, t0 + 3 * kTile);

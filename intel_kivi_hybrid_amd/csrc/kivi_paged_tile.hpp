@@ -33,10 +33,13 @@ struct TileShape {
     }
 };
 
-// 64 lanes' 16 bytes from memory to 1024 consecutive bytes of LDS.
-__device__ __forceinline__ void load_lds(const uint16_t* base, uint32_t off, unsigned char* lds) {
+// 64 lanes' 16 bytes from memory to 1024 consecutive bytes of LDS; lanes behind the
+// head's channels bring zeros (all lanes load: with some of them masked, the number
+// of loads in flight is not known, and every wait becomes one for all of them).
+__device__ __forceinline__ void load_lds(const PagedLaunch& a, const void* from, bool inside,
+                                         unsigned char* lds) {
     __builtin_amdgcn_global_load_lds(
-        (const __attribute__((address_space(1))) void*)(base + off),
+        (const __attribute__((address_space(1))) void*)(inside ? from : a.zeros),
         (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 // All but the wave's last N loads have arrived (they do in order).
@@ -44,6 +47,13 @@ template <int N = 0>
 __device__ __forceinline__ void wait_loads() {
     static_assert(N < 64, "the counter's range");
     __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+}
+
+// Workgroup barrier behind which the tiles waited for are whole, and the buffers
+// read before it free.  A fence would wait for the loads in flight too: they write
+// LDS, which it orders.
+__device__ __forceinline__ void tile_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 // Instruction kinds of __builtin_amdgcn_sched_group_barrier.
@@ -189,7 +199,7 @@ struct TileLoads {
     using M = TileShape<DP, TOKENS>;
     static constexpr int LD = TOKENS / M::ROWS / GROUP;     // loads of a wave for a tile's keys
     int wave;                                               // within the group
-    int page[LD];
+    int page[LD];                                           // (whole: the first alone)
     uint32_t k_off[LD], v_off[LD];                          // the lane's, in the tile's rows
     bool whole;                                             // pages hold tiles
 
@@ -215,47 +225,38 @@ struct TileLoads {
         return (slot ^ (key ? M::key_swizzle(t) : M::value_swizzle(t))) * 8;
     }
     __device__ __forceinline__ void pages_of(const PagedLaunch& a, const Work& w, int t0) {
-        if (whole) {
-            page[0] = block_page(a, w, t0);
-            return;
-        }
+        // (a store of page[0] on either side of a branch is merged with another's, and
+        // the array then lies in scratch memory)
+        page[0] = block_page(a, w, t0 + (whole ? 0 : block_of(0)));
+        if (whole) return;
 #pragma unroll
-        for (int i = 0; i < LD; ++i) page[i] = block_page(a, w, t0 + block_of(i));
+        for (int i = 1; i < LD; ++i) page[i] = block_page(a, w, t0 + block_of(i));
     }
     // Loads the tile at t0 (whose pages are known), then its successor's pages.
     __device__ __forceinline__ void issue(const PagedLaunch& a, const Work& w, unsigned char* buf,
                                           int t0, int next) {
-        const bool full = a.D == M::SL * 8;
         unsigned char* to = buf + wave * 1024;
-        if (whole) {
-            const uint16_t* k = block_at<uint16_t>(a, w, a.k_pages, page[0], t0);
-            const uint16_t* v = block_at<uint16_t>(a, w, a.v_pages, page[0], t0);
-            if (full) {
+        const uint16_t *k[LD], *v[LD];
+        k[0] = block_at<uint16_t>(a, w, a.k_pages, page[0], t0 + (whole ? 0 : block_of(0)));
+        v[0] = block_at<uint16_t>(a, w, a.v_pages, page[0], t0 + (whole ? 0 : block_of(0)));
 #pragma unroll
-                for (int i = 0; i < LD; ++i) {
-                    load_lds(k, k_off[i], to + i * GROUP * 1024);
-                    load_lds(v, v_off[i], to + i * GROUP * 1024 + M::BYTES);
-                }
-            } else {
+        for (int i = 1; i < LD; ++i) {
+            k[i] = k[0];
+            v[i] = v[0];
+        }
+        if (!whole) {
 #pragma unroll
-                for (int i = 0; i < LD; ++i) {
-                    if (channel(i, true) < a.D) load_lds(k, k_off[i], to + i * GROUP * 1024);
-                    if (channel(i, false) < a.D)
-                        load_lds(v, v_off[i], to + i * GROUP * 1024 + M::BYTES);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < LD; ++i) {
-                const int t = t0 + block_of(i);
-                const uint16_t* k = block_at<uint16_t>(a, w, a.k_pages, page[i], t);
-                const uint16_t* v = block_at<uint16_t>(a, w, a.v_pages, page[i], t);
-                if (channel(i, true) < a.D) load_lds(k, k_off[i], to + i * GROUP * 1024);
-                if (channel(i, false) < a.D)
-                    load_lds(v, v_off[i], to + i * GROUP * 1024 + M::BYTES);
+            for (int i = 1; i < LD; ++i) {
+                k[i] = block_at<uint16_t>(a, w, a.k_pages, page[i], t0 + block_of(i));
+                v[i] = block_at<uint16_t>(a, w, a.v_pages, page[i], t0 + block_of(i));
             }
         }
         pages_of(a, w, next);
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            load_lds(a, k[i] + k_off[i], channel(i, true) < a.D, to + i * GROUP * 1024);
+            load_lds(a, v[i] + v_off[i], channel(i, false) < a.D, to + i * GROUP * 1024 + M::BYTES);
+        }
     }
     // The lane's own part of a tile that has arrived and that some row does not see
     // to its end: zeros behind the end (weight 0 of whatever lies there) and for
