@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) paged_many_kernel(P
         if (t0 + kTile > min(wg_all, end) && loads.template mend<DT>(now, t0, end)) odd = 1;
         tile_barrier();
         if (t0 + kTile < end) loads.issue(a, w, next, t0 + kTile, t0 + 2 * kTile);
-        if (t0 < rows.last) rows.tile(now, now + M::BYTES, t0, end, a.qscale);
+        if (t0 < rows.last) rows.tile(now, 0, M::BYTES, t0, end, a.qscale);
         t0 += kTile;
     };
 

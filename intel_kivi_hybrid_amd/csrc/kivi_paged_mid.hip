@@ -54,8 +54,7 @@ __global__ void __launch_bounds__(kBlock) paged_mid_kernel(PagedLaunch a) {
         if (t0 + 3 * kTile < end) loads.issue(a, w, last, t0 + 3 * kTile, t0 + 4 * kTile);
         const int at = t0 + 32 * part;
         if (at < rows.last)
-            rows.tile(now + 32 * part * M::ROW, now + M::BYTES + 32 * part * M::ROW, at, end,
-                      a.qscale);
+            rows.tile(now, 32 * part * M::ROW, M::BYTES + 32 * part * M::ROW, at, end, a.qscale);
         t0 += kTile;
     };
 

@@ -93,8 +93,10 @@ struct TileRows {
         last = row0 < w.rows ? min(base + min(row0 + 31, w.rows - 1) / w.hg, w.it.kv_end) : 0;
     }
 
-    // A tile of keys (kb) and values (vb) in LDS, positions t0 ..
-    __device__ __forceinline__ void tile(const unsigned char* kb, const unsigned char* vb,
+    // A tile of keys (at kb of buf) and values (at vb) in LDS, positions t0 ..  (buf is
+    // the array itself and each address one sum: through a longer chain the compiler
+    // loses which array a read is of, and it then waits for the loads into the others)
+    __device__ __forceinline__ void tile(const unsigned char* buf, uint32_t kb, uint32_t vb,
                                          int t0, int end, float qscale) {
         const int lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
         f32x16_t s[M::TB];
@@ -109,7 +111,7 @@ struct TileRows {
 #pragma unroll
             for (int tb = 0; tb < M::TB; ++tb) {
                 const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(
-                    kb + (krow ^ (32 * ks)) + 32 * tb * M::ROW);
+                    buf + (kb + (krow ^ (32 * ks)) + 32 * tb * M::ROW));
                 s[tb] = mfma32<DT>(kf, qf[ks], s[tb]);
             }
         }
@@ -166,9 +168,9 @@ struct TileRows {
             }
 #pragma unroll
             for (int cb = 0; cb < M::CB; ++cb) {
-                const unsigned char* p = vb + (vrow ^ (64 * cb)) + 16 * j * M::ROW;
-                const uint2 lo = read_transposed(p);
-                const uint2 hi = read_transposed(p + 8 * M::ROW);
+                const uint32_t at = vb + (vrow ^ (64 * cb)) + 16 * j * M::ROW;
+                const uint2 lo = read_transposed(buf + at);
+                const uint2 hi = read_transposed(buf + (at + 8 * M::ROW));
                 O[cb] = mfma32<DT>(u32x4_t{lo.x, lo.y, hi.x, hi.y}, pf, O[cb]);
             }
         }
@@ -266,8 +268,8 @@ struct TileLoads {
         bool any = false;
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
-            u32x4_t* v = reinterpret_cast<u32x4_t*>(buf + M::BYTES + (i * GROUP + wave) * 1024 +
-                                                    threadIdx.x % kWave * 16);
+            u32x4_t* v = reinterpret_cast<u32x4_t*>(
+                buf + (M::BYTES + (i * GROUP + wave) * 1024 + threadIdx.x % kWave * 16));
             u32x4_t x = *v;
             if (t0 + block_of(i) + token(i) >= end) {
                 x = u32x4_t{0, 0, 0, 0};
