@@ -44,27 +44,26 @@ struct PagedMerge {
 
 static_assert(sizeof(PagedItem) == 32 && sizeof(PagedMerge) == 32, "plan records");
 
-// Kinds of attention items: kind k takes 16 << k rows (none 32), and is one launch.
+// Kinds of attention items: kind k takes 16 << k rows (none 32), and is one launch
+// (kFew64: fp32, kMany: the 16-bit types).
 enum PagedKind : int { kFew16 = 0, kFew64 = 2, kMany = 3, kPagedKinds = 4 };
 
 constexpr int paged_tile_rows(int kind) { return 16 << kind; }
 
-// The kind that takes `rows` rows of a kv head.  fp32 has a kernel of 16 rows and
-// one of 64, which takes all larger numbers; the 16-bit types one of 16, one of 64
-// (four buffers of tiles fit the LDS up to 128 channels) and one of 128.
-constexpr int paged_kind(int64_t rows, bool f32, int head_dim) {
-    if (rows <= 16) return kFew16;
-    if (f32) return kFew64;
-    return rows <= 64 && head_dim <= 128 ? kFew64 : kMany;
+// The kind that takes `rows` rows of a kv head: fp32 has kernels of 16 and 64 rows,
+// the 16-bit types of 16 and 128.  Up to 16 rows a kernel that streams them is
+// faster (64 single tokens, 32/8 heads, 8K positions: bf16 287 us, in tiles of more
+// rows 317; fp32, 4K positions: 282 and 331), from there on the larger tiles.
+constexpr int paged_kind(int64_t rows, bool f32) {
+    return rows <= 16 ? kFew16 : f32 ? kFew64 : kMany;
 }
 // Workgroups that the card works on at once: 256 CUs, and as many on each as the
-// kernels' registers or LDS leave room for (fp32's 64 rows: as bring more, more
+// kernels' registers or LDS leave room for (fp32's 64 rows: as bring more; more
 // than that share the matrix cores that bound it).
-constexpr int paged_slots(int kind, bool f32, int head_dim) {
+constexpr int paged_slots(int kind, int head_dim) {
     const int per_cu = kind == kMany    ? (head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1)
                        : kind == kFew16 ? (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1)
-                       : f32            ? 2
-                                        : (head_dim <= 64 ? 2 : 1);
+                                        : 2;
     return 256 * per_cu;
 }
 

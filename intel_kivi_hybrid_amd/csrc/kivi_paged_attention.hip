@@ -20,7 +20,9 @@ namespace {
 
 constexpr int kMergeBlock = 256;
 
-// Joins partials: a thread takes four channels of a row.
+// Joins partials: a thread takes four channels of a row.  Bound by its reads of the
+// partials, and for few of them by one trip to memory: 4 us for a single token's 8
+// splits, 17 us for the 45 MB of two chunks of 777 tokens and 30 single ones.
 template <int DT>
 __global__ void __launch_bounds__(kMergeBlock) paged_merge_kernel(PagedLaunch a) {
     const int per_row = a.D / 4;
@@ -99,7 +101,8 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
         return set_error(kErrInvalidArgument, "null pointer");
     const int per = 16 / src_size(dtype);
     if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out |
-         (uintptr_t)plan | (uintptr_t)workspace) & 15 || q_token_stride % per != 0 || q_head_stride % per != 0)
+         (uintptr_t)plan | (uintptr_t)workspace) & 15 ||
+        q_token_stride % per != 0 || q_head_stride % per != 0)
         return set_error(kErrInvalidArgument,
                          "q's rows, pages, plan, out and workspace must be 16-byte aligned");
     const int64_t floats = part_floats(info, kv_heads, head_dim);
@@ -141,8 +144,7 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
                              a.n_items);
         if (kind == kMany) launch_paged_many(a, dtype, s);
         else if (dtype == kSrcF32) launch_paged_f32(a, kind, s);
-        else if (kind == kFew16) launch_paged_few(a, dtype, s);
-        else launch_paged_mid(a, dtype, s);
+        else launch_paged_few(a, dtype, s);
         const int rc = check_launch("paged_attention");
         if (rc) return rc;
     }

@@ -230,7 +230,6 @@ __device__ __forceinline__ void join_waves(const PagedLaunch& a, const Work& w, 
 }  // namespace
 
 void launch_paged_few(const PagedLaunch& a, int dtype, hipStream_t s);
-void launch_paged_mid(const PagedLaunch& a, int dtype, hipStream_t s);
 void launch_paged_f32(const PagedLaunch& a, int kind, hipStream_t s);
 void launch_paged_many(const PagedLaunch& a, int dtype, hipStream_t s);
 

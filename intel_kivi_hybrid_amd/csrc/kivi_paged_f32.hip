@@ -388,7 +388,8 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 3 : 2) paged_f32_many_kern
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int c = 64 * cg + 16 * gq + 4 * i;
-            if (c < a.D) finish<kSrcF32>(a, w, r, c, rows.out(cg, i), rows.m, rows.l, odd != 0, kTile);
+            if (c < a.D)
+                finish<kSrcF32>(a, w, r, c, rows.out(cg, i), rows.m, rows.l, odd != 0, kTile);
         }
     }
 }

@@ -1,5 +1,5 @@
 // Tiles of keys and values in LDS and the products of 32 query rows with them
-// (16-bit types), for the kernels that load their tiles straight into LDS.
+// (16-bit types), where tiles go from memory straight into LDS.
 //
 // Such a load (64 lanes of 16 bytes) fills 1024 consecutive bytes, so token rows
 // lie unpadded there, and the vectors of a token are permuted instead, by the
@@ -34,20 +34,16 @@ struct TileShape {
 };
 
 // 64 lanes' 16 bytes from memory to 1024 consecutive bytes of LDS; lanes behind the
-// head's channels bring zeros (all lanes load: with some of them masked, the number
-// of loads in flight is not known, and every wait becomes one for all of them).
+// head's channels bring zeros, so no load stands behind a branch that depends on the
+// lane and no LDS has to be cleared.
 __device__ __forceinline__ void load_lds(const PagedLaunch& a, const void* from, bool inside,
                                          unsigned char* lds) {
     __builtin_amdgcn_global_load_lds(
         (const __attribute__((address_space(1))) void*)(inside ? from : a.zeros),
         (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
-// All but the wave's last N loads have arrived (they do in order).
-template <int N = 0>
-__device__ __forceinline__ void wait_loads() {
-    static_assert(N < 64, "the counter's range");
-    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
-}
+// The wave's loads have arrived.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 // Workgroup barrier behind which the tiles waited for are whole, and the buffers
 // read before it free.  A fence would wait for the loads in flight too: they write
@@ -191,22 +187,22 @@ struct TileRows {
     }
 };
 
-// How a workgroup's or wave's lanes load a tile: load i of GROUP waves covers
+// How a workgroup's lanes load a tile: load i of one of its WAVES waves covers
 // ROWS tokens of one block of 16 positions, whose page is the same for the whole
 // wave; a lane's place in the block is the same for every tile.  Pages of at
 // least a tile's size hold the whole tile: one page and one address for it (four
 // of each, with their 64-bit products, were 160 scalar instructions a tile).
-template <int DP, int TOKENS, int GROUP>
+template <int DP, int TOKENS, int WAVES>
 struct TileLoads {
     using M = TileShape<DP, TOKENS>;
-    static constexpr int LD = TOKENS / M::ROWS / GROUP;     // loads of a wave for a tile's keys
-    int wave;                                               // within the group
+    static constexpr int LD = TOKENS / M::ROWS / WAVES;     // loads of a wave for a tile's keys
+    int wave;
     int page[LD];                                           // (whole: the first alone)
     uint32_t k_off[LD], v_off[LD];                          // the lane's, in the tile's rows
     bool whole;                                             // pages hold tiles
 
-    __device__ __forceinline__ void init(const PagedLaunch& a, int wave_in_group) {
-        wave = wave_in_group;
+    __device__ __forceinline__ void init(const PagedLaunch& a, int w) {
+        wave = w;
         whole = 1 << a.page_shift >= TOKENS;
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
@@ -216,11 +212,11 @@ struct TileLoads {
         }
     }
     __device__ __forceinline__ int block_of(int i) const {
-        return (i * GROUP + wave) * M::ROWS / 16 * 16;
+        return (i * WAVES + wave) * M::ROWS / 16 * 16;
     }
     // the token (of its block) and channel that the lane loads
     __device__ __forceinline__ int token(int i) const {
-        return ((i * GROUP + wave) * M::ROWS + threadIdx.x % kWave / M::SL) % 16;
+        return ((i * WAVES + wave) * M::ROWS + threadIdx.x % kWave / M::SL) % 16;
     }
     __device__ __forceinline__ int channel(int i, bool key) const {
         const int t = token(i), slot = threadIdx.x % kWave % M::SL;
@@ -256,8 +252,8 @@ struct TileLoads {
         pages_of(a, w, next);
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
-            load_lds(a, k[i] + k_off[i], channel(i, true) < a.D, to + i * GROUP * 1024);
-            load_lds(a, v[i] + v_off[i], channel(i, false) < a.D, to + i * GROUP * 1024 + M::BYTES);
+            load_lds(a, k[i] + k_off[i], channel(i, true) < a.D, to + i * WAVES * 1024);
+            load_lds(a, v[i] + v_off[i], channel(i, false) < a.D, to + i * WAVES * 1024 + M::BYTES);
         }
     }
     // The lane's own part of a tile that has arrived and that some row does not see
@@ -269,7 +265,7 @@ struct TileLoads {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             u32x4_t* v = reinterpret_cast<u32x4_t*>(
-                buf + (M::BYTES + (i * GROUP + wave) * 1024 + threadIdx.x % kWave * 16));
+                buf + (M::BYTES + (i * WAVES + wave) * 1024 + threadIdx.x % kWave * 16));
             u32x4_t x = *v;
             if (t0 + block_of(i) + token(i) >= end) {
                 x = u32x4_t{0, 0, 0, 0};
