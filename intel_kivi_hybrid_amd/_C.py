@@ -755,6 +755,9 @@ class PagedPlan:
         return handle
 
 
+_PLAN_ITEMS = 1 << 13        # int32s of a plan's items that a first buffer has room for
+
+
 def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_heads, kv_heads,
                head_dim, dtype=torch.bfloat16, device="cuda") -> PagedPlan:
     """The plan of a step in which sequence s, ``context_lens[s]`` tokens long
@@ -785,7 +788,16 @@ def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_he
     p._info, p._info_ptr = info, ctypes.addressof(info)
     args = (n_seqs, new.data_ptr(), ctx.data_ptr(), table.data_ptr(), table.shape[1],
             table.shape[1], page_size, num_pages, _IO_DTYPES[dtype], q_heads, kv_heads, head_dim)
-    _native.check(_lib.kivi_paged_plan(*args, None, 0, p._info_ptr), "paged_plan")
+    # (one call where a buffer of the usual size will do; on a host that has not used
+    # its GPU yet the arguments are checked first)
+    host = None
+    if torch.cuda.is_initialized():
+        host = torch.empty(table.numel() + 2 * min(max(int(new.sum()), 0), 1 << 20) + _PLAN_ITEMS,
+                           dtype=torch.int32, pin_memory=True)
+    rc = _lib.kivi_paged_plan(*args, None if host is None else host.data_ptr(),
+                              0 if host is None else host.numel(), p._info_ptr)
+    if rc and (host is None or info[0] <= host.numel()):
+        _native.check(rc, "paged_plan")
     p.device = torch.device(_DEVICE_TYPE, device_index(dev))
     _check(not torch.cuda.is_current_stream_capturing(),
            "a plan is made outside of a graph's capture")
@@ -794,11 +806,12 @@ def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_he
     p.q_heads, p.kv_heads, p.head_dim = q_heads, kv_heads, head_dim
     p._index = p.device.index
     p._pool = torch.Size((num_pages, kv_heads, page_size, head_dim))
-    host = torch.empty(max(info[0], 1), dtype=torch.int32, pin_memory=True)
-    _native.check(_lib.kivi_paged_plan(*args, host.data_ptr(), host.numel(), p._info_ptr),
-                  "paged_plan")
+    if host is None or info[0] > host.numel():
+        host = torch.empty(max(info[0], 1), dtype=torch.int32, pin_memory=True)
+        _native.check(_lib.kivi_paged_plan(*args, host.data_ptr(), host.numel(), p._info_ptr),
+                      "paged_plan")
     with on_device(p.device):
-        p._buf = host.to(p.device, non_blocking=True)
+        p._buf = host[:max(info[0], 1)].to(p.device, non_blocking=True)
         p._event = torch.cuda.Event()
         p._event.record()
         p._stream = stream_handle(p.device)

@@ -293,11 +293,11 @@ Cut best_cut(const std::vector<Tile>& tiles, const std::vector<int>& rows, int64
             const Cut cut{keep ? rounds : 0, T};
             int64_t items = 0;
             for (size_t i = 0; i < tiles.size(); ++i) items += cut.pieces(i, tiles[i].end);
-            if (n > 1 && items > 16 * machines) continue;
+            if (n > 1 && items > 4 * machines) continue;
             busy.assign((size_t)machines, 0);
             int64_t end = 0;
             bool merge = false;
-            for (size_t i = 0; i < tiles.size(); ++i) {
+            for (size_t i = 0; i < tiles.size() && end < best_end; ++i) {
                 const int64_t k = cut.pieces(i, tiles[i].end);
                 merge |= k > 1;
                 const int64_t each =
