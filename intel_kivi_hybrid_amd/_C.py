@@ -792,6 +792,8 @@ def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_he
     # its GPU yet the arguments are checked first)
     host = None
     if torch.cuda.is_initialized():
+        _check(not torch.cuda.is_current_stream_capturing(),
+               "a plan is made outside of a graph's capture")
         host = torch.empty(table.numel() + 2 * min(max(int(new.sum()), 0), 1 << 20) + _PLAN_ITEMS,
                            dtype=torch.int32, pin_memory=True)
     rc = _lib.kivi_paged_plan(*args, None if host is None else host.data_ptr(),
@@ -799,8 +801,6 @@ def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_he
     if rc and (host is None or info[0] <= host.numel()):
         _native.check(rc, "paged_plan")
     p.device = torch.device(_DEVICE_TYPE, device_index(dev))
-    _check(not torch.cuda.is_current_stream_capturing(),
-           "a plan is made outside of a graph's capture")
     p.tokens, p.context = info[1], info[12]
     p.num_pages, p.page_size, p.dtype, p._code = num_pages, page_size, dtype, _IO_DTYPES[dtype]
     p.q_heads, p.kv_heads, p.head_dim = q_heads, kv_heads, head_dim
@@ -887,6 +887,7 @@ def paged_append(k, v, k_pages, v_pages, plan, q=None, q_out=None, cos=None, sin
         _check_inference(k, v, q, q_norm, k_norm)
     dev = plan._index
     kp, vp = _check_pages(plan, k_pages, v_pages)
+    _check(kp != vp or plan.tokens == 0, "k_pages and v_pages must be two pools")
     ks = _check_tokens(k, "k", plan, plan.kv_heads)
     vs = _check_tokens(v, "v", plan, plan.kv_heads)
     rot = cos_ptr = sin_ptr = 0
@@ -1047,7 +1048,8 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out
     _check(logits.stride(1) == 1 or logits.shape[1] == 1, "a row's logits must be contiguous")
     rows, vocab = logits.shape
     dev = logits.device
-    _check(uniforms.dtype in (torch.float32, torch.float64) and uniforms.dim() == 1
+    _check(isinstance(uniforms, torch.Tensor)
+           and uniforms.dtype in (torch.float32, torch.float64) and uniforms.dim() == 1
            and uniforms.shape[0] == rows and uniforms.is_contiguous() and uniforms.device == dev,
            "uniforms must be a contiguous [", rows, "] float32 or float64 tensor on ", dev)
     tp, t = _setting(temperature, "temperature", rows, torch.float32, dev)

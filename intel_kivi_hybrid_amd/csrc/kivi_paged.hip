@@ -497,7 +497,7 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
             }
         }
         return kOk;
-    } catch (const std::bad_alloc&) {
+    } catch (...) {                                      // (bad_alloc, length_error)
         return set_error(kErrRuntime, "out of host memory for a plan");
     }
 }

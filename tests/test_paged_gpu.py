@@ -386,3 +386,41 @@ def test_no_tokens(hip_device):
     k = torch.empty(0, 1, 64, dtype=BF, device="cuda:0")
     assert _c().paged_append(k, k, kd, kd, plan, q=q).shape == (0, 2, 64)
     assert np.count_nonzero(kd.float().cpu().numpy()) == 0
+
+
+def test_one_pool_for_both_and_a_plan_in_a_capture(hip_device):
+    case = _setup([(20, 2)], 32, BF, 4, 2, 64, seed=3)
+    table, pool, ctx, new, kp, vp, plan, q = case
+    kd, k = kp.cuda(), torch.randn(2, 2, 64, device="cuda:0").to(BF)
+    with pytest.raises(RuntimeError, match="must be two pools"):
+        _c().paged_append(k, k, kd, kd, plan)
+    # (reading one pool as both is the attention of keys that are the values)
+    same = (table, pool, ctx, new, kp, kp, plan, q)
+    _check(_c().paged_attention(q.cuda(), kd, kd, plan), same, 32)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="outside of a graph's capture"):
+            _c().paged_plan(table, ctx, new, page_size=32, num_pages=pool, q_heads=4, kv_heads=2,
+                            head_dim=64, device="cuda:0")
+        torch.zeros(1, device="cuda:0")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FF], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [3, 40])
+def test_output_in_the_queries_place(hip_device, dtype, n):
+    case = _setup([(3000, n), (70, 1)], 32, dtype, 8, 2, 128, seed=5)
+    table, pool, ctx, new, kp, vp, plan, q = case
+    kd, vd, qd = kp.cuda(), vp.cuda(), q.cuda()
+    want = _c().paged_attention(qd, kd, vd, plan)
+    assert _c().paged_attention(qd, kd, vd, plan, out=qd) is qd
+    assert torch.equal(qd, want)
+
+
+def test_plans_larger_than_the_usual(hip_device):
+    """More items than the first buffer holds, and the same plan from a host that
+    asks for its size first."""
+    lens = [(1, 1)] * 1500
+    case = _setup(lens, 16, BF, 4, 2, 64, seed=6)
+    assert case[6]._buf.numel() > 8 * 1500
+    _check(_attend(case), case, 16)

@@ -283,3 +283,8 @@ def test_sample_token_with_cuts(hip_device, where):
     x[2] = -float("inf")
     with pytest.raises(ValueError, match="none above -infinity"):
         sample_token(x.to(where), 0.8, None, True, top_p=0.9)
+
+
+def test_uniforms_must_be_a_tensor(hip_device):
+    with pytest.raises(RuntimeError, match="uniforms must be"):
+        _c().sample(torch.randn(2, 10, device="cuda:0"), 0.5)
