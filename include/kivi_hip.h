@@ -455,8 +455,9 @@ size_t kivi_paged_attention_workspace_size(const int64_t* info, int32_t kv_heads
  * context of c sees positions 0 .. c - n + i.  q is [tokens][q_heads][head_dim]
  * of dtype with strides of whole 16-byte vectors, out the same, contiguous; query
  * head h reads kv head h / (q_heads / kv_heads).  softmax_scale must be positive.
- * Scores, softmax and sums are fp32; weights are rounded to dtype for the product
- * with the values.  What lies behind a sequence's end or in positions that a
+ * Scores, softmax and sums are fp32; for the product with 16-bit values weights
+ * are rounded to dtype (up to 16 rows per kv head: split into two such pieces).
+ * plan is 16-byte aligned, and so are q's rows, the pages, out and workspace.  What lies behind a sequence's end or in positions that a
  * token does not see, infinities and NaN too, does not reach it.  Rows of out
  * behind the last token are left as they were. */
 int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
