@@ -53,7 +53,9 @@ constexpr int kMaxVocab = 1 << 20;        // (a row's rels stay below 2^57)
 constexpr int kList = 6144;               // tokens that a row's list holds
 constexpr int kOrder = kSlice + 16;       // a slice's tokens, and the ones outside of vectors
 constexpr int kStarts = kBuckets + 8;     // (whole 16 bytes)
-constexpr int kSub = 2048;                // sub-buckets of a crowded bucket
+// sub-buckets of a crowded bucket, in copies of which a lane takes one (16-bit logits
+// have few values: their tokens meet in few sub-buckets)
+constexpr int kSub = 512, kCopies = 4;
 
 struct SampleArgs {
     const void* logits;
@@ -468,8 +470,8 @@ struct Picker {
                 uint32_t count[kPickBlock / kFew][kFew];
             } few;
             struct {
-                uint64_t rel[kSub + 1];
-                uint32_t count[kSub + 1];
+                uint64_t rel[kSub + 1], part_rel[kCopies][kSub];
+                uint32_t count[kSub + 1], part_count[kCopies][kSub];
             } sub;
         };
         Wanted wanted;
@@ -633,43 +635,36 @@ struct Picker {
         __syncthreads();
     }
 
-    // The sub-buckets' running sums, in place.
+    // The sub-buckets' running sums from their copies.
     __device__ void scan_sub() {
-        constexpr int kPer = kSub / kPickBlock;
+        static_assert(kSub <= kPickBlock, "a thread for each sub-bucket");
         const int tid = threadIdx.x, lane = tid % kWave;
-        uint64_t r[kPer], sum = 0;
-        uint32_t c[kPer], n = 0;
+        uint64_t rel = 0;
+        uint32_t count = 0;
+        if (tid < kSub) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            r[i] = s.sub.rel[kPer * tid + i];
-            c[i] = s.sub.count[kPer * tid + i];
-            sum += r[i];
-            n += c[i];
-        }
-        uint64_t ir = sum;
-        uint32_t ic = n;
-        wave_scan(ir, ic);
-        if (lane == kWave - 1) {
-            s.wave_rel[tid / kWave] = ir;
-            s.wave_count[tid / kWave] = ic;
+            for (int i = 0; i < kCopies; ++i) {
+                rel += s.sub.part_rel[i][tid];
+                count += s.sub.part_count[i][tid];
+            }
+            wave_scan(rel, count);
+            if (lane == kWave - 1) {
+                s.wave_rel[tid / kWave] = rel;
+                s.wave_count[tid / kWave] = count;
+            }
         }
         __syncthreads();
-        ir -= sum;
-        ic -= n;
-        for (int i = 0; i < tid / kWave; ++i) {
-            ir += s.wave_rel[i];
-            ic += s.wave_count[i];
-        }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            s.sub.rel[kPer * tid + i] = ir;
-            s.sub.count[kPer * tid + i] = ic;
-            ir += r[i];
-            ic += c[i];
-        }
-        if (tid == kPickBlock - 1) {
-            s.sub.rel[kSub] = ir;
-            s.sub.count[kSub] = ic;
+        if (tid < kSub) {
+            for (int i = 0; i < tid / kWave; ++i) {
+                rel += s.wave_rel[i];
+                count += s.wave_count[i];
+            }
+            s.sub.rel[tid + 1] = rel;
+            s.sub.count[tid + 1] = count;
+            if (tid == 0) {
+                s.sub.rel[0] = 0;
+                s.sub.count[0] = 0;
+            }
         }
         __syncthreads();
     }
@@ -771,18 +766,18 @@ struct Picker {
         const Need x = need_of(kind, at, b);
         uint64_t lo = 0, hi = ~0ull, before_rel = 0;
         uint32_t before_count = 0, n = s.sums.count[b + 1] - s.sums.count[b];
-        // (a round leaves a 2048th of a range of 2^64 at most: 6 rounds)
-        for (int round = 0; n > kFew && round < 6; ++round) {
-            // counts and sums of 2048 stretches of the keys between lo and hi, from
+        // (a round leaves a 512th of a range of 2^64 at most: 7 rounds and a bit)
+        for (int round = 0; n > kFew && round < 8; ++round) {
+            // counts and sums of 512 stretches of the keys between lo and hi, from
             // the least to the most logit (or index, where all are equal)
             __syncthreads();
             if (tid == 0) {
                 s.bits_min = ~0u;
                 s.bits_max = 0;
             }
-            for (int i = tid; i < kSub; i += kPickBlock) {
-                s.sub.rel[i] = 0;
-                s.sub.count[i] = 0;
+            for (int i = tid; i < kCopies * kSub; i += kPickBlock) {
+                (&s.sub.part_rel[0][0])[i] = 0;
+                (&s.sub.part_count[0][0])[i] = 0;
             }
             __syncthreads();
             uint32_t mn = ~0u, mx = 0;
@@ -807,8 +802,9 @@ struct Picker {
             each(b, [&](uint64_t key, uint64_t rel) {
                 if (key < lo || key > hi) return;
                 const int i = (int)((key - first) >> shift);
-                atomicAdd((unsigned long long*)&s.sub.rel[i], (unsigned long long)rel);
-                atomicAdd(&s.sub.count[i], 1u);
+                const int copy = tid % kCopies;
+                atomicAdd((unsigned long long*)&s.sub.part_rel[copy][i], (unsigned long long)rel);
+                atomicAdd(&s.sub.part_count[copy][i], 1u);
             });
             __syncthreads();
             scan_sub();
