@@ -22,7 +22,7 @@ import threading
 import torch
 
 from . import _native
-from ._device import device_index, on_device, stream_handle
+from ._device import device_index, is_current, on_device, stream_handle
 
 _lib = _native.load()
 
@@ -706,8 +706,8 @@ def packed_attention_typed(q, store, softmax_scale=None, kv_start=None, hidden=N
 # --------------------------------------------------------------------------
 def _check_inference(*tensors) -> None:
     for t in tensors:
-        _check(t is None or not t.requires_grad, "inference only: a tensor requires a gradient; "
-               "call it under torch.no_grad()")
+        if t is not None and t.requires_grad:
+            _fail("inference only: a tensor requires a gradient; call it under torch.no_grad()")
 
 
 def _host_ints(values, name: str) -> torch.Tensor:
@@ -883,9 +883,13 @@ def paged_append(k, v, k_pages, v_pages, plan, q=None, q_out=None, cos=None, sin
     if ``interleaved``.  Both in fp32, rounded once.  Values are copied.  Rows may
     have any strides, as slices of one projection have; rows behind the plan's
     tokens are not read, and stay as they are in ``q_out``, which may be ``q``."""
+    dev = plan._index
+    if not is_current(dev):
+        with on_device(dev):
+            return paged_append(k, v, k_pages, v_pages, plan, q, q_out, cos, sin, interleaved,
+                                q_norm, k_norm, eps)
     if torch.is_grad_enabled():
         _check_inference(k, v, q, q_norm, k_norm)
-    dev = plan._index
     kp, vp = _check_pages(plan, k_pages, v_pages)
     _check(kp != vp or plan.tokens == 0, "k_pages and v_pages must be two pools")
     ks = _check_tokens(k, "k", plan, plan.kv_heads)
@@ -925,14 +929,13 @@ def paged_append(k, v, k_pages, v_pages, plan, q=None, q_out=None, cos=None, sin
         q_ptr, q_st, q_sh, out_ptr = q.data_ptr(), st[0], st[1], q_out.data_ptr()
     else:
         _check(q_out is None and q_norm is None, "q_out and q_norm need q")
-    with on_device(dev):
-        rc = _lib.kivi_paged_append(
-            q_ptr, q_st, q_sh, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-            plan._code, out_ptr, kp, vp, plan.num_pages, plan.page_size, plan.q_heads,
-            plan.kv_heads, plan.head_dim, plan._ptr, plan.tokens, cos_ptr, sin_ptr, rot,
-            1 if interleaved else 0, 0 if q_norm is None else q_norm.data_ptr(),
-            0 if k_norm is None else k_norm.data_ptr(),
-            0 if norm_dt is None else _IO_DTYPES[norm_dt], eps, plan._enter(dev))
+    rc = _lib.kivi_paged_append(
+        q_ptr, q_st, q_sh, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+        plan._code, out_ptr, kp, vp, plan.num_pages, plan.page_size, plan.q_heads,
+        plan.kv_heads, plan.head_dim, plan._ptr, plan.tokens, cos_ptr, sin_ptr, rot,
+        1 if interleaved else 0, 0 if q_norm is None else q_norm.data_ptr(),
+        0 if k_norm is None else k_norm.data_ptr(),
+        0 if norm_dt is None else _IO_DTYPES[norm_dt], eps, plan._enter(dev))
     if rc:
         _native.check(rc, "paged_append")
     return q_out
@@ -980,6 +983,10 @@ def paged_attention(q, k_pages, v_pages, plan, softmax_scale=None, out=None, wor
     Returns ``[tokens, Hq, D]`` in q's type.  Chunks of prompts, verification
     passes and single tokens may share a call.  Rows behind the plan's tokens are
     not read, and stay as they are in ``out``.  Launched on the current stream."""
+    dev = plan._index
+    if not is_current(dev):
+        with on_device(dev):
+            return paged_attention(q, k_pages, v_pages, plan, softmax_scale, out, workspace)
     if torch.is_grad_enabled():
         _check_inference(q)
     kp, vp = _check_pages(plan, k_pages, v_pages)
@@ -992,23 +999,22 @@ def paged_attention(q, k_pages, v_pages, plan, softmax_scale=None, out=None, wor
         out = _new_rows(q, plan)
     else:
         _check_out(out, "out", q)
-    dev = plan._index
     need = plan._workspace
     ws_ptr = ws_bytes = 0
-    with on_device(dev):
-        if need:
-            if workspace is None:
-                workspace = _call_workspace(dev, need)
-            ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-            _check(workspace.is_contiguous() and workspace.get_device() == dev
-                   and not ws_ptr & 15 and ws_bytes >= need,
-                   "workspace must be a contiguous, 16-byte aligned tensor of ", need,
-                   " bytes on ", plan.device)
-        rc = _lib.kivi_paged_attention(
-            q_ptr, st[0], st[1], plan._code, kp, vp, plan.num_pages, plan.page_size,
-            plan.q_heads, plan.kv_heads, plan.head_dim, plan._ptr, plan._info_ptr,
-            plan.head_dim ** -0.5 if softmax_scale is None else float(softmax_scale),
-            out.data_ptr(), ws_ptr, ws_bytes, plan._enter(dev))
+    if need and workspace is None:
+        workspace = _call_workspace(dev, need)         # (held until both launches are made)
+        ws_ptr, ws_bytes = workspace.data_ptr(), need
+    elif need:
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        _check(workspace.is_contiguous() and workspace.get_device() == dev
+               and not ws_ptr & 15 and ws_bytes >= need,
+               "workspace must be a contiguous, 16-byte aligned tensor of ", need,
+               " bytes on ", plan.device)
+    rc = _lib.kivi_paged_attention(
+        q_ptr, st[0], st[1], plan._code, kp, vp, plan.num_pages, plan.page_size,
+        plan.q_heads, plan.kv_heads, plan.head_dim, plan._ptr, plan._info_ptr,
+        plan.head_dim ** -0.5 if softmax_scale is None else float(softmax_scale),
+        out.data_ptr(), ws_ptr, ws_bytes, plan._enter(dev))
     if rc:
         _native.check(rc, "paged_attention")
     return out

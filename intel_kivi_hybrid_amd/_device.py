@@ -36,6 +36,10 @@ def stream_handle(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def is_current(index: int) -> bool:
+    return _current() == index
+
+
 def on_device(device):
     """A context in which ``device`` (a torch.device or an index) is the
     current device: no switch when it already is."""
