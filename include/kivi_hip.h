@@ -456,7 +456,8 @@ size_t kivi_paged_attention_workspace_size(const int64_t* info, int32_t kv_heads
  * of dtype with strides of whole 16-byte vectors, out the same, contiguous; query
  * head h reads kv head h / (q_heads / kv_heads).  softmax_scale must be positive.
  * Scores, softmax and sums are fp32; for the product with 16-bit values weights
- * are rounded to dtype (up to 16 rows per kv head: split into two such pieces).
+ * are rounded to dtype (where no sequence of the step brings more than 16 rows to
+ * a kv head they are split into two such pieces).
  * plan is 16-byte aligned, and so are q's rows, the pages, out and workspace.  What lies behind a sequence's end or in positions that a
  * token does not see, infinities and NaN too, does not reach it.  Rows of out
  * behind the last token are left as they were. */

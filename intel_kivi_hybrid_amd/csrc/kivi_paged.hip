@@ -390,13 +390,16 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
                                  runs[i].page);
 
         // Row tiles, and the positions that the last row of each sees.  Beside 16-bit
-        // sequences of 17 to 64 rows, which are as much bound by memory, those of
-        // fewer take tiles of the larger kind too, one launch for all (16 sequences
-        // of 2 or 3 tokens, 28/4 heads, 3K positions: 27 us, as two launches 32).
+        // sequences of more than 16 rows those of fewer take tiles of the larger kind
+        // too: one launch, in which their loads run beside the others' products (two
+        // chunks of 777 tokens and 30 single ones, 64/8 heads, fp16: 302 us, as two
+        // launches 354; 16 sequences of 2 or 3 tokens, 28/4 heads: 22 and 32).  Above
+        // 128 channels, where a CU holds one workgroup, only beside few rows (2 chunks
+        // of 300 and 18 single tokens, 28/4 heads of 256: 147 us, as two launches 137).
         int few = kFew16;
         for (int s = 0; s < n_seqs; ++s) {
             const int64_t rows = (int64_t)new_lens[s] * hg;
-            if (!f32 && rows > 16 && rows <= 64) few = kMany;
+            if (!f32 && rows > 16 && (rows <= 64 || head_dim <= 128)) few = kMany;
         }
         std::vector<Tile> tiles[kPagedKinds];
         for (int s = 0; s < n_seqs; ++s) {

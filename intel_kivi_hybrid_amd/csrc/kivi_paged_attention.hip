@@ -22,7 +22,7 @@ constexpr int kMergeBlock = 256;
 
 // Joins partials: a thread takes four channels of a row.  Bound by its reads of the
 // partials, and for few of them by one trip to memory: 4 us for a single token's 8
-// splits, 17 us for the 45 MB of two chunks of 777 tokens and 30 single ones.
+// splits, 17 us for 45 MB (80 pieces of 128 rows, 8 kv heads).
 template <int DT>
 __global__ void __launch_bounds__(kMergeBlock) paged_merge_kernel(PagedLaunch a) {
     const int per_row = a.D / 4;
