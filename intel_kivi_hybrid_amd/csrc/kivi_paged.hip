@@ -396,11 +396,20 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
         // launches 354; 16 sequences of 2 or 3 tokens, 28/4 heads: 22 and 32).  Above
         // 128 channels, where a CU holds one workgroup, only beside few rows (2 chunks
         // of 300 and 18 single tokens, 28/4 heads of 256: 147 us, as two launches 137).
+        // In fp32, where a tile of many rows takes few at the time of products that only
+        // one of its waves has, up to 2^24 elements of their keys (19 single tokens of 500
+        // positions beside a chunk of 94, 16/2 heads of 256, 4M elements: 35 us, as two
+        // launches 50; 28 of 4K beside two of 200, 32/8 heads of 128, 86M: 405 and 327).
         int few = kFew16;
+        int64_t small = 0;
+        bool large = false;
         for (int s = 0; s < n_seqs; ++s) {
             const int64_t rows = (int64_t)new_lens[s] * hg;
             if (!f32 && rows > 16 && (rows <= 64 || head_dim <= 128)) few = kMany;
+            if (rows > 0 && rows <= 16) small += context_lens[s];
+            large |= rows > 16;
         }
+        if (f32 && large && small <= (1 << 24) / head_dim / kv_heads) few = kFew64;
         std::vector<Tile> tiles[kPagedKinds];
         for (int s = 0; s < n_seqs; ++s) {
             const int64_t n = new_lens[s], rows = n * hg;
