@@ -413,7 +413,8 @@ int kivi_packed_decode_attention_append(
  * out) and is context_lens[s] tokens long with them; its pages are
  * page_table[s*table_stride + 0 .. ceil(context/page_size)-1], table_pages
  * entries at most.  Pages may be shared between sequences (a common prefix), but
- * no slot may be given to two new tokens.  With plan NULL only info is written:
+ * no slot may be given to two new tokens.  A context, and the new tokens times
+ * q_heads / kv_heads, are 2^31 - 4096 at most.  With plan NULL only info is written:
  * info[0] is the size of the plan in int32 words, info[1] its tokens.  The
  * caller copies the plan to the device once per step and gives the copy and info
  * to every layer's calls; it holds for pools of num_pages pages and the

@@ -348,6 +348,10 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
                 return set_error(kErrInvalidArgument,
                                  "sequence %d: %lld new tokens in a context of %lld", s,
                                  (long long)n, (long long)c);
+            if (c > kPagedMost)
+                return set_error(kErrInvalidArgument,
+                                 "sequence %d: a context of %lld, at most %lld positions are taken",
+                                 s, (long long)c, (long long)kPagedMost);
             const int64_t p = (c + page_size - 1) >> shift;
             if (p > table_pages)
                 return set_error(kErrInvalidArgument,
@@ -365,7 +369,7 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
             pages += p;
             longest = std::max(longest, c);
         }
-        if (tokens > INT32_MAX / 4 || tokens * (int64_t)hg > INT32_MAX || pages > INT32_MAX / 4)
+        if (tokens > INT32_MAX / 4 || tokens * (int64_t)hg > kPagedMost || pages > INT32_MAX / 4)
             return set_error(kErrInvalidArgument, "a step of %lld tokens over %lld pages is too "
                              "large", (long long)tokens, (long long)pages);
 

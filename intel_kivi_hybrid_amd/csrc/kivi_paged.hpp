@@ -67,6 +67,10 @@ constexpr int paged_slots(int kind, int head_dim) {
     return 256 * per_cu;
 }
 
+// Positions of a sequence, and rows of a step (tokens x heads of a kv head), at most:
+// kernels look a few tiles past the last one in 32 bits.
+constexpr int64_t kPagedMost = ((int64_t)1 << 31) - 4096;
+
 // info[] of kivi_paged_plan
 enum PagedInfo : int {
     kInfoInts = 0,        // int32s of the plan

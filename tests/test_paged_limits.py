@@ -1,0 +1,41 @@
+"""CPU tests of the paged cache's limits: sizes at which the kernels' 32-bit
+positions and rows would wrap."""
+
+import numpy as np
+import pytest
+
+
+def _info(table, pool, ctx, new, page_size, Hq, Hkv, D=16, dtype=1):
+    from intel_kivi_hybrid_amd import _native
+    lib = _native.load()
+    info = np.zeros(16, dtype=np.int64)
+    c, n = np.asarray(ctx, dtype=np.int32), np.asarray(new, dtype=np.int32)
+    rc = lib.kivi_paged_plan(len(ctx), n.ctypes.data, c.ctypes.data, table.ctypes.data,
+                             table.shape[1], table.shape[1], page_size, pool, dtype, Hq, Hkv, D,
+                             None, 0, info.ctypes.data)
+    return rc, (_native.last_error() if rc else info)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_contexts_whose_positions_would_wrap(dtype):
+    """A sequence of one page many times (a table that repeats): the kernels look a
+    few tiles past the end, in 32 bits."""
+    table = np.zeros((1, 1 << 23), dtype=np.int32)
+    longest = (1 << 31) - 4096
+    table[0, (longest - 1) >> 8] = 1
+    rc, info = _info(table, 2, [longest], [1], 256, 1, 1, dtype=dtype)
+    assert rc == 0 and info[12] == longest
+    for c in (longest + 1, (1 << 31) - 1):
+        rc, text = _info(table, 2, [c], [1], 256, 1, 1, dtype=dtype)
+        assert rc == 1 and "positions" in text
+
+
+def test_rows_that_would_wrap():
+    """Rows of a sequence and kv head (tokens x heads of its group) stay below
+    2^31 - 4096: a tile's last rows may lie behind them."""
+    table = np.arange(1 << 9, dtype=np.int32)[None]
+    n = 1 << 16
+    rc, text = _info(table, 1 << 9, [n], [n], 128, 1 << 15, 1)
+    assert rc == 1 and "too large" in text
+    rc, text = _info(table[:, :1], 1 << 9, [1], [1], 128, (1 << 31) - 1, 1)
+    assert rc == 1 and "too large" in text
