@@ -460,8 +460,9 @@ size_t kivi_paged_attention_workspace_size(const int64_t* info, int32_t kv_heads
  * are rounded to dtype (where no sequence of the step brings more than 16 rows to
  * a kv head they are split into two such pieces).
  * plan is 16-byte aligned, and so are q's rows, the pages, out and workspace.  What lies behind a sequence's end or in positions that a
- * token does not see, infinities and NaN too, does not reach it.  Rows of out
- * behind the last token are left as they were. */
+ * token does not see, infinities and NaN too, does not reach it; those in
+ * values that it sees reach it whatever their weights.  Rows of out behind the last
+ * token are left as they were. */
 int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                          int32_t dtype, const void* k_pages, const void* v_pages,
                          int64_t num_pages, int32_t page_size, int32_t q_heads,

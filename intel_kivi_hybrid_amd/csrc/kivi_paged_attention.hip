@@ -52,6 +52,17 @@ __global__ void __launch_bounds__(kMergeBlock) paged_merge_kernel(PagedLaunch a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = fmaf(y[i], f, o[i]);
     }
+    if (sum == sum && has_nan(o)) {
+        // (an infinity of a partial whose weight is 0 here: it is one all the same)
+        o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int s = 0; s < g.splits; ++s) {
+            const f32x4_t y = *reinterpret_cast<const f32x4_t*>(po + s * next_o);
+            const float f = exp2_fast(ml[s * next_ml] - top);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = non_finite(y[i]) ? o[i] + y[i] : fmaf(y[i], f, o[i]);
+        }
+    }
     const int i = r / a.hg;
     store4<DT>(a.out, ((int64_t)(g.tok0 + i) * a.Hq + kvh * a.hg + (r - i * a.hg)) * a.D + c,
                o * inverse_sum(sum));

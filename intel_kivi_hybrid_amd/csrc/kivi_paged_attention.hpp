@@ -72,8 +72,11 @@ __device__ __forceinline__ float half_of(uint32_t w, int hi) {
 // A value that a row must not see still meets it as 0 * value, which is NaN for
 // an infinity or a NaN.  In steps where some row stops short, such elements
 // enter the products as 0, and the rows that do see them get them back at the
-// end (odd_values()): a weight is positive, so what they make of the sum does not
-// depend on it.
+// end (add_odd()): a weight is positive, so what they make of the sum does not
+// depend on it.  In the other steps they enter as they are.  What the products hold of
+// a weight may be 0 (one that rounds to it) or less (its second piece), which makes a
+// NaN of an infinity; so where channels end as NaN in a row whose weights are numbers,
+// the sum of what it sees there is formed anew, without weights.
 
 // Zeroes the non-finite ones (an exponent of ones) of two 16-bit values.
 template <int DT>
@@ -148,6 +151,18 @@ __device__ __forceinline__ int64_t part_row(const PagedLaunch& a, const Work& w,
     return ((int64_t)w.kvh * a.n_parts + w.it.part) * a.part_rows + (r - w.it.row0);
 }
 
+// Four consecutive elements, widened.
+template <int DT>
+__device__ __forceinline__ f32x4_t load4(const void* p, int64_t i) {
+    if constexpr (DT == kSrcF32) {
+        return *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + i);
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+        return f32x4_t{half_of<DT>(x.x, 0), half_of<DT>(x.x, 1), half_of<DT>(x.y, 0),
+                       half_of<DT>(x.y, 1)};
+    }
+}
+
 // Four consecutive channels of an output row, rounded once.
 template <int DT>
 __device__ __forceinline__ void store4(void* out, int64_t i, f32x4_t x) {
@@ -158,42 +173,58 @@ __device__ __forceinline__ void store4(void* out, int64_t i, f32x4_t x) {
             make_uint2(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]));
 }
 
-// The sum of the non-finite values of positions t .. lim - 1 in four channels.
+// The sum of the non-finite values of positions t .. lim - 1 in four channels, the ones
+// asked for (done once all of these are NaN).
 template <int DT>
 __device__ __forceinline__ f32x4_t odd_values(const PagedLaunch& a, const Work& w, int t, int lim,
-                                           int c) {
+                                           int c, const bool (&asked)[4]) {
     f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
     for (; t < lim; ++t) {
         const int64_t at = (int64_t)w.pages[t >> a.page_shift] * w.page_elems + w.head_off +
                            (t & ((1 << a.page_shift) - 1)) * a.D + c;
+        const f32x4_t x = load4<DT>(a.v_pages, at);
+        bool done = true;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float x = widen<DT>(a.v_pages, at + i);
-            if (non_finite(x)) sum[i] += x;
+            sum[i] += non_finite(x[i]) ? x[i] : 0.f;
+            done &= !asked[i] || sum[i] != sum[i];
         }
+        if (done) break;
     }
     return sum;
 }
-// Where these start: the first step of `unit` positions that some row of the
-// tile (all of which see `all` positions) does not see to its end.
-__device__ __forceinline__ int odd_from(const Work& w, int all, int unit) {
-    return w.it.kv_begin + max(0, all - w.it.kv_begin) / unit * unit;
+__device__ __forceinline__ bool has_nan(f32x4_t o) {
+    return o[0] != o[0] || o[1] != o[1] || o[2] != o[2] || o[3] != o[3];
+}
+// Four channels of a row that sees the positions up to lim, of weights' sum `sum`:
+// the non-finite values added.  odd: some in the steps of `unit` positions that not all
+// rows (which all see `all`) see to their ends, where they entered as 0.
+template <int DT>
+__device__ __forceinline__ void add_odd(const PagedLaunch& a, const Work& w, int all, int unit,
+                                        int lim, int c, float sum, bool odd, f32x4_t& o) {
+    const bool lost = sum == sum && has_nan(o);
+    if (!odd && !lost) return;
+    bool asked[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asked[i] = odd || o[i] != o[i];
+    const int from = lost ? 0 : max(0, all - w.it.kv_begin) / unit * unit;
+    const f32x4_t x = odd_values<DT>(a, w, w.it.kv_begin + from, lim, c, asked);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (lost && asked[i]) o[i] = non_finite(x[i]) ? x[i] : o[i];
+        else o[i] += asked[i] ? x[i] : 0.f;
+    }
 }
 
 // 1 / sum; a row that saw nothing has sum 0 and comes out as zeros.
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
 // Four channels of row r of an item that is done: `o` of sum `sum` at maximum
-// `top`.  odd: some values of a step (of `unit` positions) that not all rows see
-// to its end were not finite.
+// `top`.
 template <int DT>
-__device__ __forceinline__ void finish(const PagedLaunch& a, const Work& w, int r, int c,
-                                       f32x4_t o, float top, float sum, bool odd, int unit) {
-    if (w.it.part < 0) o *= inverse_sum(sum);
-    if (odd) {
-        const int all = w.it.ctx - w.it.n + w.it.row0 / w.hg + 1;
-        o += odd_values<DT>(a, w, odd_from(w, all, unit), row_limit(w, r), c);
-    }
+__device__ __forceinline__ void store_row(const PagedLaunch& a, const Work& w, int r, int c,
+                                          f32x4_t o, float top, float sum) {
     if (w.it.part < 0) {
         store4<DT>(a.out, out_offset(a, w, r) + c, o);
     } else {
@@ -201,6 +232,17 @@ __device__ __forceinline__ void finish(const PagedLaunch& a, const Work& w, int 
         *reinterpret_cast<f32x4_t*>(a.part_o + at * a.D + c) = o;
         if (c == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(top, sum);
     }
+}
+// add_odd() for channels that the lane has stored (a loop over them, once in the code,
+// where the kernel has them in registers by constant numbers).
+template <int DT>
+__device__ __forceinline__ void mend_row(const PagedLaunch& a, const Work& w, int r, int c,
+                                         float top, float sum, bool odd, int unit) {
+    f32x4_t o;
+    if (w.it.part < 0) o = load4<DT>(a.out, out_offset(a, w, r) + c);
+    else o = *reinterpret_cast<const f32x4_t*>(a.part_o + part_row(a, w, r) * a.D + c);
+    add_odd<DT>(a, w, w.it.ctx - w.it.n + w.it.row0 / w.hg + 1, unit, row_limit(w, r), c, sum, odd, o);
+    store_row<DT>(a, w, r, c, o, top, sum);
 }
 
 // Joins WAVES waves' results of ROWS rows (row i of wave j at jo(j) + i * stride,
@@ -223,7 +265,10 @@ __device__ __forceinline__ void join_waves(const PagedLaunch& a, const Work& w, 
             o += *reinterpret_cast<const f32x4_t*>(jo(i) + row * stride + c);
             sum += l[i][row] * exp2_fast(m[i][row] - top);
         }
-        finish<DT>(a, w, r, c, o, top, sum, odd, unit);
+        if (w.it.part < 0) o *= inverse_sum(sum);
+        add_odd<DT>(a, w, w.it.ctx - w.it.n + w.it.row0 / w.hg + 1, unit, row_limit(w, r), c, sum,
+                    odd, o);
+        store_row<DT>(a, w, r, c, o, top, sum);
     }
 }
 

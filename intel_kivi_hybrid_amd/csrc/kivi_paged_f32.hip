@@ -383,15 +383,23 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 3 : 2) paged_f32_many_kern
     rows.sum();
     const int r = row0 + col;
     if (r >= w.rows) return;
+    const float inv = w.it.part < 0 ? inverse_sum(rows.l) : 1.0f;
+    bool lost = false;
 #pragma unroll
     for (int cg = 0; cg < R::CG; ++cg) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int c = 64 * cg + 16 * gq + 4 * i;
-            if (c < a.D)
-                finish<kSrcF32>(a, w, r, c, rows.out(cg, i), rows.m, rows.l, odd != 0, kTile);
+            if (c >= a.D) continue;
+            const f32x4_t o = rows.out(cg, i) * inv;
+            lost |= has_nan(o);
+            store_row<kSrcF32>(a, w, r, c, o, rows.m, rows.l);
         }
     }
+    if (odd == 0 && !lost) return;
+#pragma unroll 1
+    for (int c = 16 * gq; c < a.D; c += c % 16 < 12 ? 4 : 52)
+        mend_row<kSrcF32>(a, w, r, c, rows.m, rows.l, odd != 0, kTile);
 }
 
 template <int DP>

@@ -73,6 +73,7 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) paged_many_kernel(P
     const bool whole = w.it.part < 0;
     const float inv = whole ? inverse_sum(l) : 1.0f;
     const int64_t at = whole ? out_offset(a, w, r) : part_row(a, w, r);
+    bool lost = false;
 #pragma unroll
     for (int cb = 0; cb < M::CB; ++cb) {
 #pragma unroll
@@ -82,13 +83,17 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) paged_many_kernel(P
             const f32x16_t& O = rows.O[cb];
             f32x4_t o = {O[4 * i], O[4 * i + 1], O[4 * i + 2], O[4 * i + 3]};
             o *= inv;
-            if (odd != 0) o += odd_values<DT>(a, w, odd_from(w, wg_all, M::TILE), rows.lim, c);
+            lost |= has_nan(o);
             if (whole) store4<DT>(a.out, at + c, o);
             else *reinterpret_cast<f32x4_t*>(a.part_o + at * a.D + c) = o;
         }
     }
     if (!whole && half == 0)
         *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(rows.m, l);
+    if (odd == 0 && !lost) return;
+#pragma unroll 1
+    for (int c = 4 * half; c < a.D; c += 8)
+        mend_row<DT>(a, w, r, c, rows.m, l, odd != 0, M::TILE);
 }
 
 template <int DT>

@@ -1,0 +1,95 @@
+"""GPU tests of the paged cache's special values: infinities and NaN that a token
+sees."""
+
+import pytest
+import torch
+
+from tests.paged_helpers import attention64, attention_tolerance
+from tests.test_paged_gpu import _attend, _c, _setup
+
+pytestmark = pytest.mark.gpu
+BF, HF, FF = torch.bfloat16, torch.float16, torch.float32
+INF, NAN = float("inf"), float("nan")
+
+
+def _slot(pages, table, s, pos, page_size):
+    """The pool's ``[Hkv, D]`` of a sequence's position."""
+    return pages[int(table[s, pos // page_size]), :, pos % page_size]
+
+
+def _same(o, ref, tol):
+    """Finite elements within the bound, the others the same."""
+    o = o.double().cpu()
+    fine = torch.isfinite(ref)
+    assert bool(((o - ref).abs() <= tol)[fine].all())
+    assert torch.equal(torch.isnan(o), torch.isnan(ref))
+    big = torch.isinf(ref)
+    assert torch.equal(o[big], ref[big])
+    return fine
+
+
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, HF, FF], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_infinities_that_all_rows_see(hip_device, dtype, D, n):
+    """Wherever the position lies: in a step of positions that every row sees to its
+    end, in one that some do not, in a split of the context."""
+    case = _setup([(70, n), (1500, n), (9, 1)], 16, dtype, 4, 2, D, seed=9)
+    table, pool, ctx, new, kp, vp, plan, q = case
+    for s, positions in ((0, (0, 13, 40, 69)), (1, (3, 64, 700, 1499)), (2, (4,))):
+        for i, pos in enumerate(positions):
+            v = _slot(vp, table, s, pos, 16)
+            v[0, 7 * i] = INF
+            v[1, 7 * i + 1] = -INF
+            v[1, 7 * i + 2] = NAN
+            v[:, 60] = INF if i % 2 == 0 else -INF          # (both: NaN)
+    ref, mag, size = attention64(q, kp, vp, table, ctx, new, 16, D ** -0.5)
+    fine = _same(_attend(case), ref, attention_tolerance(ref, mag, size, D, max(ctx), dtype))
+    assert not fine[0, :, 60].any() and fine[:, :, 61].all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FF], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [1, 24])
+def test_an_infinity_of_little_weight(hip_device, dtype, n):
+    """Every weight is positive: e^-40 of the largest too."""
+    D = 64
+    case = _setup([(300, n)], 32, dtype, 2, 2, D, seed=4)
+    table, pool, ctx, new, kp, vp, plan, q = case
+    q[:] = 1.0
+    for pos in (5, 100):
+        _slot(kp, table, 0, pos, 32)[:] = -5.0              # score -40, the others' N(0,1)
+        _slot(vp, table, 0, pos, 32)[:, 3] = INF
+    ref, mag, size = attention64(q, kp, vp, table, ctx, new, 32, D ** -0.5)
+    assert bool((ref[:, :, 3] == INF).all())
+    _same(_attend(case), ref, attention_tolerance(ref, mag, size, D, max(ctx), dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FF], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [1, 24])
+def test_an_infinity_in_a_split_of_no_weight(hip_device, dtype, n):
+    """A split of the context whose scores all lie 140 nats below another's (2^-202:
+    nothing in fp32), with an infinity in it."""
+    D = 64
+    case = _setup([(3000, n)], 32, dtype, 2, 2, D, seed=4)
+    table, pool, ctx, new, kp, vp, plan, q = case
+    assert list(plan._info)[5] > 0
+    q[:] = 1.0
+    for pos in range(1500):
+        _slot(kp, table, 0, pos, 32)[:] = -17.5
+    _slot(vp, table, 0, 3, 32)[:, 3] = INF
+    _slot(vp, table, 0, 3, 32)[1, 4] = -INF
+    ref, mag, size = attention64(q, kp, vp, table, ctx, new, 32, D ** -0.5)
+    assert bool((ref[:, :, 3] == INF).all()) and bool((ref[:, 1, 4] == -INF).all())
+    _same(_attend(case), ref, attention_tolerance(ref, mag, size, D, max(ctx), dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FF], ids=["bf16", "f16", "f32"])
+def test_keys_that_are_not_finite_leave_no_finite_row(hip_device, dtype):
+    """A NaN score: the whole row is NaN, as the formula has it, and no other."""
+    for n in (1, 24):
+        case = _setup([(300, n), (50, 1)], 32, dtype, 4, 2, 64, seed=4)
+        table, pool, ctx, new, kp, vp, plan, q = case
+        _slot(kp, table, 0, 17, 32)[1, 3] = NAN
+        o = _attend(case).cpu()
+        assert bool(torch.isnan(o[:n, 2:]).all())
+        assert bool(torch.isfinite(o[:n, :2]).all()) and bool(torch.isfinite(o[n:]).all())
