@@ -701,9 +701,11 @@ struct Picker {
                : kind == kByMass ? r < at && at <= r + rel
                                  : r <= at && at < r + rel;
     }
+    // The running mass at `rel` rels of the bucket (one whose mass is rounded to 0 adds
+    // none: the row's total is never passed).
     static __device__ __forceinline__ uint64_t mass_at(const Need& x, uint64_t rel) {
         const uint64_t part = (uint64_t)__builtin_rint((double)rel / x.per);
-        return x.base + (part < 1 ? 1 : part > x.mass ? x.mass : part);
+        return x.base + min(max(part, (uint64_t)1), x.mass);
     }
 
     // One wave, a token of the list for each lane: its rank in its bucket.
