@@ -11,8 +11,11 @@
 // off by at most half a step of that type, as the values themselves are.
 //
 // The softmax is online in the log2 domain.  A row's maximum moves only when
-// exceeded by more than 8 (weights <= 256, in range of every type), so most
-// steps rescale nothing.
+// exceeded by more than 8, so most steps rescale nothing.  Weights are formed against
+// the maximum lowered by weight_bits(): in fp16 from 2^7 to 2^15 for a row's largest,
+// so that the type's subnormal steps of 2^-24 are 2^-31 of it or less.  (Against the
+// maximum itself weights below 2^-25 of the largest became 0: of 16K positions whose
+// values count, 25.2 log2 units below every 32nd, nothing was left.)
 #pragma once
 
 #include <float.h>
@@ -25,6 +28,8 @@ namespace kivi {
 namespace {
 
 constexpr float kMoveMax = 8.0f;       // log2 units
+template <int DT>
+constexpr float weight_bits() { return DT == kSrcF16 ? 7.0f : 0.0f; }
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));

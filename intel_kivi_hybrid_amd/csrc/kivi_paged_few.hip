@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kBlock) paged_few_kernel(PagedLaunch a) {
         }
         float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
                          fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        mx *= a.qscale;
+        mx = fmaf(mx, a.qscale, -weight_bits<DT>());
         if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax) != 0) {
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));

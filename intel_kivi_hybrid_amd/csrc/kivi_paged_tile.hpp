@@ -137,7 +137,7 @@ struct TileRows {
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tb][i]);
         }
-        mx *= qscale;
+        mx = fmaf(mx, qscale, -weight_bits<DT>());
         if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax) != 0) {
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             const float to = fmaxf(m, mx), f = exp2_fast(m - to);

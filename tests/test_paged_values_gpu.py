@@ -1,10 +1,10 @@
 """GPU tests of the paged cache's special values: infinities and NaN that a token
-sees."""
+sees, weights far below a row's largest."""
 
 import pytest
 import torch
 
-from tests.paged_helpers import attention64, attention_tolerance
+from tests.paged_helpers import EPS, attention64, attention_tolerance
 from tests.test_paged_gpu import _attend, _c, _setup
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +93,40 @@ def test_keys_that_are_not_finite_leave_no_finite_row(hip_device, dtype):
         o = _attend(case).cpu()
         assert bool(torch.isnan(o[:n, 2:]).all())
         assert bool(torch.isfinite(o[:n, :2]).all()) and bool(torch.isfinite(o[n:]).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FF], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [1, 5])
+@pytest.mark.parametrize("below,spread", [(25.2, 0.0), (22.0, 0.0), (21.0, 0.3), (12.0, 1.0)])
+def test_a_long_tail_below_the_largest(hip_device, dtype, n, below, spread):
+    """16K positions, every 32nd of them ``below`` log2 units above the others, whose
+    values alone count.
+
+    The bound: the output's rounding; the weights' (half a step of a 16-bit type; an
+    fp16 weight is held as 2^7 of the largest at least, so half a step of its smallest
+    numbers is 2^-32 of the largest weight, of which the sum has c / 32 - 1 or more);
+    and fp32's.  Of these a score is a sum of D products, off by (D + 3) 2^-24 of
+    sum |q k| scale, which moves a weight and the weights' sum by that each; a lane adds
+    at most half of the positions one after the other, each off by 2^-24 of the sum, for
+    the weights and (in matrix products of 16 positions) for the values."""
+    D, c, hg, much = 64, 16384, 4, 1000.0
+    case = _setup([(c - n, n)], 64, dtype, hg, 1, D, seed=7)
+    table, pool, ctx, new, kp, vp, plan, q = case
+    g = torch.Generator().manual_seed(3)
+    q[:] = 1.0
+    k, v = torch.zeros(c, D), torch.full((c, D), much)
+    k[:, :16] = spread * torch.randn(c, 16, generator=g)
+    k[::32] = below * 0.6931471805599453 / 8.0              # (64 channels, the scale is 1/8)
+    v[::32] = 0.0
+    for j in range(c // 64):
+        kp[int(table[0, j]), 0], vp[int(table[0, j]), 0] = (
+            x[64 * j:64 * j + 64].to(dtype) for x in (k, v))
+    ref, mag, size = attention64(q, kp, vp, table, ctx, new, 64, D ** -0.5)
+    u, half = 2.0 ** -24, EPS[dtype] / 2
+    fp32 = 2 * ((D + 3) * u * size[..., None] + (c / 2 + 64) * u)
+    tol = half * ref.abs() + ((half if dtype != FF else 0.0) + fp32) * mag * (1 + 2 * half)
+    if dtype == HF:
+        tol = tol + c * much * 2.0 ** -32 / (c / 32 - 1)
+    err = (_attend(case).double().cpu() - ref).abs()
+    print(f"[tail] {dtype} n={n} {below} worst {float((err / tol).max()):.3f} of the bound")
+    assert bool((err <= tol).all())
