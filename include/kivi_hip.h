@@ -457,12 +457,12 @@ size_t kivi_paged_attention_workspace_size(const int64_t* info, int32_t kv_heads
  * of dtype with strides of whole 16-byte vectors, out the same, contiguous; query
  * head h reads kv head h / (q_heads / kv_heads).  softmax_scale must be positive.
  * Scores, softmax and sums are fp32; for the product with 16-bit values weights
- * are rounded to dtype (where no sequence of the step brings more than 16 rows to
- * a kv head they are split into two such pieces).
- * plan is 16-byte aligned, and so are q's rows, the pages, out and workspace.  What lies behind a sequence's end or in positions that a
- * token does not see, infinities and NaN too, does not reach it; those in
- * values that it sees reach it whatever their weights.  Rows of out behind the last
- * token are left as they were. */
+ * are rounded to dtype (those of a sequence with up to 16 rows to a kv head, tokens
+ * x heads, in two pieces, whatever else the step holds).  plan is 16-byte aligned,
+ * and so are q's rows, the pages, out and workspace.  What lies behind a sequence's
+ * end or in positions that a token does not see, infinities and NaN too, does not
+ * reach it; those in values that it sees reach it whatever their weights.  Rows of
+ * out behind the last token are left as they were. */
 int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                          int32_t dtype, const void* k_pages, const void* v_pages,
                          int64_t num_pages, int32_t page_size, int32_t q_heads,

@@ -15,8 +15,14 @@
 // of 16 sequences, 28/4 heads, 3K positions: 23 us with the join, of 64 at 8K 167,
 // 5.0 TB/s (a kernel of 64 rows of its own, with its waves on both rows and
 // positions and three tiles in flight, took 27 and 186).
+//
+// A workgroup whose sequence has up to 16 rows walks it as kivi_paged_few.hpp does, in
+// the same LDS: two chunks of 777 tokens and 30 single ones, 64/8 heads, fp16: 281 us,
+// as it took with those in tiles of 128 rows (whose weights had one piece); 63 single
+// tokens of 8K beside 5 tokens, 32/8 heads, bf16: 327 and 331.
 #include <hip/hip_runtime.h>
 
+#include "kivi_paged_few.hpp"
 #include "kivi_paged_tile.hpp"
 
 namespace kivi {
@@ -31,12 +37,21 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) paged_many_kernel(P
     using M = TileShape<DP, kTile>;
     // (two arrays, not one: reads of this tile then need not wait for the next
     // one's loads, which the compiler knows to write the other array)
-    __shared__ __align__(16) unsigned char buf0[2 * M::BYTES];
-    __shared__ __align__(16) unsigned char buf1[2 * M::BYTES];
+    constexpr int kFewBytes = 2 * Few<DP>::WAVE_BYTES;
+    constexpr int kBytes = 2 * M::BYTES > kFewBytes ? 2 * M::BYTES : kFewBytes;
+    __shared__ __align__(16) unsigned char buf0[kBytes];
+    __shared__ __align__(16) unsigned char buf1[kBytes];
+    __shared__ FewJoin join;
     __shared__ int odd;                    // some values were not finite
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
     const Work w = work_of(a);
+    if (w.rows <= paged_tile_rows(kFew16)) {
+        few_rows<DT, DP>(a, w, [&](int i) {
+            return (i < 2 ? buf0 : buf1) + i % 2 * Few<DP>::WAVE_BYTES;
+        }, join);
+        return;
+    }
     const int end = w.it.kv_end;
 
     TileRows<DT, DP, kTile> rows;

@@ -130,3 +130,25 @@ def test_a_long_tail_below_the_largest(hip_device, dtype, n, below, spread):
     err = (_attend(case).double().cpu() - ref).abs()
     print(f"[tail] {dtype} n={n} {below} worst {float((err / tol).max()):.3f} of the bound")
     assert bool((err <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_single_tokens_are_as_exact_beside_many_rows(hip_device, dtype, D):
+    """Their weights enter the second product in two pieces (off by 2^-18 at most:
+    half a step of half a step), alone or in the launch of a sequence of many rows."""
+    lens, Hq, Hkv = [(60, 1), (100, 40), (90, 1), (33, 3)], 8, 2
+    case = _setup(lens, 16, dtype, Hq, Hkv, D, seed=5)
+    table, pool, ctx, new, kp, vp, plan, q = case
+    q *= 0.2
+    assert list(plan._info)[6:9] == [0, 0, 0]               # (one launch)
+    ref, mag, size = attention64(q, kp, vp, table, ctx, new, 16, D ** -0.5)
+    u = 2.0 ** -24
+    moved = 2 * ((D + 3) * u * size[..., None] + (max(ctx) + 8) * u)
+    tol = EPS[dtype] / 2 * ref.abs() + (2.0 ** -18 + moved) * mag * (1 + EPS[dtype])
+    if dtype == HF:
+        tol = tol + max(ctx) * mag * 2.0 ** -32
+    err = (_attend(case).double().cpu() - ref).abs()
+    rows = [0] + list(range(41, 45))
+    print(f"[company] {dtype} D={D} worst {float((err / tol)[rows].max()):.3f} of the bound")
+    assert bool((err <= tol)[rows].all())
