@@ -394,26 +394,27 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
                                  runs[i].page);
 
         // Row tiles, and the positions that the last row of each sees.  Beside 16-bit
-        // sequences of more than 16 rows those of fewer take tiles of the larger kind
-        // too: one launch, in which their loads run beside the others' products (two
-        // chunks of 777 tokens and 30 single ones, 64/8 heads, fp16: 302 us, as two
-        // launches 354; 16 sequences of 2 or 3 tokens, 28/4 heads: 22 and 32).  Above
-        // 128 channels, where a CU holds one workgroup, only beside few rows (2 chunks
-        // of 300 and 18 single tokens, 28/4 heads of 256: 147 us, as two launches 137).
-        // In fp32, where a tile of many rows takes few at the time of products that only
-        // one of its waves has, up to 2^24 elements of their keys (19 single tokens of 500
-        // positions beside a chunk of 94, 16/2 heads of 256, 4M elements: 35 us, as two
-        // launches 50; 28 of 4K beside two of 200, 32/8 heads of 128, 86M: 405 and 327).
-        int few = kFew16;
+        // sequences of more than 16 rows those of fewer go into the same launch, where
+        // their loads run beside the others' products (64/8 heads, fp16, two chunks of 777
+        // tokens and 30 single ones: 281 us, as two launches 354; 32/8 heads, bf16, 63
+        // single tokens of 8K beside five tokens: 327 and 354, 128 of 2K beside eight
+        // times five: 177 and 188, eight of 500 beside 200: 29 and 38; 28/4 heads of 256,
+        // where a CU holds one workgroup, 18 of 2K beside 200: 58 and 78, but 30 of 8K
+        // beside 200: 244 and 228).  In fp32, where a tile of many rows takes few at the
+        // time of products that only one of its waves has, up to 2^23 elements of their
+        // keys (32/8 heads of 128, 28 single tokens beside two of 200: 2^23 75 and 88 us,
+        // 2^24 102 and 97; eight beside 94: 2^22 31 and 35, 2^23 46 and 41, 2^24 60 and
+        // 51; 16/2 heads of 256, eight beside 94: 2^23 52 and 54, 2^24 71 and 64).
         int64_t small = 0;
         bool large = false;
         for (int s = 0; s < n_seqs; ++s) {
             const int64_t rows = (int64_t)new_lens[s] * hg;
-            if (!f32 && rows > 16 && (rows <= 64 || head_dim <= 128)) few = kMany;
             if (rows > 0 && rows <= 16) small += context_lens[s];
             large |= rows > 16;
         }
-        if (f32 && large && small <= (1 << 24) / head_dim / kv_heads) few = kFew64;
+        int few = kFew16;
+        if (large && !f32) few = kMany;
+        if (large && f32 && small <= (1 << 23) / head_dim / kv_heads) few = kFew64;
         std::vector<Tile> tiles[kPagedKinds];
         for (int s = 0; s < n_seqs; ++s) {
             const int64_t n = new_lens[s], rows = n * hg;
