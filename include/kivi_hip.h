@@ -436,7 +436,7 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
  *   rows are rotated by the angles of the token's position p, row p of cos and
  *   sin ([positions][rotary_dim/2] f32): channels i and i + rotary_dim/2, or 2i
  *   and 2i+1 with interleaved.  The tables must reach info[12] positions.
- * Values are copied bit for bit. */
+ * Values, and channels that neither of these changes, are copied bit for bit. */
 int kivi_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                       const void* k, int64_t k_token_stride, int64_t k_head_stride,
                       const void* v, int64_t v_token_stride, int64_t v_head_stride,

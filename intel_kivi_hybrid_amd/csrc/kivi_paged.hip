@@ -52,62 +52,86 @@ struct AppendArgs {
 
 typedef unsigned int kivi_u4v __attribute__((ext_vector_type(4)));
 
-// Eight elements widened: one or two 16-byte loads (vec: aligned to 16), read once
+// Eight elements as they lie: one or two 16-byte loads (vec: aligned to 16), read once
 // by this kernel.
 template <int DT>
-__device__ __forceinline__ void load8(const void* p, int64_t i, bool vec, float (&x)[8]) {
-    if (!vec) {
+struct Eight {
+    static constexpr int kWords = DT == kSrcF32 ? 8 : 4;
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ void load(const void* p, int64_t i, bool vec) {
+        const char* from = static_cast<const char*>(p) + i * src_size(DT);
+        if (vec) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = widen<DT>(p, i + j);
-    } else if constexpr (DT == kSrcF32) {
-        const float4 a = load4_vec<DT>(p, i), b = load4_vec<DT>(p, i + 4);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-        const kivi_u4v w = __builtin_nontemporal_load(
-            reinterpret_cast<const kivi_u4v*>(static_cast<const uint16_t*>(p) + i));
+            for (int j = 0; j < kWords; j += 4) {
+                const kivi_u4v x =
+                    __builtin_nontemporal_load(reinterpret_cast<const kivi_u4v*>(from + 4 * j));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (DT == kSrcBF16) {
-                x[2 * j] = __uint_as_float(w[j] << 16);
-                x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-            } else {
-                x[2 * j] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j] & 0xffffu));
-                x[2 * j + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j] >> 16));
+                for (int k = 0; k < 4; ++k) w[j + k] = x[k];
+            }
+        } else if constexpr (DT == kSrcF32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = reinterpret_cast<const uint32_t*>(from)[j];
+        } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(from);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
+        }
+    }
+    __device__ __forceinline__ void widen(float (&x)[8]) const {
+        if constexpr (DT == kSrcF32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (DT == kSrcBF16) {
+                    x[2 * j] = __uint_as_float(w[j] << 16);
+                    x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+                } else {
+                    x[2 * j] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j] & 0xffffu));
+                    x[2 * j + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j] >> 16));
+                }
             }
         }
     }
+    __device__ __forceinline__ void round(const float (&x)[8]) {
+        if constexpr (DT == kSrcF32) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(x[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint16_t lo, hi;
+                if constexpr (DT == kSrcBF16) {
+                    lo = __builtin_bit_cast(uint16_t, (__bf16)x[2 * j]);
+                    hi = __builtin_bit_cast(uint16_t, (__bf16)x[2 * j + 1]);
+                } else {
+                    lo = __builtin_bit_cast(uint16_t, (_Float16)x[2 * j]);
+                    hi = __builtin_bit_cast(uint16_t, (_Float16)x[2 * j + 1]);
+                }
+                w[j] = lo | (uint32_t)hi << 16;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(void* p, int64_t i) const {
+        uint4* to = reinterpret_cast<uint4*>(static_cast<char*>(p) + i * src_size(DT));
+#pragma unroll
+        for (int j = 0; j < kWords; j += 4)
+            to[j / 4] = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+    }
+};
+// Eight of a type known at run time, widened.
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int i, bool vec, float (&x)[8]) {
+    Eight<DT> e;
+    e.load(p, i, vec);
+    e.widen(x);
 }
-// The same of a type known at run time.
 __device__ __forceinline__ void load8_dt(const void* p, int i, int dt, bool vec, float (&x)[8]) {
     if (dt == kSrcF32) load8<kSrcF32>(p, i, vec, x);
     else if (dt == kSrcBF16) load8<kSrcBF16>(p, i, vec, x);
     else load8<kSrcF16>(p, i, vec, x);
-}
-
-template <int DT>
-__device__ __forceinline__ void store8(void* p, int64_t i, const float (&x)[8]) {
-    if constexpr (DT == kSrcF32) {
-        float4* o = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
-        o[0] = make_float4(x[0], x[1], x[2], x[3]);
-        o[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint16_t lo, hi;
-            if constexpr (DT == kSrcBF16) {
-                lo = __builtin_bit_cast(uint16_t, (__bf16)x[2 * j]);
-                hi = __builtin_bit_cast(uint16_t, (__bf16)x[2 * j + 1]);
-            } else {
-                lo = __builtin_bit_cast(uint16_t, (_Float16)x[2 * j]);
-                hi = __builtin_bit_cast(uint16_t, (_Float16)x[2 * j + 1]);
-            }
-            w[j] = lo | (uint32_t)hi << 16;
-        }
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) =
-            make_uint4(w[0], w[1], w[2], w[3]);
-    }
 }
 
 // Sum over aligned segments of 1 << log2 lanes.
@@ -152,12 +176,10 @@ __global__ void __launch_bounds__(kAppendBlock) paged_append_kernel(AppendArgs a
         norm = a.k_norm;
         from = tok * a.k_st + (int64_t)(h - a.Hq) * a.k_sh;
     }
-    float x[8], y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = y[j] = 0.f;
+    Eight<DT> ex{}, ey{};
     if (live) {
-        load8<DT>(src, from + c0, a.vec, x);
-        load8<DT>(src, from + c1, a.vec, y);
+        ex.load(src, from + c0, a.vec);
+        ey.load(src, from + c1, a.vec);
     }
     // angles: of pairs (c0 + j, c1 + j), or of the pairs in x and those in y
     const bool turned = live && inside && h < a.Hq + a.Hkv;
@@ -171,6 +193,9 @@ __global__ void __launch_bounds__(kAppendBlock) paged_append_kernel(AppendArgs a
         sn[0] = *reinterpret_cast<const float4*>(a.sin + r + i0);
         sn[1] = *reinterpret_cast<const float4*>(a.sin + r + i1);
     }
+    float x[8], y[8];
+    ex.widen(x);
+    ey.widen(y);
     if (norm != nullptr) {
         float u[8], w[8];
         if (live) {
@@ -218,8 +243,13 @@ __global__ void __launch_bounds__(kAppendBlock) paged_append_kernel(AppendArgs a
         dst = h < a.Hq + a.Hkv ? a.k_pages : a.v_pages;
         to = (((page * a.Hkv + kvh) << a.page_shift) + off) * a.D;
     }
-    store8<DT>(dst, to + c0, x);
-    store8<DT>(dst, to + c1, y);
+    // (what is only moved keeps its bits: to fp32 and back a signalling NaN loses one)
+    if (norm != nullptr || turned) {
+        ex.round(x);
+        ey.round(y);
+    }
+    ex.store(dst, to + c0);
+    ey.store(dst, to + c1);
 }
 
 int page_shift_of(int32_t page_size) {

@@ -1,5 +1,5 @@
 """GPU tests of the paged cache's special values: infinities and NaN that a token
-sees, weights far below a row's largest."""
+sees, weights far below a row's largest, the bits of a copy."""
 
 import pytest
 import torch
@@ -152,3 +152,33 @@ def test_single_tokens_are_as_exact_beside_many_rows(hip_device, dtype, D):
     rows = [0] + list(range(41, 45))
     print(f"[company] {dtype} D={D} worst {float((err / tol)[rows].max()):.3f} of the bound")
     assert bool((err <= tol)[rows].all())
+
+
+# ------------------------------------------------------- the append's copies
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "f16"])
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("rotary", [0, 32])
+def test_every_bit_of_a_copy(hip_device, dtype, offset, rotary):
+    """All 65536 patterns, signalling NaN among them: values, and channels that are
+    neither normed nor rotated, from rows on and off 16-byte borders."""
+    T, H, D, page = 512, 2, 64, 32
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16)
+    flat = torch.empty(65536 + offset, dtype=torch.int16, device="cuda:0")
+    flat[offset:] = bits.cuda()
+    x = flat[offset:].view(dtype).view(T, H, D)
+    table = torch.randperm(T // page, generator=torch.Generator().manual_seed(1))
+    table = table.to(torch.int32)[None]
+    plan = _c().paged_plan(table, [T], [T], page_size=page, num_pages=T // page, q_heads=H,
+                           kv_heads=H, head_dim=D, dtype=dtype, device="cuda:0")
+    kd, vd = (torch.zeros(T // page, H, page, D, dtype=dtype, device="cuda:0") for _ in range(2))
+    kw = {}
+    if rotary:
+        kw["cos"], kw["sin"] = _c().rotary_tables(T, rotary, device="cuda:0")
+    q = _c().paged_append(x, x, kd, vd, plan, q=x, **kw)
+    want = bits.view(T, H, D)[:, :, rotary:]
+
+    def pages(p):
+        return p.view(torch.int16).cpu()[table[0].long()].transpose(1, 2).reshape(T, H, D)
+    assert torch.equal(pages(vd), bits.view(T, H, D))
+    assert torch.equal(pages(kd)[:, :, rotary:], want)
+    assert torch.equal(q.view(torch.int16).cpu()[:, :, rotary:], want)
