@@ -20,6 +20,7 @@ import functools
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from ._device import device_index, is_current, on_device, stream_handle
@@ -704,10 +705,21 @@ def packed_attention_typed(q, store, softmax_scale=None, kv_start=None, hidden=N
 # Paged cache (no reference counterpart; see include/kivi_hip.h): sequences of
 # unequal lengths on pages of one pool.
 # --------------------------------------------------------------------------
+def _tracked() -> bool:
+    """Whether a derivative of either kind may be asked of a call made now."""
+    return torch.is_grad_enabled() or forward_ad._current_level >= 0
+
+
 def _check_inference(*tensors) -> None:
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            _fail("inference only: a tensor requires a gradient; call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _fail("inference only: a tensor requires a gradient; call it under "
+                      "torch.no_grad()")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _fail("inference only: a tensor has a forward-mode tangent")
 
 
 def _host_ints(values, name: str) -> torch.Tensor:
@@ -888,8 +900,8 @@ def paged_append(k, v, k_pages, v_pages, plan, q=None, q_out=None, cos=None, sin
         with on_device(dev):
             return paged_append(k, v, k_pages, v_pages, plan, q, q_out, cos, sin, interleaved,
                                 q_norm, k_norm, eps)
-    if torch.is_grad_enabled():
-        _check_inference(k, v, q, q_norm, k_norm)
+    if _tracked():
+        _check_inference(k, v, k_pages, v_pages, q, q_out, cos, sin, q_norm, k_norm)
     kp, vp = _check_pages(plan, k_pages, v_pages)
     _check(kp != vp or plan.tokens == 0, "k_pages and v_pages must be two pools")
     ks = _check_tokens(k, "k", plan, plan.kv_heads)
@@ -987,8 +999,8 @@ def paged_attention(q, k_pages, v_pages, plan, softmax_scale=None, out=None, wor
     if not is_current(dev):
         with on_device(dev):
             return paged_attention(q, k_pages, v_pages, plan, softmax_scale, out, workspace)
-    if torch.is_grad_enabled():
-        _check_inference(q)
+    if _tracked():
+        _check_inference(q, k_pages, v_pages, out)
     kp, vp = _check_pages(plan, k_pages, v_pages)
     st = _check_tokens(q, "q", plan, plan.q_heads)
     q_ptr = q.data_ptr()
