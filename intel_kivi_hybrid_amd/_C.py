@@ -756,14 +756,17 @@ class PagedPlan:
     def _enter(self, device: int) -> int:
         """The current stream's handle, ordered behind the plan's copy."""
         handle = stream_handle(device)
-        if handle != self._stream and not torch.cuda.is_current_stream_capturing():
+        if handle == self._stream and self._settled:
+            return handle
+        if torch.cuda.is_current_stream_capturing():
+            # (on the plan's own stream too: a replay may come on another)
+            _check(self._settled, "call the plan's wait() before capturing a graph with it")
+        elif handle != self._stream:
             stream = torch.cuda.current_stream(device)
             if not self._settled:
                 stream.wait_event(self._event)
             # (its memory is not given away while this stream may read it)
             self._buf.record_stream(stream)
-        elif handle != self._stream:
-            _check(self._settled, "call the plan's wait() before capturing a graph with it")
         return handle
 
 

@@ -1,4 +1,5 @@
-"""GPU tests of the paged cache's calls: tensors that derivatives are asked of."""
+"""GPU tests of the paged cache's calls: tensors that derivatives are asked of,
+and captures."""
 
 import pytest
 import torch
@@ -7,7 +8,7 @@ import torch.autograd.forward_ad as fwd
 from tests.test_paged_gpu import _c, _setup
 
 pytestmark = pytest.mark.gpu
-FF = torch.float32
+BF, FF = torch.bfloat16, torch.float32
 
 
 def _inputs(dtype=FF):
@@ -55,3 +56,29 @@ def test_forward_mode_tangents_are_refused(hip_device):
                     with mode(), pytest.raises(RuntimeError, match="inference only"):
                         list(_calls(plan, y))[i][1]()
             list(_calls(plan, x))[i][1]()                     # (a level without tangents)
+
+
+def test_capture_on_the_plans_own_stream_needs_a_settled_plan(hip_device):
+    s = torch.cuda.Stream()
+    table, pool, ctx, new, kp, vp, _, q = _setup([(20, 1)], 32, BF, 4, 2, 64, seed=3)
+    kd, vd, qd = kp.cuda(), vp.cuda(), q.cuda()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        plan = _c().paged_plan(table, ctx, new, page_size=32, num_pages=pool, q_heads=4,
+                               kv_heads=2, head_dim=64, device="cuda:0")
+        want = _c().paged_attention(qd, kd, vd, plan)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        with pytest.raises(RuntimeError, match="wait"):
+            _c().paged_attention(qd, kd, vd, plan)
+        torch.zeros(1, device="cuda:0")
+    plan.wait()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        out = _c().paged_attention(qd, kd, vd, plan)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
