@@ -456,17 +456,21 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
                 tiles[kind].push_back({s, (int)r, context_lens[s] - n + last / hg + 1});
             }
         }
+        auto tile_rows = [&](const Tile& t, int kind) {
+            return (int)std::min<int64_t>(paged_tile_rows(kind),
+                                          (int64_t)new_lens[t.seq] * hg - t.row0);
+        };
+        auto is_few = [&](const Tile& t) { return paged_few((int64_t)new_lens[t.seq] * hg); };
         Cut cuts[kPagedKinds];
         int64_t items = 0, merges = 0, parts = 0, part_rows = 0, kinds[kPagedKinds] = {0, 0, 0, 0};
+        int64_t few_parts = 0, few_rows = 0;
         for (int kind = 0; kind < kPagedKinds; ++kind) {
             // longest first: the last workgroups to start are short ones
             std::vector<Tile>& of = tiles[kind];
             std::stable_sort(of.begin(), of.end(),
                              [](const Tile& a, const Tile& b) { return a.end > b.end; });
             std::vector<int> rows;
-            for (const Tile& t : of)
-                rows.push_back((int)std::min<int64_t>(paged_tile_rows(kind),
-                                                      (int64_t)new_lens[t.seq] * hg - t.row0));
+            for (const Tile& t : of) rows.push_back(tile_rows(t, kind));
             const int64_t slots = paged_slots(kind, head_dim);
             cuts[kind] = best_cut(of, rows, std::max<int64_t>(1, slots / kv_heads),
                                   paged_costs(kind));
@@ -474,11 +478,13 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
                 const int64_t splits = cuts[kind].pieces(i, of[i].end);
                 items += splits;
                 kinds[kind] += splits;
-                if (splits > 1) {
-                    merges += 1;
-                    parts += splits;
-                    part_rows = std::max<int64_t>(part_rows, paged_tile_rows(kind));
-                }
+                if (splits == 1) continue;
+                merges += 1;
+                parts += splits;
+                part_rows = std::max<int64_t>(part_rows, rows[i]);
+                if (!is_few(of[i])) continue;
+                few_parts += splits;
+                few_rows = std::max<int64_t>(few_rows, rows[i]);
             }
         }
         const int64_t pages_at = 2 * tokens, items_at = (pages_at + pages + 7) / 8 * 8;
@@ -499,6 +505,8 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
         info[kInfoPartRows] = part_rows;
         info[kInfoContext] = longest;
         info[kInfoZerosAt] = zeros_at;
+        info[kInfoFewParts] = few_parts;
+        info[kInfoFewRows] = few_rows;
         if (plan == nullptr || tokens == 0) return kOk;
         if (plan_ints < ints)
             return set_error(kErrInvalidArgument, "the plan needs %lld words, got %lld",
@@ -524,7 +532,7 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
         for (int64_t i = zeros_at; i < ints; ++i) plan[i] = 0;
         PagedItem* item = reinterpret_cast<PagedItem*>(plan + items_at);
         PagedMerge* merge = reinterpret_cast<PagedMerge*>(plan + merges_at);
-        int32_t part = 0;
+        int32_t next_few = 0, next_many = (int32_t)few_parts;
         for (int kind = 0; kind < kPagedKinds; ++kind) {
             for (size_t j = 0; j < tiles[kind].size(); ++j) {
                 const Tile& x = tiles[kind][j];
@@ -532,9 +540,10 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
                 // (whole units of 64 positions, shared out evenly)
                 const int64_t units = (x.end + 63) / 64;
                 const int s = x.seq;
+                int32_t& part = is_few(x) ? next_few : next_many;
                 if (splits > 1)
                     *merge++ = PagedMerge{tok0[s], new_lens[s], x.row0, (int32_t)splits, part,
-                                          paged_tile_rows(kind), {0, 0}};
+                                          tile_rows(x, kind), {0, 0}};
                 for (int64_t i = 0; i < splits; ++i) {
                     const int64_t b = units * i / splits * 64;
                     const int64_t e = std::min(x.end, units * (i + 1) / splits * 64);

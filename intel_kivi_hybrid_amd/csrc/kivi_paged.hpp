@@ -38,7 +38,7 @@ struct PagedMerge {
     int32_t row0;
     int32_t splits;
     int32_t part;        // first partial
-    int32_t rows;        // of the tile (the last one's may end earlier)
+    int32_t rows;        // of the tile
     int32_t pad[2];
 };
 
@@ -57,6 +57,11 @@ constexpr int paged_tile_rows(int kind) { return 16 << kind; }
 constexpr int paged_kind(int64_t rows, bool f32) {
     return rows <= 16 ? kFew16 : f32 ? kFew64 : kMany;
 }
+// Sequences whose partials have rows of their own number (beside tiles of many rows
+// those of single tokens would otherwise be mostly empty: eight tokens of 32K beside
+// five of another sequence, 32/4 heads of 128, took 55 MB).
+constexpr bool paged_few(int64_t rows) { return rows <= paged_tile_rows(kFew16); }
+
 // Workgroups that the card works on at once: 256 CUs, and as many on each as the
 // kernels' registers or LDS leave room for (fp32's 64 rows: as bring more; more
 // than that share the matrix cores that bound it).
@@ -81,9 +86,11 @@ enum PagedInfo : int {
     kInfoMerges = 5,
     kInfoItems = 6,       // items of each kind, in order
     kInfoParts = 10,      // partials of a kv head
-    kInfoPartRows = 11,   // rows of a partial (the largest tile among the split ones)
+    kInfoPartRows = 11,   // rows of a partial (of the split tile that has most)
     kInfoContext = 12,    // the longest sequence
     kInfoZerosAt = 13,
+    kInfoFewParts = 14,   // partials of sequences with few rows (the first ones),
+    kInfoFewRows = 15,    // and rows of these
     kInfoCount = 16,
 };
 
@@ -93,13 +100,15 @@ struct PagedLaunch {
     const void* k_pages;
     const void* v_pages;
     void* out;                    // [tokens][q_heads][head_dim]
-    float* part_o;                // [kv head][partial][rows][head_dim]
-    float* part_ml;               // [kv head][partial][rows][2]: maximum and sum
+    float* part_o;                // [kv head][partial][its rows][head_dim]
+    float* part_ml;               // [kv head][partial][its rows][2]: maximum and sum
     const int32_t* pages;
     const PagedItem* items;
     const PagedMerge* merges;
     const int32_t* zeros;
-    int n_items, n_merges, n_parts, part_rows;
+    int n_items, n_merges, part_rows, few_rows;
+    int64_t part_total;           // rows of a kv head's partials
+    int64_t many_at;              // row of partial p with many rows: this + p * part_rows
     int Hq, Hkv, hg, D, page_shift;
     float qscale;                 // softmax scale * log2 e
 };

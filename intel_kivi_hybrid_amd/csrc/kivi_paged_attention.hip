@@ -32,12 +32,12 @@ __global__ void __launch_bounds__(kMergeBlock) paged_merge_kernel(PagedLaunch a)
     const PagedMerge g = a.merges[tile / a.Hkv];
     const int at = (blockIdx.x - tile * blocks) * kMergeBlock + threadIdx.x;
     const int row = at / per_row, c = (at - row * per_row) * 4, r = g.row0 + row;
-    // (partials are as large as the largest tile's)
-    if (row >= g.rows || r >= g.n * a.hg) return;
-    const int64_t p0 = ((int64_t)kvh * a.n_parts + g.part) * a.part_rows + row;
+    if (row >= g.rows) return;
+    const int64_t p0 = part_at(a, kvh, g.part, g.n * a.hg) + row;
     const float* ml = a.part_ml + 2 * p0;
     const float* po = a.part_o + p0 * a.D + c;
-    const int64_t next_ml = 2 * (int64_t)a.part_rows, next_o = (int64_t)a.part_rows * a.D;
+    const int64_t rows = paged_few(g.n * a.hg) ? a.few_rows : a.part_rows;
+    const int64_t next_ml = 2 * rows, next_o = rows * a.D;
     float top = -FLT_MAX;
 #pragma unroll 4
     for (int s = 0; s < g.splits; ++s) top = fmaxf(top, ml[s * next_ml]);
@@ -68,8 +68,12 @@ __global__ void __launch_bounds__(kMergeBlock) paged_merge_kernel(PagedLaunch a)
                o * inverse_sum(sum));
 }
 
+int64_t part_rows_of(const int64_t* info) {
+    return info[kInfoFewParts] * info[kInfoFewRows] +
+           (info[kInfoParts] - info[kInfoFewParts]) * info[kInfoPartRows];
+}
 int64_t part_floats(const int64_t* info, int32_t kv_heads, int32_t head_dim) {
-    return info[kInfoParts] * info[kInfoPartRows] * kv_heads * (head_dim + 2);
+    return part_rows_of(info) * kv_heads * (head_dim + 2);
 }
 
 }  // namespace
@@ -131,10 +135,12 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     a.merges = reinterpret_cast<const PagedMerge*>(plan + info[kInfoMergesAt]);
     a.zeros = plan + info[kInfoZerosAt];
     a.n_merges = (int)info[kInfoMerges];
-    a.n_parts = (int)info[kInfoParts];
     a.part_rows = (int)info[kInfoPartRows];
+    a.few_rows = (int)info[kInfoFewRows];
+    a.part_total = part_rows_of(info);
+    a.many_at = info[kInfoFewParts] * (info[kInfoFewRows] - info[kInfoPartRows]);
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + (int64_t)a.n_parts * a.part_rows * kv_heads * head_dim;
+    a.part_ml = a.part_o + a.part_total * kv_heads * head_dim;
     a.Hq = q_heads;
     a.Hkv = kv_heads;
     a.hg = q_heads / kv_heads;

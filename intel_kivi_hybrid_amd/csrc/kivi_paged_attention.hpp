@@ -152,8 +152,13 @@ __device__ __forceinline__ int64_t q_offset(const PagedLaunch& a, const Work& w,
     const int i = r / w.hg;
     return (w.it.tok0 + i) * a.q_st + (int64_t)(w.kvh * w.hg + (r - i * w.hg)) * a.q_sh;
 }
+// The first row of a partial of a sequence with `rows` rows.
+__device__ __forceinline__ int64_t part_at(const PagedLaunch& a, int kvh, int part, int rows) {
+    return kvh * a.part_total + (paged_few(rows) ? (int64_t)part * a.few_rows
+                                                 : a.many_at + (int64_t)part * a.part_rows);
+}
 __device__ __forceinline__ int64_t part_row(const PagedLaunch& a, const Work& w, int r) {
-    return ((int64_t)w.kvh * a.n_parts + w.it.part) * a.part_rows + (r - w.it.row0);
+    return part_at(a, w.kvh, w.it.part, w.rows) + (r - w.it.row0);
 }
 
 // Four consecutive elements, widened.

@@ -1,8 +1,12 @@
 """CPU tests of the paged cache's limits: sizes at which the kernels' 32-bit
-positions and rows would wrap."""
+positions and rows would wrap, and workspaces by what is live."""
 
 import numpy as np
 import pytest
+import torch
+
+from tests.paged_helpers import make_table
+from tests.test_paged_plan import _plan
 
 
 def _info(table, pool, ctx, new, page_size, Hq, Hkv, D=16, dtype=1):
@@ -39,3 +43,17 @@ def test_rows_that_would_wrap():
     assert rc == 1 and "too large" in text
     rc, text = _info(table[:, :1], 1 << 9, [1], [1], 128, (1 << 31) - 1, 1)
     assert rc == 1 and "too large" in text
+
+
+def test_workspace_follows_the_live_rows():
+    """Eight single tokens of 32K positions beside a verification of five tokens:
+    partials of 8 rows and of 40, not all of a tile of 128."""
+    from intel_kivi_hybrid_amd import _native
+    lens = [(32768, 1)] * 8 + [(32768, 5)]
+    table, pool, ctx, new = make_table(lens, 256, seed=1)
+    words, info = _plan(table, pool, ctx, new, 256, torch.bfloat16, 32, 4, 128)
+    merges = words[info[4]:info[4] + 8 * info[5]].reshape(-1, 8)
+    need = _native.load().kivi_paged_attention_workspace_size(info.ctypes.data, 4, 128)
+    assert need == sum(m[3] * (8 if m[1] == 1 else 40) for m in merges) * 4 * 130 * 4 > 0
+    # (partials of few rows come first)
+    assert max(m[4] + m[3] for m in merges if m[1] == 1) == min(m[4] for m in merges if m[1] == 5)
