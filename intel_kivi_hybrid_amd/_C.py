@@ -705,18 +705,13 @@ def packed_attention_typed(q, store, softmax_scale=None, kv_start=None, hidden=N
 # Paged cache (no reference counterpart; see include/kivi_hip.h): sequences of
 # unequal lengths on pages of one pool.
 # --------------------------------------------------------------------------
-def _tracked() -> bool:
-    """Whether a derivative of either kind may be asked of a call made now."""
-    return torch.is_grad_enabled() or forward_ad._current_level >= 0
-
-
 def _check_inference(*tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 _fail("inference only: a tensor requires a gradient; call it under "
                       "torch.no_grad()")
-    if forward_ad._current_level >= 0:
+    if forward_ad._current_level >= 0:                   # (inside a dual_level())
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 _fail("inference only: a tensor has a forward-mode tangent")
@@ -756,12 +751,12 @@ class PagedPlan:
     def _enter(self, device: int) -> int:
         """The current stream's handle, ordered behind the plan's copy."""
         handle = stream_handle(device)
-        if handle == self._stream and self._settled:
-            return handle
-        if torch.cuda.is_current_stream_capturing():
-            # (on the plan's own stream too: a replay may come on another)
-            _check(self._settled, "call the plan's wait() before capturing a graph with it")
-        elif handle != self._stream:
+        if not self._settled:
+            # (before a capture on the plan's own stream too: a replay may come on another)
+            _check(not torch.cuda.is_current_stream_capturing(),
+                   "call the plan's wait() before capturing a graph with it")
+            self._settled = self._event.query()
+        if handle != self._stream and not torch.cuda.is_current_stream_capturing():
             stream = torch.cuda.current_stream(device)
             if not self._settled:
                 stream.wait_event(self._event)
@@ -903,8 +898,7 @@ def paged_append(k, v, k_pages, v_pages, plan, q=None, q_out=None, cos=None, sin
         with on_device(dev):
             return paged_append(k, v, k_pages, v_pages, plan, q, q_out, cos, sin, interleaved,
                                 q_norm, k_norm, eps)
-    if _tracked():
-        _check_inference(k, v, k_pages, v_pages, q, q_out, cos, sin, q_norm, k_norm)
+    _check_inference(k, v, k_pages, v_pages, q, q_out, cos, sin, q_norm, k_norm)
     kp, vp = _check_pages(plan, k_pages, v_pages)
     _check(kp != vp or plan.tokens == 0, "k_pages and v_pages must be two pools")
     ks = _check_tokens(k, "k", plan, plan.kv_heads)
@@ -1002,8 +996,7 @@ def paged_attention(q, k_pages, v_pages, plan, softmax_scale=None, out=None, wor
     if not is_current(dev):
         with on_device(dev):
             return paged_attention(q, k_pages, v_pages, plan, softmax_scale, out, workspace)
-    if _tracked():
-        _check_inference(q, k_pages, v_pages, out)
+    _check_inference(q, k_pages, v_pages, out)
     kp, vp = _check_pages(plan, k_pages, v_pages)
     st = _check_tokens(q, "q", plan, plan.q_heads)
     q_ptr = q.data_ptr()

@@ -60,14 +60,13 @@ def test_forward_mode_tangents_are_refused(hip_device):
 
 def test_capture_on_the_plans_own_stream_needs_a_settled_plan(hip_device):
     s = torch.cuda.Stream()
-    table, pool, ctx, new, kp, vp, _, q = _setup([(20, 1)], 32, BF, 4, 2, 64, seed=3)
+    table, pool, ctx, new, kp, vp, other, q = _setup([(20, 1)], 32, BF, 4, 2, 64, seed=3)
     kd, vd, qd = kp.cuda(), vp.cuda(), q.cuda()
+    want = _c().paged_attention(qd, kd, vd, other)
     torch.cuda.synchronize()
     with torch.cuda.stream(s):
         plan = _c().paged_plan(table, ctx, new, page_size=32, num_pages=pool, q_heads=4,
                                kv_heads=2, head_dim=64, device="cuda:0")
-        want = _c().paged_attention(qd, kd, vd, plan)
-    torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=s):
         with pytest.raises(RuntimeError, match="wait"):
