@@ -455,7 +455,8 @@ size_t kivi_paged_attention_workspace_size(const int64_t* info, int32_t kv_heads
  * included (append them first): new token i of a sequence with n new ones in a
  * context of c sees positions 0 .. c - n + i.  q is [tokens][q_heads][head_dim]
  * of dtype with strides of whole 16-byte vectors, out the same, contiguous; query
- * head h reads kv head h / (q_heads / kv_heads).  softmax_scale must be positive.
+ * head h reads kv head h / (q_heads / kv_heads).  softmax_scale must be positive
+ * and below 2^127.
  * Scores, softmax and sums are fp32; for the product with 16-bit values weights
  * are rounded to dtype (those of a sequence with up to 16 rows to a kv head, tokens
  * x heads, in two pieces, whatever else the step holds).  plan is 16-byte aligned,

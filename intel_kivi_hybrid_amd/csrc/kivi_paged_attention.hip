@@ -107,8 +107,10 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
         return set_error(kErrInvalidArgument,
                          "unsupported geometry: page_size %d, %d query heads over %d kv heads, "
                          "head_dim %d", page_size, q_heads, kv_heads, head_dim);
-    if (!(softmax_scale > 0.f) || !isfinite(softmax_scale))
-        return set_error(kErrInvalidArgument, "softmax_scale must be positive and finite, got %g",
+    const float qscale = softmax_scale * (float)M_LOG2E;
+    if (!(softmax_scale > 0.f) || !isfinite(qscale))
+        return set_error(kErrInvalidArgument,
+                         "softmax_scale must be positive and below 2^127, got %g",
                          (double)softmax_scale);
     if (info[kInfoTokens] == 0) return kOk;
     if (q == nullptr || k_pages == nullptr || v_pages == nullptr || plan == nullptr ||
@@ -146,7 +148,7 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     a.hg = q_heads / kv_heads;
     a.D = head_dim;
     a.page_shift = shift;
-    a.qscale = softmax_scale * (float)M_LOG2E;
+    a.qscale = qscale;
     hipStream_t s = (hipStream_t)stream;
     const PagedItem* items = reinterpret_cast<const PagedItem*>(plan + info[kInfoItemsAt]);
     // (the largest tiles first: the small ones fill in behind them)

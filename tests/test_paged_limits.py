@@ -1,6 +1,8 @@
 """CPU tests of the paged cache's limits: sizes at which the kernels' 32-bit
 positions and rows would wrap, and workspaces by what is live."""
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -57,3 +59,15 @@ def test_workspace_follows_the_live_rows():
     assert need == sum(m[3] * (8 if m[1] == 1 else 40) for m in merges) * 4 * 130 * 4 > 0
     # (partials of few rows come first)
     assert max(m[4] + m[3] for m in merges if m[1] == 1) == min(m[4] for m in merges if m[1] == 5)
+
+
+def test_scales_whose_log2_units_overflow():
+    from intel_kivi_hybrid_amd import _native
+    lib = _native.load()
+    buf = (ctypes.c_float * 64)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    info = (ctypes.c_int64 * 16)()
+    info[1] = 1
+    rc = lib.kivi_paged_attention(p, 64, 64, 1, p, p, 4, 32, 4, 2, 64, p, ctypes.addressof(info),
+                                  ctypes.c_float(3e38), p, None, 0, None)
+    assert rc == 1 and "softmax_scale must be positive" in _native.last_error()
