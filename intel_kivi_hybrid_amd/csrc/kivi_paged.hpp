@@ -52,8 +52,9 @@ constexpr int paged_tile_rows(int kind) { return 16 << kind; }
 
 // The kind that takes `rows` rows of a kv head: fp32 has kernels of 16 and 64 rows,
 // the 16-bit types of 16 and 128.  Up to 16 rows a kernel that streams them is
-// faster (64 single tokens, 32/8 heads, 8K positions: bf16 287 us, in tiles of more
-// rows 317; fp32, 4K positions: 282 and 331), from there on the larger tiles.
+// faster (64 single tokens, 32/8 heads of 128: bf16, up to 8K positions, 287 us, in tiles
+// of more rows 317; fp32, 4096 positions, 361 and 390, 512 positions 43 and 52), from
+// there on the larger tiles.
 constexpr int paged_kind(int64_t rows, bool f32) {
     return rows <= 16 ? kFew16 : f32 ? kFew64 : kMany;
 }

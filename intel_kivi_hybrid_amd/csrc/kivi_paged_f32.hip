@@ -10,15 +10,15 @@
 // of 16 positions.
 //
 // Up to 16 rows are bound by memory: a workgroup's four waves walk units of their
-// own, straight from memory to registers, and join at the end.  64 sequences of 4K
-// positions, 32/8 heads of 128: 272 us, 5.7 TB/s.
+// own, straight from memory to registers, and join at the end.  64 sequences of 4096
+// positions, 32/8 heads of 128: 361 us, 5.9 TB/s.
 //
 // More are bound by the fp32 products (a sixteenth of the 16-bit rate): each wave
 // takes 16 of 64 rows, and all read the same tiles from LDS, the next one on its way
 // in registers.  1024 tokens over 8K positions of two sequences, 32/8 heads of 128:
-// 113 TFLOP/s of the 154 that a large product reaches; 638 tokens of 5 sequences,
-// 28/4 heads: 104 us (with two tiles of 16 rows for each wave and the keys split
-// over the waves, each reading all of them from L2: 157).  Small steps stay at a
+// 113 TFLOP/s of the 154 that a large product reaches; 319 to 638 tokens of each of 5
+// sequences, 28/4 heads: 95 to 104 us (with two tiles of 16 rows for each wave and the
+// keys split over the waves, each reading all of them from L2: 157).  Small steps stay at a
 // third of the rate: 256 workgroups of 36 units take 1.6 us a unit, of 132 1.2 (0.85
 // are the products), wherever their operands come from.
 #include <hip/hip_runtime.h>

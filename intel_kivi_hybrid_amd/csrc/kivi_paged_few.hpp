@@ -14,7 +14,7 @@
 // rows the same is done in their launch (kivi_paged_many.hip).
 //
 // 64 sequences of up to 8K positions, 32/8 heads of 128, bf16: 287 us, 5.75 TB/s (a
-// read-only stream reaches 6.4).  One sequence of 1K: 7.5 us, and the join 3.8.
+// read-only stream reaches 6.4).  One sequence of 1K: 7 us, and the join 3 to 4.
 #pragma once
 
 #include "kivi_paged_attention.hpp"

@@ -9,11 +9,11 @@
 // for them, two workgroups per CU.
 //
 // Many rows are bound by the products: 2048 tokens after 8200, 32/8 heads of 128,
-// bf16: 310 to 335 us, 920 to 1000 TFLOP/s, of the 1093 that a large product
+// bf16: 305 to 335 us, 920 to 1015 TFLOP/s, of the 1093 that a large product
 // reaches (the matrix cores busy for 47 % of the cycles, at a clock that they bring
 // down to 1.8 GHz).  Few rows are bound by memory, whatever the idle waves: 5 tokens
-// of 16 sequences, 28/4 heads, 3K positions: 23 us with the join, of 64 at 8K 167,
-// 5.0 TB/s (a kernel of 64 rows of its own, with its waves on both rows and
+// of 16 sequences, 28/4 heads, 3K positions: 23 us with the join, of 64 at 8K 157 to
+// 167, 5.0 TB/s (a kernel of 64 rows of its own, with its waves on both rows and
 // positions and three tiles in flight, took 27 and 186).
 //
 // A workgroup whose sequence has up to 16 rows walks it as kivi_paged_few.hpp does, in

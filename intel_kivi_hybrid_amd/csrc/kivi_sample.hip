@@ -16,7 +16,9 @@
 // last border moves the last by less than a bucket's mass); the second launch, a
 // workgroup for each row, takes their tokens from the slices and ranks those
 // against each other, by sub-buckets where they are many.  Where they are more than
-// fit its list (thousands of equal logits) it goes through the row instead.
+// fit its list (a flat distribution, or thousands of equal logits) it goes through the
+// row instead: 64 rows of 128256 normal logits of deviation 1, temperature 1.3, top_p
+// 0.9: fp32 268 us, bf16 410.
 //
 // Precision: neighbouring borders lie as close as a token's share of the mass,
 // 1e-6 and less, and sums of fp32 weights over 10^5 tokens are off by more than
@@ -25,11 +27,11 @@
 // any order; a bucket's sum is rounded to 2^-43 of the row's largest edge.  Tokens
 // below e^-32 of a slice's largest have no mass (2^-46 of it, each).
 //
-// 64 rows of 128256 bf16 logits with settings of their own: 49 us (the first launch
-// 19, bound by its 55 vector operations for each token, the second 34, bound by the
-// passes that one CU makes over a warm row's list of 4500 tokens); one row of 50257
-// fp32: 20 us (8 and 12, both the latency of their steps).  The logits' bytes alone
-// would take 3 us.
+// 64 rows of 128256 bf16 logits with settings of their own: 46 to 49 us a call (in a
+// serialised trace the first launch 19, bound by its 55 vector operations for each
+// token, the second 34, bound by the passes that one CU makes over a warm row's list of
+// 4500 tokens); one row of 50257 fp32: 20 us (8 and 12, both the latency of their
+// steps).  The logits' bytes alone would take 3 us.
 #include <hip/hip_runtime.h>
 
 #include <math.h>
