@@ -19,6 +19,8 @@ namespace kivi {
 namespace {
 
 constexpr int kMergeBlock = 256;
+// (a launch has fewer than 2^32 lanes; all of these have 256 to a workgroup)
+constexpr int64_t kMostBlocks = (int64_t)UINT32_MAX / kMergeBlock;
 
 // Joins partials: a thread takes four channels of a row.  Bound by its reads of the
 // partials, and for few of them by one trip to memory: 4 us for a single token's 8
@@ -158,7 +160,7 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
         a.items = items + before;
         a.n_items = (int)info[kInfoItems + kind];
         if (a.n_items == 0) continue;
-        if ((int64_t)a.n_items * kv_heads > INT32_MAX)
+        if ((int64_t)a.n_items * kv_heads > kMostBlocks)
             return set_error(kErrInvalidArgument, "%d items are too many for one launch",
                              a.n_items);
         if (kind == kMany) launch_paged_many(a, dtype, s);
@@ -170,7 +172,7 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     if (a.n_merges == 0) return kOk;
     const int64_t blocks = (int64_t)a.n_merges * kv_heads *
                            ((a.part_rows * (head_dim / 4) + kMergeBlock - 1) / kMergeBlock);
-    if (blocks > INT32_MAX)
+    if (blocks > kMostBlocks)
         return set_error(kErrInvalidArgument, "%d tiles to merge are too many for one launch",
                          a.n_merges);
     const dim3 grid((unsigned)blocks);

@@ -978,7 +978,8 @@ int kivi_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t r
     if (logits == nullptr || uniforms == nullptr || out == nullptr)
         return set_error(kErrInvalidArgument, "null pointer");
     const int64_t slices = slices_of(vocab);
-    if (rows * slices > INT32_MAX)
+    // (a launch has fewer than 2^32 lanes)
+    if (rows * slices > (int64_t)UINT32_MAX / kBlock || rows > (int64_t)UINT32_MAX / kPickBlock)
         return set_error(kErrInvalidArgument, "%d rows of %d tokens are too many for one launch",
                          rows, vocab);
     const size_t need = kivi_sample_workspace_size(rows, vocab);
