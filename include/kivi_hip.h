@@ -471,6 +471,51 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
                          const int64_t* info, float softmax_scale, void* out, void* workspace,
                          size_t workspace_bytes, void* stream);
 
+/* ---- paged cache of 8 bits ---------------------------------------------------
+ * The same cache with pages of codes, [num_pages][kv_heads][page_size][head_dim]
+ * int8, and a scale for each block of 16 positions of a page and kv head,
+ * [num_pages][kv_heads][page_size / 16] f32, beside each pool: a key or value is
+ * code * scale. */
+#define KIVI_PAGED8_INFO 20
+
+/* kivi_paged_plan for pages of 8 bits; dtype is that of queries and outputs.  No
+ * block of 16 positions may get new tokens of two sequences. */
+int kivi_paged8_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* context_lens,
+                     const int32_t* page_table, int64_t table_stride, int32_t table_pages,
+                     int32_t page_size, int64_t num_pages, int32_t dtype, int32_t q_heads,
+                     int32_t kv_heads, int32_t head_dim, int32_t* plan, int64_t plan_words,
+                     int64_t* info);
+
+/* kivi_paged_append to pages of 8 bits.  A block's scale is the least power of two
+ * from 2^-126 on whose 127-fold reaches every value that was appended to the block
+ * since its first position was, codes are quotients rounded to nearest even; where
+ * new tokens need a larger scale, the codes that the block holds are rounded again.
+ * Keys that are normed or rotated are formed in fp64.  A value that is not finite
+ * makes its block's scale NaN, until the block's first position is written again.
+ * Codes behind the last token are left as they are.  Scales must not be negative. */
+int kivi_paged8_append(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                       const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                       const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                       int32_t dtype, void* q_out, int8_t* k_pages, int8_t* v_pages,
+                       float* k_scales, float* v_scales, int64_t num_pages, int32_t page_size,
+                       int32_t q_heads, int32_t kv_heads, int32_t head_dim, const int32_t* plan,
+                       const int64_t* info, const float* cos, const float* sin,
+                       int32_t rotary_dim, int32_t interleaved, const void* q_norm,
+                       const void* k_norm, int32_t norm_dtype, float eps, void* stream);
+
+/* kivi_paged_attention over pages of 8 bits (its workspace function, with the info of
+ * kivi_paged8_plan).  Codes enter the products exactly; weights times value scales are
+ * rounded to bf16 (fp16 for f16 queries and more than 16 rows to a kv head), in two
+ * pieces for up to 16 rows and three for f32, whose queries enter in three pieces too.
+ * A row that sees a position of a block whose scale is NaN comes out as NaN; scales of
+ * blocks that it sees nothing of do not reach it. */
+int kivi_paged8_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                          int32_t dtype, const int8_t* k_pages, const int8_t* v_pages,
+                          const float* k_scales, const float* v_scales, int64_t num_pages,
+                          int32_t page_size, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                          const int32_t* plan, const int64_t* info, float softmax_scale, void* out,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- sampling ---------------------------------------------------------------
  * Next tokens out[rows] from logits [rows][vocab] (dtype 0 f32, 1 bf16, 2 f16;
  * rows row_stride elements apart; vocab at most 2^20) and uniforms[rows] in [0, 1)

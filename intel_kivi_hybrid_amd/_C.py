@@ -738,7 +738,8 @@ class PagedPlan:
     pools of ``num_pages`` pages and to the geometry it was made for."""
 
     __slots__ = ("device", "tokens", "context", "num_pages", "page_size", "q_heads", "kv_heads",
-                 "head_dim", "dtype", "_code", "_index", "_pool", "_buf", "_ptr", "_info",
+                 "head_dim", "dtype", "cache_dtype", "_code", "_index", "_pool", "_scales", "_buf",
+                 "_ptr", "_info",
                  "_info_ptr", "_workspace", "_stream", "_event", "_settled")
 
     def wait(self) -> None:
@@ -769,18 +770,24 @@ _PLAN_ITEMS = 1 << 13        # int32s of a plan's items that a first buffer has 
 
 
 def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_heads, kv_heads,
-               head_dim, dtype=torch.bfloat16, device="cuda") -> PagedPlan:
+               head_dim, dtype=torch.bfloat16, device="cuda", cache_dtype=None) -> PagedPlan:
     """The plan of a step in which sequence s, ``context_lens[s]`` tokens long
     with them, brings its last ``new_lens[s]`` tokens (0: it sits this step out).
     ``page_table`` (int32 host tensor ``[sequences, pages]``): its pages, position
     p on entry ``p // page_size``; entries behind its last position are not read.
-    Tokens are numbered sequence by sequence.  Host work and one copy to
-    ``device``, once per step for all layers."""
+    Tokens are numbered sequence by sequence.  ``cache_dtype``: the pages' type,
+    ``dtype`` or int8 (no block of 16 positions may then get new tokens of two
+    sequences).  Host work and one copy to ``device``, once per step for all
+    layers."""
     _check(isinstance(page_table, torch.Tensor) and page_table.dim() == 2
            and page_table.dtype is torch.int32 and page_table.device.type == "cpu",
            "page_table must be an int32 [sequences, pages] tensor on the host")
     _check(dtype in _IO_DTYPES, "dtype must be float32, bfloat16 or float16, got ",
            _dtype_name(dtype))
+    eight = cache_dtype is torch.int8
+    _check(eight or cache_dtype is None or cache_dtype is dtype, "cache_dtype must be ",
+           _dtype_name(dtype), " or int8, got ", _dtype_name(cache_dtype))
+    make = _lib.kivi_paged8_plan if eight else _lib.kivi_paged_plan
     dev = torch.device(device)
     _check(dev.type == _DEVICE_TYPE, "device must be on ", _DEVICE_TYPE, " but got ", dev.type)
     page_size, q_heads, kv_heads, head_dim = (
@@ -794,7 +801,7 @@ def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_he
            "context_lens and new_lens must hold one entry for each of the table's ", n_seqs,
            " sequences")
     p = PagedPlan()
-    info = (ctypes.c_int64 * 16)()
+    info = (ctypes.c_int64 * 20)()
     p._info, p._info_ptr = info, ctypes.addressof(info)
     args = (n_seqs, new.data_ptr(), ctx.data_ptr(), table.data_ptr(), table.shape[1],
             table.shape[1], page_size, num_pages, _IO_DTYPES[dtype], q_heads, kv_heads, head_dim)
@@ -806,8 +813,8 @@ def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_he
                "a plan is made outside of a graph's capture")
         host = torch.empty(table.numel() + 2 * min(max(int(new.sum()), 0), 1 << 20) + _PLAN_ITEMS,
                            dtype=torch.int32, pin_memory=True)
-    rc = _lib.kivi_paged_plan(*args, None if host is None else host.data_ptr(),
-                              0 if host is None else host.numel(), p._info_ptr)
+    rc = make(*args, None if host is None else host.data_ptr(),
+              0 if host is None else host.numel(), p._info_ptr)
     if rc and (host is None or info[0] <= host.numel()):
         _native.check(rc, "paged_plan")
     p.device = torch.device(_DEVICE_TYPE, device_index(dev))
@@ -816,10 +823,11 @@ def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_he
     p.q_heads, p.kv_heads, p.head_dim = q_heads, kv_heads, head_dim
     p._index = p.device.index
     p._pool = torch.Size((num_pages, kv_heads, page_size, head_dim))
+    p.cache_dtype = torch.int8 if eight else dtype
+    p._scales = torch.Size((num_pages, kv_heads, page_size // 16)) if eight else None
     if host is None or info[0] > host.numel():
         host = torch.empty(max(info[0], 1), dtype=torch.int32, pin_memory=True)
-        _native.check(_lib.kivi_paged_plan(*args, host.data_ptr(), host.numel(), p._info_ptr),
-                      "paged_plan")
+        _native.check(make(*args, host.data_ptr(), host.numel(), p._info_ptr), "paged_plan")
     with on_device(p.device):
         p._buf = host[:max(info[0], 1)].to(p.device, non_blocking=True)
         p._event = torch.cuda.Event()
@@ -836,7 +844,7 @@ def paged_plan(page_table, context_lens, new_lens, *, page_size, num_pages, q_he
 # common ways to be right) only where it fails.
 def _check_pages(plan, k_pages, v_pages):
     kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
-    pool, dt, dev = plan._pool, plan.dtype, plan._index
+    pool, dt, dev = plan._pool, plan.cache_dtype, plan._index
     if not (k_pages.shape == pool and v_pages.shape == pool and k_pages.dtype is dt
             and v_pages.dtype is dt and k_pages.is_contiguous() and v_pages.is_contiguous()
             and k_pages.get_device() == dev and v_pages.get_device() == dev
@@ -848,6 +856,28 @@ def _check_pages(plan, k_pages, v_pages):
                    _dtype_name(dt), " on ", plan.device, ", got ", list(t.shape), " of ",
                    _dtype_name(t.dtype), " on ", t.device)
     return kp, vp
+
+
+def _check_scales(plan, k_scales, v_scales):
+    """The scales of pages of 8 bits (none for others): their addresses."""
+    shape, dev = plan._scales, plan._index
+    if shape is None:
+        _check(k_scales is None and v_scales is None,
+               "k_scales and v_scales belong to pages of int8, the plan is for ",
+               _dtype_name(plan.dtype))
+        return 0, 0
+    _check(k_scales is not None and v_scales is not None,
+           "pages of int8 need k_scales and v_scales")
+    if not (k_scales.shape == shape and v_scales.shape == shape
+            and k_scales.dtype is torch.float32 and v_scales.dtype is torch.float32
+            and k_scales.is_contiguous() and v_scales.is_contiguous()
+            and k_scales.get_device() == dev and v_scales.get_device() == dev):
+        for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+            _check(t.shape == shape and t.dtype is torch.float32 and t.is_contiguous()
+                   and t.get_device() == dev, name, " must be a contiguous ", list(shape),
+                   " tensor of Float on ", plan.device, ", got ", list(t.shape), " of ",
+                   _dtype_name(t.dtype), " on ", t.device)
+    return k_scales.data_ptr(), v_scales.data_ptr()
 
 
 def _check_tokens(t, name: str, plan, heads: int):
@@ -881,7 +911,8 @@ def _check_out(out, name: str, like) -> None:
 
 
 def paged_append(k, v, k_pages, v_pages, plan, q=None, q_out=None, cos=None, sin=None,
-                 interleaved=False, q_norm=None, k_norm=None, eps=1e-6):
+                 interleaved=False, q_norm=None, k_norm=None, eps=1e-6, k_scales=None,
+                 v_scales=None):
     """Write a step's new keys and values ``[tokens, Hkv, D]`` to their pages,
     normed and rotated on the way, and return its queries ``q`` ``[tokens, Hq, D]``
     normed and rotated likewise (None without ``q``): one launch.
@@ -892,15 +923,26 @@ def paged_append(k, v, k_pages, v_pages, plan, q=None, q_out=None, cos=None, sin
     the token's position in its sequence, channel i with i + r/2, or 2i with 2i + 1
     if ``interleaved``.  Both in fp32, rounded once.  Values are copied.  Rows may
     have any strides, as slices of one projection have; rows behind the plan's
-    tokens are not read, and stay as they are in ``q_out``, which may be ``q``."""
+    tokens are not read, and stay as they are in ``q_out``, which may be ``q``.
+
+    Pages of int8 (a plan with ``cache_dtype=torch.int8``) have ``k_scales`` and
+    ``v_scales`` ``[num_pages, Hkv, page_size / 16]`` fp32 beside them, one for each
+    block of 16 positions of a page and head: the least power of two from 2^-126 on
+    whose 127-fold reaches the block's values; an element is code * scale, its code
+    the quotient rounded to nearest even.  A block's older codes are rounded again
+    where new tokens need a larger scale.  What a block's first position finds there
+    is not read.  A value that is not finite makes its block's scale NaN."""
     dev = plan._index
     if not is_current(dev):
         with on_device(dev):
             return paged_append(k, v, k_pages, v_pages, plan, q, q_out, cos, sin, interleaved,
-                                q_norm, k_norm, eps)
-    _check_inference(k, v, k_pages, v_pages, q, q_out, cos, sin, q_norm, k_norm)
+                                q_norm, k_norm, eps, k_scales, v_scales)
+    _check_inference(k, v, k_pages, v_pages, q, q_out, cos, sin, q_norm, k_norm, k_scales,
+                     v_scales)
     kp, vp = _check_pages(plan, k_pages, v_pages)
     _check(kp != vp or plan.tokens == 0, "k_pages and v_pages must be two pools")
+    ksp, vsp = _check_scales(plan, k_scales, v_scales)
+    _check(ksp != vsp or not ksp or plan.tokens == 0, "k_scales and v_scales must be two tensors")
     ks = _check_tokens(k, "k", plan, plan.kv_heads)
     vs = _check_tokens(v, "v", plan, plan.kv_heads)
     rot = cos_ptr = sin_ptr = 0
@@ -938,13 +980,17 @@ def paged_append(k, v, k_pages, v_pages, plan, q=None, q_out=None, cos=None, sin
         q_ptr, q_st, q_sh, out_ptr = q.data_ptr(), st[0], st[1], q_out.data_ptr()
     else:
         _check(q_out is None and q_norm is None, "q_out and q_norm need q")
-    rc = _lib.kivi_paged_append(
-        q_ptr, q_st, q_sh, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-        plan._code, out_ptr, kp, vp, plan.num_pages, plan.page_size, plan.q_heads,
-        plan.kv_heads, plan.head_dim, plan._ptr, plan.tokens, cos_ptr, sin_ptr, rot,
-        1 if interleaved else 0, 0 if q_norm is None else q_norm.data_ptr(),
-        0 if k_norm is None else k_norm.data_ptr(),
-        0 if norm_dt is None else _IO_DTYPES[norm_dt], eps, plan._enter(dev))
+    rows = (q_ptr, q_st, q_sh, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+            plan._code, out_ptr, kp, vp)
+    geometry = (plan.num_pages, plan.page_size, plan.q_heads, plan.kv_heads, plan.head_dim,
+                plan._ptr)
+    way = (cos_ptr, sin_ptr, rot, 1 if interleaved else 0,
+           0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(),
+           0 if norm_dt is None else _IO_DTYPES[norm_dt], eps, plan._enter(dev))
+    if ksp:
+        rc = _lib.kivi_paged8_append(*rows, ksp, vsp, *geometry, plan._info_ptr, *way)
+    else:
+        rc = _lib.kivi_paged_append(*rows, *geometry, plan.tokens, *way)
     if rc:
         _native.check(rc, "paged_append")
     return q_out
@@ -985,19 +1031,24 @@ def _call_workspace(device: int, nbytes: int):
     return buf
 
 
-def paged_attention(q, k_pages, v_pages, plan, softmax_scale=None, out=None, workspace=None):
+def paged_attention(q, k_pages, v_pages, plan, softmax_scale=None, out=None, workspace=None,
+                    k_scales=None, v_scales=None):
     """Attention of a step's new tokens ``q [tokens, Hq, D]`` over their
     sequences' pages, their own keys and values included (:func:`paged_append`
     first): token i of n new ones in a context of c sees positions 0 .. c - n + i.
     Returns ``[tokens, Hq, D]`` in q's type.  Chunks of prompts, verification
     passes and single tokens may share a call.  Rows behind the plan's tokens are
-    not read, and stay as they are in ``out``.  Launched on the current stream."""
+    not read, and stay as they are in ``out``.  ``k_scales``, ``v_scales``: the scales
+    of pages of int8, as :func:`paged_append` leaves them.  Launched on the current
+    stream."""
     dev = plan._index
     if not is_current(dev):
         with on_device(dev):
-            return paged_attention(q, k_pages, v_pages, plan, softmax_scale, out, workspace)
-    _check_inference(q, k_pages, v_pages, out)
+            return paged_attention(q, k_pages, v_pages, plan, softmax_scale, out, workspace,
+                                   k_scales, v_scales)
+    _check_inference(q, k_pages, v_pages, out, k_scales, v_scales)
     kp, vp = _check_pages(plan, k_pages, v_pages)
+    ksp, vsp = _check_scales(plan, k_scales, v_scales)
     st = _check_tokens(q, "q", plan, plan.q_heads)
     q_ptr = q.data_ptr()
     if q_ptr & 15 or (st[0] | st[1]) * q.element_size() & 15:
@@ -1018,11 +1069,15 @@ def paged_attention(q, k_pages, v_pages, plan, softmax_scale=None, out=None, wor
                and not ws_ptr & 15 and ws_bytes >= need,
                "workspace must be a contiguous, 16-byte aligned tensor of ", need,
                " bytes on ", plan.device)
-    rc = _lib.kivi_paged_attention(
-        q_ptr, st[0], st[1], plan._code, kp, vp, plan.num_pages, plan.page_size,
-        plan.q_heads, plan.kv_heads, plan.head_dim, plan._ptr, plan._info_ptr,
-        plan.head_dim ** -0.5 if softmax_scale is None else float(softmax_scale),
-        out.data_ptr(), ws_ptr, ws_bytes, plan._enter(dev))
+    geometry = (plan.num_pages, plan.page_size, plan.q_heads, plan.kv_heads, plan.head_dim,
+                plan._ptr, plan._info_ptr,
+                plan.head_dim ** -0.5 if softmax_scale is None else float(softmax_scale),
+                out.data_ptr(), ws_ptr, ws_bytes, plan._enter(dev))
+    if ksp:
+        rc = _lib.kivi_paged8_attention(q_ptr, st[0], st[1], plan._code, kp, vp, ksp, vsp,
+                                        *geometry)
+    else:
+        rc = _lib.kivi_paged_attention(q_ptr, st[0], st[1], plan._code, kp, vp, *geometry)
     if rc:
         _native.check(rc, "paged_attention")
     return out

@@ -104,6 +104,14 @@ __device__ __forceinline__ float seg_partner(float v) {
     return __builtin_bit_cast(float, r);
 }
 
+template <int M>
+__device__ __forceinline__ double seg_partner(double v) {
+    const int2 x = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(double, make_int2(
+        __float_as_int(seg_partner<M>(__int_as_float(x.x))),
+        __float_as_int(seg_partner<M>(__int_as_float(x.y)))));
+}
+
 // Reduce min and max over aligned segments of LANES consecutive lanes
 // (LANES a power of two <= 64).  Every lane of a segment ends with the result.
 template <int LANES>

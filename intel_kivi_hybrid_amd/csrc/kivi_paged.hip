@@ -11,11 +11,7 @@
 // written once.  Memory-bound for prompts (12.3K tokens of 32/8 heads of 128 with
 // norms, bf16: 59 us, 4.7 TB/s, where a copy reaches 5.0), launch-bound for single
 // tokens (64 of 64/8 heads, fp16: 3.7 us on the GPU, 12 us a call).
-//
-// A lane takes two 8-element vectors of a head, D/2 apart (r/2 in a rotated part of
-// r channels), that hold whole pairs of either kind of rotation: neighbours, or
-// i and i + r/2.  So a rotation never crosses lanes, and only the norm's sum does,
-// over the D / 16 lanes of the head (a power of two of them, DPP steps).
+// How lanes share a head: kivi_paged_rows.hpp.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -23,125 +19,11 @@
 #include <new>
 #include <vector>
 
-#include "kivi_common.hpp"
-#include "kivi_paged.hpp"
+#include "kivi_paged_rows.hpp"
 #include "../../include/kivi_hip.h"
 
 namespace kivi {
 namespace {
-
-constexpr int kAppendBlock = 256;
-
-struct AppendArgs {
-    const void* q;
-    const void* k;
-    const void* v;
-    int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
-    void* q_out;
-    void* k_pages;
-    void* v_pages;
-    const int2* tokens;          // slot, position
-    const float* cos;
-    const float* sin;
-    const void* q_norm;
-    const void* k_norm;
-    float eps, inv_d;
-    int n_tokens, Hq, Hkv, D, page_shift, rot, lanes_log2;
-    int norm_dt, norm_vec, interleaved, vec;
-};
-
-typedef unsigned int kivi_u4v __attribute__((ext_vector_type(4)));
-
-// Eight elements as they lie: one or two 16-byte loads (vec: aligned to 16), read once
-// by this kernel.
-template <int DT>
-struct Eight {
-    static constexpr int kWords = DT == kSrcF32 ? 8 : 4;
-    uint32_t w[kWords];
-
-    __device__ __forceinline__ void load(const void* p, int64_t i, bool vec) {
-        const char* from = static_cast<const char*>(p) + i * src_size(DT);
-        if (vec) {
-#pragma unroll
-            for (int j = 0; j < kWords; j += 4) {
-                const kivi_u4v x =
-                    __builtin_nontemporal_load(reinterpret_cast<const kivi_u4v*>(from + 4 * j));
-#pragma unroll
-                for (int k = 0; k < 4; ++k) w[j + k] = x[k];
-            }
-        } else if constexpr (DT == kSrcF32) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = reinterpret_cast<const uint32_t*>(from)[j];
-        } else {
-            const uint16_t* h = reinterpret_cast<const uint16_t*>(from);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
-        }
-    }
-    __device__ __forceinline__ void widen(float (&x)[8]) const {
-        if constexpr (DT == kSrcF32) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(w[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (DT == kSrcBF16) {
-                    x[2 * j] = __uint_as_float(w[j] << 16);
-                    x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-                } else {
-                    x[2 * j] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j] & 0xffffu));
-                    x[2 * j + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[j] >> 16));
-                }
-            }
-        }
-    }
-    __device__ __forceinline__ void round(const float (&x)[8]) {
-        if constexpr (DT == kSrcF32) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(x[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint16_t lo, hi;
-                if constexpr (DT == kSrcBF16) {
-                    lo = __builtin_bit_cast(uint16_t, (__bf16)x[2 * j]);
-                    hi = __builtin_bit_cast(uint16_t, (__bf16)x[2 * j + 1]);
-                } else {
-                    lo = __builtin_bit_cast(uint16_t, (_Float16)x[2 * j]);
-                    hi = __builtin_bit_cast(uint16_t, (_Float16)x[2 * j + 1]);
-                }
-                w[j] = lo | (uint32_t)hi << 16;
-            }
-        }
-    }
-    __device__ __forceinline__ void store(void* p, int64_t i) const {
-        uint4* to = reinterpret_cast<uint4*>(static_cast<char*>(p) + i * src_size(DT));
-#pragma unroll
-        for (int j = 0; j < kWords; j += 4)
-            to[j / 4] = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
-    }
-};
-// Eight of a type known at run time, widened.
-template <int DT>
-__device__ __forceinline__ void load8(const void* p, int i, bool vec, float (&x)[8]) {
-    Eight<DT> e;
-    e.load(p, i, vec);
-    e.widen(x);
-}
-__device__ __forceinline__ void load8_dt(const void* p, int i, int dt, bool vec, float (&x)[8]) {
-    if (dt == kSrcF32) load8<kSrcF32>(p, i, vec, x);
-    else if (dt == kSrcBF16) load8<kSrcBF16>(p, i, vec, x);
-    else load8<kSrcF16>(p, i, vec, x);
-}
-
-// Sum over aligned segments of 1 << log2 lanes.
-__device__ __forceinline__ float seg_sum(float v, int log2) {
-    if (log2 > 0) v += seg_partner<1>(v);
-    if (log2 > 1) v += seg_partner<2>(v);
-    if (log2 > 2) v += seg_partner<4>(v);
-    if (log2 > 3) v += seg_partner<8>(v);
-    return v;
-}
 
 // A segment of lanes takes a head of a token.  (Several heads to a segment, to
 // share the angles and have more loads in flight, cost more in waves on a SIMD
@@ -154,15 +36,8 @@ __global__ void __launch_bounds__(kAppendBlock) paged_append_kernel(AppendArgs a
     const uint32_t row = t >> a.lanes_log2;
     const int tok = (int)(row / (uint32_t)heads), h = (int)(row - (uint32_t)tok * heads);
     if (tok >= a.n_tokens) return;                       // (whole segments leave)
-    const int unit = (int)(t & ((1u << a.lanes_log2) - 1));
-    const bool live = unit < a.D / 16;
+    const HeadLane lane = head_lane(a, (int)(t & ((1u << a.lanes_log2) - 1)));
     const int2 place = a.tokens[tok];
-
-    // the lane's two vectors of 8 channels: of the rotated part's halves, or of the
-    // rest's
-    const bool inside = 16 * unit < a.rot;
-    const int start = inside ? 0 : a.rot, at = 8 * unit - start / 2;
-    const int c0 = start + at, c1 = c0 + (inside ? a.rot : a.D - a.rot) / 2;
 
     const void* src = a.v;
     const void* norm = nullptr;
@@ -176,64 +51,6 @@ __global__ void __launch_bounds__(kAppendBlock) paged_append_kernel(AppendArgs a
         norm = a.k_norm;
         from = tok * a.k_st + (int64_t)(h - a.Hq) * a.k_sh;
     }
-    Eight<DT> ex{}, ey{};
-    if (live) {
-        ex.load(src, from + c0, a.vec);
-        ey.load(src, from + c1, a.vec);
-    }
-    // angles: of pairs (c0 + j, c1 + j), or of the pairs in x and those in y
-    const bool turned = live && inside && h < a.Hq + a.Hkv;
-    const int half = a.rot / 2;
-    float4 cs[2], sn[2];
-    if (turned) {
-        const int64_t r = (int64_t)place.y * half;
-        const int i0 = a.interleaved ? c0 / 2 : c0, i1 = a.interleaved ? c1 / 2 : c0 + 4;
-        cs[0] = *reinterpret_cast<const float4*>(a.cos + r + i0);
-        cs[1] = *reinterpret_cast<const float4*>(a.cos + r + i1);
-        sn[0] = *reinterpret_cast<const float4*>(a.sin + r + i0);
-        sn[1] = *reinterpret_cast<const float4*>(a.sin + r + i1);
-    }
-    float x[8], y[8];
-    ex.widen(x);
-    ey.widen(y);
-    if (norm != nullptr) {
-        float u[8], w[8];
-        if (live) {
-            load8_dt(norm, c0, a.norm_dt, a.norm_vec, u);
-            load8_dt(norm, c1, a.norm_dt, a.norm_vec, w);
-        }
-        float s = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s = fmaf(x[j], x[j], fmaf(y[j], y[j], s));
-        s = seg_sum(s, a.lanes_log2);
-        const float r = rsqrtf(fmaf(s, a.inv_d, a.eps));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[j] = x[j] * r * u[j];
-            y[j] = y[j] * r * w[j];
-        }
-    }
-    if (!live) return;
-    if (turned) {
-        const float c[8] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w, cs[1].x, cs[1].y, cs[1].z, cs[1].w};
-        const float s[8] = {sn[0].x, sn[0].y, sn[0].z, sn[0].w, sn[1].x, sn[1].y, sn[1].z, sn[1].w};
-        if (a.interleaved) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float* v = j < 4 ? x + 2 * j : y + 2 * (j - 4);
-                const float p = v[0], q = v[1];
-                v[0] = fmaf(p, c[j], -(q * s[j]));
-                v[1] = fmaf(q, c[j], p * s[j]);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float p = x[j], q = y[j];
-                x[j] = fmaf(p, c[j], -(q * s[j]));
-                y[j] = fmaf(q, c[j], p * s[j]);
-            }
-        }
-    }
     void* dst = a.q_out;
     int64_t to = ((int64_t)tok * a.Hq + h) * a.D;
     if (h >= a.Hq) {
@@ -243,26 +60,22 @@ __global__ void __launch_bounds__(kAppendBlock) paged_append_kernel(AppendArgs a
         dst = h < a.Hq + a.Hkv ? a.k_pages : a.v_pages;
         to = (((page * a.Hkv + kvh) << a.page_shift) + off) * a.D;
     }
-    // (what is only moved keeps its bits: to fp32 and back a signalling NaN loses one)
-    if (norm != nullptr || turned) {
-        ex.round(x);
-        ey.round(y);
-    }
-    ex.store(dst, to + c0);
-    ey.store(dst, to + c1);
+    move_row<DT>(a, lane, src, from, norm, h < a.Hq + a.Hkv, place.y, dst, to);
 }
 
-int page_shift_of(int32_t page_size) {
+}  // namespace
+
+int paged_page_shift(int32_t page_size) {
     for (int s = 4; s <= 8; ++s)
         if (page_size == 1 << s) return s;
     return -1;
 }
 
-int check_pool(int32_t dtype, int64_t num_pages, int32_t page_size, int32_t q_heads,
-               int32_t kv_heads, int32_t head_dim) {
+int paged_check_pool(int32_t dtype, int64_t num_pages, int32_t page_size, int32_t q_heads,
+                     int32_t kv_heads, int32_t head_dim) {
     if (dtype < 0 || dtype > 2)
         return set_error(kErrInvalidArgument, "dtype %d is not 0 (f32), 1 (bf16) or 2 (f16)", dtype);
-    if (page_shift_of(page_size) < 0)
+    if (paged_page_shift(page_size) < 0)
         return set_error(kErrInvalidArgument,
                          "page_size must be 16, 32, 64, 128 or 256, got %d", page_size);
     if (num_pages < 1 || num_pages > INT32_MAX / page_size)
@@ -280,6 +93,8 @@ int check_pool(int32_t dtype, int64_t num_pages, int32_t page_size, int32_t q_he
         return set_error(kErrUnsupported, "a page of %d kv heads is too large", kv_heads);
     return kOk;
 }
+
+namespace {
 
 struct Tile {
     int seq, row0;
@@ -349,27 +164,21 @@ Cut best_cut(const std::vector<Tile>& tiles, const std::vector<int>& rows, int64
     return best;
 }
 
-}  // namespace
-}  // namespace kivi
-
-using namespace kivi;
-
-extern "C" {
-
-int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* context_lens,
-                    const int32_t* page_table, int64_t table_stride, int32_t table_pages,
-                    int32_t page_size, int64_t num_pages, int32_t dtype, int32_t q_heads,
-                    int32_t kv_heads, int32_t head_dim, int32_t* plan, int64_t plan_ints,
-                    int64_t* info) {
-    int rc = check_pool(dtype, num_pages, page_size, q_heads, kv_heads, head_dim);
+// The plan of kivi_paged_plan, and with `eight` of kivi_paged8_plan.
+int make_plan(bool eight, int32_t n_seqs, const int32_t* new_lens, const int32_t* context_lens,
+              const int32_t* page_table, int64_t table_stride, int32_t table_pages,
+              int32_t page_size, int64_t num_pages, int32_t dtype, int32_t q_heads,
+              int32_t kv_heads, int32_t head_dim, int32_t* plan, int64_t plan_ints,
+              int64_t* info) {
+    int rc = paged_check_pool(dtype, num_pages, page_size, q_heads, kv_heads, head_dim);
     if (rc) return rc;
     if (n_seqs < 0 || info == nullptr || table_pages < 0 || table_stride < table_pages ||
         (n_seqs > 0 && (new_lens == nullptr || context_lens == nullptr ||
                         (page_table == nullptr && table_pages > 0))))
         return set_error(kErrInvalidArgument, "null or negative plan argument");
-    const int shift = page_shift_of(page_size);
+    const int shift = paged_page_shift(page_size);
     const int hg = q_heads / kv_heads;
-    const bool f32 = dtype == 0;
+    const bool f32 = dtype == 0 && !eight;   // (8 bits: their products run on the 16-bit units)
     try {
         int64_t tokens = 0, pages = 0, longest = 0;
         for (int s = 0; s < n_seqs; ++s) {
@@ -418,10 +227,17 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
         std::sort(runs.begin(), runs.end(), [](const Run& a, const Run& b) {
             return a.page != b.page ? a.page < b.page : a.from < b.from;
         });
-        for (size_t i = 1; i < runs.size(); ++i)
-            if (runs[i].page == runs[i - 1].page && runs[i].from <= runs[i - 1].to)
+        for (size_t i = 1; i < runs.size(); ++i) {
+            if (runs[i].page != runs[i - 1].page) continue;
+            if (runs[i].from <= runs[i - 1].to)
                 return set_error(kErrInvalidArgument, "page %d: a slot is given to two new tokens",
                                  runs[i].page);
+            // (each would rescale the other's)
+            if (eight && runs[i].from / kScaleBlock <= runs[i - 1].to / kScaleBlock)
+                return set_error(kErrInvalidArgument,
+                                 "page %d: a block of %d positions is given to two sequences' new "
+                                 "tokens", runs[i].page, kScaleBlock);
+        }
 
         // Row tiles, and the positions that the last row of each sees.  Beside 16-bit
         // sequences of more than 16 rows those of fewer go into the same launch, where
@@ -489,11 +305,17 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
         }
         const int64_t pages_at = 2 * tokens, items_at = (pages_at + pages + 7) / 8 * 8;
         const int64_t merges_at = items_at + 8 * items, zeros_at = merges_at + 8 * merges;
-        const int64_t ints = tokens > 0 ? zeros_at + 8 : 0;
+        int64_t blocks = 0;
+        for (int s = 0; s < n_seqs && eight; ++s)
+            if (new_lens[s] > 0)
+                blocks += (int64_t)(context_lens[s] - 1) / kScaleBlock -
+                          (context_lens[s] - new_lens[s]) / kScaleBlock + 1;
+        const int64_t blocks_at = zeros_at + 8;
+        const int64_t ints = tokens > 0 ? blocks_at + 4 * blocks : 0;
         if (ints > INT32_MAX || parts > INT32_MAX / 64)
             return set_error(kErrInvalidArgument, "a plan of %lld words is too large",
                              (long long)ints);
-        for (int i = 0; i < kInfoCount; ++i) info[i] = 0;
+        for (int i = 0; i < (eight ? kInfoCount8 : kInfoCount); ++i) info[i] = 0;
         info[kInfoInts] = ints;
         info[kInfoTokens] = tokens;
         info[kInfoPagesAt] = pages_at;
@@ -507,6 +329,10 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
         info[kInfoZerosAt] = zeros_at;
         info[kInfoFewParts] = few_parts;
         info[kInfoFewRows] = few_rows;
+        if (eight) {
+            info[kInfoBlocksAt] = blocks_at;
+            info[kInfoBlocks] = blocks;
+        }
         if (plan == nullptr || tokens == 0) return kOk;
         if (plan_ints < ints)
             return set_error(kErrInvalidArgument, "the plan needs %lld words, got %lld",
@@ -529,7 +355,18 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
             }
         }
         for (int64_t i = pages_at + pages; i < items_at; ++i) plan[i] = 0;
-        for (int64_t i = zeros_at; i < ints; ++i) plan[i] = 0;
+        for (int64_t i = zeros_at; i < blocks_at; ++i) plan[i] = 0;
+        PagedBlock* block = reinterpret_cast<PagedBlock*>(plan + blocks_at);
+        for (int s = 0; s < n_seqs && eight; ++s) {
+            const int32_t from = context_lens[s] - new_lens[s], c = context_lens[s];
+            for (int32_t p = from; p < c; p = p / kScaleBlock * kScaleBlock + kScaleBlock) {
+                const int32_t first = p / kScaleBlock * kScaleBlock;
+                *block++ = PagedBlock{
+                    page_table[s * table_stride + (first >> shift)] * page_size +
+                        (first & (page_size - 1)),
+                    tok0[s] + (p - from), p - first, std::min(kScaleBlock, c - first) - (p - first)};
+            }
+        }
         PagedItem* item = reinterpret_cast<PagedItem*>(plan + items_at);
         PagedMerge* merge = reinterpret_cast<PagedMerge*>(plan + merges_at);
         int32_t next_few = 0, next_many = (int32_t)few_parts;
@@ -558,18 +395,20 @@ int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* cont
     }
 }
 
-int kivi_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+}  // namespace
+
+// Checks an append's arguments and fills the kernels'; n_tokens 0: there is nothing to do.
+int paged_append_args(AppendArgs& a, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                       const void* k, int64_t k_token_stride, int64_t k_head_stride,
                       const void* v, int64_t v_token_stride, int64_t v_head_stride,
                       int32_t dtype, void* q_out, void* k_pages, void* v_pages,
                       int64_t num_pages, int32_t page_size, int32_t q_heads, int32_t kv_heads,
                       int32_t head_dim, const int32_t* plan, int32_t tokens, const float* cos,
                       const float* sin, int32_t rotary_dim, int32_t interleaved,
-                      const void* q_norm, const void* k_norm, int32_t norm_dtype, float eps,
-                      void* stream) {
+                      const void* q_norm, const void* k_norm, int32_t norm_dtype, float eps) {
     const int32_t hq = q == nullptr ? 0 : q_heads;
-    int rc = check_pool(dtype, num_pages, page_size, q == nullptr ? kv_heads : q_heads, kv_heads,
-                        head_dim);
+    const int rc = paged_check_pool(dtype, num_pages, page_size,
+                                    q == nullptr ? kv_heads : q_heads, kv_heads, head_dim);
     if (rc) return rc;
     if (tokens < 0) return set_error(kErrInvalidArgument, "tokens %d must not be negative", tokens);
     if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 16 != 0)
@@ -581,6 +420,7 @@ int kivi_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stri
         return set_error(kErrInvalidArgument, "cos and sin must be 16-byte aligned");
     if (norm_dtype < 0 || norm_dtype > 2)
         return set_error(kErrInvalidArgument, "norm_dtype %d is not 0, 1 or 2", norm_dtype);
+    a = AppendArgs{};
     if (tokens == 0) return kOk;
     if (k == nullptr || v == nullptr || k_pages == nullptr || v_pages == nullptr ||
         plan == nullptr || (q != nullptr && q_out == nullptr))
@@ -589,7 +429,6 @@ int kivi_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stri
     if (((uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)(q != nullptr ? q_out : nullptr)) &
         align)
         return set_error(kErrInvalidArgument, "pages and q_out must be 16-byte aligned");
-    AppendArgs a{};
     a.q = q; a.k = k; a.v = v;
     a.q_st = q_token_stride; a.q_sh = q_head_stride;
     a.k_st = k_token_stride; a.k_sh = k_head_stride;
@@ -601,7 +440,7 @@ int kivi_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stri
     a.eps = eps;
     a.inv_d = 1.0f / (float)head_dim;
     a.n_tokens = tokens; a.Hq = hq; a.Hkv = kv_heads; a.D = head_dim;
-    a.page_shift = page_shift_of(page_size);
+    a.page_shift = paged_page_shift(page_size);
     a.rot = rotary_dim; a.interleaved = interleaved != 0;
     a.lanes_log2 = 0;
     while ((1 << a.lanes_log2) < head_dim / 16) ++a.lanes_log2;
@@ -614,7 +453,52 @@ int kivi_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stri
     }
     a.vec = (strides * src_size(dtype) & 15) == 0 && (bases & 15) == 0;
     a.norm_vec = (((uintptr_t)q_norm | (uintptr_t)k_norm) & 15) == 0;
-    const int64_t lanes = (int64_t)tokens * (hq + 2 * kv_heads) << a.lanes_log2;
+    return kOk;
+}
+
+}  // namespace kivi
+
+using namespace kivi;
+
+extern "C" {
+
+int kivi_paged_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* context_lens,
+                    const int32_t* page_table, int64_t table_stride, int32_t table_pages,
+                    int32_t page_size, int64_t num_pages, int32_t dtype, int32_t q_heads,
+                    int32_t kv_heads, int32_t head_dim, int32_t* plan, int64_t plan_ints,
+                    int64_t* info) {
+    return make_plan(false, n_seqs, new_lens, context_lens, page_table, table_stride, table_pages,
+                     page_size, num_pages, dtype, q_heads, kv_heads, head_dim, plan, plan_ints,
+                     info);
+}
+
+int kivi_paged8_plan(int32_t n_seqs, const int32_t* new_lens, const int32_t* context_lens,
+                     const int32_t* page_table, int64_t table_stride, int32_t table_pages,
+                     int32_t page_size, int64_t num_pages, int32_t dtype, int32_t q_heads,
+                     int32_t kv_heads, int32_t head_dim, int32_t* plan, int64_t plan_ints,
+                     int64_t* info) {
+    return make_plan(true, n_seqs, new_lens, context_lens, page_table, table_stride, table_pages,
+                     page_size, num_pages, dtype, q_heads, kv_heads, head_dim, plan, plan_ints,
+                     info);
+}
+
+int kivi_paged_append(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                      const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                      const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                      int32_t dtype, void* q_out, void* k_pages, void* v_pages,
+                      int64_t num_pages, int32_t page_size, int32_t q_heads, int32_t kv_heads,
+                      int32_t head_dim, const int32_t* plan, int32_t tokens, const float* cos,
+                      const float* sin, int32_t rotary_dim, int32_t interleaved,
+                      const void* q_norm, const void* k_norm, int32_t norm_dtype, float eps,
+                      void* stream) {
+    AppendArgs a;
+    const int rc = paged_append_args(a, q, q_token_stride, q_head_stride, k, k_token_stride,
+                                     k_head_stride, v, v_token_stride, v_head_stride, dtype, q_out,
+                                     k_pages, v_pages, num_pages, page_size, q_heads, kv_heads,
+                                     head_dim, plan, tokens, cos, sin, rotary_dim, interleaved,
+                                     q_norm, k_norm, norm_dtype, eps);
+    if (rc || a.n_tokens == 0) return rc;
+    const int64_t lanes = (int64_t)tokens * (a.Hq + 2 * kv_heads) << a.lanes_log2;
     if (lanes > INT32_MAX)
         return set_error(kErrInvalidArgument, "%d tokens are too many for one launch", tokens);
     hipStream_t s = (hipStream_t)stream;

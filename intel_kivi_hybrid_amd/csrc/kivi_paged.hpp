@@ -12,6 +12,8 @@
 //   items   [items][8]    PagedItem: one workgroup's work for one kv head
 //   merges  [merges][8]   PagedMerge: row tiles whose context is split
 //   zeros   [8]           what lanes behind the head's channels load
+//   blocks  [blocks][4]   PagedBlock, for pages of 8 bits: the blocks of positions
+//                         that get tokens
 #pragma once
 
 #include "kivi_common.hpp"
@@ -42,7 +44,19 @@ struct PagedMerge {
     int32_t pad[2];
 };
 
-static_assert(sizeof(PagedItem) == 32 && sizeof(PagedMerge) == 32, "plan records");
+// Positions that share a scale in pages of 8 bits: as many as the attention kernels load
+// at a time, never across a page.
+constexpr int kScaleBlock = 16;
+
+struct PagedBlock {
+    int32_t slot;        // of its first position
+    int32_t tok;         // its first new token among the step's
+    int32_t held;        // positions before that token
+    int32_t n;           // new tokens
+};
+
+static_assert(sizeof(PagedItem) == 32 && sizeof(PagedMerge) == 32 && sizeof(PagedBlock) == 16,
+              "plan records");
 
 // Kinds of attention items: kind k takes 16 << k rows (none 32), and is one launch
 // (kFew64: fp32, kMany: the 16-bit types).
@@ -93,6 +107,10 @@ enum PagedInfo : int {
     kInfoFewParts = 14,   // partials of sequences with few rows (the first ones),
     kInfoFewRows = 15,    // and rows of these
     kInfoCount = 16,
+    // and of kivi_paged8_plan
+    kInfoBlocksAt = 16,
+    kInfoBlocks = 17,
+    kInfoCount8 = 20,
 };
 
 struct PagedLaunch {

@@ -1,0 +1,334 @@
+// Attention over pages of 8 bits for more than 16 query rows per kv head: chunks of
+// prompts, verification passes.
+//
+// As kivi_paged_many.hip: a workgroup takes 128 rows of a kv head, 32 for each of its four
+// waves (v_mfma_f32_32x32x16), and walks the positions in tiles of 64 (32 above 128
+// channels) in two LDS buffers.  A tile's codes are loaded into registers while the one
+// before is computed, widened there once for all four waves and written to the other
+// buffer: one barrier per tile.
+//
+// fp16's weights stay fp16 (11 bits): value scales have no room in its range, so a row
+// keeps a second maximum, that of its weights times their blocks' scales, and its outputs
+// in units of that one.
+#include <hip/hip_runtime.h>
+
+#include "kivi_paged8_attention.hpp"
+#include "kivi_paged_tile.hpp"
+
+namespace kivi {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kBlock = kWaves * kWave;
+
+// How a workgroup's lanes load a tile: a lane takes 16 channels of a token.
+template <int DP, int TOKENS>
+struct Tile8Loads {
+    using M = TileShape<DP, TOKENS>;
+    static constexpr int CH = M::SL / 2;                    // lanes of a token
+    static constexpr int LD = TOKENS * CH / kBlock;         // loads of a lane for a tile's keys
+    static constexpr int NB = TOKENS / 16;
+    int wave;
+    int page[LD], block[NB];                                // of the loads, of the tile's blocks
+    u32x4_t k[LD], v[LD];
+    BlockScales<NB> scales;
+
+    // the first position of the block that load i lies in, and its token of the tile
+    __device__ __forceinline__ int block_of(int i) const {
+        return (i * kBlock + wave * kWave) / CH / 16 * 16;
+    }
+    __device__ __forceinline__ int token(int i) const {
+        return (i * kBlock + (int)threadIdx.x) / CH;
+    }
+    __device__ __forceinline__ int channel() const { return threadIdx.x % CH * 16; }
+
+    __device__ __forceinline__ void pages_of(const Paged8Launch& a, const Work& w, int t0) {
+#pragma unroll
+        for (int i = 0; i < LD; ++i) page[i] = block_page(a, w, t0 + block_of(i));
+#pragma unroll
+        for (int b = 0; b < NB; ++b) block[b] = block_page(a, w, t0 + 16 * b);
+    }
+    // Loads the tile at t0 (whose pages are known), then its successor's pages.
+    __device__ __forceinline__ void issue(const Paged8Launch& a, const Work& w, int t0) {
+        const int c = channel();
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const uint32_t off = token(i) % 16 * a.D + c;
+            const int t = t0 + block_of(i);
+            k[i] = u32x4_t{0, 0, 0, 0};
+            v[i] = u32x4_t{0, 0, 0, 0};
+            if (c >= a.D) continue;
+            k[i] = *reinterpret_cast<const u32x4_t*>(
+                block_at<uint8_t>(a, w, a.k_pages, page[i], t) + off);
+            v[i] = *reinterpret_cast<const u32x4_t*>(
+                block_at<uint8_t>(a, w, a.v_pages, page[i], t) + off);
+        }
+        scales.load(a, w, t0, block);
+        pages_of(a, w, t0 + TOKENS);
+    }
+    // Writes the loaded tile, widened, to LDS.
+    template <int KT, int VT>
+    __device__ __forceinline__ void store(unsigned char* buf) const {
+        const int c = channel();
+        if (c >= DP) return;                                // (96 channels: six lanes of eight)
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int t = token(i);
+            unsigned char* kr = buf + t * M::ROW;
+            unsigned char* vr = kr + M::BYTES;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int x = c / 8 + h;
+                *reinterpret_cast<u32x4_t*>(kr + ((x ^ M::key_swizzle(t)) << 4)) =
+                    operand_of_codes<KT>(k[i][2 * h], k[i][2 * h + 1]);
+                *reinterpret_cast<u32x4_t*>(vr + ((x ^ M::value_swizzle(t)) << 4)) =
+                    operand_of_codes<VT>(v[i][2 * h], v[i][2 * h + 1]);
+            }
+        }
+    }
+};
+
+// A wave's 32 query rows (lane: row lane % 32) and their softmax state.
+template <int DT, int DP, int TOKENS>
+struct Tile8Rows {
+    using M = TileShape<DP, TOKENS>;
+    static constexpr int KT = key_type<DT>(), NQ = query_pieces<DT>();
+    static constexpr int VT = DT == kSrcF16 ? kSrcF16 : kSrcBF16;
+    static constexpr int NB = TOKENS / 16;
+    u32x4_t qf[M::KS][NQ];
+    f32x16_t O[M::CB];
+    float m, l;
+    float top;               // fp16: the outputs' units, log2
+    int lim;                 // positions that the lane's row sees
+    int all, last;           // that all, and any, of the 32 rows see
+
+    __device__ __forceinline__ void init(const Paged8Launch& a, const Work& w, int row0) {
+        const int lane = threadIdx.x % kWave, half = lane / 32, r = row0 + lane % 32;
+        const bool live = r < w.rows;
+        lim = live ? row_limit(w, r) : 0;
+        m = top = -FLT_MAX;
+        l = 0.f;
+        const int64_t q = live ? q_offset(a, w, r) : 0;
+#pragma unroll
+        for (int ks = 0; ks < M::KS; ++ks) {
+            const int c = 16 * ks + 8 * half;
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) qf[ks][n] = u32x4_t{0, 0, 0, 0};
+            if (live && c < a.D) load_query<DT>(a.q, q + c, qf[ks]);
+        }
+#pragma unroll
+        for (int cb = 0; cb < M::CB; ++cb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) O[cb][i] = 0.f;
+        }
+        const int base = w.it.ctx - w.it.n + 1;
+        all = base + row0 / w.hg;
+        last = row0 < w.rows ? min(base + min(row0 + 31, w.rows - 1) / w.hg, w.it.kv_end) : 0;
+    }
+
+    // A tile of keys and values in LDS, positions t0 ..
+    __device__ __forceinline__ void tile(const unsigned char* buf, const BlockScales<NB>& sc,
+                                         int t0, int end, float qscale) {
+        const int lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
+        f32x16_t s[M::TB];
+#pragma unroll
+        for (int tb = 0; tb < M::TB; ++tb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[tb][i] = 0.f;
+        }
+        const uint32_t krow = col * M::ROW + ((half ^ M::key_swizzle(col)) << 4);
+#pragma unroll
+        for (int ks = 0; ks < M::KS; ++ks) {
+#pragma unroll
+            for (int tb = 0; tb < M::TB; ++tb) {
+                const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(
+                    buf + ((krow ^ (32 * ks)) + 32 * tb * M::ROW));
+#pragma unroll
+                for (int n = NQ - 1; n >= 0; --n) s[tb] = mfma32<KT>(kf, qf[ks][n], s[tb]);
+            }
+        }
+        // score i of 32 tokens tb: token 32 tb + 8 (i / 4) + 4 half + i % 4, of block
+        // 2 tb + i / 8
+        float units[NB], vs[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            units[b] = score_units(sc.k[b], qscale);
+            vs[b] = sc.v[b];
+        }
+        if (t0 + M::TILE > min(all, end)) {
+#pragma unroll
+            for (int tb = 0; tb < M::TB; ++tb) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (t0 + 32 * tb + 8 * (i / 4) + 4 * half + i % 4 >= lim)
+                        s[tb][i] = -INFINITY;
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                if (t0 + 16 * b >= lim) {
+                    vs[b] = 0.f;
+                    units[b] = FLT_MIN;
+                }
+        }
+        float mx = -INFINITY, mv = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float x = s[b / 2][b % 2 * 8];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) x = fmaxf(x, s[b / 2][b % 2 * 8 + i]);
+            x *= units[b];
+            mx = fmaxf(mx, x);
+            // (an exponent above the scale's)
+            if constexpr (VT == kSrcF16)
+                mv = fmaxf(mv, x + (float)((int)(__float_as_uint(sc.v[b]) >> 23 & 0xff) - 126));
+        }
+        if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax) != 0) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float to = fmaxf(m, mx), f = exp2_fast(m - to);
+            m = to;
+            l *= f;
+            if constexpr (VT != kSrcF16) {
+#pragma unroll
+                for (int cb = 0; cb < M::CB; ++cb) O[cb] *= f;
+            }
+        }
+        if constexpr (VT == kSrcF16) {
+            mv -= weight_bits<VT>();
+            if (__builtin_amdgcn_ballot_w64(mv > top + kMoveMax) != 0) {
+                mv = fmaxf(mv, __shfl_xor(mv, 32));
+                const float to = fmaxf(top, mv), f = exp2_fast(top - to);
+                top = to;
+#pragma unroll
+                for (int cb = 0; cb < M::CB; ++cb) O[cb] *= f;
+            }
+            const float f = exp2_fast(m - top);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) vs[b] *= f;
+        }
+        // transposed: lanes of 16 take tokens 4 half .. + 3 of 16 channels
+        const int t = 4 * half + lane % 16 / 4;
+        const int c = lane / 16 % 2 * 2 + lane % 4 / 2;
+        const uint32_t vrow = M::BYTES + t * M::ROW + ((c ^ M::value_swizzle(t)) << 4) + lane % 2 * 8;
+        constexpr int NP = DT == kSrcF32 ? 3 : 1;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            u32x4_t pf[NP];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = s[b / 2][b % 2 * 8 + 2 * i], y = s[b / 2][b % 2 * 8 + 2 * i + 1];
+                const float p0 = exp2_fast(fmaf(x, units[b], -m));
+                const float p1 = exp2_fast(fmaf(y, units[b], -m));
+                l += p0 + p1;
+                if constexpr (NP == 3) {
+                    uint32_t hi, mid, lo;
+                    split3_pair(p0 * vs[b], p1 * vs[b], hi, mid, lo, split_consts());
+                    pf[0][i] = hi;
+                    pf[1][i] = mid;
+                    pf[2][i] = lo;
+                } else {
+                    pf[0][i] = pack2<VT>(p0 * vs[b], p1 * vs[b]);
+                }
+            }
+#pragma unroll
+            for (int cb = 0; cb < M::CB; ++cb) {
+                const uint32_t at = (vrow ^ (64 * cb)) + 16 * b * M::ROW;
+                const uint2 lo = read_transposed(buf + at);
+                const uint2 hi = read_transposed(buf + (at + 8 * M::ROW));
+                const u32x4_t vt = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+                for (int n = NP - 1; n >= 0; --n) O[cb] = mfma32<VT>(vt, pf[n], O[cb]);
+            }
+        }
+    }
+};
+
+template <int DT, int DP>
+__global__ void __launch_bounds__(kBlock, DP <= 128 && DT != kSrcF32 ? 2 : 1)
+    paged8_many_kernel(Paged8Launch a) {
+    constexpr int kTile = DP <= 128 ? 64 : 32;
+    using M = TileShape<DP, kTile>;
+    constexpr int kFewBytes = 2 * Few8<DP>::WAVE_BYTES;
+    constexpr int kBytes = 2 * M::BYTES > kFewBytes ? 2 * M::BYTES : kFewBytes;
+    __shared__ __align__(16) unsigned char buf0[kBytes];
+    __shared__ __align__(16) unsigned char buf1[kBytes];
+    __shared__ Few8Join join;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
+    const Work w = work_of(a);
+    if (w.rows <= paged_tile_rows(kFew16)) {
+        few8_rows<DT, DP>(a, w, [&](int i) {
+            return (i < 2 ? buf0 : buf1) + i % 2 * Few8<DP>::WAVE_BYTES;
+        }, join);
+        return;
+    }
+    const int end = w.it.kv_end;
+    using R = Tile8Rows<DT, DP, kTile>;
+    R rows;
+    rows.init(a, w, w.it.row0 + 32 * wave);
+    Tile8Loads<DP, kTile> loads;
+    loads.wave = wave;
+
+    int t0 = w.it.kv_begin;
+    loads.pages_of(a, w, t0);
+    loads.issue(a, w, t0);
+    loads.template store<R::KT, R::VT>(buf0);
+    auto step = [&](unsigned char* now, unsigned char* next) {
+        const BlockScales<R::NB> scales = loads.scales;
+        // (behind it this tile is whole, and the other buffer read by all)
+        __syncthreads();
+        const bool more = t0 + kTile < end;
+        if (more) loads.issue(a, w, t0 + kTile);
+        if (t0 < rows.last) rows.tile(now, scales, t0, end, a.qscale);
+        if (more) loads.template store<R::KT, R::VT>(next);
+        t0 += kTile;
+    };
+    while (true) {
+        step(buf0, buf1);
+        if (t0 >= end) break;
+        step(buf1, buf0);
+        if (t0 >= end) break;
+    }
+
+    float l = rows.l;
+    l += __shfl_xor(l, 32);
+    const int r = w.it.row0 + 32 * wave + col;
+    if (r >= w.rows) return;
+    const bool whole = w.it.part < 0;
+    float f = whole ? inverse_sum(l) : 1.0f;
+    if constexpr (R::VT == kSrcF16) f *= exp2_fast(rows.top - rows.m);
+    const int64_t at = whole ? out_offset(a, w, r) : part_row(a, w, r);
+#pragma unroll
+    for (int cb = 0; cb < M::CB; ++cb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = 32 * cb + 8 * i + 4 * half;
+            if (c >= a.D) continue;
+            const f32x16_t& O = rows.O[cb];
+            f32x4_t o = {O[4 * i], O[4 * i + 1], O[4 * i + 2], O[4 * i + 3]};
+            o *= f;
+            if (whole) store4<DT>(a.out, at + c, o);
+            else *reinterpret_cast<f32x4_t*>(a.part_o + at * a.D + c) = o;
+        }
+    }
+    if (!whole && half == 0)
+        *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(rows.m, l);
+}
+
+template <int DT>
+void launch_dim(const Paged8Launch& a, hipStream_t s) {
+    const dim3 grid((unsigned)(a.n_items * a.Hkv));
+    if (a.D <= 64) paged8_many_kernel<DT, 64><<<grid, kBlock, 0, s>>>(a);
+    else if (a.D <= 96) paged8_many_kernel<DT, 96><<<grid, kBlock, 0, s>>>(a);
+    else if (a.D <= 128) paged8_many_kernel<DT, 128><<<grid, kBlock, 0, s>>>(a);
+    else paged8_many_kernel<DT, 256><<<grid, kBlock, 0, s>>>(a);
+}
+
+}  // namespace
+
+void launch_paged8_many(const Paged8Launch& a, int dtype, hipStream_t s) {
+    if (dtype == kSrcF32) launch_dim<kSrcF32>(a, s);
+    else if (dtype == kSrcBF16) launch_dim<kSrcBF16>(a, s);
+    else launch_dim<kSrcF16>(a, s);
+}
+
+}  // namespace kivi

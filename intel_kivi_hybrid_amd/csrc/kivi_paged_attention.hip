@@ -12,7 +12,7 @@
 
 #include <math.h>
 
-#include "kivi_paged_attention.hpp"
+#include "kivi_paged8_attention.hpp"
 #include "../../include/kivi_hip.h"
 
 namespace kivi {
@@ -78,25 +78,13 @@ int64_t part_floats(const int64_t* info, int32_t kv_heads, int32_t head_dim) {
     return part_rows_of(info) * kv_heads * (head_dim + 2);
 }
 
-}  // namespace
-}  // namespace kivi
-
-using namespace kivi;
-
-extern "C" {
-
-size_t kivi_paged_attention_workspace_size(const int64_t* info, int32_t kv_heads,
-                                           int32_t head_dim) {
-    if (info == nullptr || kv_heads < 1 || head_dim < 1) return 0;
-    return (size_t)part_floats(info, kv_heads, head_dim) * 4;
-}
-
-int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
-                         int32_t dtype, const void* k_pages, const void* v_pages,
-                         int64_t num_pages, int32_t page_size, int32_t q_heads,
-                         int32_t kv_heads, int32_t head_dim, const int32_t* plan,
-                         const int64_t* info, float softmax_scale, void* out, void* workspace,
-                         size_t workspace_bytes, void* stream) {
+// Checks a call's arguments and fills what its launches share; Hq 0: there is nothing to
+// do.
+int launch_args(PagedLaunch& a, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                int32_t dtype, const void* k_pages, const void* v_pages, int64_t num_pages,
+                int32_t page_size, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                const int32_t* plan, const int64_t* info, float softmax_scale, void* out,
+                void* workspace, size_t workspace_bytes) {
     if (info == nullptr) return set_error(kErrInvalidArgument, "null plan info");
     if (dtype < 0 || dtype > 2)
         return set_error(kErrInvalidArgument, "dtype %d is not 0 (f32), 1 (bf16) or 2 (f16)", dtype);
@@ -114,6 +102,7 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
         return set_error(kErrInvalidArgument,
                          "softmax_scale must be positive and below 2^127, got %g",
                          (double)softmax_scale);
+    a.Hq = 0;
     if (info[kInfoTokens] == 0) return kOk;
     if (q == nullptr || k_pages == nullptr || v_pages == nullptr || plan == nullptr ||
         out == nullptr)
@@ -128,7 +117,6 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     if (floats > 0 && (workspace == nullptr || workspace_bytes < (size_t)floats * 4))
         return set_error(kErrInvalidArgument, "workspace must hold %lld bytes, got %zu",
                          (long long)floats * 4, workspace_bytes);
-    PagedLaunch a{};
     a.q = q;
     a.q_st = q_token_stride;
     a.q_sh = q_head_stride;
@@ -151,7 +139,12 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     a.D = head_dim;
     a.page_shift = shift;
     a.qscale = qscale;
-    hipStream_t s = (hipStream_t)stream;
+    return kOk;
+}
+
+// The launches of a plan: launch(kind) makes that of a kind's items.
+template <class L, class F>
+int run_items(L& a, int dtype, const int32_t* plan, const int64_t* info, hipStream_t s, F launch) {
     const PagedItem* items = reinterpret_cast<const PagedItem*>(plan + info[kInfoItemsAt]);
     // (the largest tiles first: the small ones fill in behind them)
     for (int kind = kPagedKinds - 1; kind >= 0; --kind) {
@@ -160,18 +153,16 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
         a.items = items + before;
         a.n_items = (int)info[kInfoItems + kind];
         if (a.n_items == 0) continue;
-        if ((int64_t)a.n_items * kv_heads > kMostBlocks)
+        if ((int64_t)a.n_items * a.Hkv > kMostBlocks)
             return set_error(kErrInvalidArgument, "%d items are too many for one launch",
                              a.n_items);
-        if (kind == kMany) launch_paged_many(a, dtype, s);
-        else if (dtype == kSrcF32) launch_paged_f32(a, kind, s);
-        else launch_paged_few(a, dtype, s);
+        launch(kind);
         const int rc = check_launch("paged_attention");
         if (rc) return rc;
     }
     if (a.n_merges == 0) return kOk;
-    const int64_t blocks = (int64_t)a.n_merges * kv_heads *
-                           ((a.part_rows * (head_dim / 4) + kMergeBlock - 1) / kMergeBlock);
+    const int64_t blocks = (int64_t)a.n_merges * a.Hkv *
+                           ((a.part_rows * (a.D / 4) + kMergeBlock - 1) / kMergeBlock);
     if (blocks > kMostBlocks)
         return set_error(kErrInvalidArgument, "%d tiles to merge are too many for one launch",
                          a.n_merges);
@@ -180,6 +171,62 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
     else if (dtype == kSrcBF16) paged_merge_kernel<kSrcBF16><<<grid, kMergeBlock, 0, s>>>(a);
     else paged_merge_kernel<kSrcF16><<<grid, kMergeBlock, 0, s>>>(a);
     return check_launch("paged_merge");
+}
+
+}  // namespace
+}  // namespace kivi
+
+using namespace kivi;
+
+extern "C" {
+
+size_t kivi_paged_attention_workspace_size(const int64_t* info, int32_t kv_heads,
+                                           int32_t head_dim) {
+    if (info == nullptr || kv_heads < 1 || head_dim < 1) return 0;
+    return (size_t)part_floats(info, kv_heads, head_dim) * 4;
+}
+
+int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                         int32_t dtype, const void* k_pages, const void* v_pages,
+                         int64_t num_pages, int32_t page_size, int32_t q_heads,
+                         int32_t kv_heads, int32_t head_dim, const int32_t* plan,
+                         const int64_t* info, float softmax_scale, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+    PagedLaunch a{};
+    const int rc = launch_args(a, q, q_token_stride, q_head_stride, dtype, k_pages, v_pages,
+                               num_pages, page_size, q_heads, kv_heads, head_dim, plan, info, softmax_scale,
+                               out, workspace, workspace_bytes);
+    if (rc || a.Hq == 0) return rc;
+    hipStream_t s = (hipStream_t)stream;
+    return run_items(a, dtype, plan, info, s, [&](int kind) {
+        if (kind == kMany) launch_paged_many(a, dtype, s);
+        else if (dtype == kSrcF32) launch_paged_f32(a, kind, s);
+        else launch_paged_few(a, dtype, s);
+    });
+}
+
+int kivi_paged8_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                          int32_t dtype, const int8_t* k_pages, const int8_t* v_pages,
+                          const float* k_scales, const float* v_scales, int64_t num_pages,
+                          int32_t page_size, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                          const int32_t* plan, const int64_t* info, float softmax_scale, void* out,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+    Paged8Launch a{};
+    const int rc = launch_args(a, q, q_token_stride, q_head_stride, dtype, k_pages, v_pages,
+                               num_pages, page_size, q_heads, kv_heads, head_dim, plan, info, softmax_scale,
+                               out, workspace, workspace_bytes);
+    if (rc || a.Hq == 0) return rc;
+    if (k_scales == nullptr || v_scales == nullptr)
+        return set_error(kErrInvalidArgument, "null scales");
+    if (info[kInfoItems + kFew64] != 0)
+        return set_error(kErrInvalidArgument, "the plan is not one of kivi_paged8_plan");
+    a.k_scales = k_scales;
+    a.v_scales = v_scales;
+    hipStream_t s = (hipStream_t)stream;
+    return run_items(a, dtype, plan, info, s, [&](int kind) {
+        if (kind == kMany) launch_paged8_many(a, dtype, s);
+        else launch_paged8_few(a, dtype, s);
+    });
 }
 
 }  // extern "C"

@@ -268,8 +268,9 @@ __device__ __forceinline__ void mend_row(const PagedLaunch& a, const Work& w, in
 
 // Joins WAVES waves' results of ROWS rows (row i of wave j at jo(j) + i * stride,
 // each scaled to the largest of the waves' maxima) and finishes the rows from
-// row0.  By all 256 threads of a workgroup.
-template <int DT, int DP, int ROWS, int WAVES, class F>
+// row0.  By all 256 threads of a workgroup.  ODD: values may not be finite (codes always
+// are).
+template <int DT, int DP, int ROWS, int WAVES, bool ODD = true, class F>
 __device__ __forceinline__ void join_waves(const PagedLaunch& a, const Work& w, int row0, F jo,
                                            int stride, const float (*m)[ROWS],
                                            const float (*l)[ROWS], bool odd, int unit) {
@@ -287,8 +288,9 @@ __device__ __forceinline__ void join_waves(const PagedLaunch& a, const Work& w, 
             sum += l[i][row] * exp2_fast(m[i][row] - top);
         }
         if (w.it.part < 0) o *= inverse_sum(sum);
-        add_odd<DT>(a, w, w.it.ctx - w.it.n + w.it.row0 / w.hg + 1, unit, row_limit(w, r), c, sum,
-                    odd, o);
+        if constexpr (ODD)
+            add_odd<DT>(a, w, w.it.ctx - w.it.n + w.it.row0 / w.hg + 1, unit, row_limit(w, r), c,
+                        sum, odd, o);
         store_row<DT>(a, w, r, c, o, top, sum);
     }
 }
