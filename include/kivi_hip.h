@@ -516,6 +516,34 @@ int kivi_paged8_attention(const void* q, int64_t q_token_stride, int64_t q_head_
                           const int32_t* plan, const int64_t* info, float softmax_scale, void* out,
                           void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- logits before sampling --------------------------------------------------
+ * out[rows][vocab] from logits [rows][vocab] (dtype 0 f32, 1 bf16, 2 f16; out_dtype the
+ * same or 0; rows row_stride and out_stride elements apart; out may be logits).  For
+ * token v of a row, in f32 with one rounding at the end, in this order:
+ * - tokens [rows][n_tokens] (i32, or i64 with tokens_i64; rows token_stride apart): the
+ *   first lengths[row] (or length) of a row are its tokens so far, the first
+ *   prompt_lengths[row] (or prompt_length) of these its prompt.  Where v is one of them
+ *   x becomes x / repetition above 0 and x * repetition otherwise; where it is n > 0
+ *   times among those behind the prompt, x - (frequency * n + presence).  Ids outside
+ *   the vocabulary are passed over.  Settings are the scalars, or one value per row
+ *   (device arrays) where a pointer is given; a repetition that is not above 0 is 1.
+ * - bias_ids, bias [rows][biases] (rows id_stride and bias_stride apart): + the sum,
+ *   in the list's order, of the biases that are listed for v.
+ * - allowed (NULL: all): bit v % 32 of word v / 32 of a row's words, allowed_stride
+ *   apart, is 0: -infinity.
+ * A logit that none of this concerns keeps its bits.  n_tokens and biases are 2^30 at
+ * most. */
+int kivi_adjust_logits(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows,
+                       int32_t vocab, const void* tokens, int32_t tokens_i64,
+                       int64_t token_stride, int32_t n_tokens, const int32_t* lengths,
+                       int32_t length, const int32_t* prompt_lengths, int32_t prompt_length,
+                       const float* repetitions, float repetition, const float* presences,
+                       float presence, const float* frequencies, float frequency,
+                       const void* bias_ids, int32_t ids_i64, int64_t id_stride,
+                       const float* bias, int64_t bias_stride, int32_t biases,
+                       const uint32_t* allowed, int64_t allowed_stride, void* out,
+                       int32_t out_dtype, int64_t out_stride, void* stream);
+
 /* ---- sampling ---------------------------------------------------------------
  * Next tokens out[rows] from logits [rows][vocab] (dtype 0 f32, 1 bf16, 2 f16;
  * rows row_stride elements apart; vocab at most 2^20) and uniforms[rows] in [0, 1)

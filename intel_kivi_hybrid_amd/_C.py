@@ -1098,6 +1098,107 @@ def _setting(value, name: str, rows: int, dtype, dev):
     return 0, value
 
 
+def allowed_tokens(mask):
+    """The words that :func:`adjust_logits` takes from a mask ``[rows, vocab]`` (nonzero
+    or True: the token is allowed): ``[rows, ceil(vocab / 32)]`` int32, bit ``v % 32``
+    of word ``v // 32`` for token v."""
+    return ~hidden_positions(mask)
+
+
+def _row_list(t, name: str, rows: int, dtypes, dev):
+    """A list for each row, ``[rows, n]``, or one for all, ``[n]``: rows any distance
+    apart.  Its stride."""
+    _check(isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() in (1, 2)
+           and (t.dim() == 1 or t.shape[0] == rows) and t.device == dev
+           and (t.shape[-1] <= 1 or t.stride(-1) == 1), name, " must be a [", rows,
+           ", n] or [n] tensor of ", " or ".join(_dtype_name(d) for d in dtypes),
+           " with contiguous rows on ", dev)
+    return 0 if t.dim() == 1 else t.stride(0)
+
+
+_ID_DTYPES = (torch.int32, torch.int64)
+
+
+def adjust_logits(logits, tokens=None, lengths=None, prompt_lengths=0, repetition_penalty=1.0,
+                  presence_penalty=0.0, frequency_penalty=0.0, bias_ids=None, bias=None,
+                  allowed=None, out=None):
+    """``logits [rows, vocab]`` (fp32, bf16 or fp16) changed before :func:`sample`:
+    penalties for repeated tokens, then biases, then a mask, each where it is given, in
+    fp32 with one rounding at the end; launched on the current stream.
+
+    ``tokens [rows, n]`` (int32 or int64): each row's tokens so far, of which the first
+    ``lengths`` count (None: all), and of these the first ``prompt_lengths`` are its
+    prompt; ids outside the vocabulary are passed over.  A logit x of a token among them
+    becomes x / repetition_penalty above 0 and x * repetition_penalty otherwise; of one
+    that is k > 0 times behind the prompt, x - (frequency_penalty * k +
+    presence_penalty).  ``bias_ids`` (int32 or int64) and ``bias`` (fp32), ``[rows, n]``
+    or ``[n]`` for all rows: x plus the sum, in the list's order, of the biases that are
+    listed for the token.  ``allowed`` (int32, ``[rows, words]`` or ``[words]``,
+    :func:`allowed_tokens`): logits of tokens whose bit is 0 become -infinity.
+
+    Penalties and lengths are numbers or tensors with one value per row (float32;
+    lengths int32).  ``out``: where the result goes, ``logits`` itself, or another tensor
+    of its type or fp32 (None: a new one of its type).  A logit that nothing concerns
+    keeps its bits."""
+    if not (isinstance(logits, torch.Tensor) and logits.dim() == 2
+            and logits.dtype in _IO_DTYPES and logits.is_cuda):
+        _fail("logits must be a [rows, vocab] tensor of a float type on ", _DEVICE_TYPE)
+    rows, vocab = logits.shape
+    _check(vocab > 0, "a row must have logits")
+    _check(logits.stride(1) == 1 or vocab == 1, "a row's logits must be contiguous")
+    dev = logits.device
+    tok = (0, 0, 0, 0)
+    if tokens is not None:
+        _check(tokens.dim() == 2, "tokens must be a [", rows, ", n] tensor")
+        st = _row_list(tokens, "tokens", rows, _ID_DTYPES, dev)
+        tok = (tokens.data_ptr(), int(tokens.dtype is torch.int64), st, tokens.shape[1])
+    lp, length = _setting(tok[3] if lengths is None else lengths, "lengths", rows, torch.int32, dev)
+    pp, prompt = _setting(prompt_lengths, "prompt_lengths", rows, torch.int32, dev)
+    length, prompt = _check_int(length, "lengths"), _check_int(prompt, "prompt_lengths")
+    _check(0 <= length <= tok[3], "lengths must lie in [0, ", tok[3], "], got ", length)
+    _check(prompt >= 0, "prompt_lengths must not be negative, got ", prompt)
+    rp, r = _setting(repetition_penalty, "repetition_penalty", rows, torch.float32, dev)
+    sp, s = _setting(presence_penalty, "presence_penalty", rows, torch.float32, dev)
+    fp, f = _setting(frequency_penalty, "frequency_penalty", rows, torch.float32, dev)
+    _check(rp or r > 0.0, "repetition_penalty must be positive, got ", r)
+    _check(tokens is not None or not (rp or sp or fp or r != 1.0 or s != 0.0 or f != 0.0),
+           "penalties need tokens")
+    ids = (0, 0, 0, 0, 0, 0)
+    if bias_ids is not None or bias is not None:
+        _check(bias_ids is not None and bias is not None, "biases need bias_ids and bias")
+        ist = _row_list(bias_ids, "bias_ids", rows, _ID_DTYPES, dev)
+        bst = _row_list(bias, "bias", rows, (torch.float32,), dev)
+        _check(bias_ids.shape[-1] == bias.shape[-1], "bias_ids name ", bias_ids.shape[-1],
+               " tokens, bias has ", bias.shape[-1], " values")
+        ids = (bias_ids.data_ptr(), int(bias_ids.dtype is torch.int64), ist, bias.data_ptr(), bst,
+               bias.shape[-1])
+    words = (0, 0)
+    if allowed is not None:
+        st = _row_list(allowed, "allowed", rows, (torch.int32,), dev)
+        _check(allowed.shape[-1] * 32 >= vocab, "allowed has ", allowed.shape[-1],
+               " words for ", vocab, " tokens")
+        words = (allowed.data_ptr(), st)
+    _check_inference(logits, bias, out, *(x for x in (repetition_penalty, presence_penalty,
+                                                      frequency_penalty)
+                                          if isinstance(x, torch.Tensor)))
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+    else:
+        _check(out.dtype in (logits.dtype, torch.float32) and out.shape == logits.shape
+               and (out.stride(1) == 1 or vocab == 1) and out.device == dev, "out must be a [",
+               rows, ", ", vocab, "] tensor of ", _dtype_name(logits.dtype),
+               " or Float with contiguous rows on ", dev)
+    index = dev.index
+    with on_device(index):
+        rc = _lib.kivi_adjust_logits(
+            logits.data_ptr(), _IO_DTYPES[logits.dtype], logits.stride(0), rows, vocab, *tok, lp,
+            length, pp, prompt, rp, r, sp, s, fp, f, *ids, *words, out.data_ptr(),
+            _IO_DTYPES[out.dtype], out.stride(0), stream_handle(index))
+    if rc:
+        _native.check(rc, "adjust_logits")
+    return out
+
+
 def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     """Next tokens ``[rows]`` (int64) from ``logits [rows, vocab]`` (fp32, bf16 or
     fp16) and ``uniforms [rows]`` in [0, 1) (fp32 or fp64), launched on the current

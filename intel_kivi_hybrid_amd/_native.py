@@ -96,6 +96,9 @@ SIGNATURES = {
                            _vp, _vp, _i32, _f32, _vp],
     "kivi_paged8_attention": [_vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32,
                               _i32, _vp, _vp, _f32, _vp, _vp, ctypes.c_size_t, _vp],
+    "kivi_adjust_logits": [_vp, _i32, _i64, _i32, _i32, _vp, _i32, _i64, _i32, _vp, _i32, _vp, _i32,
+                           _vp, _f32, _vp, _f32, _vp, _f32, _vp, _i32, _i64, _vp, _i64, _i32, _vp,
+                           _i64, _vp, _i32, _i64, _vp],
     "kivi_sample": [_vp, _i32, _i64, _i32, _i32, _vp, _i32, _vp, ctypes.c_double, _vp, _i32, _vp,
                     ctypes.c_double, _vp, ctypes.c_double, _vp, _vp, ctypes.c_size_t, _vp],
     "kivi_sample_workspace_size": [_i32, _i32],

@@ -1,0 +1,323 @@
+// Logits changed before sampling: penalties for repeated tokens, biases, masks.
+//
+// For token v of a row with logit x, n times among the row's generated tokens:
+//   x > 0 ? x / r : x * r      where v is among its tokens, prompt or generated
+//   x - (f n + p)              where n > 0
+//   x + b                      b: the biases that the row lists for v, added up in order
+//   -infinity                  where the row's mask does not allow v
+// in fp32, rounded once; a logit that none of this concerns keeps its bits.
+//
+// One launch: a workgroup takes a slice of a row's vocabulary.  It counts the row's tokens
+// that lie in the slice in LDS (whole numbers: in any order the same), adds up the
+// slice's biases there, and goes through its logits once.  Every slice reads all of its
+// row's tokens, from L2.
+#include <hip/hip_runtime.h>
+
+#include "kivi_common.hpp"
+#include "../../include/kivi_hip.h"
+
+namespace kivi {
+namespace {
+
+constexpr int kBlock = 256;
+constexpr uint32_t kInPrompt = 1u << 31;     // of a count
+constexpr uint32_t kNoBias = 0xffffffffu;    // (of no sum: NaN is stored as 0x7fc00000)
+constexpr uint32_t kNobody = 0xffffffffu;
+constexpr int kMostEntries = 1 << 30;        // (32-bit indexes look a turn past the last one)
+
+struct AdjustArgs {
+    const void* logits;
+    void* out;
+    int64_t stride, out_stride;
+    const void* tokens;                      // NULL: no penalties
+    int64_t token_stride;
+    const int32_t* lengths;
+    const int32_t* prompts;
+    const float* repetitions;
+    const float* presences;
+    const float* frequencies;
+    const void* bias_ids;
+    const float* bias;
+    int64_t id_stride, bias_stride;
+    const uint8_t* allowed;                  // bytes of the words
+    int64_t allowed_stride;                  // in bytes
+    float repetition, presence, frequency;
+    int length, prompt, n_tokens, biases;
+    int vocab, slice, slices, token64, id64;
+};
+
+// Eight elements wherever they lie.
+typedef uint32_t loose_u4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+template <int DT>
+struct Eight {
+    static constexpr int kWords = DT == kSrcF32 ? 8 : 4;
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        const char* from = static_cast<const char*>(p) + i * src_size(DT);
+#pragma unroll
+        for (int j = 0; j < kWords; j += 4) {
+            const u4 x = *reinterpret_cast<const loose_u4*>(from + 4 * j);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[j + k] = x[k];
+        }
+    }
+    __device__ __forceinline__ void store(void* p, int64_t i) const {
+        char* to = static_cast<char*>(p) + i * src_size(DT);
+#pragma unroll
+        for (int j = 0; j < kWords; j += 4)
+            *reinterpret_cast<loose_u4*>(to + 4 * j) = u4{w[j], w[j + 1], w[j + 2], w[j + 3]};
+    }
+    __device__ __forceinline__ void load_some(const void* p, int64_t i, int n) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (DT == kSrcF32) {
+                w[j] = j < n ? static_cast<const uint32_t*>(p)[i + j] : 0u;
+            } else {
+                const uint32_t h = j < n ? static_cast<const uint16_t*>(p)[i + j] : 0u;
+                if (j % 2 == 0) w[j / 2] = h;
+                else w[j / 2] |= h << 16;
+            }
+        }
+    }
+    __device__ __forceinline__ void store_some(void* p, int64_t i, int n) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (j >= n) continue;
+            if (DT == kSrcF32) static_cast<uint32_t*>(p)[i + j] = w[j];
+            else static_cast<uint16_t*>(p)[i + j] = (uint16_t)(w[j / 2] >> (16 * (j % 2)));
+        }
+    }
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (DT == kSrcF32) return __uint_as_float(w[j]);
+        const uint32_t h = w[j / 2] >> (16 * (j % 2)) & 0xffffu;
+        if constexpr (DT == kSrcBF16) return __uint_as_float(h << 16);
+        else return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+    }
+    __device__ __forceinline__ void set(int j, float x) {
+        if constexpr (DT == kSrcF32) {
+            w[j] = __float_as_uint(x);
+        } else {
+            uint32_t h;
+            if constexpr (DT == kSrcBF16) h = __builtin_bit_cast(uint16_t, (__bf16)x);
+            else h = __builtin_bit_cast(uint16_t, (_Float16)x);
+            w[j / 2] = j % 2 ? (w[j / 2] & 0xffffu) | h << 16 : (w[j / 2] & 0xffff0000u) | h;
+        }
+    }
+};
+
+__device__ __forceinline__ float setting(const float* rows, float all, int row) {
+    return rows == nullptr ? all : rows[row];
+}
+__device__ __forceinline__ int64_t id_at(const void* ids, int64_t i, int wide) {
+    return wide ? static_cast<const int64_t*>(ids)[i] : static_cast<const int32_t*>(ids)[i];
+}
+
+// Counts tokens from .. to - 1 of the row that lie in the slice.
+__device__ __forceinline__ void count_tokens(const AdjustArgs& a, int64_t row, int from, int to,
+                                             uint32_t first, uint32_t n, bool prompt,
+                                             uint32_t* counts) {
+    constexpr int kAtOnce = 4;
+    const int64_t base = row * a.token_stride;
+    for (int i = from + threadIdx.x; i < to; i += kAtOnce * kBlock) {
+        int64_t id[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j)
+            id[j] = id_at(a.tokens, base + min(i + j * kBlock, to - 1), a.token64);
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            const uint64_t at = (uint64_t)(id[j] - (int64_t)first);
+            if (at >= n || i + j * kBlock >= to) continue;
+            if (prompt) atomicOr(counts + at, kInPrompt);
+            else atomicAdd(counts + at, 1u);
+        }
+    }
+}
+
+// The slice's biases, each token's added up in the list's order: of the entries of a turn
+// that name one token the first goes, then the next.  owner: kNobody throughout.
+__device__ __forceinline__ void add_biases(const AdjustArgs& a, int64_t row, uint32_t first,
+                                           uint32_t n, uint32_t* owner, uint32_t* sums) {
+    for (int base = 0; base < a.biases; base += kBlock) {
+        const int i = base + threadIdx.x;
+        bool waits = false;
+        uint32_t at = 0;
+        float b = 0.f;
+        if (i < a.biases) {
+            const uint64_t x =
+                (uint64_t)(id_at(a.bias_ids, row * a.id_stride + i, a.id64) - (int64_t)first);
+            waits = x < n;
+            at = (uint32_t)x;
+            if (waits) b = a.bias[row * a.bias_stride + i];
+        }
+        while (__syncthreads_or(waits)) {
+            if (waits) atomicMin(owner + at, threadIdx.x);
+            __syncthreads();
+            const bool goes = waits && owner[at] == threadIdx.x;
+            __syncthreads();
+            if (goes) {
+                const float s = sums[at] == kNoBias ? b : __uint_as_float(sums[at]) + b;
+                sums[at] = s == s ? __float_as_uint(s) : 0x7fc00000u;
+                owner[at] = kNobody;
+                waits = false;
+            }
+        }
+    }
+}
+
+template <int DT, int OUT>
+__global__ void __launch_bounds__(kBlock) adjust_logits_kernel(AdjustArgs a) {
+    extern __shared__ __align__(16) uint32_t lds[];
+    const int row = blockIdx.x / a.slices;
+    const uint32_t first = (blockIdx.x - row * a.slices) * (uint32_t)a.slice;
+    const uint32_t n = min((uint32_t)a.slice, (uint32_t)a.vocab - first);
+
+    float r = 1.f, p = 0.f, f = 0.f;
+    int length = 0, prompt = 0;
+    if (a.tokens != nullptr) {
+        r = setting(a.repetitions, a.repetition, row);
+        p = setting(a.presences, a.presence, row);
+        f = setting(a.frequencies, a.frequency, row);
+        if (!(r > 0.f)) r = 1.f;
+        length = a.lengths == nullptr ? a.length : a.lengths[row];
+        prompt = a.prompts == nullptr ? a.prompt : a.prompts[row];
+        length = min(max(length, 0), a.n_tokens);
+        prompt = min(max(prompt, 0), length);
+    }
+    const bool counted = length > 0 && (r != 1.f || p != 0.f || f != 0.f);
+    uint32_t* counts = lds;
+    uint32_t* sums = lds + (a.tokens != nullptr || a.biases > 0 ? a.slice : 0);
+    if (a.biases > 0) {
+        for (uint32_t i = threadIdx.x; i < n; i += kBlock) {
+            counts[i] = kNobody;
+            sums[i] = kNoBias;
+        }
+        __syncthreads();
+        add_biases(a, row, first, n, counts, sums);
+        __syncthreads();
+    }
+    if (counted) {
+        for (uint32_t i = threadIdx.x; i < n; i += kBlock) counts[i] = 0;
+        __syncthreads();
+        if (r != 1.f) count_tokens(a, row, 0, prompt, first, n, true, counts);
+        count_tokens(a, row, prompt, length, first, n, false, counts);
+    }
+    __syncthreads();
+
+    const int64_t in = row * a.stride + first, to = row * a.out_stride + first;
+    const uint8_t* allowed =
+        a.allowed == nullptr ? nullptr : a.allowed + row * a.allowed_stride + first / 8;
+    for (uint32_t i = 8 * threadIdx.x; i < n; i += 8 * kBlock) {
+        const int some = min(8, (int)(n - i));
+        Eight<DT> x;
+        if (some == 8) x.load(a.logits, in + i);
+        else x.load_some(a.logits, in + i, some);
+        const uint32_t bits = allowed == nullptr ? 0xffu : allowed[i / 8];
+        Eight<OUT> y;
+        if constexpr (DT == OUT) {
+            y = x;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y.set(j, x.get(j));
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // (behind the slice's end LDS holds anything: some < 8 alone)
+            const bool inside = j < some;
+            const uint32_t c = counted && inside ? counts[i + j] : 0u;
+            const uint32_t b = a.biases > 0 && inside ? sums[i + j] : kNoBias;
+            float v = x.get(j);
+            if (c != 0 && r != 1.f) v = v > 0.f ? v / r : v * r;
+            if ((c & ~kInPrompt) != 0) v = v - (f * (float)(c & ~kInPrompt) + p);
+            if (b != kNoBias) v = v + __uint_as_float(b);
+            const bool banned = (bits >> j & 1) == 0;
+            if (banned) v = -__builtin_inff();
+            if (c != 0 || b != kNoBias || banned) y.set(j, v);
+        }
+        if (some == 8) y.store(a.out, to + i);
+        else y.store_some(a.out, to + i, some);
+    }
+}
+
+}  // namespace
+}  // namespace kivi
+
+using namespace kivi;
+
+extern "C" {
+
+int kivi_adjust_logits(const void* logits, int32_t dtype, int64_t row_stride, int32_t rows,
+                       int32_t vocab, const void* tokens, int32_t tokens_i64,
+                       int64_t token_stride, int32_t n_tokens, const int32_t* lengths,
+                       int32_t length, const int32_t* prompt_lengths, int32_t prompt_length,
+                       const float* repetitions, float repetition, const float* presences,
+                       float presence, const float* frequencies, float frequency,
+                       const void* bias_ids, int32_t ids_i64, int64_t id_stride,
+                       const float* bias, int64_t bias_stride, int32_t biases,
+                       const uint32_t* allowed, int64_t allowed_stride, void* out,
+                       int32_t out_dtype, int64_t out_stride, void* stream) {
+    if (dtype < 0 || dtype > 2)
+        return set_error(kErrInvalidArgument, "dtype %d is not 0 (f32), 1 (bf16) or 2 (f16)", dtype);
+    if (out_dtype != dtype && out_dtype != kSrcF32)
+        return set_error(kErrInvalidArgument, "out_dtype %d is neither 0 (f32) nor dtype", out_dtype);
+    if (rows < 0 || vocab < 1)
+        return set_error(kErrInvalidArgument, "%d rows of %d tokens", rows, vocab);
+    if (n_tokens < 0 || n_tokens > kMostEntries || biases < 0 || biases > kMostEntries)
+        return set_error(kErrInvalidArgument, "%d tokens, %d biases: at most %d of each are taken",
+                         n_tokens, biases, kMostEntries);
+    if (rows == 0) return kOk;
+    if (logits == nullptr || out == nullptr || (n_tokens > 0 && tokens == nullptr) ||
+        (biases > 0 && (bias_ids == nullptr || bias == nullptr)))
+        return set_error(kErrInvalidArgument, "null pointer");
+    if (((uintptr_t)logits & (src_size(dtype) - 1)) || ((uintptr_t)out & (src_size(out_dtype) - 1)))
+        return set_error(kErrInvalidArgument, "logits and out must be aligned to their elements");
+    // In place is one element at a time; any other overlap would read what was written.
+    const char* from = static_cast<const char*>(logits);
+    const char* to = static_cast<const char*>(out);
+    const int64_t in_bytes = ((rows - 1) * row_stride + vocab) * src_size(dtype);
+    const int64_t out_bytes = ((rows - 1) * out_stride + vocab) * src_size(out_dtype);
+    const bool same = from == to && dtype == out_dtype && (rows == 1 || row_stride == out_stride);
+    if (out_stride < vocab && rows > 1)
+        return set_error(kErrInvalidArgument, "rows of out overlap");
+    if (!same && from < to + out_bytes && to < from + in_bytes)
+        return set_error(kErrInvalidArgument, "out must be logits or apart from them");
+    AdjustArgs a{};
+    a.logits = logits; a.out = out;
+    a.stride = row_stride; a.out_stride = out_stride;
+    a.tokens = n_tokens > 0 ? tokens : nullptr;
+    a.token64 = tokens_i64; a.token_stride = token_stride; a.n_tokens = n_tokens;
+    a.lengths = lengths; a.length = length;
+    a.prompts = prompt_lengths; a.prompt = prompt_length;
+    a.repetitions = repetitions; a.repetition = repetition;
+    a.presences = presences; a.presence = presence;
+    a.frequencies = frequencies; a.frequency = frequency;
+    a.bias_ids = bias_ids; a.id64 = ids_i64; a.id_stride = id_stride;
+    a.bias = bias; a.bias_stride = bias_stride; a.biases = biases;
+    a.allowed = reinterpret_cast<const uint8_t*>(allowed);
+    a.allowed_stride = 4 * allowed_stride;
+    a.vocab = vocab;
+    a.slice = 4096;
+    a.slices = (int)(((int64_t)vocab + a.slice - 1) / a.slice);
+    const int64_t blocks = (int64_t)rows * a.slices;
+    if (blocks > (int64_t)UINT32_MAX / kBlock)
+        return set_error(kErrInvalidArgument, "%d rows of %d tokens are too many for one launch",
+                         rows, vocab);
+    const unsigned grid = (unsigned)blocks;
+    const size_t lds = ((a.tokens != nullptr || biases > 0) + (biases > 0)) * (size_t)a.slice * 4;
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == kSrcF32)
+        adjust_logits_kernel<kSrcF32, kSrcF32><<<grid, kBlock, lds, s>>>(a);
+    else if (dtype == kSrcBF16 && out_dtype == dtype)
+        adjust_logits_kernel<kSrcBF16, kSrcBF16><<<grid, kBlock, lds, s>>>(a);
+    else if (dtype == kSrcBF16)
+        adjust_logits_kernel<kSrcBF16, kSrcF32><<<grid, kBlock, lds, s>>>(a);
+    else if (out_dtype == dtype)
+        adjust_logits_kernel<kSrcF16, kSrcF16><<<grid, kBlock, lds, s>>>(a);
+    else
+        adjust_logits_kernel<kSrcF16, kSrcF32><<<grid, kBlock, lds, s>>>(a);
+    return check_launch("adjust_logits");
+}
+
+}  // extern "C"
