@@ -1,14 +1,19 @@
 // Pieces shared by the attention kernels over pages of 8 bits (kivi_paged8.hip), and the
 // walk of up to 16 query rows.
 //
-// Codes are whole numbers up to 127, which bf16 and fp16 hold exactly, so both products
-// run on the 16-bit matrix instructions with codes as they are; the scales of a block of
-// 16 positions, numbers that all its lanes share, come in outside: the keys' into what
-// turns a score into log2 units, the values' into the weights.  The first product takes
-// queries in their own type, fp32 ones as three bf16 pieces (their 24 bits); the second
-// takes bf16 weights (fp16 has no room for scales): two pieces for up to 16 rows, three
-// for fp32, which so keeps fp32's accuracy at three times the products, where the fp32
-// instructions take sixteen times.
+// Codes are whole numbers up to 127, which fp16 holds exactly, so both products run on
+// the fp16 matrix instructions with codes as they are; the scales of a block of 16
+// positions, numbers that all its lanes share, come in outside: the keys' into what
+// turns a score into log2 units, the values' into the weights.
+//
+// Queries enter as fp16 too: a row times the power of two that brings its largest
+// element to 2^14, which keeps every bit of bf16's elements down to 2^-28 of that one,
+// and fp32's as two pieces (22 bits).  Weights times value scales have no such bounds, so
+// a row keeps a second maximum, that of these products, and its outputs in units of
+// that one: the largest lies between 2^12 and 2^15, so that fp16's last step, 2^-24, is
+// 2^-36 of it or less.  They are rounded to fp16 (as a bf16 cache's would be to bf16, or
+// better), for up to 16 rows and for fp32 in two pieces.  (bf16 operands hold codes and any scale
+// at once, but take a fifth more operations to widen codes, and fp32 three pieces.)
 //
 // Codes are finite, so what a row must not see is 0 times a number; but for a block's
 // scales that are NaN, whose place numbers take for rows that see none of the block.
@@ -25,53 +30,92 @@ struct Paged8Launch : PagedLaunch {
 
 namespace {
 
-// The type of the key operand, and the pieces that queries and weights enter in.
+// The pieces that queries enter in.
 template <int DT>
-constexpr int key_type() { return DT == kSrcF16 ? kSrcF16 : kSrcBF16; }
-template <int DT>
-constexpr int query_pieces() { return DT == kSrcF32 ? 3 : 1; }
+constexpr int query_pieces() { return DT == kSrcF32 ? 2 : 1; }
 
-// Two codes of a word's bytes 2 i and 2 i + 1, as a pair of DT.
-template <int DT>
+// Two codes of a word's bytes 2 i and 2 i + 1: 1024 + (code + 128), from which 1152 goes
+// exactly.  x: the word with the codes' signs flipped.
 __device__ __forceinline__ uint32_t pair_of_codes(uint32_t x, int i) {
-    if constexpr (DT == kSrcBF16) {
-        const float a = (float)(int8_t)(x >> (16 * i)), b = (float)(int8_t)(x >> (16 * i + 8));
-        return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-    } else {
-        // 1024 + (code + 128), from which 1152 goes exactly
-        const uint32_t u = __builtin_amdgcn_perm(0x64646464u, x ^ 0x80808080u,
-                                                 i ? 0x04030402u : 0x04010400u);
-        const f16x2_t v = __builtin_bit_cast(f16x2_t, u) - f16x2_t{(_Float16)1152, (_Float16)1152};
-        return __builtin_bit_cast(uint32_t, v);
-    }
+    const uint32_t u = __builtin_amdgcn_perm(0x64646464u, x, i ? 0x04030402u : 0x04010400u);
+    const f16x2_t v = __builtin_bit_cast(f16x2_t, u) - f16x2_t{(_Float16)1152, (_Float16)1152};
+    return __builtin_bit_cast(uint32_t, v);
 }
 // Eight codes as an operand.
-template <int DT>
 __device__ __forceinline__ u32x4_t operand_of_codes(uint32_t x, uint32_t y) {
-    return u32x4_t{pair_of_codes<DT>(x, 0), pair_of_codes<DT>(x, 1), pair_of_codes<DT>(y, 0),
-                   pair_of_codes<DT>(y, 1)};
+    x ^= 0x80808080u;
+    y ^= 0x80808080u;
+    return u32x4_t{pair_of_codes(x, 0), pair_of_codes(x, 1), pair_of_codes(y, 0),
+                   pair_of_codes(y, 1)};
 }
 
-// Eight consecutive channels of a query row as an operand of each piece.
-template <int DT>
-__device__ __forceinline__ void load_query(const void* q, int64_t i,
-                                           u32x4_t (&f)[query_pieces<DT>()]) {
-    if constexpr (DT == kSrcF32) {
-        const SplitConsts k = split_consts();
-        const f32x4_t* p = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(q) + i);
-        const f32x4_t x = p[0], y = p[1];
+// Two values as fp16 pieces: rounded, and what that left out.
+struct Pieces { uint32_t hi, lo; };
+__device__ __forceinline__ Pieces split_f16(float a, float b) {
+    const uint32_t hi = pack2<kSrcF16>(a, b);
+    const f16x2_t h = __builtin_bit_cast(f16x2_t, hi);
+    return {hi, pack2<kSrcF16>(fmaf((float)h[0], -1.0f, a), fmaf((float)h[1], -1.0f, b))};
+}
+
+// A query row's operands, k-step i's 8 channels at channel(i), by the lanes that
+// share(max) reduces over: f, and what a product with them is to be multiplied by.
+template <int DT, int KS, class C, class S>
+__device__ __forceinline__ float load_query(const PagedLaunch& a, int64_t at, bool live, C channel,
+                                            S share, u32x4_t (&f)[KS][query_pieces<DT>()]) {
+    if constexpr (DT == kSrcF16) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t hi, mid, lo;
-            split3_pair(j < 2 ? x[2 * j] : y[2 * j - 4], j < 2 ? x[2 * j + 1] : y[2 * j - 3], hi,
-                        mid, lo, k);
-            f[0][j] = hi;
-            f[1][j] = mid;
-            f[2][j] = lo;
+        for (int i = 0; i < KS; ++i) {
+            f[i][0] = u32x4_t{0, 0, 0, 0};
+            if (live && channel(i) < a.D)
+                f[i][0] = *reinterpret_cast<const u32x4_t*>(
+                    static_cast<const uint16_t*>(a.q) + at + channel(i));
         }
+        return 1.0f;
     } else {
-        f[0] = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(q) + i);
+        f32x4_t x[KS][2];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                x[i][h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                if (live && channel(i) < a.D) x[i][h] = load4<DT>(a.q, at + channel(i) + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    top = max(top, __float_as_uint(x[i][h][j]) & 0x7fffffffu);
+            }
+        }
+        const int e = (int)(share(top) >> 23);
+        // 2^14 for the largest (a row of infinities or NaN, and one below 2^-112, may stay
+        // where it is: its scores are no numbers, or 0)
+        const int up = e == 255 ? 0 : min(141 - e, 126);
+        const float factor = __int_as_float((127 + up) << 23);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float u = x[i][j / 2][j % 2 * 2] * factor;
+                const float v = x[i][j / 2][j % 2 * 2 + 1] * factor;
+                if constexpr (DT == kSrcF32) {
+                    const Pieces p = split_f16(u, v);
+                    f[i][0][j] = p.hi;
+                    f[i][1][j] = p.lo;
+                } else {
+                    f[i][0][j] = pack2<kSrcF16>(u, v);
+                }
+            }
+        }
+        return __int_as_float((127 - up) << 23);
     }
+}
+
+// The largest weight times scale of a row is 2^kWeightBits, or half of it, when its units
+// are set, and they are set anew where one comes out 2^kMoveTop times larger.
+constexpr float kWeightBits = 13.0f, kMoveTop = 2.0f;
+
+// Power of two above a scale, log2.
+__device__ __forceinline__ float above(float scale) {
+    return (float)((int)(__float_as_uint(scale) >> 23 & 0xff) - 126);
 }
 
 // The scales of blocks of 16 positions (the last one's for blocks past the end), by
@@ -141,7 +185,7 @@ template <int DT, int DP, class L>
 __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, L lds,
                                           Few8Join& join) {
     using F = Few8<DP>;
-    constexpr int NB = F::NB, KT = key_type<DT>(), NQ = query_pieces<DT>();
+    constexpr int NB = F::NB, NQ = query_pieces<DT>();
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     const int col = lane % 16, gq = lane / 16;
     unsigned char* vl = lds(wave);
@@ -154,20 +198,18 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
         return ks + 1 == F::KS && F::KS % 2 ? 32 * ks + 8 * gq : 32 * (ks & ~1) + 16 * gq + ks % 2 * 8;
     };
     u32x4_t qf[F::KS][NQ];
-    f32x4_t O[F::CB];
-    float m = -FLT_MAX, l = 0.f;
+    f32x4_t O[F::CB];                    // in units of 2^top
+    float m = -FLT_MAX, top = -FLT_MAX, l = 0.f, qscale;
     int lim = 0;
     {
         const int r = w.it.row0 + col;
         const bool live = r < w.rows;
         if (live) lim = row_limit(w, r);
-        const int64_t q = live ? q_offset(a, w, r) : 0;
-#pragma unroll
-        for (int ks = 0; ks < F::KS; ++ks) {
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) qf[ks][n] = u32x4_t{0, 0, 0, 0};
-            if (live && channel(ks) < a.D) load_query<DT>(a.q, q + channel(ks), qf[ks]);
-        }
+        qscale = a.qscale * load_query<DT, F::KS>(a, live ? q_offset(a, w, r) : 0, live, channel,
+                                                  [](uint32_t x) {
+            x = max(x, (uint32_t)__shfl_xor((int)x, 16));
+            return max(x, (uint32_t)__shfl_xor((int)x, 32));
+        }, qf);
     }
 #pragma unroll
     for (int cb = 0; cb < F::CB; ++cb) O[cb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -238,11 +280,12 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
             s[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < F::KS; ++ks) {
-                const u32x4_t x = operand_of_codes<KT>(kf[b][ks / 2][ks % 2 * 2],
-                                                       kf[b][ks / 2][ks % 2 * 2 + 1]);
+                const u32x4_t x = operand_of_codes(kf[b][ks / 2][ks % 2 * 2],
+                                                   kf[b][ks / 2][ks % 2 * 2 + 1]);
 #pragma unroll
-                for (int n = NQ - 1; n >= 0; --n) s[b] = mfma16<KT>(x, qf[ks][n], s[b]);
+                for (int n = NQ - 1; n >= 0; --n) s[b] = mfma16<kSrcF16>(x, qf[ks][n], s[b]);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         const Pages pg = ahead;
         if (next < end) {
@@ -264,7 +307,7 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
         float units[NB], vs[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            units[b] = score_units(scales.k[b], a.qscale);
+            units[b] = score_units(scales.k[b], qscale);
             vs[b] = scales.v[b];
         }
         if (t0 + F::UNIT > min(all_see, end)) {
@@ -279,46 +322,62 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
                     if (t0 + 16 * b + 4 * gq + i >= lim) s[b][i] = -INFINITY;
             }
         }
-        float mx = -INFINITY;
+        float mx = -INFINITY, mv = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-            mx = fmaxf(mx, fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])) * units[b]);
-        if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax) != 0) {
+        for (int b = 0; b < NB; ++b) {
+            const float x = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])) * units[b];
+            mx = fmaxf(mx, x);
+            mv = fmaxf(mv, x + above(scales.v[b]));
+        }
+        mv -= kWeightBits;
+        if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax || mv > top + kMoveTop) != 0) {
             mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float to = fmaxf(m, mx), f = exp2_fast(m - to);
-            m = to;
-            l *= f;
+            mv = fmaxf(mv, __shfl_xor(mv, 16));
+            mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
+            mv = fmaxf(top, fmaxf(mv, __shfl_xor(mv, 32)));
+            l *= exp2_fast(m - mx);
+            const float f = exp2_fast(top - mv);
+            m = mx;
+            top = mv;
 #pragma unroll
             for (int cb = 0; cb < F::CB; ++cb) O[cb] *= f;
         }
+        const float down = exp2_fast(m - top);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) vs[b] *= down;
         // rows of a transposed read: tokens 4 gq .. + 3 of a block and of the next, in
         // the order in which a lane holds the weights
         const unsigned char* vr = vl + (4 * gq + col / 2 % 4 + col / 8 * 16) * F::VS + col % 2 * 8;
         wave_sync();
 #pragma unroll
         for (int j = 0; j < NB / 2; ++j) {
-            constexpr int NP = DT == kSrcF32 ? 3 : 2;
-            const SplitConsts k = split_consts();
-            u32x4_t pf[NP];
+            u32x4_t hi, lo;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int b = 2 * j + i / 2;
                 const float p0 = exp2_fast(fmaf(s[b][i % 2 * 2], units[b], -m));
                 const float p1 = exp2_fast(fmaf(s[b][i % 2 * 2 + 1], units[b], -m));
                 l += p0 + p1;
-                uint32_t x[3];
-                if constexpr (NP == 3) split3_pair(p0 * vs[b], p1 * vs[b], x[0], x[1], x[2], k);
-                else split_pair(p0 * vs[b], p1 * vs[b], x[0], x[1], k);
-#pragma unroll
-                for (int n = 0; n < NP; ++n) pf[n][i] = x[n];
+                const Pieces w = split_f16(p0 * vs[b], p1 * vs[b]);
+                hi[i] = w.hi;
+                lo[i] = w.lo;
             }
+            // (four reads, then their products: left to itself the compiler widens all of
+            // a unit's codes first, in 100 registers more)
+            constexpr int kAtOnce = F::CB % 4 == 0 ? 4 : 3;
 #pragma unroll
-            for (int cb = 0; cb < F::CB; ++cb) {
-                const i32x2_t v = read_transposed8(vr + 32 * j * F::VS + cb * 16);
-                const u32x4_t vt8 = operand_of_codes<kSrcBF16>((uint32_t)v[0], (uint32_t)v[1]);
+            for (int c0 = 0; c0 < F::CB; c0 += kAtOnce) {
+                i32x2_t v[kAtOnce];
 #pragma unroll
-                for (int n = NP - 1; n >= 0; --n) O[cb] = mfma16<kSrcBF16>(vt8, pf[n], O[cb]);
+                for (int i = 0; i < kAtOnce; ++i)
+                    v[i] = read_transposed8(vr + 32 * j * F::VS + (c0 + i) * 16);
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const u32x4_t x = operand_of_codes((uint32_t)v[i][0], (uint32_t)v[i][1]);
+                    O[c0 + i] = mfma16<kSrcF16>(x, lo, O[c0 + i]);
+                    O[c0 + i] = mfma16<kSrcF16>(x, hi, O[c0 + i]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -331,8 +390,8 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
         join.l[wave][col] = l;
     }
     __syncthreads();
-    const float f = exp2_fast(m - fmaxf(fmaxf(join.m[0][col], join.m[1][col]),
-                                        fmaxf(join.m[2][col], join.m[3][col])));
+    const float f = exp2_fast(top - fmaxf(fmaxf(join.m[0][col], join.m[1][col]),
+                                          fmaxf(join.m[2][col], join.m[3][col])));
 #pragma unroll
     for (int cb = 0; cb < F::CB; ++cb)
         *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(vl) + col * F::OS + 16 * cb + 4 * gq) =

@@ -10,7 +10,7 @@ namespace {
 constexpr int kBlock = kFew8Waves * kWave;
 
 template <int DT, int DP>
-__global__ void __launch_bounds__(kBlock) paged8_few_kernel(Paged8Launch a) {
+__global__ void __launch_bounds__(kBlock, 2) paged8_few_kernel(Paged8Launch a) {
     __shared__ __align__(16) unsigned char lds[kFew8Waves * Few8<DP>::WAVE_BYTES];
     __shared__ Few8Join join;
     few8_rows<DT, DP>(a, work_of(a), [&](int i) { return lds + i * Few8<DP>::WAVE_BYTES; }, join);

@@ -6,10 +6,6 @@
 // channels) in two LDS buffers.  A tile's codes are loaded into registers while the one
 // before is computed, widened there once for all four waves and written to the other
 // buffer: one barrier per tile.
-//
-// fp16's weights stay fp16 (11 bits): value scales have no room in its range, so a row
-// keeps a second maximum, that of its weights times their blocks' scales, and its outputs
-// in units of that one.
 #include <hip/hip_runtime.h>
 
 #include "kivi_paged8_attention.hpp"
@@ -67,7 +63,6 @@ struct Tile8Loads {
         pages_of(a, w, t0 + TOKENS);
     }
     // Writes the loaded tile, widened, to LDS.
-    template <int KT, int VT>
     __device__ __forceinline__ void store(unsigned char* buf) const {
         const int c = channel();
         if (c >= DP) return;                                // (96 channels: six lanes of eight)
@@ -80,9 +75,9 @@ struct Tile8Loads {
             for (int h = 0; h < 2; ++h) {
                 const int x = c / 8 + h;
                 *reinterpret_cast<u32x4_t*>(kr + ((x ^ M::key_swizzle(t)) << 4)) =
-                    operand_of_codes<KT>(k[i][2 * h], k[i][2 * h + 1]);
+                    operand_of_codes(k[i][2 * h], k[i][2 * h + 1]);
                 *reinterpret_cast<u32x4_t*>(vr + ((x ^ M::value_swizzle(t)) << 4)) =
-                    operand_of_codes<VT>(v[i][2 * h], v[i][2 * h + 1]);
+                    operand_of_codes(v[i][2 * h], v[i][2 * h + 1]);
             }
         }
     }
@@ -92,13 +87,13 @@ struct Tile8Loads {
 template <int DT, int DP, int TOKENS>
 struct Tile8Rows {
     using M = TileShape<DP, TOKENS>;
-    static constexpr int KT = key_type<DT>(), NQ = query_pieces<DT>();
-    static constexpr int VT = DT == kSrcF16 ? kSrcF16 : kSrcBF16;
+    static constexpr int NQ = query_pieces<DT>();
     static constexpr int NB = TOKENS / 16;
     u32x4_t qf[M::KS][NQ];
     f32x16_t O[M::CB];
     float m, l;
-    float top;               // fp16: the outputs' units, log2
+    float top;               // the outputs' units, log2
+    float qscale;
     int lim;                 // positions that the lane's row sees
     int all, last;           // that all, and any, of the 32 rows see
 
@@ -108,14 +103,9 @@ struct Tile8Rows {
         lim = live ? row_limit(w, r) : 0;
         m = top = -FLT_MAX;
         l = 0.f;
-        const int64_t q = live ? q_offset(a, w, r) : 0;
-#pragma unroll
-        for (int ks = 0; ks < M::KS; ++ks) {
-            const int c = 16 * ks + 8 * half;
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) qf[ks][n] = u32x4_t{0, 0, 0, 0};
-            if (live && c < a.D) load_query<DT>(a.q, q + c, qf[ks]);
-        }
+        qscale = a.qscale * load_query<DT, M::KS>(
+            a, live ? q_offset(a, w, r) : 0, live, [&](int ks) { return 16 * ks + 8 * half; },
+            [](uint32_t x) { return max(x, (uint32_t)__shfl_xor((int)x, 32)); }, qf);
 #pragma unroll
         for (int cb = 0; cb < M::CB; ++cb) {
 #pragma unroll
@@ -128,7 +118,7 @@ struct Tile8Rows {
 
     // A tile of keys and values in LDS, positions t0 ..
     __device__ __forceinline__ void tile(const unsigned char* buf, const BlockScales<NB>& sc,
-                                         int t0, int end, float qscale) {
+                                         int t0, int end) {
         const int lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
         f32x16_t s[M::TB];
 #pragma unroll
@@ -144,7 +134,7 @@ struct Tile8Rows {
                 const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(
                     buf + ((krow ^ (32 * ks)) + 32 * tb * M::ROW));
 #pragma unroll
-                for (int n = NQ - 1; n >= 0; --n) s[tb] = mfma32<KT>(kf, qf[ks][n], s[tb]);
+                for (int n = NQ - 1; n >= 0; --n) s[tb] = mfma32<kSrcF16>(kf, qf[ks][n], s[tb]);
             }
         }
         // score i of 32 tokens tb: token 32 tb + 8 (i / 4) + 4 half + i % 4, of block
@@ -178,38 +168,27 @@ struct Tile8Rows {
             for (int i = 1; i < 8; ++i) x = fmaxf(x, s[b / 2][b % 2 * 8 + i]);
             x *= units[b];
             mx = fmaxf(mx, x);
-            // (an exponent above the scale's)
-            if constexpr (VT == kSrcF16)
-                mv = fmaxf(mv, x + (float)((int)(__float_as_uint(sc.v[b]) >> 23 & 0xff) - 126));
+            mv = fmaxf(mv, x + above(sc.v[b]));
         }
-        if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax) != 0) {
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float to = fmaxf(m, mx), f = exp2_fast(m - to);
-            m = to;
-            l *= f;
-            if constexpr (VT != kSrcF16) {
+        mv -= kWeightBits;
+        if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax || mv > top + kMoveTop) != 0) {
+            mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
+            mv = fmaxf(top, fmaxf(mv, __shfl_xor(mv, 32)));
+            l *= exp2_fast(m - mx);
+            const float f = exp2_fast(top - mv);
+            m = mx;
+            top = mv;
 #pragma unroll
-                for (int cb = 0; cb < M::CB; ++cb) O[cb] *= f;
-            }
+            for (int cb = 0; cb < M::CB; ++cb) O[cb] *= f;
         }
-        if constexpr (VT == kSrcF16) {
-            mv -= weight_bits<VT>();
-            if (__builtin_amdgcn_ballot_w64(mv > top + kMoveMax) != 0) {
-                mv = fmaxf(mv, __shfl_xor(mv, 32));
-                const float to = fmaxf(top, mv), f = exp2_fast(top - to);
-                top = to;
+        const float down = exp2_fast(m - top);
 #pragma unroll
-                for (int cb = 0; cb < M::CB; ++cb) O[cb] *= f;
-            }
-            const float f = exp2_fast(m - top);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) vs[b] *= f;
-        }
+        for (int b = 0; b < NB; ++b) vs[b] *= down;
         // transposed: lanes of 16 take tokens 4 half .. + 3 of 16 channels
         const int t = 4 * half + lane % 16 / 4;
         const int c = lane / 16 % 2 * 2 + lane % 4 / 2;
         const uint32_t vrow = M::BYTES + t * M::ROW + ((c ^ M::value_swizzle(t)) << 4) + lane % 2 * 8;
-        constexpr int NP = DT == kSrcF32 ? 3 : 1;
+        constexpr int NP = DT == kSrcF32 ? 2 : 1;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             u32x4_t pf[NP];
@@ -219,14 +198,12 @@ struct Tile8Rows {
                 const float p0 = exp2_fast(fmaf(x, units[b], -m));
                 const float p1 = exp2_fast(fmaf(y, units[b], -m));
                 l += p0 + p1;
-                if constexpr (NP == 3) {
-                    uint32_t hi, mid, lo;
-                    split3_pair(p0 * vs[b], p1 * vs[b], hi, mid, lo, split_consts());
-                    pf[0][i] = hi;
-                    pf[1][i] = mid;
-                    pf[2][i] = lo;
+                if constexpr (NP == 2) {
+                    const Pieces w = split_f16(p0 * vs[b], p1 * vs[b]);
+                    pf[0][i] = w.hi;
+                    pf[1][i] = w.lo;
                 } else {
-                    pf[0][i] = pack2<VT>(p0 * vs[b], p1 * vs[b]);
+                    pf[0][i] = pack2<kSrcF16>(p0 * vs[b], p1 * vs[b]);
                 }
             }
 #pragma unroll
@@ -236,7 +213,7 @@ struct Tile8Rows {
                 const uint2 hi = read_transposed(buf + (at + 8 * M::ROW));
                 const u32x4_t vt = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-                for (int n = NP - 1; n >= 0; --n) O[cb] = mfma32<VT>(vt, pf[n], O[cb]);
+                for (int n = NP - 1; n >= 0; --n) O[cb] = mfma32<kSrcF16>(vt, pf[n], O[cb]);
             }
         }
     }
@@ -271,15 +248,15 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 && DT != kSrcF32 ? 2 : 1)
     int t0 = w.it.kv_begin;
     loads.pages_of(a, w, t0);
     loads.issue(a, w, t0);
-    loads.template store<R::KT, R::VT>(buf0);
+    loads.store(buf0);
     auto step = [&](unsigned char* now, unsigned char* next) {
         const BlockScales<R::NB> scales = loads.scales;
         // (behind it this tile is whole, and the other buffer read by all)
         __syncthreads();
         const bool more = t0 + kTile < end;
         if (more) loads.issue(a, w, t0 + kTile);
-        if (t0 < rows.last) rows.tile(now, scales, t0, end, a.qscale);
-        if (more) loads.template store<R::KT, R::VT>(next);
+        if (t0 < rows.last) rows.tile(now, scales, t0, end);
+        if (more) loads.store(next);
         t0 += kTile;
     };
     while (true) {
@@ -294,8 +271,7 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 && DT != kSrcF32 ? 2 : 1)
     const int r = w.it.row0 + 32 * wave + col;
     if (r >= w.rows) return;
     const bool whole = w.it.part < 0;
-    float f = whole ? inverse_sum(l) : 1.0f;
-    if constexpr (R::VT == kSrcF16) f *= exp2_fast(rows.top - rows.m);
+    const float f = (whole ? inverse_sum(l) : 1.0f) * exp2_fast(rows.top - rows.m);
     const int64_t at = whole ? out_offset(a, w, r) : part_row(a, w, r);
 #pragma unroll
     for (int cb = 0; cb < M::CB; ++cb) {

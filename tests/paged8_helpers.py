@@ -75,21 +75,43 @@ def filled_pool8(table, pool, ctx, Hkv, D, page_size, seed, spread=0):
     return codes, scales
 
 
-def attention8_tolerance(ref, mag, size, D, c, dtype):
+def largest_weight(q, k, v_scales, table, ctx, new, page_size, scale):
+    """The largest softmax weight times value scale of each row, ``[T, Hq]`` (k: the
+    keys' values)."""
+    T, Hq, D = q.shape
+    hg = Hq // k.shape[1]
+    out, at = torch.zeros(T, Hq, dtype=torch.float64), 0
+    for s, (c, n) in enumerate(zip(ctx, new)):
+        pos = torch.arange(c)
+        page = table[s].long()[pos // page_size]
+        for h in range(Hq):
+            kk = k[page, h // hg, pos % page_size].double()
+            vs = v_scales[page, h // hg, pos % page_size // BLOCK].double()
+            for i in range(n):
+                m = c - n + i + 1
+                p = torch.softmax((kk[:m] @ q[at + i, h].double()) * scale, 0)
+                out[at + i, h] = (p * vs[:m]).max()
+        at += n
+    return out
+
+
+def attention8_tolerance(ref, mag, size, largest, D, c, dtype):
     """Each element's bound: the output's rounding (half a step; fp16's numbers below
-    2^-14 are 2^-24 apart, so 2^-25 there whatever their size); the weights'
-    rounding for the second product (half a step of a 16-bit type at most, for fp32
-    three bf16 pieces, 2^-24 of each); and fp32: a score is a sum of three products
-    of pieces for each of D channels at most, times a scale, so off by (3 D + 6)
-    2^-24 of sum |q k| scale, which moves a weight and the weights' sum by that much
-    relative each; exp2, the scales and the sums over c tokens add (3 c + 16) 2^-24
-    each."""
+    2^-14 are 2^-24 apart, so 2^-25 there whatever their size); the weights' rounding for
+    the second product, to fp16: half a step at most (2^-11, for fp32 two pieces, 2^-22),
+    and 2^-25 where the largest weight times scale is 2^12 or more, so 2^-37 of that one,
+    for c codes of 127 at most; and fp32: a score is a sum of two products of pieces for
+    each of D channels at most, pieces that leave 2^-22 of fp32 queries out, times a
+    scale: off by (2 D + 10) 2^-24 of sum |q k| scale, which moves a weight and the
+    weights' sum by that much relative each; exp2, the scales and the sums over c
+    tokens add (3 c + 16) 2^-24 each."""
     eps, u = EPS[dtype], 2.0 ** -24
-    moved = 2 * ((3 * D + 6) * u * size[..., None] + (3 * c + 16) * u)
-    half = u if dtype == torch.float32 else eps / 2
+    moved = 2 * ((2 * D + 10) * u * size[..., None] + (3 * c + 16) * u)
+    half = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -11
     least = 2.0 ** -25 if dtype == torch.float16 else 1e-30
-    return (eps / 2) * ref.abs() + (half + moved) * mag * (1 + eps) + least
+    small = 127 * c * 2.0 ** -37 * largest[..., None]
+    return (eps / 2) * ref.abs() + ((half + moved) * mag + small) * (1 + eps) + least
 
 
 __all__ = ["BLOCK", "EPS", "make_table", "scale_of", "fill", "values", "empty_pool",
-           "filled_pool8", "attention8_tolerance"]
+           "filled_pool8", "largest_weight", "attention8_tolerance"]

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests.paged8_helpers import (BLOCK, attention8_tolerance, empty_pool, fill, filled_pool8,
-                                  scale_of, values)
+                                  largest_weight, scale_of, values)
 from tests.paged_helpers import EPS, attention64, make_table, rows64, slots_of
 from tests.test_paged_gpu import SHAPES
 
@@ -41,12 +41,20 @@ def _attend(case, **kw):
                                 v_scales=vs.cuda(), **kw)
 
 
-def _check(o, case, page, scale=None):
+def _expected(case, page, scale=None):
+    """The outputs in float64, and their bounds."""
     table, pool, ctx, new, kc, ks, vc, vs, plan, q = case
     D = q.shape[-1]
-    ref, mag, size = attention64(q, values(kc, ks), values(vc, vs), table, ctx, new, page,
-                                 D ** -0.5 if scale is None else scale)
-    tol = attention8_tolerance(ref, mag, size, D, max(ctx), q.dtype)
+    at = (table, ctx, new, page, D ** -0.5 if scale is None else scale)
+    ref, mag, size = attention64(q, values(kc, ks), values(vc, vs), *at)
+    largest = largest_weight(q, values(kc, ks), vs, *at)
+    return ref, attention8_tolerance(ref, mag, size, largest, D, max(ctx), q.dtype)
+
+
+def _check(o, case, page, scale=None):
+    q = case[-1]
+    D = q.shape[-1]
+    ref, tol = _expected(case, page, scale)
     err = (o.double().cpu() - ref).abs()
     print(f"[paged8] {q.dtype} D={D} worst {float((err / tol).max()):.3f} of the bound", flush=True)
     assert bool((err <= tol).all()), float((err / tol).max())
@@ -121,9 +129,7 @@ def test_blocks_that_are_not_numbers(hip_device, dtype, D, n):
     ok_v, ok_k = vs.clone(), ks.clone()
     ok_v[torch.isnan(ok_v)] = 1.0
     ok_k[torch.isnan(ok_k)] = 1.0
-    ref, mag, size = attention64(q, values(kc, ok_k), values(vc, ok_v), table, ctx, new, 16,
-                                 D ** -0.5)
-    tol = attention8_tolerance(ref, mag, size, D, max(ctx), dtype)
+    ref, tol = _expected((table, pool, ctx, new, kc, ok_k, vc, ok_v, plan, q), 16)
     sees_v = torch.zeros(2 * n, 4, dtype=torch.bool)
     sees_k = torch.zeros(2 * n, 4, dtype=torch.bool)
     for i in range(n):
