@@ -118,31 +118,45 @@ __device__ __forceinline__ float above(float scale) {
     return (float)((int)(__float_as_uint(scale) >> 23 & 0xff) - 126);
 }
 
-// The scales of blocks of 16 positions (the last one's for blocks past the end), by
-// scalar loads.
+// The scales of N blocks of 16 positions (the last one's for blocks past the end).  Lane l
+// loads one of them, its block l % N's for keys or values, and before that, while the
+// tile before is loaded, its page.  (Scalar loads would do with no lanes, but LDS reads
+// wait for whatever scalar loads are on their way: a chunk of 2048 tokens after 8200 took
+// 397 us with them.)
 template <int N>
 struct BlockScales {
-    float k[N], v[N];
+    int page;
+    float own;
 
-    __device__ __forceinline__ void load(const Paged8Launch& a, const Work& w, int t0,
-                                         const int (&page)[N]) {
-        typedef const __attribute__((address_space(4))) float* scalar_t;
-        const int shift = a.page_shift - 4;
-#pragma unroll
-        for (int b = 0; b < N; ++b) {
-            const int off = min(t0 + 16 * b, (w.it.kv_end - 1) & ~15) & ((1 << a.page_shift) - 1);
-            const int64_t at = (((int64_t)page[b] * a.Hkv + w.kvh) << shift) + off / kScaleBlock;
-            k[b] = ((scalar_t)a.k_scales)[at];
-            v[b] = ((scalar_t)a.v_scales)[at];
-        }
+    __device__ __forceinline__ void pages_of(const Paged8Launch& a, const Work& w, int t0) {
+        const int t = min(t0 + 16 * ((int)threadIdx.x % N), w.it.kv_end - 1);
+        page = (a.pages + w.it.page0)[t >> a.page_shift];
     }
+    __device__ __forceinline__ void load(const Paged8Launch& a, const Work& w, int t0) {
+        const int lane = threadIdx.x % kWave;
+        const int t = min(t0 + 16 * (lane % N), (w.it.kv_end - 1) & ~15);
+        const int off = t & ((1 << a.page_shift) - 1);
+        const int64_t at = (((int64_t)page * a.Hkv + w.kvh) << (a.page_shift - 4)) + off / kScaleBlock;
+        own = (lane / N % 2 ? a.v_scales : a.k_scales)[at];
+    }
+    __device__ __forceinline__ int page_of(int b) const {
+        return __builtin_amdgcn_readlane(page, b);
+    }
+    __device__ __forceinline__ float k(int b) const { return lane_f(own, b); }
+    __device__ __forceinline__ float v(int b) const { return lane_f(own, N + b); }
 };
 
-// What turns a score of a block into log2 units.  Above 0, for what masks leave of a row
-// is -infinity (a scale of 0 belongs to codes that do not matter); NaN stays.
-__device__ __forceinline__ float score_units(float scale, float qscale) {
-    const float x = scale * qscale;
-    return x < FLT_MIN ? FLT_MIN : x;
+// A page id (one for the wave), by a vector load for the same reason.
+__device__ __forceinline__ int block_page_ahead(const Paged8Launch& a, const Work& w, int t) {
+    int at = min(t, w.it.kv_end - 1) >> a.page_shift;
+    asm("" : "+v"(at));
+    return (a.pages + w.it.page0)[at];
+}
+
+// What turns a score of a block into log2 units, where masks leave -infinity of some:
+// above 0 (a scale of 0 belongs to codes that do not matter); NaN stays.
+__device__ __forceinline__ float above_zero(float units) {
+    return units < FLT_MIN ? FLT_MIN : units;
 }
 
 constexpr int kFew8Waves = 4;
@@ -218,17 +232,10 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
     const int end = w.it.kv_end;
 
     u32x4_t kf[NB][F::KP], vf[NB][F::VB];
-    struct Pages { int p[NB]; };
-    auto pages_of = [&](int t0) {
-        Pages pg;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) pg.p[b] = block_page(a, w, t0 + 16 * b);
-        return pg;
-    };
-    auto load_k = [&](int t0, const Pages& pg) {
+    auto load_k = [&](int t0, const BlockScales<NB>& of) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const uint8_t* p = block_at<uint8_t>(a, w, a.k_pages, pg.p[b], t0 + 16 * b);
+            const uint8_t* p = block_at<uint8_t>(a, w, a.k_pages, of.page_of(b), t0 + 16 * b);
 #pragma unroll
             for (int kp = 0; kp < F::KP; ++kp) {
                 const int c = channel(2 * kp);
@@ -246,10 +253,10 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
         }
     };
     const int vt = lane / F::CH, vc = lane % F::CH * 16;
-    auto load_v = [&](int t0, const Pages& pg) {
+    auto load_v = [&](int t0, const BlockScales<NB>& of) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const uint8_t* p = block_at<uint8_t>(a, w, a.v_pages, pg.p[b], t0 + 16 * b);
+            const uint8_t* p = block_at<uint8_t>(a, w, a.v_pages, of.page_of(b), t0 + 16 * b);
 #pragma unroll
             for (int i = 0; i < F::VB; ++i) {
                 vf[b][i] = u32x4_t{0, 0, 0, 0};
@@ -262,14 +269,14 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
 
     int t0 = w.it.kv_begin + wave * F::UNIT;
     constexpr int kStep = kFew8Waves * F::UNIT;
-    Pages ahead{};
-    BlockScales<NB> scales{}, coming{};
+    // (a unit's scales and the next one's pages; the scales of the unit at hand)
+    BlockScales<NB> coming{}, scales{};
     if (t0 < end) {
-        const Pages pg = pages_of(t0);
-        load_k(t0, pg);
-        load_v(t0, pg);
-        coming.load(a, w, t0, pg.p);
-        ahead = pages_of(t0 + kStep);
+        coming.pages_of(a, w, t0);
+        load_k(t0, coming);
+        load_v(t0, coming);
+        coming.load(a, w, t0);
+        coming.pages_of(a, w, t0 + kStep);
     }
     for (; t0 < end; t0 += kStep) {
         const int next = t0 + kStep;
@@ -287,11 +294,9 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        const Pages pg = ahead;
         if (next < end) {
-            load_k(next, pg);
-            coming.load(a, w, next, pg.p);
-            ahead = pages_of(next + kStep);
+            load_k(next, coming);
+            coming.load(a, w, next);
         }
         wave_sync();                      // the last unit's reads, before these writes
 #pragma unroll
@@ -302,17 +307,22 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
                     *reinterpret_cast<u32x4_t*>(vl + (16 * b + vt + i * F::VT) * F::VS + vc) =
                         vf[b][i];
         }
-        if (next < end) load_v(next, pg);
+        if (next < end) {
+            load_v(next, coming);
+            coming.pages_of(a, w, next + kStep);
+        }
 
         float units[NB], vs[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            units[b] = score_units(scales.k[b], qscale);
-            vs[b] = scales.v[b];
+            units[b] = scales.k(b) * qscale;
+            vs[b] = scales.v(b);
         }
         if (t0 + F::UNIT > min(all_see, end)) {
+            asm volatile("");            // (or every unit does all of this and selects)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
+                units[b] = above_zero(units[b]);
                 if (t0 + 16 * b >= lim) {
                     vs[b] = 0.f;
                     units[b] = FLT_MIN;
@@ -327,7 +337,7 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
         for (int b = 0; b < NB; ++b) {
             const float x = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])) * units[b];
             mx = fmaxf(mx, x);
-            mv = fmaxf(mv, x + above(scales.v[b]));
+            mv = fmaxf(mv, x + above(scales.v(b)));
         }
         mv -= kWeightBits;
         if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax || mv > top + kMoveTop) != 0) {

@@ -25,7 +25,7 @@ struct Tile8Loads {
     static constexpr int LD = TOKENS * CH / kBlock;         // loads of a lane for a tile's keys
     static constexpr int NB = TOKENS / 16;
     int wave;
-    int page[LD], block[NB];                                // of the loads, of the tile's blocks
+    int page[LD];                                           // of the loads
     u32x4_t k[LD], v[LD];
     BlockScales<NB> scales;
 
@@ -40,26 +40,24 @@ struct Tile8Loads {
 
     __device__ __forceinline__ void pages_of(const Paged8Launch& a, const Work& w, int t0) {
 #pragma unroll
-        for (int i = 0; i < LD; ++i) page[i] = block_page(a, w, t0 + block_of(i));
-#pragma unroll
-        for (int b = 0; b < NB; ++b) block[b] = block_page(a, w, t0 + 16 * b);
+        for (int i = 0; i < LD; ++i) page[i] = block_page_ahead(a, w, t0 + block_of(i));
+        scales.pages_of(a, w, t0);
     }
-    // Loads the tile at t0 (whose pages are known), then its successor's pages.
+    // Loads the tile at t0 (whose pages are known), then its successor's pages.  (Lanes
+    // behind the head's channels bring its first ones: queries are 0 there, and outputs are
+    // not stored.)
     __device__ __forceinline__ void issue(const Paged8Launch& a, const Work& w, int t0) {
-        const int c = channel();
+        const int c = channel() < a.D ? channel() : 0;
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const uint32_t off = token(i) % 16 * a.D + c;
-            const int t = t0 + block_of(i);
-            k[i] = u32x4_t{0, 0, 0, 0};
-            v[i] = u32x4_t{0, 0, 0, 0};
-            if (c >= a.D) continue;
+            const int t = t0 + block_of(i), pg = __builtin_amdgcn_readfirstlane(page[i]);
             k[i] = *reinterpret_cast<const u32x4_t*>(
-                block_at<uint8_t>(a, w, a.k_pages, page[i], t) + off);
+                block_at<uint8_t>(a, w, a.k_pages, pg, t) + off);
             v[i] = *reinterpret_cast<const u32x4_t*>(
-                block_at<uint8_t>(a, w, a.v_pages, page[i], t) + off);
+                block_at<uint8_t>(a, w, a.v_pages, pg, t) + off);
         }
-        scales.load(a, w, t0, block);
+        scales.load(a, w, t0);
         pages_of(a, w, t0 + TOKENS);
     }
     // Writes the loaded tile, widened, to LDS.
@@ -137,15 +135,27 @@ struct Tile8Rows {
                 for (int n = NQ - 1; n >= 0; --n) s[tb] = mfma32<kSrcF16>(kf, qf[ks][n], s[tb]);
             }
         }
+        if constexpr (NQ == 1) {
+            // (key vectors three k-steps ahead of their products)
+            constexpr int kReads = M::KS * M::TB, kAhead = 3 * M::TB;
+            __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, kAhead, 0);
+#pragma unroll
+            for (int i = 0; i < kReads - kAhead; ++i) {
+                __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, kAhead, 0);
+        }
         // score i of 32 tokens tb: token 32 tb + 8 (i / 4) + 4 half + i % 4, of block
         // 2 tb + i / 8
         float units[NB], vs[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            units[b] = score_units(sc.k[b], qscale);
-            vs[b] = sc.v[b];
+            units[b] = sc.k(b) * qscale;
+            vs[b] = sc.v(b);
         }
         if (t0 + M::TILE > min(all, end)) {
+            asm volatile("");        // (or every tile does all of this and selects)
 #pragma unroll
             for (int tb = 0; tb < M::TB; ++tb) {
 #pragma unroll
@@ -154,11 +164,13 @@ struct Tile8Rows {
                         s[tb][i] = -INFINITY;
             }
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b) {
+                units[b] = above_zero(units[b]);
                 if (t0 + 16 * b >= lim) {
                     vs[b] = 0.f;
                     units[b] = FLT_MIN;
                 }
+            }
         }
         float mx = -INFINITY, mv = -INFINITY;
 #pragma unroll
@@ -168,7 +180,7 @@ struct Tile8Rows {
             for (int i = 1; i < 8; ++i) x = fmaxf(x, s[b / 2][b % 2 * 8 + i]);
             x *= units[b];
             mx = fmaxf(mx, x);
-            mv = fmaxf(mv, x + above(sc.v[b]));
+            mv = fmaxf(mv, x + above(sc.v(b)));
         }
         mv -= kWeightBits;
         if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax || mv > top + kMoveTop) != 0) {
@@ -215,6 +227,22 @@ struct Tile8Rows {
 #pragma unroll
                 for (int n = NP - 1; n >= 0; --n) O[cb] = mfma32<kSrcF16>(vt, pf[n], O[cb]);
             }
+        }
+        if constexpr (NP == 1) {
+            // A step's products run beside the next one's weights; its values are read a
+            // step ahead.
+            __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 2 * M::CB, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedValu, 36, 0);
+#pragma unroll
+            for (int j = 0; j + 1 < NB; ++j) {
+#pragma unroll
+                for (int cb = 0; cb < M::CB; ++cb) {
+                    __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 2, 0);
+                    __builtin_amdgcn_sched_group_barrier(kSchedValu, 36 / M::CB, 0);
+                }
+            }
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, M::CB, 0);
         }
     }
 };

@@ -76,8 +76,8 @@ def filled_pool8(table, pool, ctx, Hkv, D, page_size, seed, spread=0):
 
 
 def largest_weight(q, k, v_scales, table, ctx, new, page_size, scale):
-    """The largest softmax weight times value scale of each row, ``[T, Hq]`` (k: the
-    keys' values)."""
+    """The largest softmax weight times the largest value scale that each row sees,
+    ``[T, Hq]`` (k: the keys' values)."""
     T, Hq, D = q.shape
     hg = Hq // k.shape[1]
     out, at = torch.zeros(T, Hq, dtype=torch.float64), 0
@@ -90,7 +90,7 @@ def largest_weight(q, k, v_scales, table, ctx, new, page_size, scale):
             for i in range(n):
                 m = c - n + i + 1
                 p = torch.softmax((kk[:m] @ q[at + i, h].double()) * scale, 0)
-                out[at + i, h] = (p * vs[:m]).max()
+                out[at + i, h] = p.max() * vs[:m].max()
         at += n
     return out
 
@@ -99,8 +99,8 @@ def attention8_tolerance(ref, mag, size, largest, D, c, dtype):
     """Each element's bound: the output's rounding (half a step; fp16's numbers below
     2^-14 are 2^-24 apart, so 2^-25 there whatever their size); the weights' rounding for
     the second product, to fp16: half a step at most (2^-11, for fp32 two pieces, 2^-22),
-    and 2^-25 where the largest weight times scale is 2^12 or more, so 2^-37 of that one,
-    for c codes of 127 at most; and fp32: a score is a sum of two products of pieces for
+    and 2^-25 where a row's largest weight (or weight times scale) is 2^12 or more: 2^-37
+    of the largest for c codes of 127 times their scales at most; and fp32: a score is a sum of two products of pieces for
     each of D channels at most, pieces that leave 2^-22 of fp32 queries out, times a
     scale: off by (2 D + 10) 2^-24 of sum |q k| scale, which moves a weight and the
     weights' sum by that much relative each; exp2, the scales and the sums over c

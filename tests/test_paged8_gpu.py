@@ -77,13 +77,13 @@ def test_attention_scale_and_large_scores(hip_device, dtype):
     _check(_attend(case, softmax_scale=1.0), case, 32, scale=1.0)
 
 
-@pytest.mark.parametrize("dtype", [BF, HF, FF], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dtype,spread", [(BF, 3), (BF, 10), (BF, 20), (HF, 3), (HF, 10), (FF, 3),
+                                          (FF, 10), (FF, 20)])
 @pytest.mark.parametrize("n", [1, 70])
-def test_value_blocks_of_any_loudness(hip_device, dtype, n):
-    """Scales of neighbouring blocks up to 2^40 apart (fp16's own range is 2^30
-    wide), and rows whose weights lie on the quiet ones: bounds are relative to what
-    a row sums."""
-    case = _setup([(200, n), (90, n)], 32, dtype, 4, 2, 64, seed=8, spread=10 if dtype is HF else 20)
+def test_value_blocks_of_any_loudness(hip_device, dtype, spread, n):
+    """Scales of neighbouring blocks up to 2^41 apart (fp16's own range is 2^30
+    wide), and rows whose weights lie on the quiet ones."""
+    case = _setup([(200, n), (90, n)], 32, dtype, 4, 2, 64, seed=8, spread=spread)
     table, pool, ctx, new, kc, ks, vc, vs, plan, q = case
     for s in range(2):                 # the louder half of the blocks: keys of tiny scores
         for b in range(-(-ctx[s] // BLOCK)):
