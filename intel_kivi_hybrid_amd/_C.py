@@ -1108,12 +1108,26 @@ def allowed_tokens(mask):
 def _row_list(t, name: str, rows: int, dtypes, dev):
     """A list for each row, ``[rows, n]``, or one for all, ``[n]``: rows any distance
     apart.  Its stride."""
-    _check(isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() in (1, 2)
-           and (t.dim() == 1 or t.shape[0] == rows) and t.device == dev
-           and (t.shape[-1] <= 1 or t.stride(-1) == 1), name, " must be a [", rows,
-           ", n] or [n] tensor of ", " or ".join(_dtype_name(d) for d in dtypes),
-           " with contiguous rows on ", dev)
-    return 0 if t.dim() == 1 else t.stride(0)
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.get_device() == dev:
+        sh, st = t.shape, t.stride()
+        if len(sh) == 2 and sh[0] == rows and (st[1] == 1 or sh[1] <= 1):
+            return st[0]
+        if len(sh) == 1 and (st[0] == 1 or sh[0] <= 1):
+            return 0
+    _fail(name, " must be a [", rows, ", n] or [n] tensor of ",
+          " or ".join(_dtype_name(d) for d in dtypes), " with contiguous rows on ", _DEVICE_TYPE,
+          ":", dev)
+
+
+def _row_setting(value, name: str, rows: int, dtype, dev):
+    """:func:`_setting` of a device's index."""
+    if isinstance(value, torch.Tensor):
+        if not (value.dtype is dtype and value.shape == (rows,) and value.is_contiguous()
+                and value.get_device() == dev):
+            _fail(name, " must be a number or a contiguous [", rows, "] tensor of ",
+                  _dtype_name(dtype), " on ", _DEVICE_TYPE, ":", dev)
+        return value.data_ptr(), 0
+    return 0, value
 
 
 _ID_DTYPES = (torch.int32, torch.int64)
@@ -1145,55 +1159,69 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lengths=0, repetitio
         _fail("logits must be a [rows, vocab] tensor of a float type on ", _DEVICE_TYPE)
     rows, vocab = logits.shape
     _check(vocab > 0, "a row must have logits")
-    _check(logits.stride(1) == 1 or vocab == 1, "a row's logits must be contiguous")
-    dev = logits.device
-    tok = (0, 0, 0, 0)
+    stride = logits.stride()
+    _check(stride[1] == 1 or vocab == 1, "a row's logits must be contiguous")
+    dev = logits.get_device()
+    if not is_current(dev):
+        with on_device(dev):
+            return adjust_logits(logits, tokens, lengths, prompt_lengths, repetition_penalty,
+                                 presence_penalty, frequency_penalty, bias_ids, bias, allowed,
+                                 out)
+    _check_inference(logits, bias, out)
+    tok = length = 0, 0, 0, 0
+    rp, r = _row_setting(repetition_penalty, "repetition_penalty", rows, torch.float32, dev)
+    sp, s = _row_setting(presence_penalty, "presence_penalty", rows, torch.float32, dev)
+    fp, f = _row_setting(frequency_penalty, "frequency_penalty", rows, torch.float32, dev)
+    if rp or sp or fp:
+        _check_inference(*(x for x in (repetition_penalty, presence_penalty, frequency_penalty)
+                           if isinstance(x, torch.Tensor)))
+    if not (rp or r > 0.0):
+        _fail("repetition_penalty must be positive, got ", r)
     if tokens is not None:
-        _check(tokens.dim() == 2, "tokens must be a [", rows, ", n] tensor")
-        st = _row_list(tokens, "tokens", rows, _ID_DTYPES, dev)
-        tok = (tokens.data_ptr(), int(tokens.dtype is torch.int64), st, tokens.shape[1])
-    lp, length = _setting(tok[3] if lengths is None else lengths, "lengths", rows, torch.int32, dev)
-    pp, prompt = _setting(prompt_lengths, "prompt_lengths", rows, torch.int32, dev)
-    length, prompt = _check_int(length, "lengths"), _check_int(prompt, "prompt_lengths")
-    _check(0 <= length <= tok[3], "lengths must lie in [0, ", tok[3], "], got ", length)
-    _check(prompt >= 0, "prompt_lengths must not be negative, got ", prompt)
-    rp, r = _setting(repetition_penalty, "repetition_penalty", rows, torch.float32, dev)
-    sp, s = _setting(presence_penalty, "presence_penalty", rows, torch.float32, dev)
-    fp, f = _setting(frequency_penalty, "frequency_penalty", rows, torch.float32, dev)
-    _check(rp or r > 0.0, "repetition_penalty must be positive, got ", r)
-    _check(tokens is not None or not (rp or sp or fp or r != 1.0 or s != 0.0 or f != 0.0),
-           "penalties need tokens")
-    ids = (0, 0, 0, 0, 0, 0)
+        if not (isinstance(tokens, torch.Tensor) and len(tokens.shape) == 2):
+            _fail("tokens must be a [", rows, ", n] tensor")
+        st, n = _row_list(tokens, "tokens", rows, _ID_DTYPES, dev), tokens.shape[1]
+        tok = tokens.data_ptr(), 1 if tokens.dtype is torch.int64 else 0, st, n
+        lp, length = _row_setting(n if lengths is None else lengths, "lengths", rows, torch.int32,
+                                  dev)
+        pp, prompt = _row_setting(prompt_lengths, "prompt_lengths", rows, torch.int32, dev)
+        length, prompt = _check_int(length, "lengths"), _check_int(prompt, "prompt_lengths")
+        if not 0 <= length <= n:
+            _fail("lengths must lie in [0, ", n, "], got ", length)
+        if prompt < 0:
+            _fail("prompt_lengths must not be negative, got ", prompt)
+        length = lp, length, pp, prompt
+    elif rp or sp or fp or r != 1.0 or s != 0.0 or f != 0.0 or lengths is not None:
+        _fail("penalties need tokens")
+    ids = 0, 0, 0, 0, 0, 0
     if bias_ids is not None or bias is not None:
         _check(bias_ids is not None and bias is not None, "biases need bias_ids and bias")
         ist = _row_list(bias_ids, "bias_ids", rows, _ID_DTYPES, dev)
-        bst = _row_list(bias, "bias", rows, (torch.float32,), dev)
-        _check(bias_ids.shape[-1] == bias.shape[-1], "bias_ids name ", bias_ids.shape[-1],
-               " tokens, bias has ", bias.shape[-1], " values")
-        ids = (bias_ids.data_ptr(), int(bias_ids.dtype is torch.int64), ist, bias.data_ptr(), bst,
-               bias.shape[-1])
-    words = (0, 0)
+        bst, n = _row_list(bias, "bias", rows, (torch.float32,), dev), bias.shape[-1]
+        if bias_ids.shape[-1] != n:
+            _fail("bias_ids name ", bias_ids.shape[-1], " tokens, bias has ", n, " values")
+        ids = (bias_ids.data_ptr(), 1 if bias_ids.dtype is torch.int64 else 0, ist,
+               bias.data_ptr(), bst, n)
+    words = 0, 0
     if allowed is not None:
         st = _row_list(allowed, "allowed", rows, (torch.int32,), dev)
-        _check(allowed.shape[-1] * 32 >= vocab, "allowed has ", allowed.shape[-1],
-               " words for ", vocab, " tokens")
-        words = (allowed.data_ptr(), st)
-    _check_inference(logits, bias, out, *(x for x in (repetition_penalty, presence_penalty,
-                                                      frequency_penalty)
-                                          if isinstance(x, torch.Tensor)))
+        if allowed.shape[-1] * 32 < vocab:
+            _fail("allowed has ", allowed.shape[-1], " words for ", vocab, " tokens")
+        words = allowed.data_ptr(), st
+    code = _IO_DTYPES[logits.dtype]
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+        out = logits.new_empty((rows, vocab))
+        out_code, out_stride = code, vocab
     else:
-        _check(out.dtype in (logits.dtype, torch.float32) and out.shape == logits.shape
-               and (out.stride(1) == 1 or vocab == 1) and out.device == dev, "out must be a [",
-               rows, ", ", vocab, "] tensor of ", _dtype_name(logits.dtype),
-               " or Float with contiguous rows on ", dev)
-    index = dev.index
-    with on_device(index):
-        rc = _lib.kivi_adjust_logits(
-            logits.data_ptr(), _IO_DTYPES[logits.dtype], logits.stride(0), rows, vocab, *tok, lp,
-            length, pp, prompt, rp, r, sp, s, fp, f, *ids, *words, out.data_ptr(),
-            _IO_DTYPES[out.dtype], out.stride(0), stream_handle(index))
+        out_stride = out.stride(0) if len(out.shape) == 2 else 0
+        if not (out.dtype in (logits.dtype, torch.float32) and out.shape == logits.shape
+                and (out.stride(1) == 1 or vocab == 1) and out.get_device() == dev):
+            _fail("out must be a [", rows, ", ", vocab, "] tensor of ", _dtype_name(logits.dtype),
+                  " or Float with contiguous rows on ", logits.device)
+        out_code = _IO_DTYPES[out.dtype]
+    rc = _lib.kivi_adjust_logits(
+        logits.data_ptr(), code, stride[0], rows, vocab, *tok, *length, rp, r, sp, s, fp, f, *ids,
+        *words, out.data_ptr(), out_code, out_stride, stream_handle(dev))
     if rc:
         _native.check(rc, "adjust_logits")
     return out

@@ -10,8 +10,12 @@
 // One launch: a workgroup takes a slice of a row's vocabulary.  It counts the row's tokens
 // that lie in the slice in LDS (whole numbers: in any order the same), adds up the
 // slice's biases there, and goes through its logits once.  Every slice reads all of its
-// row's tokens, from L2.
+// row's tokens, from L2.  The steps wait for each other, and for memory, rather than for
+// operations, so whatever does not depend on a step before it is loaded at the start:
+// logits, mask, biases and the first 16 tokens of each lane.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "kivi_common.hpp"
 #include "../../include/kivi_hip.h"
@@ -19,11 +23,15 @@
 namespace kivi {
 namespace {
 
-constexpr int kBlock = 256;
+// Tokens of a workgroup, as measured (64 rows of 128256 with lists of 4000: workgroups of
+// 256 lanes, 2048 20.8 us, 4096 22.9; 16 rows of 32000 with lists of 30000: of 1024 lanes,
+// 4096 11.5 us).
+constexpr int slice_of(int block) { return block == 256 ? 2048 : 4096; }
 constexpr uint32_t kInPrompt = 1u << 31;     // of a count
 constexpr uint32_t kNoBias = 0xffffffffu;    // (of no sum: NaN is stored as 0x7fc00000)
-constexpr uint32_t kNobody = 0xffffffffu;
 constexpr int kMostEntries = 1 << 30;        // (32-bit indexes look a turn past the last one)
+// Longer lists are read by workgroups of 1024 lanes, shorter ones of 256.
+constexpr int kManyTokens = 8192;
 
 struct AdjustArgs {
     const void* logits;
@@ -43,7 +51,7 @@ struct AdjustArgs {
     int64_t allowed_stride;                  // in bytes
     float repetition, presence, frequency;
     int length, prompt, n_tokens, biases;
-    int vocab, slice, slices, token64, id64;
+    int vocab, slices, token64, id64;
 };
 
 // Eight elements wherever they lie.
@@ -115,64 +123,119 @@ __device__ __forceinline__ int64_t id_at(const void* ids, int64_t i, int wide) {
     return wide ? static_cast<const int64_t*>(ids)[i] : static_cast<const int32_t*>(ids)[i];
 }
 
-// Counts tokens from .. to - 1 of the row that lie in the slice.
-__device__ __forceinline__ void count_tokens(const AdjustArgs& a, int64_t row, int from, int to,
-                                             uint32_t first, uint32_t n, bool prompt,
-                                             uint32_t* counts) {
-    constexpr int kAtOnce = 4;
-    const int64_t base = row * a.token_stride;
-    for (int i = from + threadIdx.x; i < to; i += kAtOnce * kBlock) {
-        int64_t id[kAtOnce];
+// A lane's next ids of a row's list: kLoads loads of 16 bytes, a turn of the workgroup's
+// lanes apart.
+template <int BLOCK, class I>
+struct Ids {
+    static constexpr int kLoads = 16 / sizeof(I) == 2 ? 8 : 4, kEach = 16 / sizeof(I);
+    static constexpr int kTurn = BLOCK * kEach;
+    I id[kLoads][kEach];
+
+    // From `from` on, of `n` in the list; those behind its end are -1.
+    __device__ __forceinline__ void load(const I* ids, int from, int n) {
 #pragma unroll
-        for (int j = 0; j < kAtOnce; ++j)
-            id[j] = id_at(a.tokens, base + min(i + j * kBlock, to - 1), a.token64);
+        for (int j = 0; j < kLoads; ++j) {
+            const int left = n - from - j * kTurn, i = threadIdx.x * kEach;
+            if (left <= 0) continue;
+            const I* at = ids + from + j * kTurn + i;
+            if (i + kEach <= left) {
+                const u4 x = *reinterpret_cast<const loose_u4*>(at);
+                __builtin_memcpy(id[j], &x, 16);
+            } else {
 #pragma unroll
-        for (int j = 0; j < kAtOnce; ++j) {
-            const uint64_t at = (uint64_t)(id[j] - (int64_t)first);
-            if (at >= n || i + j * kBlock >= to) continue;
-            if (prompt) atomicOr(counts + at, kInPrompt);
-            else atomicAdd(counts + at, 1u);
+                for (int k = 0; k < kEach; ++k) id[j][k] = i + k < left ? at[k] : (I)-1;
+            }
         }
     }
-}
+    // Counts those that lie in the slice; the list's first `prompt` are the prompt.
+    __device__ __forceinline__ void count(int from, int length, int prompt, uint32_t first,
+                                          uint32_t n, uint32_t* counts) const {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            if (length - from - j * kTurn <= 0) continue;
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const uint32_t at = (uint32_t)id[j][k] - first;
+                if (at >= n || (sizeof(I) == 8 && (int64_t)id[j][k] >> 32 != 0)) continue;
+                if (from + j * kTurn + (int)threadIdx.x * kEach + k < prompt)
+                    atomicOr(counts + at, kInPrompt);
+                else
+                    atomicAdd(counts + at, 1u);
+            }
+        }
+    }
+};
 
 // The slice's biases, each token's added up in the list's order: of the entries of a turn
-// that name one token the first goes, then the next.  owner: kNobody throughout.
-__device__ __forceinline__ void add_biases(const AdjustArgs& a, int64_t row, uint32_t first,
-                                           uint32_t n, uint32_t* owner, uint32_t* sums) {
-    for (int base = 0; base < a.biases; base += kBlock) {
+// that name one token the first goes, then the next.  owner: 0 throughout, before and
+// after.
+template <int BLOCK>
+struct Biases {
+    int64_t id;
+    float b;
+
+    __device__ __forceinline__ void load(const AdjustArgs& a, int64_t row, int base) {
         const int i = base + threadIdx.x;
-        bool waits = false;
-        uint32_t at = 0;
-        float b = 0.f;
-        if (i < a.biases) {
-            const uint64_t x =
-                (uint64_t)(id_at(a.bias_ids, row * a.id_stride + i, a.id64) - (int64_t)first);
-            waits = x < n;
-            at = (uint32_t)x;
-            if (waits) b = a.bias[row * a.bias_stride + i];
-        }
+        id = -1;
+        b = 0.f;
+        if (i >= a.biases) return;
+        id = id_at(a.bias_ids, row * a.id_stride + i, a.id64);
+        b = a.bias[row * a.bias_stride + i];
+    }
+    __device__ __forceinline__ void add(uint32_t first, uint32_t n, uint32_t* owner,
+                                        uint32_t* sums) const {
+        const uint64_t at = (uint64_t)(id - (int64_t)first);
+        bool waits = at < n;
         while (__syncthreads_or(waits)) {
-            if (waits) atomicMin(owner + at, threadIdx.x);
+            if (waits) atomicMax(owner + at, BLOCK - threadIdx.x);
             __syncthreads();
-            const bool goes = waits && owner[at] == threadIdx.x;
+            const bool goes = waits && owner[at] == BLOCK - threadIdx.x;
             __syncthreads();
             if (goes) {
                 const float s = sums[at] == kNoBias ? b : __uint_as_float(sums[at]) + b;
                 sums[at] = s == s ? __float_as_uint(s) : 0x7fc00000u;
-                owner[at] = kNobody;
+                owner[at] = 0;
                 waits = false;
             }
         }
     }
+};
+
+template <int BLOCK, class I>
+__device__ __forceinline__ void count_all(const AdjustArgs& a, int64_t row, int start, int length,
+                                          int prompt, uint32_t first, uint32_t n,
+                                          Ids<BLOCK, I>& ids, uint32_t* counts) {
+    for (int from = start; from < length;) {
+        ids.count(from, length, prompt, first, n, counts);
+        if (length - from <= Ids<BLOCK, I>::kLoads * Ids<BLOCK, I>::kTurn) break;
+        from += Ids<BLOCK, I>::kLoads * Ids<BLOCK, I>::kTurn;
+        ids.load(static_cast<const I*>(a.tokens) + row * a.token_stride, from, length);
+    }
 }
 
-template <int DT, int OUT>
-__global__ void __launch_bounds__(kBlock) adjust_logits_kernel(AdjustArgs a) {
-    extern __shared__ __align__(16) uint32_t lds[];
+// BIASED: sums of biases in LDS, behind the counts.
+template <int DT, int OUT, int BLOCK, class I, bool BIASED>
+__global__ void __launch_bounds__(BLOCK) adjust_logits_kernel(AdjustArgs a) {
+    constexpr int kSlice = slice_of(BLOCK);
+    static_assert(kSlice <= 8 * BLOCK, "eight logits of a lane");
+    __shared__ __align__(16) uint32_t counts[kSlice];
+    __shared__ __align__(16) uint32_t sums[BIASED ? kSlice : 4];
     const int row = blockIdx.x / a.slices;
-    const uint32_t first = (blockIdx.x - row * a.slices) * (uint32_t)a.slice;
-    const uint32_t n = min((uint32_t)a.slice, (uint32_t)a.vocab - first);
+    const uint32_t first = (blockIdx.x - row * a.slices) * (uint32_t)kSlice;
+    const uint32_t n = min((uint32_t)kSlice, (uint32_t)a.vocab - first);
+
+    const int64_t in = row * a.stride + first, to = row * a.out_stride + first;
+    const uint8_t* allowed =
+        a.allowed == nullptr ? nullptr : a.allowed + row * a.allowed_stride + first / 8;
+    const uint32_t i = 8 * threadIdx.x;
+    const int some = (int)min(8u, n - min(i, n));
+    Eight<DT> x{};
+    uint32_t bits = 0xff;
+    if (some == 8) x.load(a.logits, in + i);
+    else if (some > 0) x.load_some(a.logits, in + i, some);
+    if (some > 0 && allowed != nullptr) bits = allowed[i / 8];
+    Biases<BLOCK> biases;
+    if constexpr (BIASED) biases.load(a, row, 0);
 
     float r = 1.f, p = 0.f, f = 0.f;
     int length = 0, prompt = 0;
@@ -186,59 +249,81 @@ __global__ void __launch_bounds__(kBlock) adjust_logits_kernel(AdjustArgs a) {
         length = min(max(length, 0), a.n_tokens);
         prompt = min(max(prompt, 0), length);
     }
-    const bool counted = length > 0 && (r != 1.f || p != 0.f || f != 0.f);
-    uint32_t* counts = lds;
-    uint32_t* sums = lds + (a.tokens != nullptr || a.biases > 0 ? a.slice : 0);
-    if (a.biases > 0) {
-        for (uint32_t i = threadIdx.x; i < n; i += kBlock) {
-            counts[i] = kNobody;
-            sums[i] = kNoBias;
+    const int start = r != 1.f ? 0 : prompt;
+    const bool counted = start < length && (r != 1.f || p != 0.f || f != 0.f);
+    Ids<BLOCK, I> ids;
+    if (counted) ids.load(static_cast<const I*>(a.tokens) + row * a.token_stride, start, length);
+
+    if (counted || BIASED) {
+        for (uint32_t i = threadIdx.x; i < n; i += BLOCK) {
+            counts[i] = 0;
+            if constexpr (BIASED) sums[i] = kNoBias;
         }
         __syncthreads();
-        add_biases(a, row, first, n, counts, sums);
-        __syncthreads();
+    }
+    if constexpr (BIASED) {
+        biases.add(first, n, counts, sums);
+        for (int base = BLOCK; base < a.biases; base += BLOCK) {
+            biases.load(a, row, base);
+            biases.add(first, n, counts, sums);
+        }
     }
     if (counted) {
-        for (uint32_t i = threadIdx.x; i < n; i += kBlock) counts[i] = 0;
+        count_all<BLOCK, I>(a, row, start, length, prompt, first, n, ids, counts);
         __syncthreads();
-        if (r != 1.f) count_tokens(a, row, 0, prompt, first, n, true, counts);
-        count_tokens(a, row, prompt, length, first, n, false, counts);
     }
-    __syncthreads();
 
-    const int64_t in = row * a.stride + first, to = row * a.out_stride + first;
-    const uint8_t* allowed =
-        a.allowed == nullptr ? nullptr : a.allowed + row * a.allowed_stride + first / 8;
-    for (uint32_t i = 8 * threadIdx.x; i < n; i += 8 * kBlock) {
-        const int some = min(8, (int)(n - i));
-        Eight<DT> x;
-        if (some == 8) x.load(a.logits, in + i);
-        else x.load_some(a.logits, in + i, some);
-        const uint32_t bits = allowed == nullptr ? 0xffu : allowed[i / 8];
-        Eight<OUT> y;
-        if constexpr (DT == OUT) {
-            y = x;
-        } else {
+    if (some == 0) return;
+    Eight<OUT> y;
+    if constexpr (DT == OUT) {
+        y = x;
+    } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y.set(j, x.get(j));
-        }
+        for (int j = 0; j < 8; ++j) y.set(j, x.get(j));
+    }
+    // (few lanes have a token that something concerns)
+    uint32_t c[8], b[8], seen = 0, free = kNoBias;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        // (behind the slice's end LDS holds anything)
+        c[j] = counted && j < some ? counts[i + j] : 0u;
+        b[j] = BIASED && j < some ? sums[i + j] : kNoBias;
+        seen |= c[j];
+        free &= b[j];
+    }
+    if (seen != 0 || free != kNoBias) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            // (behind the slice's end LDS holds anything: some < 8 alone)
-            const bool inside = j < some;
-            const uint32_t c = counted && inside ? counts[i + j] : 0u;
-            const uint32_t b = a.biases > 0 && inside ? sums[i + j] : kNoBias;
             float v = x.get(j);
-            if (c != 0 && r != 1.f) v = v > 0.f ? v / r : v * r;
-            if ((c & ~kInPrompt) != 0) v = v - (f * (float)(c & ~kInPrompt) + p);
-            if (b != kNoBias) v = v + __uint_as_float(b);
-            const bool banned = (bits >> j & 1) == 0;
-            if (banned) v = -__builtin_inff();
-            if (c != 0 || b != kNoBias || banned) y.set(j, v);
+            if (c[j] != 0 && r != 1.f) v = v > 0.f ? v / r : v * r;
+            const uint32_t k = c[j] & ~kInPrompt;
+            if (k != 0) v = v - (f * (float)k + p);
+            if (b[j] != kNoBias) v = v + __uint_as_float(b[j]);
+            if (c[j] != 0 || b[j] != kNoBias) y.set(j, v);
         }
-        if (some == 8) y.store(a.out, to + i);
-        else y.store_some(a.out, to + i, some);
     }
+    if (bits != 0xff) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if ((bits >> j & 1) == 0) y.set(j, -__builtin_inff());
+    }
+    if (some == 8) y.store(a.out, to + i);
+    else y.store_some(a.out, to + i, some);
+}
+
+template <int DT, int OUT>
+void launch(const AdjustArgs& a, unsigned grid, hipStream_t s) {
+    auto with = [&](auto block, auto id) {
+        constexpr int kBlock = decltype(block)::value;
+        using I = decltype(id);
+        if (a.biases > 0) adjust_logits_kernel<DT, OUT, kBlock, I, true><<<grid, kBlock, 0, s>>>(a);
+        else adjust_logits_kernel<DT, OUT, kBlock, I, false><<<grid, kBlock, 0, s>>>(a);
+    };
+    const bool many = a.n_tokens > kManyTokens;
+    if (many && a.token64) with(std::integral_constant<int, 1024>{}, int64_t{});
+    else if (many) with(std::integral_constant<int, 1024>{}, int32_t{});
+    else if (a.token64) with(std::integral_constant<int, 256>{}, int64_t{});
+    else with(std::integral_constant<int, 256>{}, int32_t{});
 }
 
 }  // namespace
@@ -298,25 +383,20 @@ int kivi_adjust_logits(const void* logits, int32_t dtype, int64_t row_stride, in
     a.allowed = reinterpret_cast<const uint8_t*>(allowed);
     a.allowed_stride = 4 * allowed_stride;
     a.vocab = vocab;
-    a.slice = 4096;
-    a.slices = (int)(((int64_t)vocab + a.slice - 1) / a.slice);
+    const bool many = n_tokens > kManyTokens;
+    const int slice = slice_of(many ? 1024 : 256);
+    a.slices = (int)(((int64_t)vocab + slice - 1) / slice);
     const int64_t blocks = (int64_t)rows * a.slices;
-    if (blocks > (int64_t)UINT32_MAX / kBlock)
+    if (blocks > (int64_t)UINT32_MAX / 1024)
         return set_error(kErrInvalidArgument, "%d rows of %d tokens are too many for one launch",
                          rows, vocab);
     const unsigned grid = (unsigned)blocks;
-    const size_t lds = ((a.tokens != nullptr || biases > 0) + (biases > 0)) * (size_t)a.slice * 4;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == kSrcF32)
-        adjust_logits_kernel<kSrcF32, kSrcF32><<<grid, kBlock, lds, s>>>(a);
-    else if (dtype == kSrcBF16 && out_dtype == dtype)
-        adjust_logits_kernel<kSrcBF16, kSrcBF16><<<grid, kBlock, lds, s>>>(a);
-    else if (dtype == kSrcBF16)
-        adjust_logits_kernel<kSrcBF16, kSrcF32><<<grid, kBlock, lds, s>>>(a);
-    else if (out_dtype == dtype)
-        adjust_logits_kernel<kSrcF16, kSrcF16><<<grid, kBlock, lds, s>>>(a);
-    else
-        adjust_logits_kernel<kSrcF16, kSrcF32><<<grid, kBlock, lds, s>>>(a);
+    if (dtype == kSrcF32) launch<kSrcF32, kSrcF32>(a, grid, s);
+    else if (dtype == kSrcBF16 && out_dtype == dtype) launch<kSrcBF16, kSrcBF16>(a, grid, s);
+    else if (dtype == kSrcBF16) launch<kSrcBF16, kSrcF32>(a, grid, s);
+    else if (out_dtype == dtype) launch<kSrcF16, kSrcF16>(a, grid, s);
+    else launch<kSrcF16, kSrcF32>(a, grid, s);
     return check_launch("adjust_logits");
 }
 
