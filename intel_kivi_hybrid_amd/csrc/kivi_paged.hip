@@ -364,7 +364,8 @@ int make_plan(bool eight, int32_t n_seqs, const int32_t* new_lens, const int32_t
                 *block++ = PagedBlock{
                     page_table[s * table_stride + (first >> shift)] * page_size +
                         (first & (page_size - 1)),
-                    tok0[s] + (p - from), p - first, std::min(kScaleBlock, c - first) - (p - first)};
+                    tok0[s] + (p - from), p, (int16_t)(p - first),
+                    (int16_t)(std::min(kScaleBlock, c - first) - (p - first))};
             }
         }
         PagedItem* item = reinterpret_cast<PagedItem*>(plan + items_at);

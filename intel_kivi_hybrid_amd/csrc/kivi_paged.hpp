@@ -51,8 +51,9 @@ constexpr int kScaleBlock = 16;
 struct PagedBlock {
     int32_t slot;        // of its first position
     int32_t tok;         // its first new token among the step's
-    int32_t held;        // positions before that token
-    int32_t n;           // new tokens
+    int32_t position;    // of that token
+    int16_t held;        // positions before it
+    int16_t n;           // new tokens
 };
 
 static_assert(sizeof(PagedItem) == 32 && sizeof(PagedMerge) == 32 && sizeof(PagedBlock) == 16,

@@ -17,9 +17,14 @@
 // definition's code.  It costs nothing that shows beside the memory traffic.  Queries
 // are as in paged_append_kernel.
 //
-// A wave takes a block of a kv head, keys or values: its tokens' rows, read once and held
-// in registers until their largest is known; the scale; and the older codes, read only
-// where the scale grows.
+// A wave takes the tokens of a block of a kv head, keys or values, that fit its lanes
+// (8 of 128 channels; as many waves of a workgroup as that takes share a block and meet
+// once, over the scale): their rows, read once and held in registers until the block's
+// largest is known; the scale; and the older codes, read only where the scale grows.
+// Memory-bound for prompts, with the latency of a wave's steps beside it (9.3K tokens of
+// 32/8 heads of 128 with norms, bf16: 60 us, 3.6 TB/s; blocks alone 27, queries alone 38,
+// as two launches 65; a whole block to a wave, 162 registers in place of 108: 72),
+// launch-bound for single tokens (64 of 64/8 heads, fp16: 5.3 us on the GPU).
 #include <hip/hip_runtime.h>
 
 #include <float.h>
@@ -35,8 +40,8 @@ struct Append8Args {
     float* k_scales;
     float* v_scales;
     const PagedBlock* blocks;
-    uint32_t n_waves;            // blocks x kv heads x 2
-    uint32_t block_wgs;          // workgroups that these take, the first ones
+    uint32_t n_parts;            // blocks x kv heads
+    uint32_t block_wgs;          // workgroups that their keys and values take, the first ones
 };
 
 constexpr int kLeast = -126;     // exponent of the smallest scale
@@ -81,118 +86,121 @@ __device__ __forceinline__ uint2 codes_again(uint2 c, float ratio) {
     return codes_of(x, ratio);
 }
 
-// A block's new rows into it, by a wave; PASSES: how many times its tokens go into 64
-// lanes.  T: what norm and rotation are formed in.
-template <int DT, int PASSES, class T>
+// A block's new rows into it, by WAVES waves (this one's tokens: `part`).  T: what norm
+// and rotation are formed in.  meet(k): the largest of the waves' k.
+template <int DT, int WAVES, class T, class M>
 __device__ __forceinline__ void fill_block(const Append8Args& g, const PagedBlock& b, int kvh,
-                                           bool key) {
+                                           bool key, int part, M meet) {
     const AppendArgs& a = g.a;
-    const int lane = threadIdx.x % kWave, per = kWave >> a.lanes_log2;
+    const int lane = threadIdx.x % kWave;
     const HeadLane l = head_lane(a, lane & ((1 << a.lanes_log2) - 1));
-    const int slot0 = lane >> a.lanes_log2;
+    const int slot = part * (kScaleBlock / WAVES) + (lane >> a.lanes_log2), i = slot - b.held;
     const void* src = key ? a.k : a.v;
     const int64_t st = key ? a.k_st : a.v_st;
-    const int64_t from = b.tok * st + kvh * (key ? a.k_sh : a.v_sh);
+    const int64_t from = (b.tok + i) * st + kvh * (key ? a.k_sh : a.v_sh);
     const void* norm = key ? a.k_norm : nullptr;
-    const bool turned = key && l.live && l.inside;
+    const bool fresh = l.live && i >= 0 && i < b.n, turned = fresh && key && l.inside;
 
     const int64_t page = b.slot >> a.page_shift;
     const int off = b.slot & ((1 << a.page_shift) - 1);
     const int64_t row = ((page * a.Hkv + kvh) << a.page_shift) + off;
-    int8_t* codes = static_cast<int8_t*>(key ? a.k_pages : a.v_pages) + row * a.D;
+    int8_t* codes = static_cast<int8_t*>(key ? a.k_pages : a.v_pages) + row * a.D + slot * a.D;
     float* scale = (key ? g.k_scales : g.v_scales) + row / kScaleBlock;
-    const float old = b.held > 0 ? *scale : 0.f;
 
-    Eight<DT> ex[PASSES], ey[PASSES];
-    Angles at[PASSES];
-    bool fresh[PASSES];
+    Eight<DT> ex{}, ey{};
+    Angles at;
+    if (fresh) {
+        ex.load(src, from + l.c0, a.vec);
+        ey.load(src, from + l.c1, a.vec);
+    }
+    if (turned) at.load(a, l, b.position + i);
+    const float old = b.held > 0 ? *scale : 0.f;
+    T x[8], y[8];
+    {
+        float u[8], w[8];
+        ex.widen(u);
+        ey.widen(w);
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-        const int slot = slot0 + p * per, i = slot - b.held;
-        fresh[p] = l.live && i >= 0 && i < b.n;
-        ex[p] = Eight<DT>{};
-        ey[p] = Eight<DT>{};
-        if (fresh[p]) {
-            ex[p].load(src, from + i * st + l.c0, a.vec);
-            ey[p].load(src, from + i * st + l.c1, a.vec);
-            if (turned) at[p].load(a, l, a.tokens[b.tok + i].y);
+        for (int j = 0; j < 8; ++j) {
+            x[j] = u[j];
+            y[j] = w[j];
         }
     }
-    T x[PASSES][8], y[PASSES][8];
+    if (norm != nullptr) norm_row<T>(a, l, norm, x, y);
+    if (turned) turn_row<T>(a, at, x, y);
     T top = 0;
     bool finite = true;
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-        float u[8], w[8];
-        ex[p].widen(u);
-        ey[p].widen(w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[p][j] = u[j];
-            y[p][j] = w[j];
-        }
-        if (norm != nullptr) norm_row<T>(a, l, norm, x[p], y[p]);
-        if (!fresh[p]) continue;
-        if (turned) turn_row<T>(a, at[p], x[p], y[p]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const T m = x[p][j] < 0 ? -x[p][j] : x[p][j], n = y[p][j] < 0 ? -y[p][j] : y[p][j];
-            finite &= m <= (T)FLT_MAX && n <= (T)FLT_MAX;
-            top = m > top ? m : top;
-            top = n > top ? n : top;
-        }
+    for (int j = 0; j < 8; ++j) {
+        const T m = x[j] < 0 ? -x[j] : x[j], n = y[j] < 0 ? -y[j] : y[j];
+        finite &= m <= (T)FLT_MAX && n <= (T)FLT_MAX;
+        top = m > top ? m : top;
+        top = n > top ? n : top;
     }
-    const int k = wave_max_int(finite ? max(scale_exponent(top), kLeast) : kNotFinite);
+    const int k = meet(wave_max_int(
+        !fresh ? kLeast : finite ? max(scale_exponent(top), kLeast) : kNotFinite));
     // (what a block holds that is not a number keeps it so, until it starts anew)
     float s = k == kNotFinite ? __int_as_float(0x7fc00000) : __int_as_float((k + 127) << 23);
     if (old != old || (s == s && old > s)) s = old;
     const bool number = s == s;
     const T inverse = number ? (T)1 / (T)s : (T)0;
-    if (lane == 0 && __float_as_uint(s) != __float_as_uint(old)) *scale = s;
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-        if (!fresh[p]) continue;
-        int8_t* to = codes + (slot0 + p * per) * a.D;
+    if (part == 0 && lane == 0 && b.n > 0 && __float_as_uint(s) != __float_as_uint(old)) *scale = s;
+    if (fresh) {
         const uint2 zero = make_uint2(0, 0);
-        *reinterpret_cast<uint2*>(to + l.c0) = number ? codes_of(x[p], inverse) : zero;
-        *reinterpret_cast<uint2*>(to + l.c1) = number ? codes_of(y[p], inverse) : zero;
+        *reinterpret_cast<uint2*>(codes + l.c0) = number ? codes_of(x, inverse) : zero;
+        *reinterpret_cast<uint2*>(codes + l.c1) = number ? codes_of(y, inverse) : zero;
     }
-    if (b.held == 0 || !number || s == old) return;
+    if (b.held == 0 || !number || s == old || !l.live || slot >= b.held) return;
     const float ratio = old / s;
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-        const int slot = slot0 + p * per;
-        if (!l.live || slot >= b.held) continue;
-        uint2* to = reinterpret_cast<uint2*>(codes + slot * a.D + l.c0);
-        uint2* too = reinterpret_cast<uint2*>(codes + slot * a.D + l.c1);
-        const uint2 c = *to, d = *too;
-        *to = codes_again(c, ratio);
-        *too = codes_again(d, ratio);
-    }
+    uint2* to = reinterpret_cast<uint2*>(codes + l.c0);
+    uint2* too = reinterpret_cast<uint2*>(codes + l.c1);
+    const uint2 c = *to, d = *too;
+    *to = codes_again(c, ratio);
+    *too = codes_again(d, ratio);
 }
 
-template <int DT, int PASSES>
-__global__ void __launch_bounds__(kAppendBlock) paged8_append_kernel(Append8Args g) {
-    const AppendArgs& a = g.a;
-    if (blockIdx.x < g.block_wgs) {
-        const uint32_t w = blockIdx.x * (kAppendBlock / kWave) +
-                           __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-        if (w >= g.n_waves) return;
-        const uint32_t half = w / (uint32_t)a.Hkv;
-        const int kvh = (int)(w - half * (uint32_t)a.Hkv);
-        const PagedBlock b = g.blocks[half / 2];
-        const bool key = half % 2 == 0;
-        if (key && (a.k_norm != nullptr || a.rot > 0)) fill_block<DT, PASSES, double>(g, b, kvh, true);
-        else fill_block<DT, PASSES, float>(g, b, kvh, key);
-        return;
-    }
-    const uint32_t t = (blockIdx.x - g.block_wgs) * kAppendBlock + threadIdx.x;
+// Query rows of workgroup `wg`, a segment of lanes each.
+template <int DT>
+__device__ __forceinline__ void move_query(const AppendArgs& a, uint32_t wg) {
+    const uint32_t t = wg * kAppendBlock + threadIdx.x;
     const uint32_t row = t >> a.lanes_log2;
     const int tok = (int)(row / (uint32_t)a.Hq), h = (int)(row - (uint32_t)tok * (uint32_t)a.Hq);
     if (tok >= a.n_tokens) return;                       // (whole segments leave)
     move_row<DT>(a, head_lane(a, (int)(t & ((1u << a.lanes_log2) - 1))), a.q,
                  tok * a.q_st + (int64_t)h * a.q_sh, a.q_norm, true, a.tokens[tok].y, a.q_out,
                  ((int64_t)tok * a.Hq + h) * a.D);
+}
+
+template <int DT, int WAVES>
+__global__ void __launch_bounds__(kAppendBlock) paged8_append_kernel(Append8Args g) {
+    constexpr int kParts = kAppendBlock / kWave / WAVES;      // blocks of a workgroup
+    const AppendArgs& a = g.a;
+    if (blockIdx.x < g.block_wgs) {
+        __shared__ int largest[kAppendBlock / kWave];
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+        // (keys by the first half of the workgroups, values by the others)
+        const bool key = blockIdx.x < g.block_wgs / 2;
+        const uint32_t p = (blockIdx.x - (key ? 0 : g.block_wgs / 2)) * kParts + wave / WAVES;
+        const uint32_t at = min(p, g.n_parts - 1), block = at / (uint32_t)a.Hkv;
+        const int kvh = (int)(at - block * (uint32_t)a.Hkv);
+        PagedBlock b = g.blocks[block];
+        if (p >= g.n_parts) b.n = b.held = 0;
+        auto meet = [&](int k) {
+            if constexpr (WAVES > 1) {
+                largest[wave] = k;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < WAVES; ++i) k = max(k, largest[wave / WAVES * WAVES + i]);
+            }
+            return k;
+        };
+        if (key && (a.k_norm != nullptr || a.rot > 0))
+            fill_block<DT, WAVES, double>(g, b, kvh, true, wave % WAVES, meet);
+        else
+            fill_block<DT, WAVES, float>(g, b, kvh, key, wave % WAVES, meet);
+        return;
+    }
+    move_query<DT>(a, blockIdx.x - g.block_wgs);
 }
 
 template <int DT>
@@ -232,12 +240,14 @@ int kivi_paged8_append(const void* q, int64_t q_token_stride, int64_t q_head_str
     g.k_scales = k_scales;
     g.v_scales = v_scales;
     g.blocks = reinterpret_cast<const PagedBlock*>(plan + info[kInfoBlocksAt]);
-    const int64_t waves = info[kInfoBlocks] * kv_heads * 2;
+    const int64_t parts = info[kInfoBlocks] * kv_heads;
     const int64_t lanes = (int64_t)a.n_tokens * a.Hq << a.lanes_log2;
-    const int64_t wgs = (waves + kAppendBlock / kWave - 1) / (kAppendBlock / kWave);
-    if (waves * kWave > INT32_MAX || lanes > INT32_MAX)
+    // waves of a block: 16 tokens in 64 lanes
+    const int waves = a.lanes_log2 <= 2 ? 1 : 1 << (a.lanes_log2 - 2);
+    const int64_t wgs = (parts * waves + kAppendBlock / kWave - 1) / (kAppendBlock / kWave) * 2;
+    if (parts * waves * kWave > INT32_MAX / 2 || lanes > INT32_MAX)
         return set_error(kErrInvalidArgument, "%d tokens are too many for one launch", a.n_tokens);
-    g.n_waves = (uint32_t)waves;
+    g.n_parts = (uint32_t)parts;
     g.block_wgs = (uint32_t)wgs;
     const unsigned grid = (unsigned)(wgs + (lanes + kAppendBlock - 1) / kAppendBlock);
     hipStream_t s = (hipStream_t)stream;

@@ -41,7 +41,9 @@ def test_blocks_hold_every_new_token_once(lens, page_size):
     before = [c - n for c, n in zip(ctx, new) for _ in range(n)]
     slots = slots_of(table, ctx, new, page_size)
     got = []
-    for slot, tok, held, n in blocks.tolist():
+    for slot, tok, first, packed in blocks.tolist():
+        held, n = packed & 0xffff, packed >> 16
+        assert first == slots[tok][2]
         assert slot % 16 == 0 and 0 <= held and n >= 1 and held + n <= 16
         for i in range(n):
             page, off, pos = slots[tok + i]
