@@ -106,6 +106,7 @@ struct Tile {
 struct Cut {
     size_t whole;
     int64_t length;
+    int64_t end;                 // when the last piece ends, in positions
     int64_t pieces(size_t tile, int64_t len) const {
         return tile < whole ? 1 : std::max<int64_t>(1, (len + length - 1) / length);
     }
@@ -116,17 +117,22 @@ struct Cut {
 struct Costs {
     int64_t start, partial_row, merge;
 };
-constexpr Costs paged_costs(int kind) {
-    // (fp32's products of 64 rows take four times as long for a position)
-    return kind == kFew64 ? Costs{16, 1, 24} : Costs{64, 4, 96};
+constexpr Costs paged_costs(int kind, bool eight) {
+    // (fp32's products of 64 rows take four times as long for a position; the eight waves
+    // of kWide8 write twice the rows in the time of one)
+    return kind != kFew64 ? Costs{64, 4, 96} : eight ? Costs{64, 2, 96} : Costs{16, 1, 24};
 }
+
+// Pages of 8 bits: a position's time in tiles of 256 rows (one workgroup on a CU), in
+// hundredths of its time in tiles of 128 (two), and the positions on the longest way from
+// which on they are taken.
+constexpr int64_t kWideCost = 93, kWideFrom = 2048;
 
 // The cut whose items, dealt in order to `machines` workgroups as these come
 // free, end first.
 Cut best_cut(const std::vector<Tile>& tiles, const std::vector<int>& rows, int64_t machines,
              Costs cost) {
-    Cut best{tiles.size(), 64};
-    int64_t best_end = INT64_MAX;
+    Cut best{tiles.size(), 64, INT64_MAX};
     const int64_t longest = tiles.empty() ? 0 : tiles.front().end;
     std::vector<int64_t> busy;                    // a heap: when each comes free
     const size_t rounds = tiles.size() / (size_t)machines * (size_t)machines;
@@ -135,14 +141,14 @@ Cut best_cut(const std::vector<Tile>& tiles, const std::vector<int>& rows, int64
         if (n > 1 && T < 128) break;
         // (with whole rounds of tiles first, only the rest is cut)
         for (int keep = 0; keep < (n > 1 && rounds > 0 ? 2 : 1); ++keep) {
-            const Cut cut{keep ? rounds : 0, T};
+            Cut cut{keep ? rounds : 0, T, 0};
             int64_t items = 0;
             for (size_t i = 0; i < tiles.size(); ++i) items += cut.pieces(i, tiles[i].end);
             if (n > 1 && items > 4 * machines) continue;
             busy.assign((size_t)machines, 0);
-            int64_t end = 0;
+            int64_t& end = cut.end;
             bool merge = false;
-            for (size_t i = 0; i < tiles.size() && end < best_end; ++i) {
+            for (size_t i = 0; i < tiles.size() && end < best.end; ++i) {
                 const int64_t k = cut.pieces(i, tiles[i].end);
                 merge |= k > 1;
                 const int64_t each =
@@ -155,10 +161,7 @@ Cut best_cut(const std::vector<Tile>& tiles, const std::vector<int>& rows, int64
                 }
             }
             if (merge) end += cost.merge;
-            if (end < best_end) {
-                best_end = end;
-                best = cut;
-            }
+            if (end < best.end) best = cut;
         }
     }
     return best;
@@ -262,34 +265,53 @@ int make_plan(bool eight, int32_t n_seqs, const int32_t* new_lens, const int32_t
         if (large && !f32) few = kMany;
         if (large && f32 && small <= (1 << 23) / head_dim / kv_heads) few = kFew64;
         std::vector<Tile> tiles[kPagedKinds];
-        for (int s = 0; s < n_seqs; ++s) {
+        auto add_tiles = [&](int s, int kind) {
             const int64_t n = new_lens[s], rows = n * hg;
-            if (n == 0) continue;
-            const int kind = std::max(few, paged_kind(rows, f32));
-            const int step = paged_tile_rows(kind);
+            const int step = paged_tile_rows(kind, eight);
             for (int64_t r = 0; r < rows; r += step) {
                 const int64_t last = std::min(rows, r + step) - 1;
                 tiles[kind].push_back({s, (int)r, context_lens[s] - n + last / hg + 1});
             }
+        };
+        for (int s = 0; s < n_seqs; ++s) {
+            const int64_t rows = (int64_t)new_lens[s] * hg;
+            if (rows > 0) add_tiles(s, std::max(few, paged_kind(rows, f32)));
         }
         auto tile_rows = [&](const Tile& t, int kind) {
-            return (int)std::min<int64_t>(paged_tile_rows(kind),
+            return (int)std::min<int64_t>(paged_tile_rows(kind, eight),
                                           (int64_t)new_lens[t.seq] * hg - t.row0);
         };
-        auto is_few = [&](const Tile& t) { return paged_few((int64_t)new_lens[t.seq] * hg); };
-        Cut cuts[kPagedKinds];
-        int64_t items = 0, merges = 0, parts = 0, part_rows = 0, kinds[kPagedKinds] = {0, 0, 0, 0};
-        int64_t few_parts = 0, few_rows = 0;
-        for (int kind = 0; kind < kPagedKinds; ++kind) {
+        auto cut_tiles = [&](int kind) {
             // longest first: the last workgroups to start are short ones
             std::vector<Tile>& of = tiles[kind];
             std::stable_sort(of.begin(), of.end(),
                              [](const Tile& a, const Tile& b) { return a.end > b.end; });
             std::vector<int> rows;
             for (const Tile& t : of) rows.push_back(tile_rows(t, kind));
-            const int64_t slots = paged_slots(kind, head_dim);
-            cuts[kind] = best_cut(of, rows, std::max<int64_t>(1, slots / kv_heads),
-                                  paged_costs(kind));
+            const int64_t slots = paged_slots(kind, head_dim, eight);
+            return best_cut(of, rows, std::max<int64_t>(1, slots / kv_heads),
+                            paged_costs(kind, eight));
+        };
+        Cut cuts[kPagedKinds];
+        for (int kind = 0; kind < kPagedKinds; ++kind) cuts[kind] = cut_tiles(kind);
+        // Tiles of 256 rows, whose eight waves share the widening of a tile of codes, where by
+        // these costs they end first (bf16, heads of 128, in tiles of 256 and of 128 rows: a
+        // chunk of 2048 tokens after 8200, 32/8 heads, 348 and 373 us; 400 after 30000, 32/32,
+        // 255 and 289; four of 256 after 3000, 32/8, 72 and 75; 520 after 8000, 32/32, whose
+        // third tile is nearly empty, 135 and 117; shorter ways, as eight of 256 after
+        // 1000, 32/32: 50 and 44).  Sequences of few rows would need a launch of their own.
+        if (eight && large && small == 0 && paged_wide(dtype == 0, head_dim) &&
+            cuts[kMany].end >= kWideFrom) {
+            for (int s = 0; s < n_seqs; ++s)
+                if (new_lens[s] > 0) add_tiles(s, kWide8);
+            cuts[kWide8] = cut_tiles(kWide8);
+            tiles[cuts[kWide8].end * kWideCost < cuts[kMany].end * 100 ? kMany : kWide8].clear();
+        }
+        auto is_few = [&](const Tile& t) { return paged_few((int64_t)new_lens[t.seq] * hg); };
+        int64_t items = 0, merges = 0, parts = 0, part_rows = 0, kinds[kPagedKinds] = {0, 0, 0, 0};
+        int64_t few_parts = 0, few_rows = 0;
+        for (int kind = 0; kind < kPagedKinds; ++kind) {
+            const std::vector<Tile>& of = tiles[kind];
             for (size_t i = 0; i < of.size(); ++i) {
                 const int64_t splits = cuts[kind].pieces(i, of[i].end);
                 items += splits;
@@ -297,10 +319,10 @@ int make_plan(bool eight, int32_t n_seqs, const int32_t* new_lens, const int32_t
                 if (splits == 1) continue;
                 merges += 1;
                 parts += splits;
-                part_rows = std::max<int64_t>(part_rows, rows[i]);
+                part_rows = std::max<int64_t>(part_rows, tile_rows(of[i], kind));
                 if (!is_few(of[i])) continue;
                 few_parts += splits;
-                few_rows = std::max<int64_t>(few_rows, rows[i]);
+                few_rows = std::max<int64_t>(few_rows, tile_rows(of[i], kind));
             }
         }
         const int64_t pages_at = 2 * tokens, items_at = (pages_at + pages + 7) / 8 * 8;

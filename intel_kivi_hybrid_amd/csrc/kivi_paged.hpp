@@ -60,10 +60,20 @@ static_assert(sizeof(PagedItem) == 32 && sizeof(PagedMerge) == 32 && sizeof(Page
               "plan records");
 
 // Kinds of attention items: kind k takes 16 << k rows (none 32), and is one launch
-// (kFew64: fp32, kMany: the 16-bit types).
-enum PagedKind : int { kFew16 = 0, kFew64 = 2, kMany = 3, kPagedKinds = 4 };
+// (kFew64: fp32, kMany: the 16-bit types; pages of 8 bits have kMany for all types and, in
+// kFew64's place, kWide8 of 256 rows).
+enum PagedKind : int { kFew16 = 0, kWide8 = 2, kFew64 = 2, kMany = 3, kPagedKinds = 4 };
 
-constexpr int paged_tile_rows(int kind) { return 16 << kind; }
+constexpr int paged_tile_rows(int kind, bool eight = false) {
+    return eight && kind == kWide8 ? 256 : 16 << kind;
+}
+// Whether pages of 8 bits have tiles of 256 rows.  (In fp32 and above 128 channels a
+// wave's registers are too many for eight waves; up to 96 channels, where more of 128 rows
+// fit a CU, they lose: 64 channels, 12/12 heads, four chunks of 1024 after 3000, 95 and
+// 77 us; 96 channels, 16/4 heads, four of 256, 47 and 44.)
+constexpr bool paged_wide(bool f32, int head_dim) {
+    return !f32 && head_dim > 96 && head_dim <= 128;
+}
 
 // The kind that takes `rows` rows of a kv head: fp32 has kernels of 16 and 64 rows,
 // the 16-bit types of 16 and 128.  Up to 16 rows a kernel that streams them is
@@ -81,8 +91,9 @@ constexpr bool paged_few(int64_t rows) { return rows <= paged_tile_rows(kFew16);
 // Workgroups that the card works on at once: 256 CUs, and as many on each as the
 // kernels' registers or LDS leave room for (fp32's 64 rows: as bring more; more
 // than that share the matrix cores that bound it).
-constexpr int paged_slots(int kind, int head_dim) {
-    const int per_cu = kind == kMany    ? (head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1)
+constexpr int paged_slots(int kind, int head_dim, bool eight = false) {
+    const int per_cu = eight && kind == kWide8 ? 1
+                       : kind == kMany  ? (head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1)
                        : kind == kFew16 ? (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1)
                                         : 2;
     return 256 * per_cu;

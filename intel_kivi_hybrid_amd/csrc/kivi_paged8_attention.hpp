@@ -415,6 +415,6 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
 }  // namespace
 
 void launch_paged8_few(const Paged8Launch& a, int dtype, hipStream_t s);
-void launch_paged8_many(const Paged8Launch& a, int dtype, hipStream_t s);
+void launch_paged8_many(const Paged8Launch& a, int dtype, bool wide, hipStream_t s);
 
 }  // namespace kivi

@@ -1,11 +1,19 @@
 // Attention over pages of 8 bits for more than 16 query rows per kv head: chunks of
 // prompts, verification passes.
 //
-// As kivi_paged_many.hip: a workgroup takes 128 rows of a kv head, 32 for each of its four
-// waves (v_mfma_f32_32x32x16), and walks the positions in tiles of 64 (32 above 128
-// channels) in two LDS buffers.  A tile's codes are loaded into registers while the one
-// before is computed, widened there once for all four waves and written to the other
-// buffer: one barrier per tile.
+// As kivi_paged_many.hip: a workgroup takes 128 rows of a kv head (256 where the plan says
+// so), 32 for each of its four (eight) waves (v_mfma_f32_32x32x16), and walks the positions
+// in tiles of 64 (32 above 128 channels) in two LDS buffers.  A tile's codes are loaded
+// into registers while the one before is computed, widened there once for all waves and
+// written to the other buffer: one barrier per tile.
+//
+// What bounds it is the sum of two units: a SIMD's two waves do not hide a product behind
+// the other's vector instructions (32 products of 16.4 ns and about 390 instructions of 1.4
+// for a wave's tile of 64 positions at 128 channels; the products alone are two thirds of
+// the time).  Hence little else is done per score: one multiply-add, one exponential, one
+// sum, half a packing; scales enter once per block of 16 positions.  A chunk of 2048
+// tokens after 8200, 32/8 heads of 128, bf16: 348 us in tiles of 256 rows (890 TFLOP/s), 373
+// in tiles of 128; sixteen times five tokens after 3000, 28/4 heads: 24 us.
 #include <hip/hip_runtime.h>
 
 #include "kivi_paged8_attention.hpp"
@@ -14,13 +22,11 @@
 namespace kivi {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kBlock = kWaves * kWave;
-
 // How a workgroup's lanes load a tile: a lane takes 16 channels of a token.
-template <int DP, int TOKENS>
+template <int DP, int TOKENS, int WAVES>
 struct Tile8Loads {
     using M = TileShape<DP, TOKENS>;
+    static constexpr int kBlock = WAVES * kWave;
     static constexpr int CH = M::SL / 2;                    // lanes of a token
     static constexpr int LD = TOKENS * CH / kBlock;         // loads of a lane for a tile's keys
     static constexpr int NB = TOKENS / 16;
@@ -247,8 +253,8 @@ struct Tile8Rows {
     }
 };
 
-template <int DT, int DP>
-__global__ void __launch_bounds__(kBlock, DP <= 128 && DT != kSrcF32 ? 2 : 1)
+template <int DT, int DP, int WAVES>
+__global__ void __launch_bounds__(WAVES * kWave, DP <= 128 && DT != kSrcF32 && WAVES == 4 ? 2 : 1)
     paged8_many_kernel(Paged8Launch a) {
     constexpr int kTile = DP <= 128 ? 64 : 32;
     using M = TileShape<DP, kTile>;
@@ -260,17 +266,19 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 && DT != kSrcF32 ? 2 : 1)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, col = lane % 32, half = lane / 32;
     const Work w = work_of(a);
-    if (w.rows <= paged_tile_rows(kFew16)) {
-        few8_rows<DT, DP>(a, w, [&](int i) {
-            return (i < 2 ? buf0 : buf1) + i % 2 * Few8<DP>::WAVE_BYTES;
-        }, join);
-        return;
+    if constexpr (WAVES == kFew8Waves) {
+        if (w.rows <= paged_tile_rows(kFew16)) {
+            few8_rows<DT, DP>(a, w, [&](int i) {
+                return (i < 2 ? buf0 : buf1) + i % 2 * Few8<DP>::WAVE_BYTES;
+            }, join);
+            return;
+        }
     }
     const int end = w.it.kv_end;
     using R = Tile8Rows<DT, DP, kTile>;
     R rows;
     rows.init(a, w, w.it.row0 + 32 * wave);
-    Tile8Loads<DP, kTile> loads;
+    Tile8Loads<DP, kTile, WAVES> loads;
     loads.wave = wave;
 
     int t0 = w.it.kv_begin;
@@ -318,21 +326,32 @@ __global__ void __launch_bounds__(kBlock, DP <= 128 && DT != kSrcF32 ? 2 : 1)
         *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(rows.m, l);
 }
 
-template <int DT>
-void launch_dim(const Paged8Launch& a, hipStream_t s) {
+template <int DT, int DP>
+void launch_waves(const Paged8Launch& a, bool wide, hipStream_t s) {
     const dim3 grid((unsigned)(a.n_items * a.Hkv));
-    if (a.D <= 64) paged8_many_kernel<DT, 64><<<grid, kBlock, 0, s>>>(a);
-    else if (a.D <= 96) paged8_many_kernel<DT, 96><<<grid, kBlock, 0, s>>>(a);
-    else if (a.D <= 128) paged8_many_kernel<DT, 128><<<grid, kBlock, 0, s>>>(a);
-    else paged8_many_kernel<DT, 256><<<grid, kBlock, 0, s>>>(a);
+    if constexpr (DP == 128 && DT != kSrcF32) {
+        if (wide) {
+            paged8_many_kernel<DT, DP, 8><<<grid, 8 * kWave, 0, s>>>(a);
+            return;
+        }
+    }
+    paged8_many_kernel<DT, DP, 4><<<grid, 4 * kWave, 0, s>>>(a);
+}
+
+template <int DT>
+void launch_dim(const Paged8Launch& a, bool wide, hipStream_t s) {
+    if (a.D <= 64) launch_waves<DT, 64>(a, wide, s);
+    else if (a.D <= 96) launch_waves<DT, 96>(a, wide, s);
+    else if (a.D <= 128) launch_waves<DT, 128>(a, wide, s);
+    else launch_waves<DT, 256>(a, wide, s);
 }
 
 }  // namespace
 
-void launch_paged8_many(const Paged8Launch& a, int dtype, hipStream_t s) {
-    if (dtype == kSrcF32) launch_dim<kSrcF32>(a, s);
-    else if (dtype == kSrcBF16) launch_dim<kSrcBF16>(a, s);
-    else launch_dim<kSrcF16>(a, s);
+void launch_paged8_many(const Paged8Launch& a, int dtype, bool wide, hipStream_t s) {
+    if (dtype == kSrcF32) launch_dim<kSrcF32>(a, wide, s);
+    else if (dtype == kSrcBF16) launch_dim<kSrcBF16>(a, wide, s);
+    else launch_dim<kSrcF16>(a, wide, s);
 }
 
 }  // namespace kivi

@@ -218,13 +218,13 @@ int kivi_paged8_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     if (rc || a.Hq == 0) return rc;
     if (k_scales == nullptr || v_scales == nullptr)
         return set_error(kErrInvalidArgument, "null scales");
-    if (info[kInfoItems + kFew64] != 0)
+    if (info[kInfoItems + kWide8] != 0 && !paged_wide(dtype == kSrcF32, head_dim))
         return set_error(kErrInvalidArgument, "the plan is not one of kivi_paged8_plan");
     a.k_scales = k_scales;
     a.v_scales = v_scales;
     hipStream_t s = (hipStream_t)stream;
     return run_items(a, dtype, plan, info, s, [&](int kind) {
-        if (kind == kMany) launch_paged8_many(a, dtype, s);
+        if (kind == kMany || kind == kWide8) launch_paged8_many(a, dtype, kind == kWide8, s);
         else launch_paged8_few(a, dtype, s);
     });
 }

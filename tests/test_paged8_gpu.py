@@ -71,6 +71,23 @@ def test_attention_against_float64(hip_device, shape, dtype):
     _check(_attend(case), case, page)
 
 
+WIDE = [([(3900, 512)], 64, 64, 32, 128),              # each split in two
+        ([(1100, 340), (2100, 341), (2003, 511), (1500, 171)], 16, 96, 32, 112)]
+
+
+@pytest.mark.parametrize("shape", WIDE, ids=range(len(WIDE)))
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "f16"])
+def test_tiles_of_256_rows(hip_device, shape, dtype):
+    """Three kv heads of them against float64."""
+    lens, page, Hq, Hkv, D = shape
+    case = _setup(lens, page, dtype, Hq, Hkv, D, seed=3)
+    assert case[-2]._info[8] > 0 and case[-2]._info[9] == 0
+    heads = [0, 1, Hkv - 1]
+    rows = [h * (Hq // Hkv) + i for h in heads for i in range(Hq // Hkv)]
+    few = case[:4] + tuple(t[:, heads] for t in case[4:8]) + (None, case[-1][:, rows])
+    _check(_attend(case)[:, rows], few, page)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, FF], ids=["bf16", "f16", "f32"])
 def test_attention_scale_and_large_scores(hip_device, dtype):
     case = _setup([(100, 20), (700, 1)], 32, dtype, 8, 2, 64, seed=5)

@@ -69,6 +69,17 @@ def test_fp32_rows_go_into_the_tiles_of_the_16_bit_types():
     assert info[8] == 0 and info[9] > 0
 
 
+@pytest.mark.parametrize("lens,dtype,dim,wide", [
+    ([(8200, 2048)], torch.bfloat16, 128, True), ([(8200, 2048)], torch.float32, 128, False),
+    ([(8200, 2048)], torch.float16, 64, False), ([(8200, 2048), (700, 1)], torch.float16, 128, False),
+    ([(100, 256)], torch.bfloat16, 128, False), ([(30000, 100)] * 2, torch.float16, 112, True)])
+def test_long_chunks_of_128_channels_are_in_tiles_of_256_rows(lens, dtype, dim, wide):
+    """Unless sequences of few rows are beside them."""
+    table, pool, ctx, new = make_table(lens, 64, seed=3)
+    info = _plan(table, pool, ctx, new, 64, dtype, 32, 8, dim)[1]
+    assert (info[8] > 0) == wide and (info[9] > 0) == (not wide)
+
+
 def test_a_block_of_two_sequences_is_refused():
     """Disjoint slots of one page are fine in pages of the model's type; here each
     sequence would rescale the other's tokens."""
@@ -105,7 +116,8 @@ def test_entry_points_reject_bad_arguments():
     assert "softmax_scale must be positive" in attend(scale=-1.0)
     assert "null pointer" in attend(q=None)
     assert "null scales" in attend(ks=None)
-    info[8] = 1
+    info[8] = 1                                  # (tiles of 256 rows: 16 bits, 128 channels)
+    assert "not one of kivi_paged8_plan" in attend(dtype=0)
     assert "not one of kivi_paged8_plan" in attend()
     info[8] = 0
     info[6] = 1 << 24
