@@ -504,9 +504,10 @@ int kivi_paged8_append(const void* q, int64_t q_token_stride, int64_t q_head_str
                        const void* k_norm, int32_t norm_dtype, float eps, void* stream);
 
 /* kivi_paged_attention over pages of 8 bits (its workspace function, with the info of
- * kivi_paged8_plan).  Codes enter the products exactly; weights times value scales are
- * rounded to bf16 (fp16 for f16 queries and more than 16 rows to a kv head), in two
- * pieces for up to 16 rows and three for f32, whose queries enter in three pieces too.
+ * kivi_paged8_plan).  Codes enter the products exactly; queries and weights times value
+ * scales as fp16, in units of a power of two of each row's own that keep the largest
+ * within fp16's range (f32 queries, their weights, and those of a sequence with up to 16
+ * rows to a kv head in two pieces).  Scores, softmax and sums are f32.
  * A row that sees a position of a block whose scale is NaN comes out as NaN; scales of
  * blocks that it sees nothing of do not reach it. */
 int kivi_paged8_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
