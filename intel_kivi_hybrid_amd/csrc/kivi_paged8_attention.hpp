@@ -52,7 +52,11 @@ __device__ __forceinline__ u32x4_t operand_of_codes(uint32_t x, uint32_t y) {
 // Two values as fp16 pieces: rounded, and what that left out.
 struct Pieces { uint32_t hi, lo; };
 __device__ __forceinline__ Pieces split_f16(float a, float b) {
-    const uint32_t hi = pack2<kSrcF16>(a, b);
+    uint32_t hi = pack2<kSrcF16>(a, b);
+    // (What is taken off must be the word that is multiplied: of a product the compiler
+    // otherwise rounds it a second time, from the exact product, and one in 2^13 of
+    // those lies on the other side of a border.)
+    asm("" : "+v"(hi));
     const f16x2_t h = __builtin_bit_cast(f16x2_t, hi);
     return {hi, pack2<kSrcF16>(fmaf((float)h[0], -1.0f, a), fmaf((float)h[1], -1.0f, b))};
 }

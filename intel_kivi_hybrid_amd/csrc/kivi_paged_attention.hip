@@ -153,7 +153,7 @@ int run_items(L& a, int dtype, const int32_t* plan, const int64_t* info, hipStre
         a.items = items + before;
         a.n_items = (int)info[kInfoItems + kind];
         if (a.n_items == 0) continue;
-        if ((int64_t)a.n_items * a.Hkv > kMostBlocks)
+        if ((int64_t)a.n_items * a.Hkv > kMostBlocks / (kind == kWide8 ? 2 : 1))
             return set_error(kErrInvalidArgument, "%d items are too many for one launch",
                              a.n_items);
         launch(kind);

@@ -94,6 +94,17 @@ def test_attention_scale_and_large_scores(hip_device, dtype):
     _check(_attend(case, softmax_scale=1.0), case, 32, scale=1.0)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF, FF], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("lens", [[(0, 8)] * 40, [(7, 1)] * 200], ids=["many", "few"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_pieces_make_up_their_weight(hip_device, D, lens, dtype):
+    """A hundred thousand weights of rows of a few positions and small scores, whose
+    bound leaves no room for a weight whose second piece belongs to another rounding
+    of it (one in 2^13 lies that near a border)."""
+    case = _setup(lens, 16, dtype, 64, 8, D, seed=21)
+    _check(_attend(case, softmax_scale=2.0 ** -9), case, 16, scale=2.0 ** -9)
+
+
 @pytest.mark.parametrize("dtype,spread", [(BF, 3), (BF, 10), (BF, 20), (HF, 3), (HF, 10), (FF, 3),
                                           (FF, 10), (FF, 20)])
 @pytest.mark.parametrize("n", [1, 70])
