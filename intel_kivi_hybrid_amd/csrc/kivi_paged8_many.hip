@@ -12,7 +12,7 @@
 // for a wave's tile of 64 positions at 128 channels; the products alone are two thirds of
 // the time).  Hence little else is done per score: one multiply-add, one exponential, one
 // sum, half a packing; scales enter once per block of 16 positions.  A chunk of 2048
-// tokens after 8200, 32/8 heads of 128, bf16: 348 us in tiles of 256 rows (890 TFLOP/s), 373
+// tokens after 8200, 32/8 heads of 128, bf16: 345 us in tiles of 256 rows (900 TFLOP/s), 373
 // in tiles of 128; sixteen times five tokens after 3000, 28/4 heads: 24 us.
 #include <hip/hip_runtime.h>
 

@@ -12,6 +12,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "kivi_paged8_attention.hpp"
 #include "../../include/kivi_hip.h"
 
@@ -19,7 +21,8 @@ namespace kivi {
 namespace {
 
 constexpr int kMergeBlock = 256;
-// (a launch has fewer than 2^32 lanes; all of these have 256 to a workgroup)
+// (a launch has fewer than 2^32 lanes; all of these have 256 to a workgroup, but for
+// tiles of 256 rows, which have 512)
 constexpr int64_t kMostBlocks = (int64_t)UINT32_MAX / kMergeBlock;
 
 // Joins partials: a thread takes four channels of a row.  Bound by its reads of the
@@ -153,7 +156,8 @@ int run_items(L& a, int dtype, const int32_t* plan, const int64_t* info, hipStre
         a.items = items + before;
         a.n_items = (int)info[kInfoItems + kind];
         if (a.n_items == 0) continue;
-        if ((int64_t)a.n_items * a.Hkv > kMostBlocks / (kind == kWide8 ? 2 : 1))
+        const bool wide = std::is_same_v<L, Paged8Launch> && kind == kWide8;
+        if ((int64_t)a.n_items * a.Hkv > kMostBlocks / (wide ? 2 : 1))
             return set_error(kErrInvalidArgument, "%d items are too many for one launch",
                              a.n_items);
         launch(kind);
@@ -194,8 +198,8 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
                          size_t workspace_bytes, void* stream) {
     PagedLaunch a{};
     const int rc = launch_args(a, q, q_token_stride, q_head_stride, dtype, k_pages, v_pages,
-                               num_pages, page_size, q_heads, kv_heads, head_dim, plan, info, softmax_scale,
-                               out, workspace, workspace_bytes);
+                               num_pages, page_size, q_heads, kv_heads, head_dim, plan, info,
+                               softmax_scale, out, workspace, workspace_bytes);
     if (rc || a.Hq == 0) return rc;
     hipStream_t s = (hipStream_t)stream;
     return run_items(a, dtype, plan, info, s, [&](int kind) {
@@ -213,8 +217,8 @@ int kivi_paged8_attention(const void* q, int64_t q_token_stride, int64_t q_head_
                           void* workspace, size_t workspace_bytes, void* stream) {
     Paged8Launch a{};
     const int rc = launch_args(a, q, q_token_stride, q_head_stride, dtype, k_pages, v_pages,
-                               num_pages, page_size, q_heads, kv_heads, head_dim, plan, info, softmax_scale,
-                               out, workspace, workspace_bytes);
+                               num_pages, page_size, q_heads, kv_heads, head_dim, plan, info,
+                               softmax_scale, out, workspace, workspace_bytes);
     if (rc || a.Hq == 0) return rc;
     if (k_scales == nullptr || v_scales == nullptr)
         return set_error(kErrInvalidArgument, "null scales");
