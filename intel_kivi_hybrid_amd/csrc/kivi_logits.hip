@@ -14,10 +14,11 @@
 // operations, so whatever does not depend on a step before it is loaded at the start:
 // logits, mask, biases and the first 16 tokens of each lane.
 //
-// A batch is bound by the instructions of its counting (64 rows of 128256, bf16, lists of
-// 4000, 40 biases and a mask: 18.8 us, 1.9 TB/s; 63 slices read each list), one row and
-// long lists by the chain of their steps (50257 fp32 with a list of 300: 9.9 us a call, 4.6
-// on the GPU; 16 rows of 32000 with lists of 30000: 11.2).
+// A batch is bound by the instructions of counting and of what the counts change, half of
+// the vector units' time (64 rows of 128256, bf16, lists of 4000, 40 biases and a mask:
+// 16.0 us, 2.2 TB/s; in a captured graph 17.3, without tokens 9.7, with nothing 6.5), one row and long lists by the
+// chain of their steps (50257 fp32 with a list of 300: 10 us a call, 3.9 on the GPU; 16 rows
+// of 32000 with lists of 30000: 11).
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -28,9 +29,9 @@
 namespace kivi {
 namespace {
 
-// Tokens of a workgroup, as measured (64 rows of 128256 with lists of 4000: workgroups of
-// 256 lanes, 2048 20.8 us, 4096 22.9; 16 rows of 32000 with lists of 30000: of 1024 lanes,
-// 4096 11.5 us).
+// Tokens of a workgroup, as measured (64 rows of 128256 with lists of 4000: 256 lanes and
+// 2048 tokens 17.3 us, 512 and 4096 17.7, 1024 and 8192 18.8; 16 rows of 32000 with lists of
+// 30000: 1024 lanes and 4096 11 us).
 constexpr int slice_of(int block) { return block == 256 ? 2048 : 4096; }
 constexpr uint32_t kInPrompt = 1u << 31;     // of a count
 constexpr uint32_t kNoBias = 0xffffffffu;    // (of no sum: NaN is stored as 0x7fc00000)
@@ -187,10 +188,13 @@ struct Biases {
         id = id_at(a.bias_ids, row * a.id_stride + i, a.id64);
         b = a.bias[row * a.bias_stride + i];
     }
+    __device__ __forceinline__ bool inside(uint32_t first, uint32_t n) const {
+        return (uint64_t)(id - (int64_t)first) < n;
+    }
     __device__ __forceinline__ void add(uint32_t first, uint32_t n, uint32_t* owner,
                                         uint32_t* sums) const {
         const uint64_t at = (uint64_t)(id - (int64_t)first);
-        bool waits = at < n;
+        bool waits = inside(first, n);
         while (__syncthreads_or(waits)) {
             if (waits) atomicMax(owner + at, BLOCK - threadIdx.x);
             __syncthreads();
@@ -259,14 +263,22 @@ __global__ void __launch_bounds__(BLOCK) adjust_logits_kernel(AdjustArgs a) {
     Ids<BLOCK, I> ids;
     if (counted) ids.load(static_cast<const I*>(a.tokens) + row * a.token_stride, start, length);
 
+    // (most slices have none of a short list's biases)
+    bool biased = false;
     if (counted || BIASED) {
-        for (uint32_t i = threadIdx.x; i < n; i += BLOCK) {
-            counts[i] = 0;
-            if constexpr (BIASED) sums[i] = kNoBias;
-        }
-        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kSlice; i += 4 * BLOCK)
+            *reinterpret_cast<u4*>(counts + i + 4 * threadIdx.x) = u4{0, 0, 0, 0};
+        if constexpr (BIASED)
+            biased = __syncthreads_or(biases.inside(first, n)) || a.biases > BLOCK;
+        else
+            __syncthreads();
     }
-    if constexpr (BIASED) {
+    if (biased) {
+#pragma unroll
+        for (int i = 0; i < kSlice; i += 4 * BLOCK)
+            *reinterpret_cast<u4*>(sums + i + 4 * threadIdx.x) =
+                u4{kNoBias, kNoBias, kNoBias, kNoBias};
         biases.add(first, n, counts, sums);
         for (int base = BLOCK; base < a.biases; base += BLOCK) {
             biases.load(a, row, base);
@@ -289,12 +301,17 @@ __global__ void __launch_bounds__(BLOCK) adjust_logits_kernel(AdjustArgs a) {
     // (few lanes have a token that something concerns)
     uint32_t c[8], b[8], seen = 0, free = kNoBias;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        // (behind the slice's end LDS holds anything)
-        c[j] = counted && j < some ? counts[i + j] : 0u;
-        b[j] = BIASED && j < some ? sums[i + j] : kNoBias;
-        seen |= c[j];
-        free &= b[j];
+    for (int h = 0; h < 8; h += 4) {
+        const u4 k = counted ? *reinterpret_cast<const u4*>(counts + i + h) : u4{0, 0, 0, 0};
+        const u4 sum = biased ? *reinterpret_cast<const u4*>(sums + i + h)
+                              : u4{kNoBias, kNoBias, kNoBias, kNoBias};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            c[h + j] = k[j];
+            b[h + j] = sum[j];
+            seen |= k[j];
+            free &= sum[j];
+        }
     }
     if (seen != 0 || free != kNoBias) {
 #pragma unroll
