@@ -117,7 +117,13 @@ struct Cut {
 struct Costs {
     int64_t start, partial_row, merge;
 };
-constexpr Costs paged_costs(int kind, bool eight) {
+constexpr Costs paged_costs(int kind, bool eight, int head_dim) {
+    // A position of 8 bits takes few rows half the time up to 128 channels, so what is
+    // not positions weighs more (64 single tokens of 4K to 8K positions, 32/8 heads of 128,
+    // 152 us and 163 with {64, 4, 96}; 16 of 3000, 24 and 31; 64 of 8K, 12/12 of 64, 115 and
+    // 126; 116 steps of four geometries 0.97 of the time, none above 1.04; with 256
+    // channels 29 steps 1.01).
+    if (eight && kind == kFew16 && head_dim <= 128) return Costs{256, 8, 256};
     // (fp32's products of 64 rows take four times as long for a position; the eight waves
     // of kWide8 write twice the rows in the time of one)
     return kind != kFew64 ? Costs{64, 4, 96} : eight ? Costs{64, 2, 96} : Costs{16, 1, 24};
@@ -290,7 +296,7 @@ int make_plan(bool eight, int32_t n_seqs, const int32_t* new_lens, const int32_t
             for (const Tile& t : of) rows.push_back(tile_rows(t, kind));
             const int64_t slots = paged_slots(kind, head_dim, eight);
             return best_cut(of, rows, std::max<int64_t>(1, slots / kv_heads),
-                            paged_costs(kind, eight));
+                            paged_costs(kind, eight, head_dim));
         };
         Cut cuts[kPagedKinds];
         for (int kind = 0; kind < kPagedKinds; ++kind) cuts[kind] = cut_tiles(kind);

@@ -55,7 +55,7 @@ def test_blocks_hold_every_new_token_once(lens, page_size):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-def test_the_rest_is_the_plan_of_16_bit_pages(dtype):
+def test_the_rest_is_the_plan_of_16_bit_pages_where_costs_agree(dtype):
     table, pool, ctx, new = make_table(LENS[2], 32, seed=3)
     words, info = _plan(table, pool, ctx, new, dtype=dtype)
     plain, plain_info = plain_plan(table, pool, ctx, new, dtype=dtype)
