@@ -89,6 +89,18 @@ def test_tiles_of_256_rows(hip_device, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF, FF], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("Hq,Hkv", [(4, 1), (32, 2)])
+def test_single_tokens_in_the_launch_of_many_rows(hip_device, dtype, D, Hq, Hkv):
+    """Both split: rows of a few tokens and of whole tiles."""
+    lens = [(3000, 80), (3000, 1), (700, 1), (0, 1), (1500, 24)]
+    case = _setup(lens, 64, dtype, Hq, Hkv, D, seed=8)
+    info = list(case[-2]._info)
+    assert info[6:9] == [0, 0, 0] and info[5] > 1
+    _check(_attend(case), case, 64)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FF], ids=["bf16", "f16", "f32"])
 def test_attention_scale_and_large_scores(hip_device, dtype):
     case = _setup([(100, 20), (700, 1)], 32, dtype, 8, 2, 64, seed=5)
     _check(_attend(case, softmax_scale=1.0), case, 32, scale=1.0)
