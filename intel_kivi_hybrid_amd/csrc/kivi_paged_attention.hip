@@ -201,6 +201,9 @@ int kivi_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
                                num_pages, page_size, q_heads, kv_heads, head_dim, plan, info,
                                softmax_scale, out, workspace, workspace_bytes);
     if (rc || a.Hq == 0) return rc;
+    // (a kind that the type's plans do not have: those of pages of 8 bits do)
+    if (info[kInfoItems + (dtype == kSrcF32 ? kMany : kFew64)] != 0)
+        return set_error(kErrInvalidArgument, "the plan is not one of kivi_paged_plan");
     hipStream_t s = (hipStream_t)stream;
     return run_items(a, dtype, plan, info, s, [&](int kind) {
         if (kind == kMany) launch_paged_many(a, dtype, s);

@@ -80,6 +80,21 @@ def test_long_chunks_of_128_channels_are_in_tiles_of_256_rows(lens, dtype, dim, 
     assert (info[8] > 0) == wide and (info[9] > 0) == (not wide)
 
 
+@pytest.mark.parametrize("lens,dtype", [([(8200, 2048)], torch.bfloat16),
+                                        ([(40, 50)], torch.float32)])
+def test_pages_of_the_models_type_refuse_tiles_that_they_do_not_have(lens, dtype):
+    from intel_kivi_hybrid_amd import _native
+    lib = _native.load()
+    table, pool, ctx, new = make_table(lens, 64, seed=3)
+    words, info = _plan(table, pool, ctx, new, 64, dtype, 32, 8, 128)
+    size = lib.kivi_paged_attention_workspace_size(info.ctypes.data, 8, 128)
+    buf = (ctypes.c_float * 64)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    rc = lib.kivi_paged_attention(p, 4096, 128, DT[dtype], p, p, pool, 64, 32, 8, 128, p,
+                                  info.ctypes.data, ctypes.c_float(0.1), p, p, size, None)
+    assert rc == 1 and "not one of kivi_paged_plan" in _native.last_error()
+
+
 def test_a_block_of_two_sequences_is_refused():
     """Disjoint slots of one page are fine in pages of the model's type; here each
     sequence would rescale the other's tokens."""
