@@ -11,7 +11,7 @@
 // and fp32's as two pieces (22 bits).  Weights times value scales have no such bounds, so
 // a row keeps a second maximum, that of these products, and its outputs in units of
 // that one: the largest lies between 2^12 and 2^15, so that fp16's last step, 2^-24, is
-// 2^-36 of it or less.  They are rounded to fp16 (as a bf16 cache's would be to bf16, or
+// 2^-36 of it or less (lowered() and drop_far() say how fp32 holds what lies between).  They are rounded to fp16 (as a bf16 cache's would be to bf16, or
 // better), for up to 16 rows and for fp32 in two pieces.  (bf16 operands hold codes and any scale
 // at once, but take a fifth more operations to widen codes, and fp32 three pieces.)
 //
@@ -117,6 +117,26 @@ __device__ __forceinline__ float load_query(const PagedLaunch& a, int64_t at, bo
 // are set, and they are set anew where one comes out 2^kMoveTop times larger.
 constexpr float kWeightBits = 13.0f, kMoveTop = 2.0f;
 
+// A row's weights are 2^(score - m), times 2^(m - top) in its units, and fp32 has to hold
+// both.  Where the values at its largest scores are quiet (zeros have the smallest scale,
+// 2^-126) m lies below the largest score, so that m - top is kMostDown at most: by 75,
+// since top is the largest score less 126 + 13 at least.  Rows with values of a scale of
+// 2^-51 or more at their largest score have it at m.
+constexpr float kMostDown = 64.0f;
+__device__ __forceinline__ float lowered(float m, float top) { return fminf(m, top + kMostDown); }
+
+// Value scales from 2^60 on may leave fp32 on the way into such units, where the scores
+// of their block are 2^112 or more below the row's largest, and an infinity is NaN beside
+// a weight of 0: such a block's weights count as 0.  x: the lane's largest scores of the
+// blocks, most: the row's.
+constexpr float kLoud = 0x1p60f;
+template <int N>
+__device__ __forceinline__ void drop_far(float (&vs)[N], const float (&x)[N], float most) {
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+        if (vs[b] >= kLoud && x[b] < most - 112.0f) vs[b] = 0.f;       // (NaN stays)
+}
+
 // Power of two above a scale, log2.
 __device__ __forceinline__ float above(float scale) {
     return (float)((int)(__float_as_uint(scale) >> 23 & 0xff) - 126);
@@ -148,6 +168,13 @@ struct BlockScales {
     }
     __device__ __forceinline__ float k(int b) const { return lane_f(own, b); }
     __device__ __forceinline__ float v(int b) const { return lane_f(own, N + b); }
+    // whether a value's is
+    __device__ __forceinline__ bool loud() const {
+        uint32_t most = 0;
+#pragma unroll
+        for (int b = 0; b < N; ++b) most = max(most, __float_as_uint(v(b)));
+        return most >= __float_as_uint(kLoud);
+    }
 };
 
 // A page id (one for the wave), by a vector load for the same reason.
@@ -322,7 +349,8 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
             units[b] = scales.k(b) * qscale;
             vs[b] = scales.v(b);
         }
-        if (t0 + F::UNIT > min(all_see, end)) {
+        const bool loud = scales.loud();
+        if (t0 + F::UNIT > min(all_see, end) || loud) {
             asm volatile("");            // (or every unit does all of this and selects)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -334,6 +362,16 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (t0 + 16 * b + 4 * gq + i >= lim) s[b][i] = -INFINITY;
+            }
+            if (loud) {
+                float x[NB], most = m;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    x[b] = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])) * units[b];
+                    most = fmaxf(most, x[b]);
+                }
+                most = fmaxf(most, __shfl_xor(most, 16));
+                drop_far(vs, x, fmaxf(most, __shfl_xor(most, 32)));
             }
         }
         float mx = -INFINITY, mv = -INFINITY;
@@ -349,6 +387,7 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
             mv = fmaxf(mv, __shfl_xor(mv, 16));
             mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
             mv = fmaxf(top, fmaxf(mv, __shfl_xor(mv, 32)));
+            mx = lowered(mx, mv);
             l *= exp2_fast(m - mx);
             const float f = exp2_fast(top - mv);
             m = mx;
@@ -404,12 +443,14 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
         join.l[wave][col] = l;
     }
     __syncthreads();
-    const float f = exp2_fast(top - fmaxf(fmaxf(join.m[0][col], join.m[1][col]),
-                                          fmaxf(join.m[2][col], join.m[3][col])));
+    const float apart = top - fmaxf(fmaxf(join.m[0][col], join.m[1][col]),
+                                    fmaxf(join.m[2][col], join.m[3][col]));
+    // (below 2^-126 in two steps: the outputs may be large)
+    const float f = exp2_fast(fmaxf(apart, -100.0f)), rest = exp2_fast(fminf(apart + 100.0f, 0.f));
 #pragma unroll
     for (int cb = 0; cb < F::CB; ++cb)
         *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(vl) + col * F::OS + 16 * cb + 4 * gq) =
-            O[cb] * f;
+            O[cb] * f * rest;
     __syncthreads();
     join_waves<DT, DP, 16, kFew8Waves, false>(
         a, w, w.it.row0, [&](int i) { return reinterpret_cast<const float*>(lds(i)); }, F::OS,

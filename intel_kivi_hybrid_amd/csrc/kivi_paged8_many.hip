@@ -120,6 +120,14 @@ struct Tile8Rows {
         last = row0 < w.rows ? min(base + min(row0 + 31, w.rows - 1) / w.hg, w.it.kv_end) : 0;
     }
 
+    // the lane's largest of a block's scores
+    static __device__ __forceinline__ float block_top(const f32x16_t (&s)[M::TB], int b) {
+        float x = s[b / 2][b % 2 * 8];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) x = fmaxf(x, s[b / 2][b % 2 * 8 + i]);
+        return x;
+    }
+
     // A tile of keys and values in LDS, positions t0 ..
     __device__ __forceinline__ void tile(const unsigned char* buf, const BlockScales<NB>& sc,
                                          int t0, int end) {
@@ -160,7 +168,8 @@ struct Tile8Rows {
             units[b] = sc.k(b) * qscale;
             vs[b] = sc.v(b);
         }
-        if (t0 + M::TILE > min(all, end)) {
+        const bool loud = sc.loud();
+        if (t0 + M::TILE > min(all, end) || loud) {
             asm volatile("");        // (or every tile does all of this and selects)
 #pragma unroll
             for (int tb = 0; tb < M::TB; ++tb) {
@@ -177,14 +186,20 @@ struct Tile8Rows {
                     units[b] = FLT_MIN;
                 }
             }
+            if (loud) {
+                float x[NB], most = m;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    x[b] = block_top(s, b) * units[b];
+                    most = fmaxf(most, x[b]);
+                }
+                drop_far(vs, x, fmaxf(most, __shfl_xor(most, 32)));
+            }
         }
         float mx = -INFINITY, mv = -INFINITY;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            float x = s[b / 2][b % 2 * 8];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) x = fmaxf(x, s[b / 2][b % 2 * 8 + i]);
-            x *= units[b];
+            const float x = block_top(s, b) * units[b];
             mx = fmaxf(mx, x);
             mv = fmaxf(mv, x + above(sc.v(b)));
         }
@@ -192,6 +207,7 @@ struct Tile8Rows {
         if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax || mv > top + kMoveTop) != 0) {
             mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
             mv = fmaxf(top, fmaxf(mv, __shfl_xor(mv, 32)));
+            mx = lowered(mx, mv);
             l *= exp2_fast(m - mx);
             const float f = exp2_fast(top - mv);
             m = mx;
