@@ -1,6 +1,6 @@
-"""GPU tests of attention over 8-bit pages whose values are zero or next to it, against
+"""GPU tests of attention over 8-bit pages whose blocks' scales are far apart, against
 float64: blocks of zeros have the smallest scale, and what a row sees, or sees first, may
-be nothing else."""
+be nothing else; and bounds by each weight's own scale."""
 
 import pytest
 import torch
@@ -216,6 +216,23 @@ def test_loud_values_far_below_a_quiet_leader(hip_device, lens, dtype):
                         case.vs[page, 0, b] = 2.0 ** -126
                         case.vc[page, 0, b * BLOCK:(b + 1) * BLOCK] = 0
             case.check(f"2^{e} {lead} and {below} below")
+
+
+@pytest.mark.parametrize("dtype,spread", [(BF, 3), (BF, 10), (BF, 20), (HF, 3), (HF, 10), (FF, 3),
+                                          (FF, 10), (FF, 20)])
+@pytest.mark.parametrize("n", [1, 70])
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_whose_weights_lie_on_quiet_blocks(hip_device, D, n, dtype, spread):
+    """Beside blocks up to 2^41 times louder, whose keys have tiny scores: the bound is by
+    the largest product of a weight and its own scale."""
+    case = Case([(200, n), (90, n)], 32, dtype, 4, 2, D, seed=8, spread=spread)
+    for s, c in enumerate(case.ctx):
+        for page, j in case.blocks(s, 0, c):
+            for h in range(2):
+                if case.vs[page, h, j] > case.vs[int(case.table[s, 0]), h, 0]:
+                    case.kc[page, h, j * BLOCK:(j + 1) * BLOCK] = 0
+    case.q *= 4
+    case.check(f"spread {spread}")
 
 
 @TYPES
