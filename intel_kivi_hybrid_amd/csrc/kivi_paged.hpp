@@ -125,6 +125,12 @@ enum PagedInfo : int {
     kInfoCount8 = 20,
 };
 
+// Whether info is that of a plan of kivi_paged_plan, which ends behind the zeros: its caller's
+// array may hold kInfoCount entries and no more.
+inline bool paged_plain_info(const int64_t* info) {
+    return info[kInfoInts] == info[kInfoZerosAt] + 8;
+}
+
 struct PagedLaunch {
     const void* q;
     int64_t q_st, q_sh;           // strides of tokens and heads, in elements

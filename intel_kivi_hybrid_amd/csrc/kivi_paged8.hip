@@ -237,6 +237,8 @@ int kivi_paged8_append(const void* q, int64_t q_token_stride, int64_t q_head_str
     if (rc || a.n_tokens == 0) return rc;
     if (k_scales == nullptr || v_scales == nullptr)
         return set_error(kErrInvalidArgument, "null scales");
+    if (paged_plain_info(info))
+        return set_error(kErrInvalidArgument, "the plan is not one of kivi_paged8_plan");
     g.k_scales = k_scales;
     g.v_scales = v_scales;
     g.blocks = reinterpret_cast<const PagedBlock*>(plan + info[kInfoBlocksAt]);

@@ -225,7 +225,8 @@ int kivi_paged8_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     if (rc || a.Hq == 0) return rc;
     if (k_scales == nullptr || v_scales == nullptr)
         return set_error(kErrInvalidArgument, "null scales");
-    if (info[kInfoItems + kWide8] != 0 && !paged_wide(dtype == kSrcF32, head_dim))
+    if (paged_plain_info(info) ||
+        (info[kInfoItems + kWide8] != 0 && !paged_wide(dtype == kSrcF32, head_dim)))
         return set_error(kErrInvalidArgument, "the plan is not one of kivi_paged8_plan");
     a.k_scales = k_scales;
     a.v_scales = v_scales;

@@ -153,6 +153,27 @@ def test_entry_points_reject_bad_arguments():
     assert "too many for one launch" in append(blocks=1 << 24)
 
 
+@pytest.mark.parametrize("lens", LENS, ids=range(len(LENS)))
+def test_entry_points_refuse_plans_of_the_models_type(lens):
+    """Whose info ends before the blocks of 8-bit pages: nothing behind it is read."""
+    from intel_kivi_hybrid_amd import _native
+    lib = _native.load()
+    table, pool, ctx, new = make_table(lens, 32, seed=3)
+    words, plain = plain_plan(table, pool, ctx, new)
+    info = np.full(20, 1 << 40, dtype=np.int64)
+    info[:16] = plain[:16]
+    buf = (ctypes.c_float * 64)()
+    p = (ctypes.addressof(buf) + 15) // 16 * 16
+    ip = info.ctypes.data
+    calls = (lambda: lib.kivi_paged8_append(
+        None, 0, 0, p, 0, 0, p, 0, 0, 1, None, p, p, p, p, pool, 32, 8, 2, 64, p, ip, None, None,
+        0, 0, None, None, 1, ctypes.c_float(1e-6), None),
+        lambda: lib.kivi_paged8_attention(p, 512, 64, 1, p, p, p, p, pool, 32, 8, 2, 64, p, ip,
+                                          ctypes.c_float(0.1), p, p, 1 << 40, None))
+    for call in calls:
+        assert call() == 1 and "not one of kivi_paged8_plan" in _native.last_error()
+
+
 def test_python_plan_refuses_other_cache_types():
     from intel_kivi_hybrid_amd import _C
     t = torch.zeros(1, 2, dtype=torch.int32)
