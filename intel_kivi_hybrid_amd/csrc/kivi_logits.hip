@@ -388,7 +388,14 @@ int kivi_adjust_logits(const void* logits, int32_t dtype, int64_t row_stride, in
     const bool same = from == to && dtype == out_dtype && (rows == 1 || row_stride == out_stride);
     if (out_stride < vocab && rows > 1)
         return set_error(kErrInvalidArgument, "rows of out overlap");
-    if (!same && from < to + out_bytes && to < from + in_bytes)
+    // (rows may lie between the other's, the same distance apart)
+    const int64_t apart = row_stride * src_size(dtype), row = (int64_t)vocab * src_size(dtype);
+    bool between = false;
+    if (rows > 1 && apart > row && apart == out_stride * src_size(out_dtype)) {
+        const int64_t off = ((to - from) % apart + apart) % apart;
+        between = off >= row && off + (int64_t)vocab * src_size(out_dtype) <= apart;
+    }
+    if (!same && !between && from < to + out_bytes && to < from + in_bytes)
         return set_error(kErrInvalidArgument, "out must be logits or apart from them");
     AdjustArgs a{};
     a.logits = logits; a.out = out;

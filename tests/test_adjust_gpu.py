@@ -312,3 +312,23 @@ def test_calls_that_are_refused(hip_device):
             o = a.view(-1).view(torch.float32)[:70].expand(2, 70)
         with pytest.raises(RuntimeError, match="overlap|apart from"):
             C.adjust_logits(a, out=o)
+
+
+def test_rows_between_the_rows_of_out(hip_device):
+    """Logits and results as two halves of one buffer's rows, either way round."""
+    V = 700
+    for dtype in (FF, BF):
+        for a in (0, V + 3):
+            wide = torch.full((3, 2 * V + 5), 5.0, dtype=dtype, device=DEV)
+            b = V + 3 - a
+            wide[:, a:a + V] = _logits(3, V, dtype).to(DEV)
+            _check(wide[:, a:a + V], out=wide[:, b:b + V], tokens=_history(3, V, 50, 3),
+                   repetition_penalty=1.25)
+            assert bool((wide[:, V:V + 3] == 5).all() and (wide[:, 2 * V + 3:] == 5).all())
+            # from the second row on: still between them
+            _check(wide[:2, a:a + V], out=wide[1:, b:b + V], frequency_penalty=0.5,
+                   tokens=_history(2, V, 50, 4))
+            with pytest.raises(RuntimeError, match="apart from"):
+                _c().adjust_logits(wide[:, a:a + V], out=wide[:, b - 4 if b else 4:][:, :V])
+            with pytest.raises(RuntimeError, match="apart from"):
+                _c().adjust_logits(wide[:2, a:a + V], out=wide[1:, a:a + V])
