@@ -294,7 +294,7 @@ int make_plan(bool eight, int32_t n_seqs, const int32_t* new_lens, const int32_t
                              [](const Tile& a, const Tile& b) { return a.end > b.end; });
             std::vector<int> rows;
             for (const Tile& t : of) rows.push_back(tile_rows(t, kind));
-            const int64_t slots = paged_slots(kind, head_dim, eight);
+            const int64_t slots = paged_slots(kind, head_dim, eight, dtype == 0);
             return best_cut(of, rows, std::max<int64_t>(1, slots / kv_heads),
                             paged_costs(kind, eight, head_dim));
         };

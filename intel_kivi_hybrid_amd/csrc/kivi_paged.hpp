@@ -90,12 +90,20 @@ constexpr bool paged_few(int64_t rows) { return rows <= paged_tile_rows(kFew16);
 
 // Workgroups that the card works on at once: 256 CUs, and as many on each as the
 // kernels' registers or LDS leave room for (fp32's 64 rows: as bring more; more
-// than that share the matrix cores that bound it).
-constexpr int paged_slots(int kind, int head_dim, bool eight = false) {
-    const int per_cu = eight && kind == kWide8 ? 1
-                       : kind == kMany  ? (head_dim <= 64 ? 4 : head_dim <= 128 ? 2 : 1)
-                       : kind == kFew16 ? (head_dim <= 64 ? 3 : head_dim <= 128 ? 2 : 1)
-                                        : 2;
+// than that share the matrix cores that bound it).  Pages of 8 bits have kernels of their
+// own: kMany in fp32 half as many (dealt to as many as 16 bits: one chunk of 64 tokens after
+// 20000, 32/8 heads of 128, 77 us for 66; 48 steps of six geometries 1.04 of the time), and
+// single tokens of 256 channels two (dealt to one, 64 of 8K, 28/4 heads, fp32, 188 us for
+// 167; 16 of 3000 35 for 26).  (16-bit ones of 64 channels have room for four; dealt to
+// four, 64 of 8K, 12/12 heads, took 123 us for 116.)
+constexpr int paged_slots(int kind, int head_dim, bool eight = false, bool f32 = false) {
+    const int to64 = head_dim <= 64, to128 = head_dim <= 128;
+    int per_cu = 2;                                      // kFew64
+    if (kind == kMany) per_cu = to64 ? 4 : to128 ? 2 : 1;
+    if (kind == kFew16) per_cu = to64 ? 3 : to128 ? 2 : 1;
+    if (eight && kind == kWide8) per_cu = 1;
+    if (eight && kind == kMany) per_cu = to64 ? (f32 ? 2 : 3) : to128 && !f32 ? 2 : 1;
+    if (eight && kind == kFew16) per_cu = to64 ? 3 : 2;
     return 256 * per_cu;
 }
 

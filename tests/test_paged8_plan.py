@@ -153,6 +153,18 @@ def test_entry_points_reject_bad_arguments():
     assert "too many for one launch" in append(blocks=1 << 24)
 
 
+@pytest.mark.parametrize("lens,dtype,Hq,Hkv,D,per_cu", [
+    ([(20000, 64)], torch.float32, 32, 8, 128, 1), ([(8000, 200)], torch.float32, 16, 4, 96, 1),
+    ([(8000, 200)], torch.float32, 8, 2, 64, 2), ([(20000, 64)], torch.float16, 32, 8, 64, 3),
+    ([(20000, 64)], torch.bfloat16, 32, 8, 128, 2), ([(3000, 1)] * 16, torch.float32, 28, 4, 256, 2),
+    ([(3000, 1)] * 16, torch.bfloat16, 12, 12, 64, 3)])
+def test_contexts_are_split_for_the_workgroups_that_a_cu_holds(lens, dtype, Hq, Hkv, D, per_cu):
+    """So many pieces that most of them run at once, and none behind them."""
+    table, pool, ctx, new = make_table(lens, 64, seed=3)
+    info = _plan(table, pool, ctx, new, 64, dtype, Hq, Hkv, D)[1]
+    assert 256 * (per_cu - 1) < info[6:10].sum() * Hkv <= 256 * per_cu
+
+
 @pytest.mark.parametrize("lens", LENS, ids=range(len(LENS)))
 def test_entry_points_refuse_plans_of_the_models_type(lens):
     """Whose info ends before the blocks of 8-bit pages: nothing behind it is read."""
