@@ -507,8 +507,9 @@ int kivi_paged8_append(const void* q, int64_t q_token_stride, int64_t q_head_str
  * kivi_paged8_plan).  Codes enter the products exactly; queries and weights times value
  * scales as fp16, in units of a power of two of each row's own that keep the largest
  * within fp16's range (f32 queries, their weights, and those of a sequence with up to 16
- * rows to a kv head in two pieces).  Scores, softmax and sums are f32; a weight below
- * 2^-112 of its row's largest, of a value whose scale is above 2^36, may count for less.
+ * rows to a kv head in two pieces).  Scores, softmax and sums are f32; what may count for
+ * less is a weight below 2^-112 of its row's largest, of a value whose scale is above
+ * 2^36, and, beside scores of 2^29 (in log2) and more, a value whose scale is below 2^-51.
  * A row that sees a position of a block whose scale is NaN comes out as NaN; scales of
  * blocks that it sees nothing of do not reach it. */
 int kivi_paged8_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,

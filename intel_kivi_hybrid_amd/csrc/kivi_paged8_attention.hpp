@@ -1,5 +1,5 @@
-// Pieces shared by the attention kernels over pages of 8 bits (kivi_paged8.hip), and the
-// walk of up to 16 query rows.
+// Pieces shared by the attention kernels over pages of 8 bits (kivi_paged8_few.hip,
+// kivi_paged8_many.hip), and the walk of up to 16 query rows.
 //
 // Codes are whole numbers up to 127, which fp16 holds exactly, so both products run on
 // the fp16 matrix instructions with codes as they are; the scales of a block of 16
@@ -11,7 +11,7 @@
 // and fp32's as two pieces (22 bits).  Weights times value scales have no such bounds, so
 // a row keeps a second maximum, that of these products, and its outputs in units of
 // that one: the largest lies between 2^12 and 2^15, so that fp16's last step, 2^-24, is
-// 2^-36 of it or less (lowered() and drop_far() say how fp32 holds what lies between).  They are rounded to fp16 (as a bf16 cache's would be to bf16, or
+// 2^-36 of it or less (RowState and drop_far() say how fp32 holds what lies between).  They are rounded to fp16 (as a bf16 cache's would be to bf16, or
 // better), for up to 16 rows and for fp32 in two pieces.  (bf16 operands hold codes and any scale
 // at once, but take a fifth more operations to widen codes, and fp32 three pieces.)
 //
@@ -117,29 +117,52 @@ __device__ __forceinline__ float load_query(const PagedLaunch& a, int64_t at, bo
 // are set, and they are set anew where one comes out 2^kMoveTop times larger.
 constexpr float kWeightBits = 13.0f, kMoveTop = 2.0f;
 
-// A row's weights are 2^(score - m), times 2^(m - top) in its units, and fp32 has to hold
-// both.  Where the values at its largest scores are quiet (zeros have the smallest scale,
-// 2^-126) m lies below the largest score, so that m - top is kMostDown at most: by 75,
-// since top is the largest score less 126 + 13 at least.  Rows with values of a scale of
-// 2^-51 or more at their largest score have it at m.
-constexpr float kMostDown = 64.0f;
-__device__ __forceinline__ float lowered(float m, float top) { return fminf(m, top + kMostDown); }
-
-// Value scales from 2^60 on may leave fp32 on the way into such units, where the scores
-// of their block are 2^112 or more below the row's largest, and an infinity is NaN beside
-// a weight of 0: such a block's weights count as 0.  x: the lane's largest scores of the
-// blocks, most: the row's.
-constexpr float kLoud = 0x1p60f;
-template <int N>
-__device__ __forceinline__ void drop_far(float (&vs)[N], const float (&x)[N], float most) {
-#pragma unroll
-    for (int b = 0; b < N; ++b)
-        if (vs[b] >= kLoud && x[b] < most - 112.0f) vs[b] = 0.f;       // (NaN stays)
-}
-
 // Power of two above a scale, log2.
 __device__ __forceinline__ float above(float scale) {
     return (float)((int)(__float_as_uint(scale) >> 23 & 0xff) - 126);
+}
+
+// A row's softmax state: weights are 2^(score - m), l their sum, outputs in units of
+// 2^(m + lead).  (Units relative to m: beside a score of 2^28 fp32 holds no distance of 13.)
+//
+// fp32 has to hold 2^-lead too.  Where the values at a row's largest scores are quiet (zeros
+// have the smallest scale, 2^-126) m lies below the largest score, by 75 at most, so that
+// lead is -64 or more.  Rows with values of a scale of 2^-51 or more at their largest score
+// have it at m.
+constexpr float kLeastLead = -64.0f;
+struct RowState {
+    float m, lead, l;
+
+    // Moves m to `to`, or below, where `next` is the least lead that the row's outputs and
+    // the tile at hand ask for.  What the outputs are to be multiplied by.
+    __device__ __forceinline__ float move(float to, float next) {
+        float low = to + fminf(next - kLeastLead, 0.f);
+        // (from 2^31 on the nearest number below is 128 away: weights of 2^128)
+        if (to - low > 96.0f) low = to;
+        next = fmaxf(next + (to - low), kLeastLead);
+        const float gone = low - m, f = exp2_fast(lead - gone - next);
+        l *= exp2_fast(-gone);
+        m = low;
+        lead = next;
+        return f;
+    }
+};
+
+// Value scales from 2^60 on may leave fp32 on the way into such units, where the scores
+// of their block are 2^112 or more below the row's largest, and an infinity is NaN beside
+// a weight of 0: such a block's weights count as 0.  most: the lane's largest of the blocks'
+// scores, whose units these are, of(x): the row's of the lanes' x.
+constexpr float kLoud = 0x1p60f;
+template <int N, class F>
+__device__ __forceinline__ void drop_far(float (&vs)[N], const float (&most)[N],
+                                         const float (&units)[N], float m, F of) {
+    float top = m;
+#pragma unroll
+    for (int b = 0; b < N; ++b) top = fmaxf(top, most[b] * units[b]);
+    top = of(top);
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+        if (vs[b] >= kLoud && fmaf(most[b], units[b], -top) < -112.0f) vs[b] = 0.f;  // (NaN stays)
 }
 
 // The scales of N blocks of 16 positions (the last one's for blocks past the end).  Lane l
@@ -168,14 +191,68 @@ struct BlockScales {
     }
     __device__ __forceinline__ float k(int b) const { return lane_f(own, b); }
     __device__ __forceinline__ float v(int b) const { return lane_f(own, N + b); }
-    // whether a value's is
+    // Whether a value's reaches kLoud, and a key's far_keys().
     __device__ __forceinline__ bool loud() const {
         uint32_t most = 0;
 #pragma unroll
         for (int b = 0; b < N; ++b) most = max(most, __float_as_uint(v(b)));
         return most >= __float_as_uint(kLoud);
     }
+    __device__ __forceinline__ bool far(uint32_t from) const {
+        uint32_t most = 0;
+#pragma unroll
+        for (int b = 0; b < N; ++b) most = max(most, __float_as_uint(k(b)));
+        return most >= from;
+    }
 };
+
+// Key scales (as bits) from which on scores of a wave's rows may pass 2^29, products with
+// codes being 2^31 at most.  The largest score's distance from m is then no longer small, since
+// m is its product with the units rounded: such scores are rounded themselves first.
+__device__ __forceinline__ uint32_t far_keys(float qscale) {
+    const int e = __float_as_int(wave_max(qscale)) >> 23;
+    return (uint32_t)min(max(252 - e, 1), 255) << 23;
+}
+
+// Moves a row where a tile's blocks (most, units: as in drop_far()) ask for it: whether any
+// row of the wave moved, and what outputs are then to be multiplied by.  of(x): the row's
+// largest of its lanes' x.
+template <int N, class F>
+__device__ __forceinline__ bool move_row(RowState& row, const BlockScales<N>& scales,
+                                         const float (&most)[N], const float (&units)[N], F of,
+                                         float& f) {
+    // the largest score less m, and of these plus above() of their value scales
+    float x = -INFINITY, xv = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < N; ++b) {
+        const float y = fmaf(most[b], units[b], -row.m);
+        x = fmaxf(x, y);
+        xv = fmaxf(xv, y + above(scales.v(b)));
+    }
+    if (__builtin_amdgcn_ballot_w64((x > kMoveMax) |
+                                    (xv > row.lead + (kWeightBits + kMoveTop))) == 0)
+        return false;
+    x = of(x);
+    xv = of(xv);
+    float to, next;
+    if (__builtin_amdgcn_ballot_w64(x > 0x1p16f) == 0) {
+        to = row.m + fmaxf(x, 0.f);
+        next = fmaxf(row.lead, xv - kWeightBits) - (to - row.m);
+    } else {
+        // (a first tile's, or so far from m that the difference says little)
+        to = row.m;
+#pragma unroll
+        for (int b = 0; b < N; ++b) to = fmaxf(to, most[b] * units[b]);
+        to = of(to);
+        xv = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < N; ++b)
+            xv = fmaxf(xv, fmaf(most[b], units[b], -to) + above(scales.v(b)));
+        next = fmaxf(row.lead - (to - row.m), of(xv) - kWeightBits);
+    }
+    f = row.move(to, next);
+    return true;
+}
 
 // A page id (one for the wave), by a vector load for the same reason.
 __device__ __forceinline__ int block_page_ahead(const Paged8Launch& a, const Work& w, int t) {
@@ -243,8 +320,10 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
         return ks + 1 == F::KS && F::KS % 2 ? 32 * ks + 8 * gq : 32 * (ks & ~1) + 16 * gq + ks % 2 * 8;
     };
     u32x4_t qf[F::KS][NQ];
-    f32x4_t O[F::CB];                    // in units of 2^top
-    float m = -FLT_MAX, top = -FLT_MAX, l = 0.f, qscale;
+    f32x4_t O[F::CB];
+    RowState row{-FLT_MAX, 0.f, 0.f};
+    float qscale;
+    uint32_t far_from;
     int lim = 0;
     {
         const int r = w.it.row0 + col;
@@ -255,6 +334,7 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
             x = max(x, (uint32_t)__shfl_xor((int)x, 16));
             return max(x, (uint32_t)__shfl_xor((int)x, 32));
         }, qf);
+        far_from = far_keys(qscale);
     }
 #pragma unroll
     for (int cb = 0; cb < F::CB; ++cb) O[cb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -343,14 +423,23 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
             coming.pages_of(a, w, next + kStep);
         }
 
-        float units[NB], vs[NB];
+        float units[NB], vs[NB], most[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             units[b] = scales.k(b) * qscale;
             vs[b] = scales.v(b);
         }
-        const bool loud = scales.loud();
-        if (t0 + F::UNIT > min(all_see, end) || loud) {
+        auto each_most = [&] {                // the lane's largest of each block's
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                most[b] = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3]));
+        };
+        auto row_most = [](float x) {
+            x = fmaxf(x, __shfl_xor(x, 16));
+            return fmaxf(x, __shfl_xor(x, 32));
+        };
+        const bool loud = scales.loud(), far = scales.far(far_from);
+        if (t0 + F::UNIT > min(all_see, end) || loud || far) {
             asm volatile("");            // (or every unit does all of this and selects)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -363,39 +452,25 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
                 for (int i = 0; i < 4; ++i)
                     if (t0 + 16 * b + 4 * gq + i >= lim) s[b][i] = -INFINITY;
             }
-            if (loud) {
-                float x[NB], most = m;
+            if (__builtin_expect(far, 0)) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    x[b] = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])) * units[b];
-                    most = fmaxf(most, x[b]);
+                    s[b] *= units[b];
+                    units[b] = 1.0f;
                 }
-                most = fmaxf(most, __shfl_xor(most, 16));
-                drop_far(vs, x, fmaxf(most, __shfl_xor(most, 32)));
+            }
+            if (__builtin_expect(loud, 0)) {
+                each_most();
+                drop_far<NB>(vs, most, units, row.m, row_most);
             }
         }
-        float mx = -INFINITY, mv = -INFINITY;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const float x = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3])) * units[b];
-            mx = fmaxf(mx, x);
-            mv = fmaxf(mv, x + above(scales.v(b)));
-        }
-        mv -= kWeightBits;
-        if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax || mv > top + kMoveTop) != 0) {
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mv = fmaxf(mv, __shfl_xor(mv, 16));
-            mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
-            mv = fmaxf(top, fmaxf(mv, __shfl_xor(mv, 32)));
-            mx = lowered(mx, mv);
-            l *= exp2_fast(m - mx);
-            const float f = exp2_fast(top - mv);
-            m = mx;
-            top = mv;
+        each_most();
+        float f;
+        if (move_row<NB>(row, scales, most, units, row_most, f)) {
 #pragma unroll
             for (int cb = 0; cb < F::CB; ++cb) O[cb] *= f;
         }
-        const float down = exp2_fast(m - top);
+        const float down = exp2_fast(-row.lead);
 #pragma unroll
         for (int b = 0; b < NB; ++b) vs[b] *= down;
         // rows of a transposed read: tokens 4 gq .. + 3 of a block and of the next, in
@@ -408,9 +483,9 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int b = 2 * j + i / 2;
-                const float p0 = exp2_fast(fmaf(s[b][i % 2 * 2], units[b], -m));
-                const float p1 = exp2_fast(fmaf(s[b][i % 2 * 2 + 1], units[b], -m));
-                l += p0 + p1;
+                const float p0 = exp2_fast(fmaf(s[b][i % 2 * 2], units[b], -row.m));
+                const float p1 = exp2_fast(fmaf(s[b][i % 2 * 2 + 1], units[b], -row.m));
+                row.l += p0 + p1;
                 const Pieces w = split_f16(p0 * vs[b], p1 * vs[b]);
                 hi[i] = w.hi;
                 lo[i] = w.lo;
@@ -436,15 +511,15 @@ __device__ __forceinline__ void few8_rows(const Paged8Launch& a, const Work& w, 
     }
 
     // Join the waves: a row's largest maximum, then the rescaled sums.
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    row.l += __shfl_xor(row.l, 16);
+    row.l += __shfl_xor(row.l, 32);
     if (gq == 0) {
-        join.m[wave][col] = m;
-        join.l[wave][col] = l;
+        join.m[wave][col] = row.m;
+        join.l[wave][col] = row.l;
     }
     __syncthreads();
-    const float apart = top - fmaxf(fmaxf(join.m[0][col], join.m[1][col]),
-                                    fmaxf(join.m[2][col], join.m[3][col]));
+    const float apart = row.lead + (row.m - fmaxf(fmaxf(join.m[0][col], join.m[1][col]),
+                                                  fmaxf(join.m[2][col], join.m[3][col])));
     // (below 2^-126 in two steps: the outputs may be large)
     const float f = exp2_fast(fmaxf(apart, -100.0f)), rest = exp2_fast(fminf(apart + 100.0f, 0.f));
 #pragma unroll

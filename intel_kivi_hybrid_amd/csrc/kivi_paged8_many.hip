@@ -95,9 +95,9 @@ struct Tile8Rows {
     static constexpr int NB = TOKENS / 16;
     u32x4_t qf[M::KS][NQ];
     f32x16_t O[M::CB];
-    float m, l;
-    float top;               // the outputs' units, log2
+    RowState row;
     float qscale;
+    uint32_t far_from;
     int lim;                 // positions that the lane's row sees
     int all, last;           // that all, and any, of the 32 rows see
 
@@ -105,11 +105,11 @@ struct Tile8Rows {
         const int lane = threadIdx.x % kWave, half = lane / 32, r = row0 + lane % 32;
         const bool live = r < w.rows;
         lim = live ? row_limit(w, r) : 0;
-        m = top = -FLT_MAX;
-        l = 0.f;
+        row = RowState{-FLT_MAX, 0.f, 0.f};
         qscale = a.qscale * load_query<DT, M::KS>(
             a, live ? q_offset(a, w, r) : 0, live, [&](int ks) { return 16 * ks + 8 * half; },
             [](uint32_t x) { return max(x, (uint32_t)__shfl_xor((int)x, 32)); }, qf);
+        far_from = far_keys(qscale);
 #pragma unroll
         for (int cb = 0; cb < M::CB; ++cb) {
 #pragma unroll
@@ -118,14 +118,6 @@ struct Tile8Rows {
         const int base = w.it.ctx - w.it.n + 1;
         all = base + row0 / w.hg;
         last = row0 < w.rows ? min(base + min(row0 + 31, w.rows - 1) / w.hg, w.it.kv_end) : 0;
-    }
-
-    // the lane's largest of a block's scores
-    static __device__ __forceinline__ float block_top(const f32x16_t (&s)[M::TB], int b) {
-        float x = s[b / 2][b % 2 * 8];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) x = fmaxf(x, s[b / 2][b % 2 * 8 + i]);
-        return x;
     }
 
     // A tile of keys and values in LDS, positions t0 ..
@@ -162,14 +154,23 @@ struct Tile8Rows {
         }
         // score i of 32 tokens tb: token 32 tb + 8 (i / 4) + 4 half + i % 4, of block
         // 2 tb + i / 8
-        float units[NB], vs[NB];
+        float units[NB], vs[NB], most[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             units[b] = sc.k(b) * qscale;
             vs[b] = sc.v(b);
         }
-        const bool loud = sc.loud();
-        if (t0 + M::TILE > min(all, end) || loud) {
+        auto each_most = [&] {       // the lane's largest of each block's
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                most[b] = s[b / 2][b % 2 * 8];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) most[b] = fmaxf(most[b], s[b / 2][b % 2 * 8 + i]);
+            }
+        };
+        auto row_most = [](float x) { return fmaxf(x, __shfl_xor(x, 32)); };
+        const bool loud = sc.loud(), far = sc.far(far_from);
+        if (t0 + M::TILE > min(all, end) || loud || far) {
             asm volatile("");        // (or every tile does all of this and selects)
 #pragma unroll
             for (int tb = 0; tb < M::TB; ++tb) {
@@ -186,36 +187,26 @@ struct Tile8Rows {
                     units[b] = FLT_MIN;
                 }
             }
-            if (loud) {
-                float x[NB], most = m;
+            if (__builtin_expect(far, 0)) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
-                    x[b] = block_top(s, b) * units[b];
-                    most = fmaxf(most, x[b]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s[b / 2][b % 2 * 8 + i] *= units[b];
+                    units[b] = 1.0f;
                 }
-                drop_far(vs, x, fmaxf(most, __shfl_xor(most, 32)));
+            }
+            if (__builtin_expect(loud, 0)) {
+                each_most();
+                drop_far<NB>(vs, most, units, row.m, row_most);
             }
         }
-        float mx = -INFINITY, mv = -INFINITY;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const float x = block_top(s, b) * units[b];
-            mx = fmaxf(mx, x);
-            mv = fmaxf(mv, x + above(sc.v(b)));
-        }
-        mv -= kWeightBits;
-        if (__builtin_amdgcn_ballot_w64(mx > m + kMoveMax || mv > top + kMoveTop) != 0) {
-            mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
-            mv = fmaxf(top, fmaxf(mv, __shfl_xor(mv, 32)));
-            mx = lowered(mx, mv);
-            l *= exp2_fast(m - mx);
-            const float f = exp2_fast(top - mv);
-            m = mx;
-            top = mv;
+        each_most();
+        float f;
+        if (move_row<NB>(row, sc, most, units, row_most, f)) {
 #pragma unroll
             for (int cb = 0; cb < M::CB; ++cb) O[cb] *= f;
         }
-        const float down = exp2_fast(m - top);
+        const float down = exp2_fast(-row.lead);
 #pragma unroll
         for (int b = 0; b < NB; ++b) vs[b] *= down;
         // transposed: lanes of 16 take tokens 4 half .. + 3 of 16 channels
@@ -229,9 +220,9 @@ struct Tile8Rows {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float x = s[b / 2][b % 2 * 8 + 2 * i], y = s[b / 2][b % 2 * 8 + 2 * i + 1];
-                const float p0 = exp2_fast(fmaf(x, units[b], -m));
-                const float p1 = exp2_fast(fmaf(y, units[b], -m));
-                l += p0 + p1;
+                const float p0 = exp2_fast(fmaf(x, units[b], -row.m));
+                const float p1 = exp2_fast(fmaf(y, units[b], -row.m));
+                row.l += p0 + p1;
                 if constexpr (NP == 2) {
                     const Pieces w = split_f16(p0 * vs[b], p1 * vs[b]);
                     pf[0][i] = w.hi;
@@ -318,12 +309,12 @@ __global__ void __launch_bounds__(WAVES * kWave, DP <= 128 && DT != kSrcF32 && W
         if (t0 >= end) break;
     }
 
-    float l = rows.l;
+    float l = rows.row.l;
     l += __shfl_xor(l, 32);
     const int r = w.it.row0 + 32 * wave + col;
     if (r >= w.rows) return;
     const bool whole = w.it.part < 0;
-    const float f = (whole ? inverse_sum(l) : 1.0f) * exp2_fast(rows.top - rows.m);
+    const float f = (whole ? inverse_sum(l) : 1.0f) * exp2_fast(rows.row.lead);
     const int64_t at = whole ? out_offset(a, w, r) : part_row(a, w, r);
 #pragma unroll
     for (int cb = 0; cb < M::CB; ++cb) {
@@ -339,7 +330,7 @@ __global__ void __launch_bounds__(WAVES * kWave, DP <= 128 && DT != kSrcF32 && W
         }
     }
     if (!whole && half == 0)
-        *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(rows.m, l);
+        *reinterpret_cast<float2*>(a.part_ml + 2 * at) = make_float2(rows.row.m, l);
 }
 
 template <int DT, int DP>

@@ -236,6 +236,46 @@ def test_rows_whose_weights_lie_on_quiet_blocks(hip_device, D, n, dtype, spread)
 
 
 @TYPES
+@ROWS
+@pytest.mark.parametrize("e", [4, 12, 14, 15, 16, 17, 20, 40])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_beyond_the_whole_numbers_of_fp32(hip_device, sign, e, lens, dtype):
+    """Scores of 2^(e + 14) (in log2), where one position's leads the others', which lie 0
+    or below: what sees it has its values, loud, ordinary or quiet, by weights that are 1
+    or 0, off by the weight's and the output's rounding alone; a position before it has
+    the mean of the others.  From 2^29 on fp32's numbers are 32 apart and more: a maximum
+    that weights are formed against cannot lie up to 75 below the largest score there, as
+    values below 2^-51 ask for, so those may count for less, down to nothing."""
+    D = 64
+    for scale in (2.0 ** -126, 2.0 ** -60, 1.0, 4.0 if dtype == HF else 2.0 ** 21):
+        case = Case(lens, 32, dtype, 4, 1, D, seed=e)
+        case.q[:] = 0
+        case.q[..., 0] = 1024
+        case.kc[:] = 0
+        leads = []
+        for s, c in enumerate(case.ctx):
+            lead = (c - case.new[s]) * 2 // 3 + (3 if case.new[s] > 5 else 0)
+            leads += [c - case.new[s] + i >= lead for i in range(case.new[s])]
+            for page, b in case.blocks(s, 0, c):
+                case.kc[page, 0, b * BLOCK:(b + 1) * BLOCK, 0] = -100 if sign < 0 else 0
+                case.ks[page, 0, b] = 2.0 ** e
+                case.vs[page, 0, b] = 1.0 if scale < 1 else scale
+            page, b = next(case.blocks(s, lead // BLOCK * BLOCK, lead + 1))
+            case.kc[page, 0, b * BLOCK + lead % BLOCK, 0] = -64 if sign < 0 else 127
+            case.vs[page, 0, b] = scale
+        o = case.run().double().cpu()
+        ref, tol = case.expected()
+        half = 2.0 ** -22 if dtype == FF else 2.0 ** -11
+        least = 2.0 ** -25 if dtype == HF else 2.0 ** -126
+        one = (EPS[dtype] / 2 + half + 32 * 2.0 ** -24) * ref.abs() + least
+        if e >= 15 and scale < 2.0 ** -51:
+            one += ref.abs()
+        tol = torch.where(torch.tensor(leads)[:, None, None], one, tol)
+        err = (o - ref).abs()
+        assert bool((err <= tol).all()), (e, scale, float((err / tol).max()))
+
+
+@TYPES
 def test_an_appended_context_of_zeros(hip_device, dtype):
     """Through the append: a prompt of zeros, then tokens of zeros, then one of numbers."""
     C, page, Hq, Hkv, D = _c(), 32, 8, 2, 64
