@@ -460,3 +460,37 @@ def test_a_step_of_no_tokens(hip_device):
     q = torch.zeros(3, 4, 64, dtype=BF, device=DEV)
     assert _c().paged_append(k, k, *pages, plan, **scales) is None
     assert bool((_c().paged_attention(q, *pages, plan, **scales) == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FF], ids=["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [48, 128])
+def test_append_of_rows_at_any_alignment_and_in_place(hip_device, D, dtype):
+    """Rows whose strides are no whole vectors give the codes of contiguous ones; queries
+    may be turned where they lie."""
+    page, Hq, Hkv = 32, 4, 2
+    table, pool, ctx, new = make_table([(7, 30), (40, 1)], page, 3)
+    T = sum(new)
+    q, k, v = _rows(new, Hq, Hkv, D, dtype, 9)
+    cos, sin = _c().rotary_tables(max(ctx), 32, device=DEV)
+    weights = torch.rand(2, D, generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    kw = dict(cos=cos, sin=sin, q_norm=weights[0], k_norm=weights[1])
+    plan = _plan(table, ctx, new, pool, page, Hq, Hkv, D, dtype)
+    pools = [t.cuda() for t in (*filled_pool8(table, pool, ctx, Hkv, D, page, 1),
+                                *filled_pool8(table, pool, ctx, Hkv, D, page, 2))]
+
+    def append(q, k, v, q_out=None):
+        kc, ks, vc, vs = (t.clone() for t in pools)
+        got = _c().paged_append(k, v, kc, vc, plan, q=q, q_out=q_out, k_scales=ks, v_scales=vs,
+                                **kw)
+        return got.clone(), kc, ks, vc, vs
+
+    want = append(q.cuda(), k.cuda(), v.cuda())
+    odd = torch.full((T + 2, (Hq + 2 * Hkv) * D + 3), float("nan"), dtype=dtype, device=DEV)
+    rows = odd[:T, 1:1 + (Hq + 2 * Hkv) * D].unflatten(1, (-1, D))
+    rows.copy_(torch.cat([q, k, v], 1))
+    got = append(rows[:, :Hq], rows[:, Hq:Hq + Hkv], rows[:, Hq + Hkv:])
+    place = q.cuda().contiguous()
+    there = append(place, k.cuda(), v.cuda(), q_out=place)
+    for a, b, c in zip(want, got, there):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        assert torch.equal(a.view(torch.uint8), c.view(torch.uint8))
