@@ -928,8 +928,9 @@ def paged_append(k, v, k_pages, v_pages, plan, q=None, q_out=None, cos=None, sin
     Pages of int8 (a plan with ``cache_dtype=torch.int8``) have ``k_scales`` and
     ``v_scales`` ``[num_pages, Hkv, page_size / 16]`` fp32 beside them, one for each
     block of 16 positions of a page and head: the least power of two from 2^-126 on
-    whose 127-fold reaches the block's values; an element is code * scale, its code
-    the quotient rounded to nearest even.  A block's older codes are rounded again
+    whose 127-fold reaches every value appended to the block since its first position
+    was (tokens taken back among them); an element is code * scale, its code the
+    quotient rounded to nearest even.  A block's older codes are rounded again
     where new tokens need a larger scale.  What a block's first position finds there
     is not read.  A value that is not finite makes its block's scale NaN."""
     dev = plan._index

@@ -12,8 +12,18 @@
 // for a wave's tile of 64 positions at 128 channels; the products alone are two thirds of
 // the time).  Hence little else is done per score: one multiply-add, one exponential, one
 // sum, half a packing; scales enter once per block of 16 positions.  A chunk of 2048
-// tokens after 8200, 32/8 heads of 128, bf16: 345 us in tiles of 256 rows (900 TFLOP/s), 373
-// in tiles of 128; sixteen times five tokens after 3000, 28/4 heads: 24 us.
+// tokens after 8200, 32/8 heads of 128, bf16: 338 to 375 us from card to card (825 to 915
+// TFLOP/s) in tiles of 256 rows, 373 in tiles of 128 where those took 345; sixteen times five
+// tokens after 3000, 28/4 heads, fp16: 24 us.  At 64 channels a score has half the products
+// and as many vector operations, which take 69 % of the cycles beside the products' 25 (four
+// chunks of 1024 after 3000, 12/12 heads: 80 to 85 us, 400 to 425 TFLOP/s); at 256 a SIMD has
+// one wave, whose operations (44 %) and products (25 %) nothing runs beside (2048 after 8200,
+// 28/4 heads: 1005 us, 540 TFLOP/s).
+//
+// 16-bit types' weights are rounded once here.  A second piece would take the chunk from 338
+// to 450 us and the verification from 24.2 to 27.5; with one the verification is off from
+// float64 by 0.00024 of the outputs (fp16; their own rounding alone by 0.00021), the chunk
+// by 0.0017 (bf16, as its rounding alone).
 #include <hip/hip_runtime.h>
 
 #include "kivi_paged8_attention.hpp"
